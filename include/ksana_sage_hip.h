@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define KSANA_SAGE_ABI_VERSION 24
+#define KSANA_SAGE_ABI_VERSION 25
 
 /* element types of q/k/v/o */
 #define KSANA_SAGE_BF16 0
@@ -444,6 +444,37 @@ typedef struct ksana_sage_call {
 } ksana_sage_call;
 int ksana_sage_forward_call(const ksana_sage_call* call, const void* q, const void* k, const void* v, void* o,
                             void* workspace, void* stream);
+
+/* ---- Operators with gradients: what a block's attention half needs where it is trained.  No counterpart in the reference,
+ * which only generates. ---- */
+
+/* Attention on 16-bit tensors [B, L, H, D] without quantization: o = softmax(sm_scale q k^T) v, and its backward pass, which
+ * recomputes the probabilities.  D = 128 or 64, Hq a multiple of Hkv; products of 16-bit operands accumulated in fp32, softmax statistics in
+ * fp32, probabilities and their gradients rounded to the tensors' type where they are multiplied on.  Repeated calls give the
+ * same bits. */
+typedef struct ksana_sage_train_attn {
+  ksana_sage_shape shape;
+  int32_t dtype;          /* of q, k, v, o and all gradients                                                       */
+  int32_t causal;         /* row i sees keys 0 .. i                                                                */
+  float sm_scale;
+  int32_t reserved;       /* 0                                                                                     */
+  int64_t q_strides[4], k_strides[4], v_strides[4], o_strides[4];
+  const int32_t* q_lens;  /* device, [B] or NULL: only the first q_lens[b] query rows are computed, the others are zeros */
+  const int32_t* k_lens;  /* device, [B] or NULL: only the first k_lens[b] keys are seen; what lies behind them is not    */
+                          /* read.  Rows without any key: o = 0, lse = -inf, gradients 0.  Any int32, clamped.            */
+} ksana_sage_train_attn;
+/* Device scratch (256-byte aligned, 0 bytes: none needed) of the two calls below; any out-pointer may be NULL.  Not kept
+ * between calls. */
+int ksana_sage_train_attn_scratch(const ksana_sage_train_attn* call, uint64_t* fwd_bytes, uint64_t* bwd_bytes);
+/* lse: fp32 [B, Hq, Lq], contiguous, natural logarithm of each row's sum of exp(sm_scale q k); NULL if no backward follows. */
+int ksana_sage_train_attn_fwd(const ksana_sage_train_attn* call, const void* q, const void* k, const void* v, void* o,
+                              float* lse, void* scratch, void* stream);
+/* o and lse: as the forward call of the same arguments wrote them.  d_o: the result's gradient, [B, Lq, Hq, D] with
+ * do_strides.  dq, dk, dv: contiguous [B, L, H, D], written whole (zeros where nothing takes part); dq may be NULL, dk and
+ * dv may be NULL together: what nobody wants is not computed. */
+int ksana_sage_train_attn_bwd(const ksana_sage_train_attn* call, const void* q, const void* k, const void* v, const void* o,
+                              const float* lse, const void* d_o, const int64_t do_strides[4], void* dq, void* dk, void* dv,
+                              void* scratch, void* stream);
 
 #ifdef __cplusplus
 }

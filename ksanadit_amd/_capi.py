@@ -11,7 +11,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libksana_sage_hip.so"
-ABI_VERSION = 24
+ABI_VERSION = 25
 
 BF16, FP16 = 0, 1
 OK, EINVAL, ENOTSUP, EHIP = 0, -1, -2, -3
@@ -59,6 +59,9 @@ EXPORTS = (
     "ksana_sage_forward_scratch",
     "ksana_sage_sla_forward_bytes",
     "ksana_sage_sla_forward",
+    "ksana_sage_train_attn_scratch",
+    "ksana_sage_train_attn_fwd",
+    "ksana_sage_train_attn_bwd",
 )
 
 
@@ -102,6 +105,13 @@ class Call(C.Structure):
 
     _fields_ = [("shape", Shape)] + [(n, C.c_int32) for n in ("dtype", "o_dtype", "smooth_k", "causal", "flags")] + \
         [("sm_scale", C.c_float)] + [(n, C.c_int64 * 4) for n in ("q_strides", "k_strides", "v_strides", "o_strides")]
+
+
+class TrainAttn(C.Structure):
+    """``ksana_sage_train_attn``: an attention call with gradients but for its buffers and its stream."""
+
+    _fields_ = [("shape", Shape), ("dtype", C.c_int32), ("causal", C.c_int32), ("sm_scale", C.c_float), ("reserved", C.c_int32)] + \
+        [(n, C.c_int64 * 4) for n in ("q_strides", "k_strides", "v_strides", "o_strides")] + [("q_lens", C.c_void_p), ("k_lens", C.c_void_p)]
 
 
 class SageLibraryError(RuntimeError):
@@ -168,6 +178,9 @@ def _declare(lib):
     lib.ksana_sage_forward_varlen.argtypes = [vp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, f, i, i, i, vp, vp]
     lib.ksana_sage_forward_varlen.restype = i
     lib.ksana_sage_forward_call.argtypes, lib.ksana_sage_forward_call.restype = [vp] * 7, i
+    lib.ksana_sage_train_attn_scratch.argtypes, lib.ksana_sage_train_attn_scratch.restype = [vp] * 3, i
+    lib.ksana_sage_train_attn_fwd.argtypes, lib.ksana_sage_train_attn_fwd.restype = [vp] * 8, i
+    lib.ksana_sage_train_attn_bwd.argtypes, lib.ksana_sage_train_attn_bwd.restype = [vp] * 13, i
 
 
 def library_present() -> bool:

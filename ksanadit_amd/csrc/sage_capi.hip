@@ -12,6 +12,7 @@
 
 #include "../../include/ksana_sage_hip.h"
 #include "sage_kernels.h"
+#include "sage_train.h"
 
 // Scratch of ksana_sage_quant_k_static: the chunk sums of K's channel means, [B * Hkv * ceil(Lk / 256)][128]
 // fp32, followed by the counters and flags through which the workgroups of a head meet (cleared by a small kernel
@@ -1033,3 +1034,118 @@ int forward_impl(const void* q, const void* k, const void* v, void* o, int dtype
                    attn_flags, own_q ? &q_rows : nullptr, q_premul_of(sm_scale), stream, nullptr, numbered);
 }
 }  // namespace
+
+// ------------------------------------------------------------------------------------ operators with gradients
+
+namespace {
+// The call as the launchers take it, its extents and strides checked
+int train_attn_params(const ksana_sage_train_attn* c, ksana_sage::TrainAttnParams* p) {
+  if (!c) return fail(KSANA_SAGE_EINVAL, "call is null");
+  const ksana_sage_shape& s = c->shape;
+  if (s.B < 1 || s.Hq < 1 || s.Hkv < 1 || s.Lq < 1 || s.Lk < 1)
+    return fail(KSANA_SAGE_EINVAL, "shape has a non-positive extent (B=%d Hq=%d Hkv=%d Lq=%d Lk=%d)", s.B, s.Hq, s.Hkv, s.Lq, s.Lk);
+  if (s.Hq % s.Hkv != 0) return fail(KSANA_SAGE_EINVAL, "Hq=%d is not a multiple of Hkv=%d", s.Hq, s.Hkv);
+  if (s.D != 128 && s.D != 64) return fail(KSANA_SAGE_ENOTSUP, "head size %d not supported (128 or 64)", s.D);
+  if (c->dtype != KSANA_SAGE_BF16 && c->dtype != KSANA_SAGE_FP16) return fail(KSANA_SAGE_EINVAL, "dtype %d unknown", c->dtype);
+  if (c->reserved != 0) return fail(KSANA_SAGE_EINVAL, "reserved is %d, must be 0", c->reserved);
+  if (!(c->sm_scale > -INFINITY && c->sm_scale < INFINITY)) return fail(KSANA_SAGE_EINVAL, "sm_scale is not finite");
+  if (s.Lq > (1 << 24) || s.Lk > (1 << 24)) return fail(KSANA_SAGE_ENOTSUP, "Lq=%d Lk=%d: at most %d", s.Lq, s.Lk, 1 << 24);
+  // query rows of the heads of a key head are numbered together: their number in an int, its division by a product of 32 x 32 bits
+  const int64_t group = s.Hq / s.Hkv;
+  if ((int64_t)s.Lq * group > (1 << 28) || (int64_t)s.Lq * group * group > (INT64_C(1) << 32) - 1)
+    return fail(KSANA_SAGE_ENOTSUP, "Lq=%d with %lld query heads to a key head: too many rows", s.Lq, (long long)group);
+  if ((int64_t)s.B * s.Hkv > 65535) return fail(KSANA_SAGE_ENOTSUP, "B*Hkv = %lld exceeds the launch grid (65535)", (long long)s.B * s.Hkv);
+  const int64_t most = (s.Lq * group > s.Lk ? s.Lq * group : s.Lk) / 64 + 2;
+  if ((int64_t)s.B * s.Hkv * most > (INT64_C(1) << 30)) return fail(KSANA_SAGE_ENOTSUP, "the call's workgroups exceed the launch grid");
+  if (reinterpret_cast<uintptr_t>(c->q_lens) & 3) return fail(KSANA_SAGE_EINVAL, "q_lens is not 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(c->k_lens) & 3) return fail(KSANA_SAGE_EINVAL, "k_lens is not 4-byte aligned");
+  *p = ksana_sage::TrainAttnParams{};
+  p->q_lens = c->q_lens;
+  p->k_lens = c->k_lens;
+  p->dtype = c->dtype;
+  p->B = s.B;
+  p->Hq = s.Hq;
+  p->Hkv = s.Hkv;
+  p->Lq = s.Lq;
+  p->Lk = s.Lk;
+  p->D = s.D;
+  p->causal = c->causal ? 1 : 0;
+  p->sm_scale = c->sm_scale;
+  return 0;
+}
+
+int train_tensor(const char* name, const void* ptr, const ksana_sage_train_attn* c, const int64_t st[4], int L, int H, ksana_sage::TrainTensor* out) {
+  if (int rc = check_tensor(name, ptr, c->dtype, st, c->shape.B, L, H)) return rc;
+  // a tile's rows are addressed by 32-bit byte offsets from its first one
+  const int64_t group = c->shape.Hq / c->shape.Hkv;
+  if ((L > 1 && st[1] > (INT64_C(1) << 23)) || (H > 1 && st[2] > (INT64_C(1) << 30) / group))
+    return fail(KSANA_SAGE_ENOTSUP, "%s: strides %lld, %lld of its rows and heads are beyond the kernels' offsets", name, (long long)st[1], (long long)st[2]);
+  *out = ksana_sage::TrainTensor{st[0], st[1], st[2]};
+  return 0;
+}
+
+int train_scratch_given(uint64_t bytes, const void* scratch) {
+  if (bytes == 0) return 0;
+  if (!scratch) return fail(KSANA_SAGE_EINVAL, "scratch is null, the call needs %llu bytes", (unsigned long long)bytes);
+  if (reinterpret_cast<uintptr_t>(scratch) & 255) return fail(KSANA_SAGE_EINVAL, "scratch is not 256-byte aligned");
+  return 0;
+}
+}  // namespace
+
+extern "C" int ksana_sage_train_attn_scratch(const ksana_sage_train_attn* call, uint64_t* fwd_bytes, uint64_t* bwd_bytes) {
+  ksana_sage::TrainAttnParams p;
+  if (int rc = train_attn_params(call, &p)) return rc;
+  if (fwd_bytes) *fwd_bytes = ksana_sage::train_attn_scratch(p, false).bytes;
+  if (bwd_bytes) *bwd_bytes = ksana_sage::train_attn_scratch(p, true).bytes;
+  return 0;
+}
+
+extern "C" int ksana_sage_train_attn_fwd(const ksana_sage_train_attn* call, const void* q, const void* k, const void* v, void* o, float* lse,
+                                         void* scratch, void* stream) {
+  ksana_sage::TrainAttnParams p;
+  if (int rc = train_attn_params(call, &p)) return rc;
+  if (int rc = train_tensor("q", q, call, call->q_strides, p.Lq, p.Hq, &p.qs)) return rc;
+  if (int rc = train_tensor("k", k, call, call->k_strides, p.Lk, p.Hkv, &p.ks)) return rc;
+  if (int rc = train_tensor("v", v, call, call->v_strides, p.Lk, p.Hkv, &p.vs)) return rc;
+  if (int rc = train_tensor("o", o, call, call->o_strides, p.Lq, p.Hq, &p.os)) return rc;
+  if (reinterpret_cast<uintptr_t>(lse) & 3) return fail(KSANA_SAGE_EINVAL, "lse is not 4-byte aligned");
+  if (int rc = train_scratch_given(ksana_sage::train_attn_scratch(p, false).bytes, scratch)) return rc;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.o = static_cast<uint16_t*>(o);
+  p.lse = lse;
+  const StageRange range("ksana_sage.train_attn_fwd");
+  const hipError_t e = ksana_sage::launch_train_attn_fwd(p, scratch, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "training attention, forward");
+}
+
+extern "C" int ksana_sage_train_attn_bwd(const ksana_sage_train_attn* call, const void* q, const void* k, const void* v, const void* o,
+                                         const float* lse, const void* d_o, const int64_t do_strides[4], void* dq, void* dk, void* dv,
+                                         void* scratch, void* stream) {
+  ksana_sage::TrainAttnParams p;
+  if (int rc = train_attn_params(call, &p)) return rc;
+  if (int rc = train_tensor("q", q, call, call->q_strides, p.Lq, p.Hq, &p.qs)) return rc;
+  if (int rc = train_tensor("k", k, call, call->k_strides, p.Lk, p.Hkv, &p.ks)) return rc;
+  if (int rc = train_tensor("v", v, call, call->v_strides, p.Lk, p.Hkv, &p.vs)) return rc;
+  if (int rc = train_tensor("o", o, call, call->o_strides, p.Lq, p.Hq, &p.os)) return rc;
+  if (int rc = train_tensor("d_o", d_o, call, do_strides, p.Lq, p.Hq, &p.dos)) return rc;
+  if (!lse || (reinterpret_cast<uintptr_t>(lse) & 3)) return fail(KSANA_SAGE_EINVAL, "lse is null or not 4-byte aligned");
+  if ((dk == nullptr) != (dv == nullptr)) return fail(KSANA_SAGE_EINVAL, "dk and dv are computed together: give both or neither");
+  for (const void* x : {dq, dk, dv})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return fail(KSANA_SAGE_EINVAL, "a gradient is not 16-byte aligned");
+  if (dq == nullptr && dk == nullptr) return 0;
+  if (int rc = train_scratch_given(ksana_sage::train_attn_scratch(p, true).bytes, scratch)) return rc;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.o_in = static_cast<const uint16_t*>(o);
+  p.d_o = static_cast<const uint16_t*>(d_o);
+  p.lse = const_cast<float*>(lse);
+  p.dq = static_cast<uint16_t*>(dq);
+  p.dk = static_cast<uint16_t*>(dk);
+  p.dv = static_cast<uint16_t*>(dv);
+  const StageRange range("ksana_sage.train_attn_bwd");
+  const hipError_t e = ksana_sage::launch_train_attn_bwd(p, scratch, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "training attention, backward");
+}

@@ -1,0 +1,44 @@
+// Launch interface of the differentiable operators (sage_train_attn.hip, sage_train_norm.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ksana_sage {
+
+struct TrainTensor {
+  int64_t sB, sL, sH;  // element strides of [B, L, H, D]; D stride is 1
+};
+
+struct TrainAttnParams {
+  const uint16_t *q, *k, *v, *d_o;
+  const uint16_t* o_in;  // backward: the result
+  uint16_t *o, *dq, *dk, *dv;  // dq, dk, dv: contiguous [B, L, H, D]
+  float* lse;  // [B, Hq, Lq], natural logarithm; -inf where a row has no key
+  TrainTensor qs, ks, vs, os, dos;
+  const int32_t *q_lens, *k_lens;  // nullptr: all rows, all keys
+  int dtype, B, Hq, Hkv, Lq, Lk, D, causal;
+  float sm_scale;
+  // filled in by the launchers
+  int group;            // Hq / Hkv
+  unsigned group_inv;   // ceil(2^32 / group)
+  float c;              // |sm_scale| log2(e)
+  uint32_t flip;        // sign bits of two 16-bit values where sm_scale is negative
+  int row_pad;          // rows of row_l and row_d of a key head: Lq * group up to a multiple of 64
+  float *row_l, *row_d; // backward: -log2(e) lse (-inf where a row takes no part) and -sum(dO o), [B Hkv, row_pad]
+  float* norms;         // backward in fp16: largest squared norms of rows of dO and of v, [B Hkv, norm_blocks]
+  int norm_blocks, norm_q_blocks;
+  int runs;             // of tiles that a block's loop is cut into
+  float* part;          // their results
+};
+
+struct TrainAttnScratch {
+  uint64_t bytes, row_l, row_d, norms, part;
+};
+
+// What the launchers need of scratch memory (256-byte aligned)
+TrainAttnScratch train_attn_scratch(const TrainAttnParams& p, bool backward);
+hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s);
+hipError_t launch_train_attn_bwd(TrainAttnParams p, void* scratch, hipStream_t s);
+
+}  // namespace ksana_sage

@@ -1,0 +1,661 @@
+// Attention for training: o = softmax(c q k^T) v on 16-bit tensors with its backward pass, which recomputes the probabilities.
+//
+//   forward   S = c q k^T,  lse = log sum exp S,  P = exp(S - lse),  o = P v
+//   backward  dv = P^T dO,  dP = dO v^T,  d = rowsum(dO o),  dS = P (dP - d),  dq = c dS k,  dk = c dS^T q
+//
+// Nothing of the size of S is kept: the forward pass walks the keys with a running maximum and sum, the backward pass forms S
+// again from q, k and lse, once for dk and dv (a workgroup keeps keys and walks the query rows) and once for dq (it
+// keeps query rows and walks the keys).  That is seven products of the backward pass where five would do with dq summed by
+// atomic additions of all workgroups: their order would change the result from call to call.
+//
+// P and dS are rounded to the tensors' type where they become matrix operands; S, dP, all sums and accumulators are fp32.
+#include "sage_train_device.h"
+
+#include <atomic>
+#include <cmath>
+
+namespace ksana_sage {
+
+namespace {
+
+extern __shared__ __align__(1024) char train_lds[];
+__device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)train_lds; }
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+// Rounded to fp16, probabilities relative to a row's largest would lose bits from 2^-14 on and vanish at 2^-25; scaled up as far as
+// the format goes, they do so a factor of 2^6 (forward, where the reference point may lag by 2^kLazy) or 2^15 (backward) later.
+constexpr float kLazy = 8.0f;
+template <int DT>
+constexpr float kForwardShift = DT == KSANA_SAGE_FP16 ? 6.0f : 0.0f;
+template <int DT>
+constexpr float kBackwardShift = DT == KSANA_SAGE_FP16 ? 15.0f : 0.0f;
+
+struct Extent {
+  int rows, keys;  // of a batch entry that take part; rows: numbered over the heads of a key head
+};
+__device__ __forceinline__ Extent extent_of(const TrainAttnParams& p, int b) {
+  int lq = p.Lq, lk = p.Lk;
+  take_counts(p.q_lens, p.k_lens, b, lq, lk);
+  return Extent{lk > 0 ? lq * p.group : 0, lk};
+}
+
+// A lane's query row as B operands: channels 16 s + 8 hh ..
+template <int D>
+__device__ __forceinline__ void load_row(const uint16_t* row, int hh, uint32_t flip, v4i (&out)[Tile<D>::kSteps]) {
+#pragma unroll
+  for (int s = 0; s < Tile<D>::kSteps; ++s) {
+    uint4 x = *reinterpret_cast<const uint4*>(row + 16 * s + 8 * hh);
+    out[s] = v4i{(int)(x.x ^ flip), (int)(x.y ^ flip), (int)(x.z ^ flip), (int)(x.w ^ flip)};
+  }
+}
+
+// Numbers of the keys of accumulator i of 32-key block t: 32 t + 8 (i / 4) + 4 hh + i % 4
+__device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+// ------------------------------------------------------------------------------------------------------------ forward
+
+template <int DT, int D, int kCols>
+__global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel(const TrainAttnParams p) {
+  using T = Tile<D>;
+  constexpr int kWaves = 4, kRowsWg = kWaves * 32 * kCols, kStages = 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
+  const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
+  const int w = xcd_run_number();
+  if (w >= p.B * p.Hkv * blocks) return;
+  const int bh = w / blocks, block = blocks - 1 - (w - bh * blocks), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const Extent e = extent_of(p, b);
+  const int row0 = block * kRowsWg;
+  int keys = e.keys;
+  if (p.causal) keys = min(keys, row_position(p, min(row0 + kRowsWg, all_rows) - 1) + 1);
+  const int tiles = row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0;
+
+  const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
+  const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
+  const unsigned lds = lds_base();
+  v16f acc[kCols][T::kBlocks];
+  float top[kCols], minus[kCols], sum[kCols];  // reference point of the row (unscaled), what is added to its scaled scores, its sum
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) {
+    top[n] = -INFINITY;
+    minus[n] = kForwardShift<DT>;
+    sum[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < T::kBlocks; ++d) acc[n][d] = v16f{};
+  }
+  int row[kCols], limit[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) {
+    row[n] = row0 + (wave * kCols + n) * 32 + m;
+    limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
+  }
+  if (tiles > 0) {
+    auto copy = [&](int t) {
+      const int at = min(t, tiles - 1) * kTrainTile;
+      const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
+      copy_key_tile<D, kWaves>(k_head, p.ks.sL, at, e.keys, stage, wave, lane);
+      copy_key_tile<D, kWaves>(v_head, p.vs.sL, at, e.keys, stage + T::kBytes, wave, lane);
+    };
+    copy(0);
+    v4i q[kCols][T::kSteps];
+#pragma unroll
+    for (int n = 0; n < kCols; ++n)
+      load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, min(row[n], e.rows - 1)), hh, p.flip, q[n]);
+    const RowReader<D> k_reader(lane);
+    const ColumnReader<D> v_reader(lane);
+    // keys that every row of the wave sees
+    const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
+    const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      tile_ready<0>();
+      copy(t + 1);
+      const unsigned k_tile = lds + (t % kStages) * 2 * T::kBytes, v_tile = k_tile + T::kBytes;
+      v16f s[kCols][2];
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) s[n][0] = s[n][1] = v16f{};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
+          const v4i a = k_reader.read(k_tile, h, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) s[n][h] = mfma16<DT>(a, q[n][st], s[n][h]);
+        }
+      if ((t + 1) * kTrainTile > all_see) {
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          const int left = limit[n] - t * kTrainTile - 4 * hh;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[n][h][i] = 32 * h + acc_row(i) < left ? s[n][h][i] : -INFINITY;
+        }
+      }
+      float most[kCols];
+      bool move = false;
+#pragma unroll
+      for (int n = 0; n < kCols; ++n) {
+        float x = fmaxf(s[n][0][0], s[n][1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) x = fmaxf(x, fmaxf(s[n][0][i], s[n][1][i]));
+        most[n] = over_halves<Max>(x);
+        move = move || most[n] * p.c > kLazy + kForwardShift<DT> - minus[n] || (top[n] == -INFINITY && most[n] > -INFINITY);
+      }
+      if (__any(move)) {
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          const float next = fmaxf(top[n], most[n]);
+          const float factor = next == -INFINITY ? 1.0f : fast_exp2((top[n] - next) * p.c);
+          top[n] = next;
+          minus[n] = next == -INFINITY ? kForwardShift<DT> : kForwardShift<DT> - next * p.c;
+          sum[n] *= factor;
+#pragma unroll
+          for (int d = 0; d < T::kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][d][i] *= factor;
+        }
+      }
+      v4i pr[kCols][4];
+#pragma unroll
+      for (int n = 0; n < kCols; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[i] = fast_exp2(__fmaf_rn(s[n][h][i], p.c, minus[n]));
+            sum[n] += x[i];
+          }
+          pr[n][2 * h] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+          pr[n][2 * h + 1] = pack8<DT>(x[8], x[9], x[10], x[11], x[12], x[13], x[14], x[15]);
+        }
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int d = 0; d < T::kBlocks; ++d) {
+          const v4i a = v_reader.read(v_tile, d, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) acc[n][d] = mfma16<DT>(a, pr[n][st], acc[n][d]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup's LDS
+  }
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) {
+    const bool takes_part = row[n] < e.rows, exists = row[n] < all_rows;
+    const float total = over_halves<Sum>(sum[n]);
+    const float factor = !takes_part || total == 0.0f ? 0.0f : 1.0f / total;
+    const int r = min(row[n], all_rows - 1), l = row_position(p, r), h = hk * p.group + r - l * p.group;
+    if (!takes_part) {
+#pragma unroll
+      for (int d = 0; d < T::kBlocks; ++d) acc[n][d] = v16f{};
+    }
+    store_column<DT, D>(acc[n], factor, p.o + b * p.os.sB + l * p.os.sL + h * p.os.sH, hh, exists);
+    if (exists && hh == 0 && p.lse != nullptr)
+      p.lse[((int64_t)b * p.Hq + h) * p.Lq + l] = factor == 0.0f ? -INFINITY : (log2f(total) - minus[n]) * kLn2;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ backward
+
+// Per query row -log2(e) lse and -sum(dO o); in fp16 besides the largest squared norms of rows of dO and of v per block of rows.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void sage_train_rows_kernel(const TrainAttnParams p) {
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes;  // lanes of a row, rows at a time
+  constexpr int kBlockRows = 256;
+  const int lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+  const int bh = blockIdx.y, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const Extent e = extent_of(p, b);
+  float largest = 0.0f;
+  const bool of_v = (int)blockIdx.x >= p.norm_q_blocks;  // fp16 only
+  if (!of_v) {
+#pragma unroll 2
+    for (int i = 0; i < kBlockRows / kRows; ++i) {
+      const int r = blockIdx.x * kBlockRows + i * kRows + slot;
+      float d = 0.0f, square = 0.0f;
+      if (r < e.rows) {
+        const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
+        const uint4 x = *reinterpret_cast<const uint4*>(p.d_o + b * p.dos.sB + l * p.dos.sL + h * p.dos.sH + 8 * lane);
+        const uint4 y = *reinterpret_cast<const uint4*>(p.o_in + b * p.os.sB + l * p.os.sL + h * p.os.sH + 8 * lane);
+        float a[8], c[8];
+        widen8<DT>(x, a);
+        widen8<DT>(y, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          d = __fmaf_rn(a[j], c[j], d);
+          square = __fmaf_rn(a[j], a[j], square);
+        }
+      }
+#pragma unroll
+      for (int j = kLanes / 2; j > 0; j >>= 1) {
+        d += __shfl_xor(d, j);
+        if (DT == KSANA_SAGE_FP16) square += __shfl_xor(square, j);
+      }
+      largest = fmaxf(largest, square);
+      if (lane == 0 && r < p.row_pad) {
+        float minus = -INFINITY;
+        if (r < e.rows) {
+          const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
+          const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + l];
+          minus = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+        }
+        p.row_l[(int64_t)bh * p.row_pad + r] = minus;
+        p.row_d[(int64_t)bh * p.row_pad + r] = -d;
+      }
+    }
+  } else {
+    const int first = ((int)blockIdx.x - p.norm_q_blocks) * kBlockRows;
+#pragma unroll 2
+    for (int i = 0; i < kBlockRows / kRows; ++i) {
+      const int r = first + i * kRows + slot;
+      float square = 0.0f;
+      if (r < e.keys) {
+        float a[8];
+        widen8<DT>(*reinterpret_cast<const uint4*>(p.v + b * p.vs.sB + r * p.vs.sL + hk * p.vs.sH + 8 * lane), a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) square = __fmaf_rn(a[j], a[j], square);
+      }
+#pragma unroll
+      for (int j = kLanes / 2; j > 0; j >>= 1) square += __shfl_xor(square, j);
+      largest = fmaxf(largest, square);
+    }
+  }
+  if (DT == KSANA_SAGE_FP16) {
+    __shared__ float of_wave[4];
+    largest = over_lanes<Max>(largest);
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = largest;
+    __syncthreads();
+    if (threadIdx.x == 0)
+      p.norms[(int64_t)bh * p.norm_blocks + blockIdx.x] = fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
+  }
+}
+
+// In fp16 dS is scaled by the power of two that brings its bound, 2 max|dO| max|v|, to one (and by 2^15 with P): gradients of any
+// size, 1e-8 or 1e4, then keep the format's bits and cannot overflow it.
+__device__ __forceinline__ float ds_scale(const TrainAttnParams& p, int bh, int lane) {
+  const float* n = p.norms + (int64_t)bh * p.norm_blocks;
+  float q = 0.0f, v = 0.0f;
+  for (int i = lane; i < p.norm_blocks; i += 64) {
+    const float x = n[i];
+    if (i < p.norm_q_blocks)
+      q = fmaxf(q, x);
+    else
+      v = fmaxf(v, x);
+  }
+  q = over_lanes<Max>(q);
+  v = over_lanes<Max>(v);
+  const float most = 2.0f * sqrtf(q) * sqrtf(v);
+  // (not a number, infinite or zero: no scaling)
+  if (!(most > 0.0f && most < INFINITY)) return 1.0f;
+  int ex;
+  frexpf(most, &ex);
+  return ldexpf(1.0f, max(-100, min(100, -ex)));
+}
+
+template <int DT, int D, int kCols>
+__global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel(const TrainAttnParams p) {
+  using T = Tile<D>;
+  constexpr int kWaves = 4, kKeysWg = kWaves * 32 * kCols, kStages = 2;
+  constexpr int kStage = 2 * T::kBytes + 2 * kTrainTile * 4;  // q, dO, row_l, row_d
+  constexpr bool kHalf = DT == KSANA_SAGE_FP16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
+  const int blocks = (p.Lk + kKeysWg - 1) / kKeysWg;
+  const int w = xcd_run_number();
+  if (w >= p.B * p.Hkv * blocks) return;
+  const int bh = w / blocks, block = w - bh * blocks, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const Extent e = extent_of(p, b);
+  const int key0 = block * kKeysWg;
+  const int tiles = key0 < e.keys ? (e.rows + kTrainTile - 1) / kTrainTile : 0;
+  const int first_tile = p.causal ? (int)min((int64_t)key0 * p.group / kTrainTile, (int64_t)tiles) : 0;
+
+  const unsigned lds = lds_base();
+  v16f dk[kCols][T::kBlocks], dv[kCols][T::kBlocks];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n)
+#pragma unroll
+    for (int d = 0; d < T::kBlocks; ++d) dk[n][d] = dv[n][d] = v16f{};
+  float scale = 1.0f;
+  int key[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) key[n] = key0 + (wave * kCols + n) * 32 + m;
+  if (first_tile < tiles) {
+    const uint16_t* q_heads = p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH;
+    const uint16_t* do_heads = p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH;
+    const float* row_l = p.row_l + (int64_t)bh * p.row_pad;
+    const float* row_d = p.row_d + (int64_t)bh * p.row_pad;
+    auto copy = [&](int t) {
+      const int at = min(t, tiles - 1) * kTrainTile;
+      const unsigned stage = lds + (t % kStages) * kStage;
+      copy_query_tile<D, kWaves>(p, q_heads, p.qs, at, e.rows, stage, wave, lane);
+      copy_query_tile<D, kWaves>(p, do_heads, p.dos, at, e.rows, stage + T::kBytes, wave, lane);
+      // (two waves each, so that every wave has as many copies in flight)
+      lds_copy4_at((wave & 1 ? row_d : row_l) + at, lane * 4, stage + 2 * T::kBytes + (wave & 1) * kTrainTile * 4);
+    };
+    copy(first_tile);
+    v4i k[kCols][T::kSteps], v[kCols][T::kSteps];
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      const int at = min(key[n], e.keys - 1);
+      load_row<D>(p.k + b * p.ks.sB + at * p.ks.sL + hk * p.ks.sH, hh, p.flip, k[n]);
+      load_row<D>(p.v + b * p.vs.sB + at * p.vs.sL + hk * p.vs.sH, hh, 0, v[n]);
+    }
+    if constexpr (kHalf) scale = ds_scale(p, bh, lane);
+    const RowReader<D> rows(lane);
+    const ColumnReader<D> columns(lane);
+    const int64_t sees_all = (int64_t)(key0 + (wave + 1) * 32 * kCols - 1) * p.group;  // the first row that sees every key of the wave
+#pragma unroll 1
+    for (int t = first_tile; t < tiles; ++t) {
+      tile_ready<0>();
+      copy(t + 1);
+      const unsigned q_tile = lds + (t % kStages) * kStage, do_tile = q_tile + T::kBytes, stats = do_tile + T::kBytes;
+      const bool diagonal = p.causal && (int64_t)t * kTrainTile < sees_all;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v16f s[kCols], dp[kCols];
+        v4f l[4], d[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          l[g] = *(LdsF4)(uintptr_t)(stats + (32 * h + 8 * g + 4 * hh) * 4);
+          d[g] = *(LdsF4)(uintptr_t)(stats + (kTrainTile + 32 * h + 8 * g + 4 * hh) * 4);
+        }
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          s[n] = v16f{};
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[n][i] = d[i >> 2][i & 3];
+        }
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
+          const v4i a = rows.read(q_tile, h, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) s[n] = mfma16<DT>(a, k[n][st], s[n]);
+        }
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
+          const v4i a = rows.read(do_tile, h, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, v[n][st], dp[n]);
+        }
+        v4i pr[kCols][2], ds[kCols][2];
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          float x[16], y[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[i >> 2][i & 3] + kBackwardShift<DT>));
+          if (diagonal) {
+            const int64_t from = (int64_t)key[n] * p.group - t * kTrainTile - 32 * h - 4 * hh;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = acc_row(i) < from ? 0.0f : x[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = x[i] * (kHalf ? dp[n][i] * scale : dp[n][i]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            pr[n][j] = pack8<DT>(x[8 * j], x[8 * j + 1], x[8 * j + 2], x[8 * j + 3], x[8 * j + 4], x[8 * j + 5], x[8 * j + 6], x[8 * j + 7]);
+            ds[n][j] = pack8<DT>(y[8 * j], y[8 * j + 1], y[8 * j + 2], y[8 * j + 3], y[8 * j + 4], y[8 * j + 5], y[8 * j + 6], y[8 * j + 7]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < T::kBlocks; ++c) {
+            const v4i a = columns.read(do_tile, c, 2 * h + j);
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) dv[n][c] = mfma16<DT>(a, pr[n][j], dv[n][c]);
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < T::kBlocks; ++c) {
+            const v4i a = columns.read(q_tile, c, 2 * h + j);
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) dk[n][c] = mfma16<DT>(a, ds[n][j], dk[n][c]);
+          }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  const float unshift = fast_exp2(-kBackwardShift<DT>);
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) {
+    const bool exists = key[n] < p.Lk;
+    if (key[n] >= e.keys) {
+#pragma unroll
+      for (int c = 0; c < T::kBlocks; ++c) dk[n][c] = dv[n][c] = v16f{};
+    }
+    const int64_t at = (((int64_t)b * p.Lk + min(key[n], p.Lk - 1)) * p.Hkv + hk) * D;
+    store_column<DT, D>(dk[n], p.sm_scale * unshift / scale, p.dk + at, hh, exists);
+    store_column<DT, D>(dv[n], unshift, p.dv + at, hh, exists);
+  }
+}
+
+template <int DT, int D, int kCols>
+__global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(const TrainAttnParams p) {
+  using T = Tile<D>;
+  constexpr int kWaves = 4, kRowsWg = kWaves * 32 * kCols, kStages = 2;
+  constexpr bool kHalf = DT == KSANA_SAGE_FP16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
+  const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
+  const int w = xcd_run_number();
+  if (w >= p.B * p.Hkv * blocks) return;
+  const int bh = w / blocks, block = blocks - 1 - (w - bh * blocks), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const Extent e = extent_of(p, b);
+  const int row0 = block * kRowsWg;
+  int keys = e.keys;
+  if (p.causal) keys = min(keys, row_position(p, min(row0 + kRowsWg, all_rows) - 1) + 1);
+  const int tiles = row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0;
+
+  const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
+  const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
+  const unsigned lds = lds_base();
+  v16f dq[kCols][T::kBlocks];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n)
+#pragma unroll
+    for (int c = 0; c < T::kBlocks; ++c) dq[n][c] = v16f{};
+  float scale = 1.0f;
+  int row[kCols], limit[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) {
+    row[n] = row0 + (wave * kCols + n) * 32 + m;
+    limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
+  }
+  if (tiles > 0) {
+    auto copy = [&](int t) {
+      const int at = min(t, tiles - 1) * kTrainTile;
+      const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
+      copy_key_tile<D, kWaves>(k_head, p.ks.sL, at, e.keys, stage, wave, lane);
+      copy_key_tile<D, kWaves>(v_head, p.vs.sL, at, e.keys, stage + T::kBytes, wave, lane);
+    };
+    copy(0);
+    v4i q[kCols][T::kSteps], g[kCols][T::kSteps];
+    float l[kCols], d[kCols];
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+      const int r = min(row[n], e.rows - 1);
+      load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, r), hh, p.flip, q[n]);
+      load_row<D>(p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH + row_offset(p, p.dos, r), hh, 0, g[n]);
+      l[n] = p.row_l[(int64_t)bh * p.row_pad + r] + kBackwardShift<DT>;
+      d[n] = p.row_d[(int64_t)bh * p.row_pad + r];
+    }
+    if constexpr (kHalf) scale = ds_scale(p, bh, lane);
+    const RowReader<D> rows(lane);
+    const ColumnReader<D> columns(lane);
+    const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
+    const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      tile_ready<0>();
+      copy(t + 1);
+      const unsigned k_tile = lds + (t % kStages) * 2 * T::kBytes, v_tile = k_tile + T::kBytes;
+      const bool edge = (t + 1) * kTrainTile > all_see;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v16f s[kCols], dp[kCols];
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          s[n] = v16f{};
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[n][i] = d[n];
+        }
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
+          const v4i a = rows.read(k_tile, h, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) s[n] = mfma16<DT>(a, q[n][st], s[n]);
+        }
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
+          const v4i a = rows.read(v_tile, h, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, g[n][st], dp[n]);
+        }
+        v4i ds[kCols][2];
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          float y[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[n]));
+          if (edge) {
+            const int left = limit[n] - t * kTrainTile - 32 * h - 4 * hh;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = acc_row(i) < left ? y[i] : 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] *= kHalf ? dp[n][i] * scale : dp[n][i];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            ds[n][j] = pack8<DT>(y[8 * j], y[8 * j + 1], y[8 * j + 2], y[8 * j + 3], y[8 * j + 4], y[8 * j + 5], y[8 * j + 6], y[8 * j + 7]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < T::kBlocks; ++c) {
+            const v4i a = columns.read(k_tile, c, 2 * h + j);
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) dq[n][c] = mfma16<DT>(a, ds[n][j], dq[n][c]);
+          }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  const float unshift = fast_exp2(-kBackwardShift<DT>);
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) {
+    const bool exists = row[n] < all_rows;
+    const int r = min(row[n], all_rows - 1), at = row_position(p, r), h = hk * p.group + r - at * p.group;
+    if (row[n] >= e.rows) {
+#pragma unroll
+      for (int c = 0; c < T::kBlocks; ++c) dq[n][c] = v16f{};
+    }
+    store_column<DT, D>(dq[n], p.sm_scale * unshift / scale, p.dq + (((int64_t)b * p.Lq + at) * p.Hq + h) * D, hh, exists);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ launches
+
+constexpr int kNormRows = 256;  // rows per block of sage_train_rows_kernel
+
+// 64 KiB of dynamic LDS and more has to be requested per kernel, once per device.
+struct LdsRequest {
+  std::atomic<bool> done[64];
+  hipError_t make(const void* kernel, int bytes) {
+    if (bytes < 65536) return hipSuccess;
+    int dev = 0;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
+    if (done[dev].load(std::memory_order_acquire)) return hipSuccess;
+    const hipError_t f = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (f == hipSuccess) done[dev].store(true, std::memory_order_release);
+    return f;
+  }
+};
+
+void fill_in(TrainAttnParams& p) {
+  p.group = p.Hq / p.Hkv;
+  p.group_inv = (unsigned)((UINT64_C(0x100000000) + p.group - 1) / p.group);
+  p.c = fabsf(p.sm_scale) * kLog2e;
+  p.flip = p.sm_scale < 0.0f ? 0x80008000u : 0u;
+  p.row_pad = (p.Lq * p.group + kTrainTile - 1) / kTrainTile * kTrainTile;
+  p.norm_q_blocks = (p.row_pad + kNormRows - 1) / kNormRows;
+  p.norm_blocks = p.norm_q_blocks + (p.dtype == KSANA_SAGE_FP16 ? (p.Lk + kNormRows - 1) / kNormRows : 0);
+}
+
+unsigned eighths(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
+
+template <int DT, int D>
+hipError_t fwd(const TrainAttnParams& p, hipStream_t s) {
+  constexpr int kCols = 1, kLds = 2 * 2 * Tile<D>::kBytes;
+  const int rows = p.Lq * p.group, blocks = (rows + 128 * kCols - 1) / (128 * kCols);
+  static LdsRequest request;
+  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D, kCols>), kLds);
+  if (e != hipSuccess) return e;
+  sage_train_fwd_kernel<DT, D, kCols><<<eighths((int64_t)p.B * p.Hkv * blocks), 256, kLds, s>>>(p);
+  return hipGetLastError();
+}
+
+template <int DT, int D>
+hipError_t bwd(const TrainAttnParams& p, hipStream_t s) {
+  sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, p.B * p.Hkv), 256, 0, s>>>(p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (p.dk != nullptr) {
+    constexpr int kCols = 2, kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
+    const int blocks = (p.Lk + 128 * kCols - 1) / (128 * kCols);
+    static LdsRequest request;
+    e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
+    if (e != hipSuccess) return e;
+    sage_train_dkv_kernel<DT, D, kCols><<<eighths((int64_t)p.B * p.Hkv * blocks), 256, kLds, s>>>(p);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (p.dq == nullptr) return hipSuccess;
+  constexpr int kCols = 2, kLds = 2 * 2 * Tile<D>::kBytes;
+  const int blocks = (p.Lq * p.group + 128 * kCols - 1) / (128 * kCols);
+  static LdsRequest request;
+  e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);
+  if (e != hipSuccess) return e;
+  sage_train_dq_kernel<DT, D, kCols><<<eighths((int64_t)p.B * p.Hkv * blocks), 256, kLds, s>>>(p);
+  return hipGetLastError();
+}
+
+uint64_t up256(uint64_t x) { return (x + 255) & ~UINT64_C(255); }
+
+}  // namespace
+
+TrainAttnScratch train_attn_scratch(const TrainAttnParams& call, bool backward) {
+  TrainAttnParams p = call;
+  fill_in(p);
+  TrainAttnScratch out{};
+  if (!backward) return out;
+  const uint64_t heads = (uint64_t)p.B * p.Hkv, rows = up256(heads * p.row_pad * 4);
+  out.row_l = 0;
+  out.row_d = rows;
+  out.norms = 2 * rows;
+  out.part = out.norms + up256(heads * p.norm_blocks * 4);
+  out.bytes = out.part;
+  return out;
+}
+
+hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s) {
+  fill_in(p);
+  (void)scratch;
+  const bool bf16 = p.dtype == KSANA_SAGE_BF16;
+  if (p.D == 128) return bf16 ? fwd<KSANA_SAGE_BF16, 128>(p, s) : fwd<KSANA_SAGE_FP16, 128>(p, s);
+  return bf16 ? fwd<KSANA_SAGE_BF16, 64>(p, s) : fwd<KSANA_SAGE_FP16, 64>(p, s);
+}
+
+hipError_t launch_train_attn_bwd(TrainAttnParams p, void* scratch, hipStream_t s) {
+  const TrainAttnScratch at = train_attn_scratch(p, true);
+  fill_in(p);
+  char* base = static_cast<char*>(scratch);
+  p.row_l = reinterpret_cast<float*>(base + at.row_l);
+  p.row_d = reinterpret_cast<float*>(base + at.row_d);
+  p.norms = reinterpret_cast<float*>(base + at.norms);
+  const bool bf16 = p.dtype == KSANA_SAGE_BF16;
+  if (p.D == 128) return bf16 ? bwd<KSANA_SAGE_BF16, 128>(p, s) : bwd<KSANA_SAGE_FP16, 128>(p, s);
+  return bf16 ? bwd<KSANA_SAGE_BF16, 64>(p, s) : bwd<KSANA_SAGE_FP16, 64>(p, s);
+}
+
+}  // namespace ksana_sage
