@@ -100,8 +100,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
 #pragma unroll
     for (int n = 0; n < kCols; ++n)
       load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, min(row[n], e.rows - 1)), hh, p.flip, q[n]);
-    const RowReader<D> k_reader(lane);
-    const ColumnReader<D> v_reader(lane);
+    const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     // keys that every row of the wave sees
     const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
     const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
@@ -117,7 +116,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = k_reader.read(k_tile, h, st);
+          const v4i a = read_row<D>(k_tile + row_at, h, st);
 #pragma unroll
           for (int n = 0; n < kCols; ++n) s[n][h] = mfma16<DT>(a, q[n][st], s[n][h]);
         }
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
       for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int d = 0; d < T::kBlocks; ++d) {
-          const v4i a = v_reader.read(v_tile, d, st);
+          const v4i a = read_column<D>(v_tile + column_at, d, st);
 #pragma unroll
           for (int n = 0; n < kCols; ++n) acc[n][d] = mfma16<DT>(a, pr[n][st], acc[n][d]);
         }
@@ -340,8 +339,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
       load_row<D>(p.v + b * p.vs.sB + at * p.vs.sL + hk * p.vs.sH, hh, 0, v[n]);
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
-    const RowReader<D> rows(lane);
-    const ColumnReader<D> columns(lane);
+    const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     const int64_t sees_all = (int64_t)(key0 + (wave + 1) * 32 * kCols - 1) * p.group;  // the first row that sees every key of the wave
 #pragma unroll 1
     for (int t = first_tile; t < tiles; ++t) {
@@ -351,65 +349,78 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
       const bool diagonal = p.causal && (int64_t)t * kTrainTile < sees_all;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        // S, P, dv += P^T dO, dP, dS, dk += dS^T q in turn: what one part leaves is used up by the next, or the
+        // accumulators and the keys and values would not fit the registers of two waves
         v16f s[kCols], dp[kCols];
-        v4f l[4], d[4];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          l[g] = *(LdsF4)(uintptr_t)(stats + (32 * h + 8 * g + 4 * hh) * 4);
-          d[g] = *(LdsF4)(uintptr_t)(stats + (kTrainTile + 32 * h + 8 * g + 4 * hh) * 4);
-        }
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-          s[n] = v16f{};
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dp[n][i] = d[i >> 2][i & 3];
-        }
+        for (int n = 0; n < kCols; ++n) s[n] = v16f{};
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = rows.read(q_tile, h, st);
+          const v4i a = read_row<D>(q_tile + row_at, h, st);
 #pragma unroll
           for (int n = 0; n < kCols; ++n) s[n] = mfma16<DT>(a, k[n][st], s[n]);
         }
+        float x[kCols][16];
+        {
+          v4f l[4];
 #pragma unroll
-        for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = rows.read(do_tile, h, st);
+          for (int g = 0; g < 4; ++g) l[g] = *(LdsF4)(uintptr_t)(stats + (32 * h + 8 * g + 4 * hh) * 4);
 #pragma unroll
-          for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, v[n][st], dp[n]);
+          for (int n = 0; n < kCols; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[n][i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[i >> 2][i & 3] + kBackwardShift<DT>));
         }
-        v4i pr[kCols][2], ds[kCols][2];
+        if (diagonal) {
 #pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-          float x[16], y[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[i >> 2][i & 3] + kBackwardShift<DT>));
-          if (diagonal) {
+          for (int n = 0; n < kCols; ++n) {
             const int64_t from = (int64_t)key[n] * p.group - t * kTrainTile - 32 * h - 4 * hh;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = acc_row(i) < from ? 0.0f : x[i];
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = x[i] * (kHalf ? dp[n][i] * scale : dp[n][i]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            pr[n][j] = pack8<DT>(x[8 * j], x[8 * j + 1], x[8 * j + 2], x[8 * j + 3], x[8 * j + 4], x[8 * j + 5], x[8 * j + 6], x[8 * j + 7]);
-            ds[n][j] = pack8<DT>(y[8 * j], y[8 * j + 1], y[8 * j + 2], y[8 * j + 3], y[8 * j + 4], y[8 * j + 5], y[8 * j + 6], y[8 * j + 7]);
+            for (int i = 0; i < 16; ++i) x[n][i] = acc_row(i) < from ? 0.0f : x[n][i];
           }
         }
+        v4i pr[kCols][2];
+#pragma unroll
+        for (int n = 0; n < kCols; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            pr[n][j] = pack8<DT>(x[n][8 * j], x[n][8 * j + 1], x[n][8 * j + 2], x[n][8 * j + 3], x[n][8 * j + 4], x[n][8 * j + 5], x[n][8 * j + 6], x[n][8 * j + 7]);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
-            const v4i a = columns.read(do_tile, c, 2 * h + j);
+            const v4i a = read_column<D>(do_tile + column_at, c, 2 * h + j);
 #pragma unroll
             for (int n = 0; n < kCols; ++n) dv[n][c] = mfma16<DT>(a, pr[n][j], dv[n][c]);
           }
 #pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const v4f d = *(LdsF4)(uintptr_t)(stats + (kTrainTile + 32 * h + 8 * g + 4 * hh) * 4);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[n][4 * g + i] = d[i];
+        }
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) {
+          const v4i a = read_row<D>(do_tile + row_at, h, st);
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, v[n][st], dp[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[n][i] *= kHalf ? dp[n][i] * scale : dp[n][i];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            pr[n][j] = pack8<DT>(x[n][8 * j], x[n][8 * j + 1], x[n][8 * j + 2], x[n][8 * j + 3], x[n][8 * j + 4], x[n][8 * j + 5], x[n][8 * j + 6], x[n][8 * j + 7]);
+        }
+#pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
-            const v4i a = columns.read(q_tile, c, 2 * h + j);
+            const v4i a = read_column<D>(q_tile + column_at, c, 2 * h + j);
 #pragma unroll
-            for (int n = 0; n < kCols; ++n) dk[n][c] = mfma16<DT>(a, ds[n][j], dk[n][c]);
+            for (int n = 0; n < kCols; ++n) dk[n][c] = mfma16<DT>(a, pr[n][j], dk[n][c]);
           }
       }
     }
@@ -479,8 +490,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
       d[n] = p.row_d[(int64_t)bh * p.row_pad + r];
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
-    const RowReader<D> rows(lane);
-    const ColumnReader<D> columns(lane);
+    const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
     const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
 #pragma unroll 1
@@ -500,13 +510,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
         }
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = rows.read(k_tile, h, st);
+          const v4i a = read_row<D>(k_tile + row_at, h, st);
 #pragma unroll
           for (int n = 0; n < kCols; ++n) s[n] = mfma16<DT>(a, q[n][st], s[n]);
         }
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = rows.read(v_tile, h, st);
+          const v4i a = read_row<D>(v_tile + row_at, h, st);
 #pragma unroll
           for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, g[n][st], dp[n]);
         }
@@ -531,7 +541,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
-            const v4i a = columns.read(k_tile, c, 2 * h + j);
+            const v4i a = read_column<D>(k_tile + column_at, c, 2 * h + j);
 #pragma unroll
             for (int n = 0; n < kCols; ++n) dq[n][c] = mfma16<DT>(a, ds[n][j], dq[n][c]);
           }
@@ -601,7 +611,7 @@ hipError_t bwd(const TrainAttnParams& p, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (p.dk != nullptr) {
-    constexpr int kCols = 2, kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
+    constexpr int kCols = 1, kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
     const int blocks = (p.Lk + 128 * kCols - 1) / (128 * kCols);
     static LdsRequest request;
     e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
@@ -611,7 +621,7 @@ hipError_t bwd(const TrainAttnParams& p, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   if (p.dq == nullptr) return hipSuccess;
-  constexpr int kCols = 2, kLds = 2 * 2 * Tile<D>::kBytes;
+  constexpr int kCols = 1, kLds = 2 * 2 * Tile<D>::kBytes;
   const int blocks = (p.Lq * p.group + 128 * kCols - 1) / (128 * kCols);
   static LdsRequest request;
   e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);

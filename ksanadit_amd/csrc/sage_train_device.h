@@ -36,21 +36,28 @@ __device__ __forceinline__ v4i pack8(float a, float b, float c, float d, float e
   return v4i{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
 }
 
-// A tile: 64 rows of D 16-bit channels, 16-byte pieces, a row's pieces exchanged by an exclusive or with a number of the row, so that
-// neither lanes that read one piece of 32 rows nor lanes that read two pieces of four rows (the transposing read) meet in a
-// bank.  The copies into LDS are linear there: a lane fetches the piece that belongs where it writes.
+// A tile: 64 rows of D 16-bit channels.  A copy instruction of a wave fills 1 KiB in a row with 64 pieces of 16 bytes: whole rows, that
+// are not neighbours.  Which rows share a copy and how far apart the copies lie is chosen so that row r starts 64 (r % 4) + 16 (r / 4 % 4)
+// bytes into the 256 that the banks hold side by side: sixteen lanes that read one piece of sixteen rows, and 32 lanes that read 64 bytes
+// of four rows (the transposing read), then meet in no bank, and every read of a lane is one address and a constant.  (Rows 32 bytes
+// apart in the banks cost both reads twice the cycles, 16 bytes the transposing one four times.)
 template <int D>
 struct Tile {
   static constexpr int kPieces = D / 8;                       // of a row
   static constexpr int kRowBytes = 2 * D;
-  static constexpr int kBytes = kTrainTile * kRowBytes;
-  static constexpr int kRowsPerCopy = 64 / kPieces;           // one copy instruction of a wave: 1 KiB
-  static constexpr int kCopies = kBytes / 1024;               // of a tile
+  static constexpr int kCopies = kTrainTile * kPieces / 64;   // of a tile
   static constexpr int kSteps = D / 16;                       // of a product over the channels
   static constexpr int kBlocks = D / 32;                      // channel blocks of a result
-  static __device__ __forceinline__ int twist(int row) {
-    return D == 128 ? ((row & 7) << 1 | (row >> 3 & 1)) : ((row >> 1 & 3) << 1 | (row >> 3 & 1));
+  // where copy c starts, the row that lane `lane` of it holds, and where a row is; `at` is a sum over the bits of the row
+  static constexpr __device__ __forceinline__ int copy_at(int c) { return D == 128 ? c * 1088 + c / 4 * 16 : c * 1088 + c / 2 * 144; }
+  static constexpr __device__ __forceinline__ int row_of(int c, int lane) {
+    const int slot = lane / kPieces;
+    return D == 128 ? c + 16 * slot : (c & 1) + 2 * (slot & 1) + 4 * (c >> 1) + 16 * (slot >> 1);
   }
+  static constexpr __device__ __forceinline__ int at(int r) {
+    return D == 128 ? copy_at(r & 15) + (r >> 4) * kRowBytes : copy_at((r & 1) + 2 * (r >> 2 & 3)) + ((r >> 1 & 1) + 2 * (r >> 4)) * kRowBytes;
+  }
+  static constexpr int kBytes = (copy_at(kCopies - 1) + 1024 + 63) / 64 * 64;
 };
 
 // lds_copy16 (sage_attn_device.h) with the destination as the LDS address it is
@@ -73,43 +80,28 @@ typedef const __attribute__((address_space(3))) v4i* LdsV4;
 typedef const __attribute__((address_space(3))) v4f* LdsF4;
 typedef __attribute__((address_space(3))) v4s* LdsS4;
 
-// The eight values of rows 32 block + m: byte offsets in a tile of the lane's piece of step s = at[s] + block * 32 rows
+// The eight values of row 32 block + m, channels 16 step + 8 hh ..: `lane_at` of the lane, and constants
 template <int D>
-struct RowReader {
-  unsigned at[Tile<D>::kSteps];
-  __device__ __forceinline__ explicit RowReader(int lane) {
-    const int row = lane & 31, hh = lane >> 5;
-#pragma unroll
-    for (int s = 0; s < Tile<D>::kSteps; ++s) at[s] = row * Tile<D>::kRowBytes + (((2 * s + hh) ^ Tile<D>::twist(row)) << 4);
-  }
-  __device__ __forceinline__ v4i read(unsigned tile, int block, int s) const {
-    return *(LdsV4)(uintptr_t)(tile + at[s] + block * 32 * Tile<D>::kRowBytes);
-  }
-};
+__device__ __forceinline__ unsigned row_lane_at(int lane) {
+  return Tile<D>::at(lane & 31) + (lane >> 5) * 16;
+}
+template <int D>
+__device__ __forceinline__ v4i read_row(unsigned tile_and_lane, int block, int step) {
+  return *(LdsV4)(uintptr_t)(tile_and_lane + Tile<D>::at(32 * block) + 32 * step);
+}
 
 // A's operand where the sum goes over the tile's rows: channels 32 block + m, rows 16 t + 8 (j / 4) + 4 hh + j % 4
 template <int D>
-struct ColumnReader {
-  unsigned at[2][Tile<D>::kBlocks];
-  __device__ __forceinline__ explicit ColumnReader(int lane) {
-    const int hh = lane >> 5, half = lane >> 4 & 1, i = lane & 15;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = 8 * j + 4 * hh + (i >> 2);
-#pragma unroll
-      for (int b = 0; b < Tile<D>::kBlocks; ++b) {
-        const int piece = 4 * b + 2 * half + (i >> 1 & 1);
-        at[j][b] = row * Tile<D>::kRowBytes + ((piece ^ Tile<D>::twist(row)) << 4) + (i & 1) * 8;
-      }
-    }
-  }
-  __device__ __forceinline__ v4i read(unsigned tile, int block, int t) const {
-    const unsigned step = tile + t * 16 * Tile<D>::kRowBytes;
-    const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(uintptr_t)(step + at[0][block])));
-    const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(uintptr_t)(step + at[1][block])));
-    return v4i{lo[0], lo[1], hi[0], hi[1]};
-  }
-};
+__device__ __forceinline__ unsigned column_lane_at(int lane) {
+  const int i = lane & 15;
+  return Tile<D>::at(4 * (lane >> 5) + (i >> 2)) + (lane >> 4 & 1) * 32 + (i & 3) * 8;
+}
+template <int D>
+__device__ __forceinline__ v4i read_column(unsigned tile_and_lane, int block, int t) {
+  const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(uintptr_t)(tile_and_lane + Tile<D>::at(16 * t) + 64 * block)));
+  const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4)(uintptr_t)(tile_and_lane + Tile<D>::at(16 * t + 8) + 64 * block)));
+  return v4i{lo[0], lo[1], hi[0], hi[1]};
+}
 
 // Query rows of the heads that share a key head, numbered together: row r is position r / group of head r % group.
 __device__ __forceinline__ int row_position(const TrainAttnParams& p, int r) {
@@ -130,9 +122,8 @@ __device__ __forceinline__ void copy_key_tile(const uint16_t* head, int64_t sL, 
   const int left = rows - row - 1;
 #pragma unroll
   for (int c = 0; c < T::kCopies / kWaves; ++c) {
-    const int r = (c * kWaves + wave) * T::kRowsPerCopy + lane / T::kPieces;
-    const int piece = (lane % T::kPieces) ^ T::twist(r);
-    lds_copy16_at(base, (unsigned)min(r, left) * row_bytes + piece * 16, tile + (c * kWaves + wave) * 1024);
+    const int i = c * kWaves + wave;
+    lds_copy16_at(base, (unsigned)min(T::row_of(i, lane), left) * row_bytes + lane % T::kPieces * 16, tile + T::copy_at(i));
   }
 }
 // .. and of query rows, numbered as above
@@ -145,10 +136,8 @@ __device__ __forceinline__ void copy_query_tile(const TrainAttnParams& p, const 
   const unsigned l_bytes = (unsigned)(t.sL * 2), h_bytes = (unsigned)(t.sH * 2);
 #pragma unroll
   for (int c = 0; c < T::kCopies / kWaves; ++c) {
-    const int i = (c * kWaves + wave) * T::kRowsPerCopy + lane / T::kPieces;
-    const int piece = (lane % T::kPieces) ^ T::twist(i);
-    const int r = min(row + i, rows - 1), l = row_position(p, r);
-    lds_copy16_at(base, (unsigned)(l - first) * l_bytes + (unsigned)(r - l * p.group) * h_bytes + piece * 16, tile + (c * kWaves + wave) * 1024);
+    const int i = c * kWaves + wave, r = min(row + T::row_of(i, lane), rows - 1), l = row_position(p, r);
+    lds_copy16_at(base, (unsigned)(l - first) * l_bytes + (unsigned)(r - l * p.group) * h_bytes + lane % T::kPieces * 16, tile + T::copy_at(i));
   }
 }
 
