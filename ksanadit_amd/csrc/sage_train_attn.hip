@@ -89,11 +89,12 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
     limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
   }
   if (tiles > 0) {
+    const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
     auto copy = [&](int t) {
       const int at = min(t, tiles - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
-      copy_key_tile<D, kWaves>(k_head, p.ks.sL, at, e.keys, stage, wave, lane);
-      copy_key_tile<D, kWaves>(v_head, p.vs.sL, at, e.keys, stage + T::kBytes, wave, lane);
+      k_copy.start(at, e.keys, stage, wave, lane);
+      v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
     };
     copy(0);
     v4i q[kCols][T::kSteps];
@@ -123,7 +124,8 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
       if ((t + 1) * kTrainTile > all_see) {
 #pragma unroll
         for (int n = 0; n < kCols; ++n) {
-          const int left = limit[n] - t * kTrainTile - 4 * hh;
+          int left = limit[n] - t * kTrainTile - 4 * hh;
+          pin(left);  // (a branch that stays one: 64 instructions for every tile otherwise)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -134,9 +136,9 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
       bool move = false;
 #pragma unroll
       for (int n = 0; n < kCols; ++n) {
-        float x = fmaxf(s[n][0][0], s[n][1][0]);
+        float x = s[n][0][0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) x = fmaxf(x, fmaxf(s[n][0][i], s[n][1][i]));
+        for (int i = 0; i < 16; ++i) x = largest(x, s[n][0][i], s[n][1][i]);
         most[n] = over_halves<Max>(x);
         move = move || most[n] * p.c > kLazy + kForwardShift<DT> - minus[n] || (top[n] == -INFINITY && most[n] > -INFINITY);
       }
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
-// Per query row -log2(e) lse and -sum(dO o); in fp16 besides the largest squared norms of rows of dO and of v per block of rows.
+// Per query row -log2(e) lse (plus the shift) and -sum(dO o); in fp16 besides the largest squared norms of rows of dO and of v per block of rows.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void sage_train_rows_kernel(const TrainAttnParams p) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes;  // lanes of a row, rows at a time
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(256) void sage_train_rows_kernel(const TrainAttnPar
         if (r < e.rows) {
           const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
           const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + l];
-          minus = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+          minus = lse == -INFINITY ? -INFINITY : kBackwardShift<DT> - lse * kLog2e;
         }
         p.row_l[(int64_t)bh * p.row_pad + r] = minus;
         p.row_d[(int64_t)bh * p.row_pad + r] = -d;
@@ -320,13 +322,14 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
   if (first_tile < tiles) {
     const uint16_t* q_heads = p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH;
     const uint16_t* do_heads = p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH;
+    const TileCopy<D, kWaves> q_copy(q_heads, p.qs.sL, wave, lane), do_copy(do_heads, p.dos.sL, wave, lane);
     const float* row_l = p.row_l + (int64_t)bh * p.row_pad;
     const float* row_d = p.row_d + (int64_t)bh * p.row_pad;
     auto copy = [&](int t) {
       const int at = min(t, tiles - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * kStage;
-      copy_query_tile<D, kWaves>(p, q_heads, p.qs, at, e.rows, stage, wave, lane);
-      copy_query_tile<D, kWaves>(p, do_heads, p.dos, at, e.rows, stage + T::kBytes, wave, lane);
+      q_copy.start_grouped(p, p.qs, at, e.rows, stage, wave, lane);
+      do_copy.start_grouped(p, p.dos, at, e.rows, stage + T::kBytes, wave, lane);
       // (two waves each, so that every wave has as many copies in flight)
       lds_copy4_at((wave & 1 ? row_d : row_l) + at, lane * 4, stage + 2 * T::kBytes + (wave & 1) * kTrainTile * 4);
     };
@@ -368,12 +371,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
 #pragma unroll
           for (int n = 0; n < kCols; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[n][i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[i >> 2][i & 3] + kBackwardShift<DT>));
+            for (int i = 0; i < 16; ++i) x[n][i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[i >> 2][i & 3]));
         }
         if (diagonal) {
 #pragma unroll
           for (int n = 0; n < kCols; ++n) {
-            const int64_t from = (int64_t)key[n] * p.group - t * kTrainTile - 32 * h - 4 * hh;
+            int from = (int)min((int64_t)key[n] * p.group - t * kTrainTile - 32 * h - 4 * hh, (int64_t)kTrainTile);
+            pin(from);
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[n][i] = acc_row(i) < from ? 0.0f : x[n][i];
           }
@@ -472,11 +476,12 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
     limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
   }
   if (tiles > 0) {
+    const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
     auto copy = [&](int t) {
       const int at = min(t, tiles - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
-      copy_key_tile<D, kWaves>(k_head, p.ks.sL, at, e.keys, stage, wave, lane);
-      copy_key_tile<D, kWaves>(v_head, p.vs.sL, at, e.keys, stage + T::kBytes, wave, lane);
+      k_copy.start(at, e.keys, stage, wave, lane);
+      v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
     };
     copy(0);
     v4i q[kCols][T::kSteps], g[kCols][T::kSteps];
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
       const int r = min(row[n], e.rows - 1);
       load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, r), hh, p.flip, q[n]);
       load_row<D>(p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH + row_offset(p, p.dos, r), hh, 0, g[n]);
-      l[n] = p.row_l[(int64_t)bh * p.row_pad + r] + kBackwardShift<DT>;
+      l[n] = p.row_l[(int64_t)bh * p.row_pad + r];
       d[n] = p.row_d[(int64_t)bh * p.row_pad + r];
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
@@ -527,7 +532,8 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[n]));
           if (edge) {
-            const int left = limit[n] - t * kTrainTile - 32 * h - 4 * hh;
+            int left = limit[n] - t * kTrainTile - 32 * h - 4 * hh;
+            pin(left);
 #pragma unroll
             for (int i = 0; i < 16; ++i) y[i] = acc_row(i) < left ? y[i] : 0.0f;
           }

@@ -64,10 +64,10 @@ struct Tile {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_copy16_at(const void* base, unsigned lane_off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(lane_off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_copy4_at(const void* base, unsigned lane_off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(lane_off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 // All copies of this wave but the youngest kLater are in LDS, its LDS reads are done, and so are the other waves'.
@@ -112,34 +112,49 @@ __device__ __forceinline__ int64_t row_offset(const TrainAttnParams& p, const Tr
   return (int64_t)l * t.sL + (int64_t)(r - l * p.group) * t.sH;
 }
 
-// Starts a wave's share of the copy of 64 rows of keys or values from `row` on, of which `rows` exist.  Rows that do not are
-// copies of the last one: they are finite where the tensor is, and what the products make of them is not looked at.
+// A wave's copies of tiles of a tensor's rows.  Of a whole tile they are one lane offset and addresses that the wave shares; of one with
+// fewer rows, those that do not exist are copies of the last one: they are finite where the tensor is, and what the products make of
+// them is not looked at.
 template <int D, int kWaves>
-__device__ __forceinline__ void copy_key_tile(const uint16_t* head, int64_t sL, int row, int rows, unsigned tile, int wave, int lane) {
+struct TileCopy {
   using T = Tile<D>;
-  const char* base = reinterpret_cast<const char*>(head + (int64_t)row * sL);
-  const unsigned row_bytes = (unsigned)(sL * 2);
-  const int left = rows - row - 1;
+  const char* base;      // of the head
+  int64_t row_bytes;
+  unsigned whole;        // the lane's offset in a whole tile
+  __device__ __forceinline__ TileCopy(const uint16_t* head, int64_t sL, int wave, int lane)
+      : base(reinterpret_cast<const char*>(head)), row_bytes(sL * 2),
+        whole((unsigned)T::row_of(wave, lane) * (unsigned)(sL * 2) + lane % T::kPieces * 16) {}
+  // keys or values (or query rows, where each key head has one query head) from `row` on, of which `rows` exist
+  __device__ __forceinline__ void start(int row, int rows, unsigned tile, int wave, int lane) const {
+    const char* at = base + row * row_bytes;
+    if (rows - row >= kTrainTile) {
 #pragma unroll
-  for (int c = 0; c < T::kCopies / kWaves; ++c) {
-    const int i = c * kWaves + wave;
-    lds_copy16_at(base, (unsigned)min(T::row_of(i, lane), left) * row_bytes + lane % T::kPieces * 16, tile + T::copy_at(i));
-  }
-}
-// .. and of query rows, numbered as above
-template <int D, int kWaves>
-__device__ __forceinline__ void copy_query_tile(const TrainAttnParams& p, const uint16_t* heads, const TrainTensor& t, int row, int rows, unsigned tile,
-                                                int wave, int lane) {
-  using T = Tile<D>;
-  const int first = row_position(p, row);
-  const char* base = reinterpret_cast<const char*>(heads + (int64_t)first * t.sL);
-  const unsigned l_bytes = (unsigned)(t.sL * 2), h_bytes = (unsigned)(t.sH * 2);
+      for (int c = 0; c < T::kCopies / kWaves; ++c)
+        lds_copy16_at(at + (T::row_of(c * kWaves, 0)) * row_bytes, whole, tile + T::copy_at(c * kWaves + wave));
+    } else {
 #pragma unroll
-  for (int c = 0; c < T::kCopies / kWaves; ++c) {
-    const int i = c * kWaves + wave, r = min(row + T::row_of(i, lane), rows - 1), l = row_position(p, r);
-    lds_copy16_at(base, (unsigned)(l - first) * l_bytes + (unsigned)(r - l * p.group) * h_bytes + lane % T::kPieces * 16, tile + T::copy_at(i));
+      for (int c = 0; c < T::kCopies / kWaves; ++c)
+        lds_copy16_at(at, (unsigned)min(T::row_of(c * kWaves + wave, lane), rows - row - 1) * (unsigned)row_bytes + lane % T::kPieces * 16,
+                      tile + T::copy_at(c * kWaves + wave));
+    }
   }
-}
+  // query rows numbered over the heads of a key head
+  __device__ __forceinline__ void start_grouped(const TrainAttnParams& p, const TrainTensor& t, int row, int rows, unsigned tile, int wave, int lane) const {
+    if (p.group == 1) return start(row, rows, tile, wave, lane);
+    const int first = row_position(p, row);
+    const char* at = base + first * row_bytes;
+#pragma unroll
+    for (int c = 0; c < T::kCopies / kWaves; ++c) {
+      const int i = c * kWaves + wave, r = min(row + T::row_of(i, lane), rows - 1), l = row_position(p, r);
+      lds_copy16_at(at, (unsigned)(l - first) * (unsigned)row_bytes + (unsigned)(r - l * p.group) * (unsigned)(t.sH * 2) + lane % T::kPieces * 16,
+                    tile + T::copy_at(i));
+    }
+  }
+};
+
+// The largest of three, not a number if one is not (one instruction each; fmaxf on results of matrix instructions costs one more
+// to make signalling values quiet)
+__device__ __forceinline__ float largest(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
 // Number `blockIdx.x` of a launch of a multiple of eight workgroups.  Consecutive ones land on consecutive XCDs: every XCD takes a run
 // of the work, so that workgroups of one head share an L2.
