@@ -60,14 +60,14 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
   constexpr int kWaves = 4, kRowsWg = kWaves * 32 * kCols, kStages = 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
   const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
-  const int w = xcd_run_number();
-  if (w >= p.B * p.Hkv * blocks) return;
-  const int bh = w / blocks, block = blocks - 1 - (w - bh * blocks), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const TrainPlace place = train_place(p, blocks);
+  if (place.bh < 0) return;
+  const int bh = place.bh, block = blocks - 1 - place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   const int row0 = block * kRowsWg;
   int keys = e.keys;
   if (p.causal) keys = min(keys, row_position(p, min(row0 + kRowsWg, all_rows) - 1) + 1);
-  const int tiles = row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0;
+  const TileRange range = run_tiles(0, row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0, place.run, p.runs);
 
   const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
   const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
@@ -88,15 +88,15 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
     row[n] = row0 + (wave * kCols + n) * 32 + m;
     limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
   }
-  if (tiles > 0) {
+  if (range.from < range.to) {
     const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
     auto copy = [&](int t) {
-      const int at = min(t, tiles - 1) * kTrainTile;
+      const int at = min(t, range.to - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
       k_copy.start(at, e.keys, stage, wave, lane);
       v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
     };
-    copy(0);
+    copy(range.from);
     v4i q[kCols][T::kSteps];
 #pragma unroll
     for (int n = 0; n < kCols; ++n)
@@ -104,11 +104,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     // keys that every row of the wave sees
     const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
+    const bool idle = row0 + wave * 32 * kCols >= e.rows;  // a wave without rows copies its share
     const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
 #pragma unroll 1
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = range.from; t < range.to; ++t) {
       tile_ready<0>();
       copy(t + 1);
+      if (idle) continue;
       const unsigned k_tile = lds + (t % kStages) * 2 * T::kBytes, v_tile = k_tile + T::kBytes;
       v16f s[kCols][2];
 #pragma unroll
@@ -187,6 +189,14 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
     const float total = over_halves<Sum>(sum[n]);
     const float factor = !takes_part || total == 0.0f ? 0.0f : 1.0f / total;
     const int r = min(row[n], all_rows - 1), l = row_position(p, r), h = hk * p.group + r - l * p.group;
+    if (p.runs > 1) {
+      const int64_t at = ((int64_t)place.run * p.B * p.Hkv + bh) * all_rows + r;
+      store_column_part<D>(acc[n], 1.0f, p.part + at * D, hh, takes_part && range.from < range.to);
+      // (a run without tiles: nothing to add)
+      if (takes_part && hh == 0)
+        *reinterpret_cast<float2*>(p.part + (int64_t)p.runs * p.B * p.Hkv * all_rows * D + 2 * at) = make_float2(minus[n], total);
+      continue;
+    }
     if (!takes_part) {
 #pragma unroll
       for (int d = 0; d < T::kBlocks; ++d) acc[n][d] = v16f{};
@@ -301,13 +311,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
   constexpr bool kHalf = DT == KSANA_SAGE_FP16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
   const int blocks = (p.Lk + kKeysWg - 1) / kKeysWg;
-  const int w = xcd_run_number();
-  if (w >= p.B * p.Hkv * blocks) return;
-  const int bh = w / blocks, block = w - bh * blocks, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const TrainPlace place = train_place(p, blocks);
+  if (place.bh < 0) return;
+  const int bh = place.bh, block = place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   const int key0 = block * kKeysWg;
   const int tiles = key0 < e.keys ? (e.rows + kTrainTile - 1) / kTrainTile : 0;
-  const int first_tile = p.causal ? (int)min((int64_t)key0 * p.group / kTrainTile, (int64_t)tiles) : 0;
+  const TileRange range = run_tiles(p.causal ? (int)min((int64_t)key0 * p.group / kTrainTile, (int64_t)tiles) : 0, tiles, place.run, p.runs);
 
   const unsigned lds = lds_base();
   v16f dk[kCols][T::kBlocks], dv[kCols][T::kBlocks];
@@ -319,21 +329,21 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
   int key[kCols];
 #pragma unroll
   for (int n = 0; n < kCols; ++n) key[n] = key0 + (wave * kCols + n) * 32 + m;
-  if (first_tile < tiles) {
+  if (range.from < range.to) {
     const uint16_t* q_heads = p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH;
     const uint16_t* do_heads = p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH;
     const TileCopy<D, kWaves> q_copy(q_heads, p.qs.sL, wave, lane), do_copy(do_heads, p.dos.sL, wave, lane);
     const float* row_l = p.row_l + (int64_t)bh * p.row_pad;
     const float* row_d = p.row_d + (int64_t)bh * p.row_pad;
     auto copy = [&](int t) {
-      const int at = min(t, tiles - 1) * kTrainTile;
+      const int at = min(t, range.to - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * kStage;
       q_copy.start_grouped(p, p.qs, at, e.rows, stage, wave, lane);
       do_copy.start_grouped(p, p.dos, at, e.rows, stage + T::kBytes, wave, lane);
       // (two waves each, so that every wave has as many copies in flight)
       lds_copy4_at((wave & 1 ? row_d : row_l) + at, lane * 4, stage + 2 * T::kBytes + (wave & 1) * kTrainTile * 4);
     };
-    copy(first_tile);
+    copy(range.from);
     v4i k[kCols][T::kSteps], v[kCols][T::kSteps];
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
@@ -343,11 +353,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
+    const bool idle = key0 + wave * 32 * kCols >= e.keys;  // a wave without keys copies its share
     const int64_t sees_all = (int64_t)(key0 + (wave + 1) * 32 * kCols - 1) * p.group;  // the first row that sees every key of the wave
 #pragma unroll 1
-    for (int t = first_tile; t < tiles; ++t) {
+    for (int t = range.from; t < range.to; ++t) {
       tile_ready<0>();
       copy(t + 1);
+      if (idle) continue;
       const unsigned q_tile = lds + (t % kStages) * kStage, do_tile = q_tile + T::kBytes, stats = do_tile + T::kBytes;
       const bool diagonal = p.causal && (int64_t)t * kTrainTile < sees_all;
 #pragma unroll
@@ -438,6 +450,12 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
 #pragma unroll
       for (int c = 0; c < T::kBlocks; ++c) dk[n][c] = dv[n][c] = v16f{};
     }
+    if (p.runs > 1) {
+      float* at = p.part + (((int64_t)place.run * p.B * p.Hkv + bh) * p.Lk + min(key[n], p.Lk - 1)) * 2 * D;
+      store_column_part<D>(dk[n], p.sm_scale * unshift / scale, at, hh, exists);
+      store_column_part<D>(dv[n], unshift, at + D, hh, exists);
+      continue;
+    }
     const int64_t at = (((int64_t)b * p.Lk + min(key[n], p.Lk - 1)) * p.Hkv + hk) * D;
     store_column<DT, D>(dk[n], p.sm_scale * unshift / scale, p.dk + at, hh, exists);
     store_column<DT, D>(dv[n], unshift, p.dv + at, hh, exists);
@@ -451,14 +469,14 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
   constexpr bool kHalf = DT == KSANA_SAGE_FP16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
   const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
-  const int w = xcd_run_number();
-  if (w >= p.B * p.Hkv * blocks) return;
-  const int bh = w / blocks, block = blocks - 1 - (w - bh * blocks), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const TrainPlace place = train_place(p, blocks);
+  if (place.bh < 0) return;
+  const int bh = place.bh, block = blocks - 1 - place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   const int row0 = block * kRowsWg;
   int keys = e.keys;
   if (p.causal) keys = min(keys, row_position(p, min(row0 + kRowsWg, all_rows) - 1) + 1);
-  const int tiles = row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0;
+  const TileRange range = run_tiles(0, row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0, place.run, p.runs);
 
   const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
   const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
@@ -475,15 +493,15 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
     row[n] = row0 + (wave * kCols + n) * 32 + m;
     limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
   }
-  if (tiles > 0) {
+  if (range.from < range.to) {
     const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
     auto copy = [&](int t) {
-      const int at = min(t, tiles - 1) * kTrainTile;
+      const int at = min(t, range.to - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
       k_copy.start(at, e.keys, stage, wave, lane);
       v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
     };
-    copy(0);
+    copy(range.from);
     v4i q[kCols][T::kSteps], g[kCols][T::kSteps];
     float l[kCols], d[kCols];
 #pragma unroll
@@ -497,11 +515,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
+    const bool idle = row0 + wave * 32 * kCols >= e.rows;  // a wave without rows copies its share
     const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
 #pragma unroll 1
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = range.from; t < range.to; ++t) {
       tile_ready<0>();
       copy(t + 1);
+      if (idle) continue;
       const unsigned k_tile = lds + (t % kStages) * 2 * T::kBytes, v_tile = k_tile + T::kBytes;
       const bool edge = (t + 1) * kTrainTile > all_see;
 #pragma unroll
@@ -564,8 +584,80 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
 #pragma unroll
       for (int c = 0; c < T::kBlocks; ++c) dq[n][c] = v16f{};
     }
+    if (p.runs > 1) {
+      store_column_part<D>(dq[n], p.sm_scale * unshift / scale, p.part + (((int64_t)place.run * p.B * p.Hkv + bh) * all_rows + r) * D, hh, exists);
+      continue;
+    }
     store_column<DT, D>(dq[n], p.sm_scale * unshift / scale, p.dq + (((int64_t)b * p.Lq + at) * p.Hq + h) * D, hh, exists);
   }
+}
+
+// ------------------------------------------------------------------------------------------------------------ runs joined
+
+// Eight channels per lane.  A run's sums stand against a reference point of its own.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void sage_train_join_fwd_kernel(const TrainAttnParams p) {
+  constexpr int kLanes = D / 8;
+  const int all_rows = p.Lq * p.group, lane = threadIdx.x % kLanes;
+  const int64_t rows = (int64_t)p.B * p.Hkv * all_rows, at = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (at >= rows) return;
+  const int bh = (int)(at / all_rows), r = (int)(at - (int64_t)bh * all_rows), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
+  float sum[8] = {}, total = 0.0f, top = -INFINITY;
+  const float2* ml = reinterpret_cast<const float2*>(p.part + p.runs * rows * D);
+  if (r < extent_of(p, b).rows) {
+    for (int i = 0; i < p.runs; ++i) {
+      const float2 x = ml[i * rows + at];
+      if (x.y != 0.0f) top = fmaxf(top, -x.x);
+    }
+#pragma unroll 4
+    for (int i = 0; i < p.runs; ++i) {
+      const float2 x = ml[i * rows + at];
+      if (x.y == 0.0f) continue;  // (its sums are not written)
+      const float factor = fast_exp2(-x.x - top);
+      const float4* o = reinterpret_cast<const float4*>(p.part + (i * rows + at) * D + 8 * lane);
+      const float4 lo = o[0], hi = o[1];
+      total = __fmaf_rn(x.y, factor, total);
+      sum[0] = __fmaf_rn(lo.x, factor, sum[0]);
+      sum[1] = __fmaf_rn(lo.y, factor, sum[1]);
+      sum[2] = __fmaf_rn(lo.z, factor, sum[2]);
+      sum[3] = __fmaf_rn(lo.w, factor, sum[3]);
+      sum[4] = __fmaf_rn(hi.x, factor, sum[4]);
+      sum[5] = __fmaf_rn(hi.y, factor, sum[5]);
+      sum[6] = __fmaf_rn(hi.z, factor, sum[6]);
+      sum[7] = __fmaf_rn(hi.w, factor, sum[7]);
+    }
+  }
+  const float factor = total == 0.0f ? 0.0f : 1.0f / total;
+  *reinterpret_cast<v4i*>(p.o + b * p.os.sB + l * p.os.sL + h * p.os.sH + 8 * lane) =
+      pack8<DT>(sum[0] * factor, sum[1] * factor, sum[2] * factor, sum[3] * factor, sum[4] * factor, sum[5] * factor, sum[6] * factor, sum[7] * factor);
+  if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Lq + l] = total == 0.0f ? -INFINITY : (log2f(total) + top) * kLn2;
+}
+
+// Sums of the runs' gradients: of query rows (kKeys false) or of keys, whose two gradients lie side by side
+template <int DT, int D, bool kKeys>
+__global__ __launch_bounds__(256) void sage_train_join_bwd_kernel(const TrainAttnParams p) {
+  constexpr int kWidth = kKeys ? 2 * D : D, kLanes = kWidth / 8;
+  const int lane = threadIdx.x % kLanes, per_head = kKeys ? p.Lk : p.Lq * p.group;
+  const int64_t rows = (int64_t)p.B * p.Hkv * per_head, at = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (at >= rows) return;
+  float4 lo = make_float4(0, 0, 0, 0), hi = lo;
+#pragma unroll 4
+  for (int i = 0; i < p.runs; ++i) {
+    const float4* x = reinterpret_cast<const float4*>(p.part + (i * rows + at) * kWidth + 8 * lane);
+    const float4 a = x[0], c = x[1];
+    lo = make_float4(lo.x + a.x, lo.y + a.y, lo.z + a.z, lo.w + a.w);
+    hi = make_float4(hi.x + c.x, hi.y + c.y, hi.z + c.z, hi.w + c.w);
+  }
+  const int bh = (int)(at / per_head), r = (int)(at - (int64_t)bh * per_head), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  uint16_t* out;
+  if constexpr (kKeys) {
+    out = (8 * lane < D ? p.dk : p.dv) + (((int64_t)b * p.Lk + r) * p.Hkv + hk) * D + 8 * lane % D;
+  } else {
+    const int l = row_position(p, r);
+    out = p.dq + (((int64_t)b * p.Lq + l) * p.Hq + hk * p.group + r - l * p.group) * D + 8 * lane;
+  }
+  *reinterpret_cast<v4i*>(out) = pack8<DT>(lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w);
 }
 
 // ------------------------------------------------------------------------------------------------------------ launches
@@ -600,39 +692,92 @@ void fill_in(TrainAttnParams& p) {
 
 unsigned eighths(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
 
+// How many runs a launch cuts its blocks' loops of `tiles` tiles into, with `blocks` blocks in all and `bytes` of results to a run.
+// Two workgroups to each of 256 compute units; in units of a tile's time (about 2 us with both there), a workgroup costs kSetup besides
+// its tiles, a launch that joins runs kJoin and what its bytes take at 4 TB/s, written and read.
+int runs_of(int64_t blocks, int tiles, double bytes) {
+  constexpr double kSetup = 2.0, kJoin = 2.0, kBytesPerTile = 4e12 * 2e-6;
+  constexpr int kPlaces = 512;
+  int best = 1;
+  double least = 1e30;
+  for (int n = 1; n <= 128 && n <= tiles; ++n) {
+    const double rounds = (double)((blocks * n + kPlaces - 1) / kPlaces), each = (tiles + n - 1) / n;
+    const double cost = rounds * (each + kSetup) + (n > 1 ? kJoin + 2.0 * n * bytes / kBytesPerTile : 0.0);
+    if (cost < 0.97 * least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
+constexpr int kBlockRows = 128;  // rows, or keys, of a workgroup
+struct TrainRuns {
+  int fwd, dkv, dq;
+  uint64_t fwd_bytes, dkv_bytes, dq_bytes;  // of their partial results
+};
+TrainRuns train_runs(const TrainAttnParams& p) {
+  const int64_t heads = (int64_t)p.B * p.Hkv, rows = (int64_t)p.Lq * p.group;
+  const int64_t row_blocks = heads * ((rows + kBlockRows - 1) / kBlockRows), key_blocks = heads * ((p.Lk + kBlockRows - 1) / kBlockRows);
+  const int key_tiles = (p.Lk + kTrainTile - 1) / kTrainTile, row_tiles = (int)((rows + kTrainTile - 1) / kTrainTile);
+  const double row_bytes = 4.0 * heads * rows * p.D, key_bytes = 8.0 * heads * p.Lk * p.D;
+  TrainRuns r{};
+  r.fwd = runs_of(row_blocks, key_tiles, row_bytes);
+  r.dkv = runs_of(key_blocks, row_tiles, key_bytes);
+  r.dq = runs_of(row_blocks, key_tiles, row_bytes);
+  r.fwd_bytes = r.fwd > 1 ? (uint64_t)r.fwd * heads * rows * (p.D + 2) * 4 : 0;
+  r.dkv_bytes = r.dkv > 1 ? (uint64_t)r.dkv * heads * p.Lk * p.D * 8 : 0;
+  r.dq_bytes = r.dq > 1 ? (uint64_t)r.dq * heads * rows * p.D * 4 : 0;
+  return r;
+}
+
 template <int DT, int D>
-hipError_t fwd(const TrainAttnParams& p, hipStream_t s) {
+hipError_t fwd(TrainAttnParams p, hipStream_t s) {
   constexpr int kCols = 1, kLds = 2 * 2 * Tile<D>::kBytes;
-  const int rows = p.Lq * p.group, blocks = (rows + 128 * kCols - 1) / (128 * kCols);
+  static_assert(kBlockRows == 128 * kCols);
+  const int64_t rows = (int64_t)p.Lq * p.group, heads = (int64_t)p.B * p.Hkv, blocks = (rows + kBlockRows - 1) / kBlockRows;
   static LdsRequest request;
-  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D, kCols>), kLds);
+  hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D, kCols>), kLds);
   if (e != hipSuccess) return e;
-  sage_train_fwd_kernel<DT, D, kCols><<<eighths((int64_t)p.B * p.Hkv * blocks), 256, kLds, s>>>(p);
+  sage_train_fwd_kernel<DT, D, kCols><<<eighths(heads * blocks * p.runs), 256, kLds, s>>>(p);
+  e = hipGetLastError();
+  if (e != hipSuccess || p.runs == 1) return e;
+  constexpr int kJoined = 256 / (D / 8);
+  sage_train_join_fwd_kernel<DT, D><<<(unsigned)((heads * rows + kJoined - 1) / kJoined), 256, 0, s>>>(p);
   return hipGetLastError();
 }
 
 template <int DT, int D>
-hipError_t bwd(const TrainAttnParams& p, hipStream_t s) {
-  sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, p.B * p.Hkv), 256, 0, s>>>(p);
+hipError_t bwd(TrainAttnParams p, const TrainRuns& runs, hipStream_t s) {
+  const int64_t rows = (int64_t)p.Lq * p.group, heads = (int64_t)p.B * p.Hkv;
+  sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, (unsigned)heads), 256, 0, s>>>(p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
+  constexpr int kCols = 1;
   if (p.dk != nullptr) {
-    constexpr int kCols = 1, kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
-    const int blocks = (p.Lk + 128 * kCols - 1) / (128 * kCols);
+    constexpr int kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
     static LdsRequest request;
     e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
     if (e != hipSuccess) return e;
-    sage_train_dkv_kernel<DT, D, kCols><<<eighths((int64_t)p.B * p.Hkv * blocks), 256, kLds, s>>>(p);
+    p.runs = runs.dkv;
+    sage_train_dkv_kernel<DT, D, kCols><<<eighths(heads * ((p.Lk + kBlockRows - 1) / kBlockRows) * p.runs), 256, kLds, s>>>(p);
+    if (p.runs > 1) {
+      constexpr int kJoined = 256 / (D / 4);
+      sage_train_join_bwd_kernel<DT, D, true><<<(unsigned)((heads * p.Lk + kJoined - 1) / kJoined), 256, 0, s>>>(p);
+    }
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   if (p.dq == nullptr) return hipSuccess;
-  constexpr int kCols = 1, kLds = 2 * 2 * Tile<D>::kBytes;
-  const int blocks = (p.Lq * p.group + 128 * kCols - 1) / (128 * kCols);
+  constexpr int kLds = 2 * 2 * Tile<D>::kBytes;
   static LdsRequest request;
   e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);
   if (e != hipSuccess) return e;
-  sage_train_dq_kernel<DT, D, kCols><<<eighths((int64_t)p.B * p.Hkv * blocks), 256, kLds, s>>>(p);
+  p.runs = runs.dq;
+  sage_train_dq_kernel<DT, D, kCols><<<eighths(heads * ((rows + kBlockRows - 1) / kBlockRows) * p.runs), 256, kLds, s>>>(p);
+  if (p.runs > 1) {
+    constexpr int kJoined = 256 / (D / 8);
+    sage_train_join_bwd_kernel<DT, D, false><<<(unsigned)((heads * rows + kJoined - 1) / kJoined), 256, 0, s>>>(p);
+  }
   return hipGetLastError();
 }
 
@@ -643,20 +788,25 @@ uint64_t up256(uint64_t x) { return (x + 255) & ~UINT64_C(255); }
 TrainAttnScratch train_attn_scratch(const TrainAttnParams& call, bool backward) {
   TrainAttnParams p = call;
   fill_in(p);
+  const TrainRuns runs = train_runs(p);
   TrainAttnScratch out{};
-  if (!backward) return out;
+  if (!backward) {
+    out.bytes = up256(runs.fwd_bytes);
+    return out;
+  }
   const uint64_t heads = (uint64_t)p.B * p.Hkv, rows = up256(heads * p.row_pad * 4);
   out.row_l = 0;
   out.row_d = rows;
   out.norms = 2 * rows;
   out.part = out.norms + up256(heads * p.norm_blocks * 4);
-  out.bytes = out.part;
+  out.bytes = out.part + up256(runs.dkv_bytes > runs.dq_bytes ? runs.dkv_bytes : runs.dq_bytes);  // (one after the other)
   return out;
 }
 
 hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s) {
   fill_in(p);
-  (void)scratch;
+  p.runs = train_runs(p).fwd;
+  p.part = static_cast<float*>(scratch);
   const bool bf16 = p.dtype == KSANA_SAGE_BF16;
   if (p.D == 128) return bf16 ? fwd<KSANA_SAGE_BF16, 128>(p, s) : fwd<KSANA_SAGE_FP16, 128>(p, s);
   return bf16 ? fwd<KSANA_SAGE_BF16, 64>(p, s) : fwd<KSANA_SAGE_FP16, 64>(p, s);
@@ -665,13 +815,15 @@ hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s
 hipError_t launch_train_attn_bwd(TrainAttnParams p, void* scratch, hipStream_t s) {
   const TrainAttnScratch at = train_attn_scratch(p, true);
   fill_in(p);
+  const TrainRuns runs = train_runs(p);
   char* base = static_cast<char*>(scratch);
   p.row_l = reinterpret_cast<float*>(base + at.row_l);
   p.row_d = reinterpret_cast<float*>(base + at.row_d);
   p.norms = reinterpret_cast<float*>(base + at.norms);
+  p.part = reinterpret_cast<float*>(base + at.part);
   const bool bf16 = p.dtype == KSANA_SAGE_BF16;
-  if (p.D == 128) return bf16 ? bwd<KSANA_SAGE_BF16, 128>(p, s) : bwd<KSANA_SAGE_FP16, 128>(p, s);
-  return bf16 ? bwd<KSANA_SAGE_BF16, 64>(p, s) : bwd<KSANA_SAGE_FP16, 64>(p, s);
+  if (p.D == 128) return bf16 ? bwd<KSANA_SAGE_BF16, 128>(p, runs, s) : bwd<KSANA_SAGE_FP16, 128>(p, runs, s);
+  return bf16 ? bwd<KSANA_SAGE_BF16, 64>(p, runs, s) : bwd<KSANA_SAGE_FP16, 64>(p, runs, s);
 }
 
 }  // namespace ksana_sage

@@ -156,9 +156,33 @@ struct TileCopy {
 // to make signalling values quiet)
 __device__ __forceinline__ float largest(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
-// Number `blockIdx.x` of a launch of a multiple of eight workgroups.  Consecutive ones land on consecutive XCDs: every XCD takes a run
-// of the work, so that workgroups of one head share an L2.
-__device__ __forceinline__ int xcd_run_number() { return (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3); }
+// What workgroup `blockIdx.x` of a launch works on: a key head, a block of its rows or keys, and a run of the block's loop.
+// Consecutive workgroups land on consecutive XCDs.  Where all blocks cost the same, every XCD takes a run of heads after heads, so that
+// workgroups of one head share an L2.  Causal blocks and the entries of a padded batch differ: there the same block of
+// all heads comes before the next block, so that XCDs share long and short ones (and still keep heads to themselves where their number is
+// a multiple of eight).
+struct TrainPlace {
+  int bh, block, run;  // bh < 0: no such workgroup
+};
+__device__ __forceinline__ TrainPlace train_place(const TrainAttnParams& p, int blocks) {
+  const int heads = p.B * p.Hkv, all = heads * blocks;
+  if (p.causal || p.q_lens != nullptr || p.k_lens != nullptr) {
+    const int run = (int)blockIdx.x / all, at = (int)blockIdx.x - run * all, block = at / heads;
+    return run < p.runs ? TrainPlace{at - block * heads, block, run} : TrainPlace{-1, 0, 0};
+  }
+  const int i = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  if (i >= all * p.runs) return TrainPlace{-1, 0, 0};
+  const int part = i / blocks, bh = part / p.runs;
+  return TrainPlace{bh, i - part * blocks, part - bh * p.runs};
+}
+// The tiles of a run, of tiles `first` to `last`
+struct TileRange {
+  int from, to;
+};
+__device__ __forceinline__ TileRange run_tiles(int first, int last, int run, int runs) {
+  const int each = (max(0, last - first) + runs - 1) / runs;
+  return TileRange{min(last, first + run * each), min(last, first + (run + 1) * each)};
+}
 
 // A lane's column of a result whose rows are channels (32 dt + 8 g + 4 hh + c): two lanes hold a column's halves and exchange
 // them, so that each stores runs of eight channels.
@@ -175,6 +199,18 @@ __device__ __forceinline__ void store_column(const v16f (&acc)[Tile<D>::kBlocks]
       if (store) *reinterpret_cast<uint4*>(row + 32 * b + 8 * g + 8 * hh) = make_uint4(x[0], y[0], x[1], y[1]);
     }
   }
+}
+
+// .. and unrounded, for a run of a block
+template <int D>
+__device__ __forceinline__ void store_column_part(const v16f (&acc)[Tile<D>::kBlocks], float factor, float* row, int hh, bool store) {
+  if (!store) return;
+#pragma unroll
+  for (int b = 0; b < Tile<D>::kBlocks; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(row + 32 * b + 8 * g + 4 * hh) =
+          make_float4(acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor, acc[b][4 * g + 2] * factor, acc[b][4 * g + 3] * factor);
 }
 
 }  // namespace ksana_sage

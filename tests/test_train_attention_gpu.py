@@ -96,7 +96,7 @@ def _check(q, k, v, do, device, **kw):
     (1, 1, 1, 1, 2, 128, False), (1, 2, 2, 1, 1, 128, False), (2, 2, 1, 33, 31, 128, False), (1, 3, 3, 64, 64, 128, True),
     (1, 2, 2, 128, 64, 64, False), (2, 4, 2, 65, 129, 64, True), (1, 2, 2, 257, 300, 128, False), (1, 2, 2, 300, 257, 128, True),
     (1, 6, 2, 100, 321, 128, True), (1, 5, 1, 77, 200, 128, False), (1, 1, 1, 1, 1000, 128, False), (1, 8, 1, 1, 777, 64, False),
-    (1, 1, 1, 900, 3, 128, False), (1, 2, 2, 513, 513, 128, True), (3, 1, 1, 130, 190, 128, False),
+    (1, 260, 260, 70, 66, 128, False), (2, 264, 132, 129, 65, 64, True), (1, 1, 1, 900, 3, 128, False), (1, 2, 2, 513, 513, 128, True), (3, 1, 1, 130, 190, 128, False),
 ])
 def test_result_and_gradients_follow_the_formula(hip_device, dtype, B, Hq, Hkv, Lq, Lk, D, causal):
     _check(*_draw(Lq * 1000 + Lk, B, Hq, Hkv, Lq, Lk, D, dtype), hip_device, causal=causal)
