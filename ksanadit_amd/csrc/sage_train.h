@@ -28,8 +28,10 @@ struct TrainAttnParams {
   float *row_l, *row_d; // backward: -log2(e) lse (-inf where a row takes no part) and -sum(dO o), [B Hkv, row_pad]
   float* norms;         // backward in fp16: largest squared norms of rows of dO and of v, [B Hkv, norm_blocks]
   int norm_blocks, norm_q_blocks;
-  int runs;             // of tiles that a block's loop is cut into
-  float* part;          // their results
+  // of one launch: the first `whole` blocks are walked by a workgroup each, the loops of the others are cut into runs of run_tiles tiles,
+  // at most `runs` of them; their results, [blocks cut, runs, 128, ..], go to `part`
+  int whole, cut, runs, run_tiles;
+  float* part;
 };
 
 struct TrainAttnScratch {

@@ -11,6 +11,7 @@
 // P and dS are rounded to the tensors' type where they become matrix operands; S, dP, all sums and accumulators are fp32.
 #include "sage_train_device.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 
@@ -21,6 +22,7 @@ namespace {
 extern __shared__ __align__(1024) char train_lds[];
 __device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)train_lds; }
 
+constexpr int kTrainBlock = 128;  // query rows, or keys, of a workgroup
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // Rounded to fp16, probabilities relative to a row's largest would lose bits from 2^-14 on and vanish at 2^-25; scaled up as far as
 // the format goes, they do so a factor of 2^6 (forward, where the reference point may lag by 2^kLazy) or 2^15 (backward) later.
@@ -37,6 +39,18 @@ __device__ __forceinline__ Extent extent_of(const TrainAttnParams& p, int b) {
   int lq = p.Lq, lk = p.Lk;
   take_counts(p.q_lens, p.k_lens, b, lq, lk);
   return Extent{lk > 0 ? lq * p.group : 0, lk};
+}
+
+// Tiles that a block of rows (of keys) walks
+__device__ __forceinline__ int key_tiles_of(const TrainAttnParams& p, const Extent& e, int row0) {
+  int keys = e.keys;
+  if (p.causal) keys = min(keys, row_position(p, min(row0 + kTrainBlock, p.Lq * p.group) - 1) + 1);
+  return row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0;
+}
+__device__ __forceinline__ int row_tiles_of(const TrainAttnParams& p, const Extent& e, int key0, int& first) {
+  const int tiles = key0 < e.keys ? (e.rows + kTrainTile - 1) / kTrainTile : 0;
+  first = p.causal ? (int)min((int64_t)key0 * p.group / kTrainTile, (int64_t)tiles) : 0;
+  return tiles;
 }
 
 // A lane's query row as B operands: channels 16 s + 8 hh ..
@@ -61,13 +75,11 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
   const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
   const TrainPlace place = train_place(p, blocks);
-  if (place.bh < 0) return;
   const int bh = place.bh, block = blocks - 1 - place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   const int row0 = block * kRowsWg;
-  int keys = e.keys;
-  if (p.causal) keys = min(keys, row_position(p, min(row0 + kRowsWg, all_rows) - 1) + 1);
-  const TileRange range = run_tiles(0, row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0, place.run, p.runs);
+  const TileRange range = run_tiles(p, place, 0, key_tiles_of(p, e, row0));
+  if (place.run >= range.runs) return;
 
   const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
   const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
@@ -189,12 +201,10 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
     const float total = over_halves<Sum>(sum[n]);
     const float factor = !takes_part || total == 0.0f ? 0.0f : 1.0f / total;
     const int r = min(row[n], all_rows - 1), l = row_position(p, r), h = hk * p.group + r - l * p.group;
-    if (p.runs > 1) {
-      const int64_t at = ((int64_t)place.run * p.B * p.Hkv + bh) * all_rows + r;
-      store_column_part<D>(acc[n], 1.0f, p.part + at * D, hh, takes_part && range.from < range.to);
-      // (a run without tiles: nothing to add)
-      if (takes_part && hh == 0)
-        *reinterpret_cast<float2*>(p.part + (int64_t)p.runs * p.B * p.Hkv * all_rows * D + 2 * at) = make_float2(minus[n], total);
+    if (range.runs > 1) {
+      const int64_t at = ((int64_t)place.cut * p.runs + place.run) * kTrainBlock + row[n] - row0;
+      store_column_part<D>(acc[n], 1.0f, p.part + at * D, hh, takes_part);
+      if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.cut * p.runs * kTrainBlock * D + 2 * at) = make_float2(minus[n], total);
       continue;
     }
     if (!takes_part) {
@@ -209,18 +219,20 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
+constexpr int kNormRows = 64;  // rows of a workgroup (256 and a loop: 18.8 us of 40 heads of 1560 rows where this takes 8)
+
 // Per query row -log2(e) lse (plus the shift) and -sum(dO o); in fp16 besides the largest squared norms of rows of dO and of v per block of rows.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void sage_train_rows_kernel(const TrainAttnParams p) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes;  // lanes of a row, rows at a time
-  constexpr int kBlockRows = 256;
+  constexpr int kBlockRows = kNormRows;
   const int lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
   const int bh = blockIdx.y, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   float largest = 0.0f;
   const bool of_v = (int)blockIdx.x >= p.norm_q_blocks;  // fp16 only
   if (!of_v) {
-#pragma unroll 2
+#pragma unroll
     for (int i = 0; i < kBlockRows / kRows; ++i) {
       const int r = blockIdx.x * kBlockRows + i * kRows + slot;
       float d = 0.0f, square = 0.0f;
@@ -256,7 +268,7 @@ __global__ __launch_bounds__(256) void sage_train_rows_kernel(const TrainAttnPar
     }
   } else {
     const int first = ((int)blockIdx.x - p.norm_q_blocks) * kBlockRows;
-#pragma unroll 2
+#pragma unroll
     for (int i = 0; i < kBlockRows / kRows; ++i) {
       const int r = first + i * kRows + slot;
       float square = 0.0f;
@@ -312,12 +324,13 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
   const int blocks = (p.Lk + kKeysWg - 1) / kKeysWg;
   const TrainPlace place = train_place(p, blocks);
-  if (place.bh < 0) return;
   const int bh = place.bh, block = place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   const int key0 = block * kKeysWg;
-  const int tiles = key0 < e.keys ? (e.rows + kTrainTile - 1) / kTrainTile : 0;
-  const TileRange range = run_tiles(p.causal ? (int)min((int64_t)key0 * p.group / kTrainTile, (int64_t)tiles) : 0, tiles, place.run, p.runs);
+  int first_tile;
+  const int tiles = row_tiles_of(p, e, key0, first_tile);
+  const TileRange range = run_tiles(p, place, first_tile, tiles);
+  if (place.run >= range.runs) return;
 
   const unsigned lds = lds_base();
   v16f dk[kCols][T::kBlocks], dv[kCols][T::kBlocks];
@@ -450,8 +463,8 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
 #pragma unroll
       for (int c = 0; c < T::kBlocks; ++c) dk[n][c] = dv[n][c] = v16f{};
     }
-    if (p.runs > 1) {
-      float* at = p.part + (((int64_t)place.run * p.B * p.Hkv + bh) * p.Lk + min(key[n], p.Lk - 1)) * 2 * D;
+    if (range.runs > 1) {
+      float* at = p.part + (((int64_t)place.cut * p.runs + place.run) * kTrainBlock + key[n] - key0) * 2 * D;
       store_column_part<D>(dk[n], p.sm_scale * unshift / scale, at, hh, exists);
       store_column_part<D>(dv[n], unshift, at + D, hh, exists);
       continue;
@@ -470,13 +483,11 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
   const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
   const TrainPlace place = train_place(p, blocks);
-  if (place.bh < 0) return;
   const int bh = place.bh, block = blocks - 1 - place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
   const int row0 = block * kRowsWg;
-  int keys = e.keys;
-  if (p.causal) keys = min(keys, row_position(p, min(row0 + kRowsWg, all_rows) - 1) + 1);
-  const TileRange range = run_tiles(0, row0 < e.rows ? (keys + kTrainTile - 1) / kTrainTile : 0, place.run, p.runs);
+  const TileRange range = run_tiles(p, place, 0, key_tiles_of(p, e, row0));
+  if (place.run >= range.runs) return;
 
   const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
   const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
@@ -584,8 +595,9 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
 #pragma unroll
       for (int c = 0; c < T::kBlocks; ++c) dq[n][c] = v16f{};
     }
-    if (p.runs > 1) {
-      store_column_part<D>(dq[n], p.sm_scale * unshift / scale, p.part + (((int64_t)place.run * p.B * p.Hkv + bh) * all_rows + r) * D, hh, exists);
+    if (range.runs > 1) {
+      store_column_part<D>(dq[n], p.sm_scale * unshift / scale, p.part + (((int64_t)place.cut * p.runs + place.run) * kTrainBlock + row[n] - row0) * D, hh,
+                           exists);
       continue;
     }
     store_column<DT, D>(dq[n], p.sm_scale * unshift / scale, p.dq + (((int64_t)b * p.Lq + at) * p.Hq + h) * D, hh, exists);
@@ -594,30 +606,54 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
 
 // ------------------------------------------------------------------------------------------------------------ runs joined
 
-// Eight channels per lane.  A run's sums stand against a reference point of its own.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void sage_train_join_fwd_kernel(const TrainAttnParams p) {
-  constexpr int kLanes = D / 8;
-  const int all_rows = p.Lq * p.group, lane = threadIdx.x % kLanes;
-  const int64_t rows = (int64_t)p.B * p.Hkv * all_rows, at = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (at >= rows) return;
-  const int bh = (int)(at / all_rows), r = (int)(at - (int64_t)bh * all_rows), b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
-  float sum[8] = {}, total = 0.0f, top = -INFINITY;
-  const float2* ml = reinterpret_cast<const float2*>(p.part + p.runs * rows * D);
-  if (r < extent_of(p, b).rows) {
-    for (int i = 0; i < p.runs; ++i) {
-      const float2 x = ml[i * rows + at];
-      if (x.y != 0.0f) top = fmaxf(top, -x.x);
+// Eight channels per lane; kSlots groups of lanes share a row's runs and add their sums up in a fixed order.
+template <int kSlots>
+__device__ __forceinline__ void add_slots(float (&x)[9], int slot, int lanes, int lane) {
+  if constexpr (kSlots > 1) {
+    __shared__ float all[256 * 9];
+#pragma unroll
+    for (int i = 0; i < 9; ++i) all[i * 256 + threadIdx.x] = x[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      float sum = 0.0f;
+      for (int j = 0; j < kSlots; ++j) sum += all[i * 256 + j * lanes + lane];
+      x[i] = sum;
     }
+  }
+}
+
+// A run's sums stand against a reference point of its own.
+template <int DT, int D, int kSlots>
+__global__ __launch_bounds__(256) void sage_train_join_fwd_kernel(const TrainAttnParams p, const int groups) {
+  constexpr int kLanes = D / 8, kRows = 256 / (kLanes * kSlots);
+  const int lane = threadIdx.x % kLanes, slot = kSlots > 1 ? threadIdx.x / kLanes : 0, own = kSlots > 1 ? 0 : threadIdx.x / kLanes;
+  static_assert(kSlots == 1 || kRows == 1);
+  const int all_rows = p.Lq * p.group, blocks = (all_rows + kTrainBlock - 1) / kTrainBlock;
+  TrainPlace place = block_place(p, blocks, p.whole + (int)blockIdx.x / groups);
+  place.cut = (int)blockIdx.x / groups;
+  const int bh = place.bh, b = bh / p.Hkv, hk = bh - b * p.Hkv, row0 = (blocks - 1 - place.block) * kTrainBlock;
+  const int i = (int)blockIdx.x % groups * kRows + own, r = row0 + i;
+  const Extent e = extent_of(p, b);
+  const int runs = run_tiles(p, place, 0, key_tiles_of(p, e, row0)).runs;
+  if (runs == 1 || r >= all_rows) return;  // (with slots, of the whole workgroup)
+  const int64_t first = (int64_t)place.cut * p.runs * kTrainBlock + i;
+  const float2* ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.cut * p.runs * kTrainBlock * D);
+  float sum[9] = {}, top = -INFINITY;
+  if (r < e.rows) {
+    for (int j = lane; j < runs; j += kLanes) {  // (a lane after the other: 20 us for the 64 runs of one row, 4 so)
+      const float2 x = ml[first + (int64_t)j * kTrainBlock];
+      top = x.y != 0.0f ? fmaxf(top, -x.x) : top;  // (a run whose keys are all hidden has no reference point)
+    }
+#pragma unroll
+    for (int j = kLanes / 2; j > 0; j >>= 1) top = fmaxf(top, __shfl_xor(top, j));
 #pragma unroll 4
-    for (int i = 0; i < p.runs; ++i) {
-      const float2 x = ml[i * rows + at];
-      if (x.y == 0.0f) continue;  // (its sums are not written)
-      const float factor = fast_exp2(-x.x - top);
-      const float4* o = reinterpret_cast<const float4*>(p.part + (i * rows + at) * D + 8 * lane);
+    for (int j = slot; j < runs; j += kSlots) {
+      const float2 x = ml[first + (int64_t)j * kTrainBlock];
+      const float factor = x.y != 0.0f ? fast_exp2(-x.x - top) : 0.0f;
+      const float4* o = reinterpret_cast<const float4*>(p.part + (first + (int64_t)j * kTrainBlock) * D + 8 * lane);
       const float4 lo = o[0], hi = o[1];
-      total = __fmaf_rn(x.y, factor, total);
+      sum[8] = __fmaf_rn(x.y, factor, sum[8]);
       sum[0] = __fmaf_rn(lo.x, factor, sum[0]);
       sum[1] = __fmaf_rn(lo.y, factor, sum[1]);
       sum[2] = __fmaf_rn(lo.z, factor, sum[2]);
@@ -628,28 +664,48 @@ __global__ __launch_bounds__(256) void sage_train_join_fwd_kernel(const TrainAtt
       sum[7] = __fmaf_rn(hi.w, factor, sum[7]);
     }
   }
-  const float factor = total == 0.0f ? 0.0f : 1.0f / total;
+  add_slots<kSlots>(sum, slot, kLanes, lane);
+  if (slot != 0) return;
+  const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
+  const float factor = sum[8] == 0.0f ? 0.0f : 1.0f / sum[8];
   *reinterpret_cast<v4i*>(p.o + b * p.os.sB + l * p.os.sL + h * p.os.sH + 8 * lane) =
       pack8<DT>(sum[0] * factor, sum[1] * factor, sum[2] * factor, sum[3] * factor, sum[4] * factor, sum[5] * factor, sum[6] * factor, sum[7] * factor);
-  if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Lq + l] = total == 0.0f ? -INFINITY : (log2f(total) + top) * kLn2;
+  if (lane == 0 && p.lse != nullptr) p.lse[((int64_t)b * p.Hq + h) * p.Lq + l] = sum[8] == 0.0f ? -INFINITY : (log2f(sum[8]) + top) * kLn2;
 }
 
 // Sums of the runs' gradients: of query rows (kKeys false) or of keys, whose two gradients lie side by side
-template <int DT, int D, bool kKeys>
-__global__ __launch_bounds__(256) void sage_train_join_bwd_kernel(const TrainAttnParams p) {
-  constexpr int kWidth = kKeys ? 2 * D : D, kLanes = kWidth / 8;
-  const int lane = threadIdx.x % kLanes, per_head = kKeys ? p.Lk : p.Lq * p.group;
-  const int64_t rows = (int64_t)p.B * p.Hkv * per_head, at = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  if (at >= rows) return;
-  float4 lo = make_float4(0, 0, 0, 0), hi = lo;
+template <int DT, int D, bool kKeys, int kSlots>
+__global__ __launch_bounds__(256) void sage_train_join_bwd_kernel(const TrainAttnParams p, const int groups) {
+  constexpr int kWidth = kKeys ? 2 * D : D, kLanes = kWidth / 8, kRows = kSlots > 1 ? 1 : 256 / kLanes;
+  static_assert(kSlots == 1 || kLanes * kSlots == 256);
+  const int lane = threadIdx.x % kLanes, slot = kSlots > 1 ? threadIdx.x / kLanes : 0, own = kSlots > 1 ? 0 : threadIdx.x / kLanes;
+  const int all = kKeys ? p.Lk : p.Lq * p.group, blocks = (all + kTrainBlock - 1) / kTrainBlock;
+  TrainPlace place = block_place(p, blocks, p.whole + (int)blockIdx.x / groups);
+  place.cut = (int)blockIdx.x / groups;
+  const int bh = place.bh, b = bh / p.Hkv, hk = bh - b * p.Hkv, row0 = (kKeys ? place.block : blocks - 1 - place.block) * kTrainBlock;
+  const int i = (int)blockIdx.x % groups * kRows + own, r = row0 + i;
+  const Extent e = extent_of(p, b);
+  int from = 0;
+  const int to = kKeys ? row_tiles_of(p, e, row0, from) : key_tiles_of(p, e, row0);
+  const int runs = run_tiles(p, place, from, to).runs;
+  if (runs == 1 || r >= all) return;
+  const int64_t first = (int64_t)place.cut * p.runs * kTrainBlock + i;
+  float sum[9] = {};
 #pragma unroll 4
-  for (int i = 0; i < p.runs; ++i) {
-    const float4* x = reinterpret_cast<const float4*>(p.part + (i * rows + at) * kWidth + 8 * lane);
-    const float4 a = x[0], c = x[1];
-    lo = make_float4(lo.x + a.x, lo.y + a.y, lo.z + a.z, lo.w + a.w);
-    hi = make_float4(hi.x + c.x, hi.y + c.y, hi.z + c.z, hi.w + c.w);
+  for (int j = slot; j < runs; j += kSlots) {
+    const float4* x = reinterpret_cast<const float4*>(p.part + (first + (int64_t)j * kTrainBlock) * kWidth + 8 * lane);
+    const float4 lo = x[0], hi = x[1];
+    sum[0] += lo.x;
+    sum[1] += lo.y;
+    sum[2] += lo.z;
+    sum[3] += lo.w;
+    sum[4] += hi.x;
+    sum[5] += hi.y;
+    sum[6] += hi.z;
+    sum[7] += hi.w;
   }
-  const int bh = (int)(at / per_head), r = (int)(at - (int64_t)bh * per_head), b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  add_slots<kSlots>(sum, slot, kLanes, lane);
+  if (slot != 0) return;
   uint16_t* out;
   if constexpr (kKeys) {
     out = (8 * lane < D ? p.dk : p.dv) + (((int64_t)b * p.Lk + r) * p.Hkv + hk) * D + 8 * lane % D;
@@ -657,12 +713,10 @@ __global__ __launch_bounds__(256) void sage_train_join_bwd_kernel(const TrainAtt
     const int l = row_position(p, r);
     out = p.dq + (((int64_t)b * p.Lq + l) * p.Hq + hk * p.group + r - l * p.group) * D + 8 * lane;
   }
-  *reinterpret_cast<v4i*>(out) = pack8<DT>(lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w);
+  *reinterpret_cast<v4i*>(out) = pack8<DT>(sum[0], sum[1], sum[2], sum[3], sum[4], sum[5], sum[6], sum[7]);
 }
 
 // ------------------------------------------------------------------------------------------------------------ launches
-
-constexpr int kNormRows = 256;  // rows per block of sage_train_rows_kernel
 
 // 64 KiB of dynamic LDS and more has to be requested per kernel, once per device.
 struct LdsRequest {
@@ -690,66 +744,92 @@ void fill_in(TrainAttnParams& p) {
   p.norm_blocks = p.norm_q_blocks + (p.dtype == KSANA_SAGE_FP16 ? (p.Lk + kNormRows - 1) / kNormRows : 0);
 }
 
-unsigned eighths(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
-
-// How many runs a launch cuts its blocks' loops of `tiles` tiles into, with `blocks` blocks in all and `bytes` of results to a run.
-// Two workgroups to each of 256 compute units; in units of a tile's time (about 2 us with both there), a workgroup costs kSetup besides
-// its tiles, a launch that joins runs kJoin and what its bytes take at 4 TB/s, written and read.
-int runs_of(int64_t blocks, int tiles, double bytes) {
+// How a launch of `blocks` blocks that walk at most `tiles` tiles each is cut, with `bytes` of results to a block.  Two workgroups to each of
+// 256 compute units; in units of a tile's time (about 2 us with both there), a workgroup costs kSetup besides its tiles, a launch
+// that joins runs kJoin and what its bytes take, written and read.  Blocks that cost the same: as many as fill whole rounds are
+// left whole, the others are cut so that they fill one more.  Others (`differ`, `share` of the tiles being there at all): runs of one
+// length, which even out what a workgroup has to do.
+struct TrainCut {
+  int whole, cut, runs, run_tiles;
+  uint64_t part(int width) const { return runs > 1 ? (uint64_t)cut * runs * kTrainBlock * width * 4 : 0; }
+};
+TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double share) {
   constexpr double kSetup = 2.0, kJoin = 2.0, kBytesPerTile = 4e12 * 2e-6;
   constexpr int kPlaces = 512;
-  int best = 1;
+  const int whole = differ ? 0 : (int)(blocks / kPlaces * kPlaces);
+  const int64_t rest = blocks - whole;
   double least = 1e30;
+  int best = tiles;  // of a run
   for (int n = 1; n <= 128 && n <= tiles; ++n) {
-    const double rounds = (double)((blocks * n + kPlaces - 1) / kPlaces), each = (tiles + n - 1) / n;
-    const double cost = rounds * (each + kSetup) + (n > 1 ? kJoin + 2.0 * n * bytes / kBytesPerTile : 0.0);
+    const int each = (tiles + n - 1) / n;
+    const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * rest * bytes * share / kBytesPerTile;
+    const double cost = differ ? std::max((double)blocks * tiles * share / kPlaces * (1.0 + kSetup / each) + 0.5 * each, each + kSetup) + join
+                               : (double)((rest * n + kPlaces - 1) / kPlaces) * (each + kSetup) + join;
     if (cost < 0.97 * least) {
       least = cost;
-      best = n;
+      best = each;
     }
   }
-  return best;
+  const int runs = (tiles + best - 1) / best;
+  if (runs == 1 && !differ) return TrainCut{(int)(blocks / 8 * 8), (int)(blocks % 8), 1, tiles};
+  return TrainCut{whole, (int)rest, runs, best};
 }
-constexpr int kBlockRows = 128;  // rows, or keys, of a workgroup
-struct TrainRuns {
-  int fwd, dkv, dq;
-  uint64_t fwd_bytes, dkv_bytes, dq_bytes;  // of their partial results
+struct TrainCuts {
+  TrainCut fwd, dkv, dq;
 };
-TrainRuns train_runs(const TrainAttnParams& p) {
+TrainCuts train_cuts(const TrainAttnParams& p) {
   const int64_t heads = (int64_t)p.B * p.Hkv, rows = (int64_t)p.Lq * p.group;
-  const int64_t row_blocks = heads * ((rows + kBlockRows - 1) / kBlockRows), key_blocks = heads * ((p.Lk + kBlockRows - 1) / kBlockRows);
+  const int64_t row_blocks = heads * ((rows + kTrainBlock - 1) / kTrainBlock), key_blocks = heads * ((p.Lk + kTrainBlock - 1) / kTrainBlock);
   const int key_tiles = (p.Lk + kTrainTile - 1) / kTrainTile, row_tiles = (int)((rows + kTrainTile - 1) / kTrainTile);
-  const double row_bytes = 4.0 * heads * rows * p.D, key_bytes = 8.0 * heads * p.Lk * p.D;
-  TrainRuns r{};
-  r.fwd = runs_of(row_blocks, key_tiles, row_bytes);
-  r.dkv = runs_of(key_blocks, row_tiles, key_bytes);
-  r.dq = runs_of(row_blocks, key_tiles, row_bytes);
-  r.fwd_bytes = r.fwd > 1 ? (uint64_t)r.fwd * heads * rows * (p.D + 2) * 4 : 0;
-  r.dkv_bytes = r.dkv > 1 ? (uint64_t)r.dkv * heads * p.Lk * p.D * 8 : 0;
-  r.dq_bytes = r.dq > 1 ? (uint64_t)r.dq * heads * rows * p.D * 4 : 0;
-  return r;
+  const bool differ = p.causal || p.q_lens != nullptr || p.k_lens != nullptr;
+  const double share = p.causal && p.Lq > 1 ? 0.5 : 1.0, row_bytes = 4.0 * std::min<int64_t>(rows, kTrainBlock) * p.D;
+  const TrainCut of_rows = cut_of(row_blocks, key_tiles, row_bytes, differ, share);
+  return TrainCuts{of_rows, cut_of(key_blocks, row_tiles, 8.0 * std::min(p.Lk, kTrainBlock) * p.D, differ, share), of_rows};
 }
+void take_cut(TrainAttnParams& p, const TrainCut& c) {
+  p.whole = c.whole;
+  p.cut = c.cut;
+  p.runs = c.runs;
+  p.run_tiles = c.run_tiles;
+}
+unsigned workgroups(const TrainAttnParams& p) { return (unsigned)(p.whole + (int64_t)p.cut * p.runs); }
+// Rows of a block that the joins look at
+int joined_rows(int64_t all) { return (int)std::min<int64_t>(all, kTrainBlock); }
+constexpr int kManyRuns = 16;  // from here on lanes share a row's runs
 
 template <int DT, int D>
 hipError_t fwd(TrainAttnParams p, hipStream_t s) {
   constexpr int kCols = 1, kLds = 2 * 2 * Tile<D>::kBytes;
-  static_assert(kBlockRows == 128 * kCols);
-  const int64_t rows = (int64_t)p.Lq * p.group, heads = (int64_t)p.B * p.Hkv, blocks = (rows + kBlockRows - 1) / kBlockRows;
+  static_assert(kTrainBlock == 128 * kCols);
   static LdsRequest request;
-  hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D, kCols>), kLds);
+  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D, kCols>), kLds);
   if (e != hipSuccess) return e;
-  sage_train_fwd_kernel<DT, D, kCols><<<eighths(heads * blocks * p.runs), 256, kLds, s>>>(p);
-  e = hipGetLastError();
-  if (e != hipSuccess || p.runs == 1) return e;
-  constexpr int kJoined = 256 / (D / 8);
-  sage_train_join_fwd_kernel<DT, D><<<(unsigned)((heads * rows + kJoined - 1) / kJoined), 256, 0, s>>>(p);
+  sage_train_fwd_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+  if (p.runs > 1) {
+    constexpr int kLanes = D / 8;
+    const int rows = joined_rows((int64_t)p.Lq * p.group), groups = (rows * kLanes + 255) / 256;  // workgroups of a block
+    if (p.runs >= kManyRuns)
+      sage_train_join_fwd_kernel<DT, D, 256 / kLanes><<<(unsigned)((int64_t)rows * p.cut), 256, 0, s>>>(p, rows);
+    else
+      sage_train_join_fwd_kernel<DT, D, 1><<<(unsigned)((int64_t)groups * p.cut), 256, 0, s>>>(p, groups);
+  }
   return hipGetLastError();
 }
 
+template <int DT, int D, bool kKeys>
+void join_bwd(const TrainAttnParams& p, int64_t all, hipStream_t s) {
+  if (p.runs == 1) return;
+  constexpr int kLanes = (kKeys ? 2 : 1) * D / 8;
+  const int rows = joined_rows(all), groups = (rows * kLanes + 255) / 256;
+  if (p.runs >= kManyRuns)
+    sage_train_join_bwd_kernel<DT, D, kKeys, 256 / kLanes><<<(unsigned)((int64_t)rows * p.cut), 256, 0, s>>>(p, rows);
+  else
+    sage_train_join_bwd_kernel<DT, D, kKeys, 1><<<(unsigned)((int64_t)groups * p.cut), 256, 0, s>>>(p, groups);
+}
+
 template <int DT, int D>
-hipError_t bwd(TrainAttnParams p, const TrainRuns& runs, hipStream_t s) {
-  const int64_t rows = (int64_t)p.Lq * p.group, heads = (int64_t)p.B * p.Hkv;
-  sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, (unsigned)heads), 256, 0, s>>>(p);
+hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
+  sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, p.B * p.Hkv), 256, 0, s>>>(p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   constexpr int kCols = 1;
@@ -758,12 +838,9 @@ hipError_t bwd(TrainAttnParams p, const TrainRuns& runs, hipStream_t s) {
     static LdsRequest request;
     e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
     if (e != hipSuccess) return e;
-    p.runs = runs.dkv;
-    sage_train_dkv_kernel<DT, D, kCols><<<eighths(heads * ((p.Lk + kBlockRows - 1) / kBlockRows) * p.runs), 256, kLds, s>>>(p);
-    if (p.runs > 1) {
-      constexpr int kJoined = 256 / (D / 4);
-      sage_train_join_bwd_kernel<DT, D, true><<<(unsigned)((heads * p.Lk + kJoined - 1) / kJoined), 256, 0, s>>>(p);
-    }
+    take_cut(p, cuts.dkv);
+    sage_train_dkv_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+    join_bwd<DT, D, true>(p, p.Lk, s);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -772,12 +849,9 @@ hipError_t bwd(TrainAttnParams p, const TrainRuns& runs, hipStream_t s) {
   static LdsRequest request;
   e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);
   if (e != hipSuccess) return e;
-  p.runs = runs.dq;
-  sage_train_dq_kernel<DT, D, kCols><<<eighths(heads * ((rows + kBlockRows - 1) / kBlockRows) * p.runs), 256, kLds, s>>>(p);
-  if (p.runs > 1) {
-    constexpr int kJoined = 256 / (D / 8);
-    sage_train_join_bwd_kernel<DT, D, false><<<(unsigned)((heads * rows + kJoined - 1) / kJoined), 256, 0, s>>>(p);
-  }
+  take_cut(p, cuts.dq);
+  sage_train_dq_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+  join_bwd<DT, D, false>(p, (int64_t)p.Lq * p.group, s);
   return hipGetLastError();
 }
 
@@ -788,10 +862,10 @@ uint64_t up256(uint64_t x) { return (x + 255) & ~UINT64_C(255); }
 TrainAttnScratch train_attn_scratch(const TrainAttnParams& call, bool backward) {
   TrainAttnParams p = call;
   fill_in(p);
-  const TrainRuns runs = train_runs(p);
+  const TrainCuts cuts = train_cuts(p);
   TrainAttnScratch out{};
   if (!backward) {
-    out.bytes = up256(runs.fwd_bytes);
+    out.bytes = up256(cuts.fwd.part(p.D + 2));
     return out;
   }
   const uint64_t heads = (uint64_t)p.B * p.Hkv, rows = up256(heads * p.row_pad * 4);
@@ -799,13 +873,13 @@ TrainAttnScratch train_attn_scratch(const TrainAttnParams& call, bool backward) 
   out.row_d = rows;
   out.norms = 2 * rows;
   out.part = out.norms + up256(heads * p.norm_blocks * 4);
-  out.bytes = out.part + up256(runs.dkv_bytes > runs.dq_bytes ? runs.dkv_bytes : runs.dq_bytes);  // (one after the other)
+  out.bytes = out.part + up256(std::max(cuts.dkv.part(2 * p.D), cuts.dq.part(p.D)));  // (one after the other)
   return out;
 }
 
 hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s) {
   fill_in(p);
-  p.runs = train_runs(p).fwd;
+  take_cut(p, train_cuts(p).fwd);
   p.part = static_cast<float*>(scratch);
   const bool bf16 = p.dtype == KSANA_SAGE_BF16;
   if (p.D == 128) return bf16 ? fwd<KSANA_SAGE_BF16, 128>(p, s) : fwd<KSANA_SAGE_FP16, 128>(p, s);
@@ -815,15 +889,15 @@ hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s
 hipError_t launch_train_attn_bwd(TrainAttnParams p, void* scratch, hipStream_t s) {
   const TrainAttnScratch at = train_attn_scratch(p, true);
   fill_in(p);
-  const TrainRuns runs = train_runs(p);
+  const TrainCuts cuts = train_cuts(p);
   char* base = static_cast<char*>(scratch);
   p.row_l = reinterpret_cast<float*>(base + at.row_l);
   p.row_d = reinterpret_cast<float*>(base + at.row_d);
   p.norms = reinterpret_cast<float*>(base + at.norms);
   p.part = reinterpret_cast<float*>(base + at.part);
   const bool bf16 = p.dtype == KSANA_SAGE_BF16;
-  if (p.D == 128) return bf16 ? bwd<KSANA_SAGE_BF16, 128>(p, runs, s) : bwd<KSANA_SAGE_FP16, 128>(p, runs, s);
-  return bf16 ? bwd<KSANA_SAGE_BF16, 64>(p, runs, s) : bwd<KSANA_SAGE_FP16, 64>(p, runs, s);
+  if (p.D == 128) return bf16 ? bwd<KSANA_SAGE_BF16, 128>(p, cuts, s) : bwd<KSANA_SAGE_FP16, 128>(p, cuts, s);
+  return bf16 ? bwd<KSANA_SAGE_BF16, 64>(p, cuts, s) : bwd<KSANA_SAGE_FP16, 64>(p, cuts, s);
 }
 
 }  // namespace ksana_sage

@@ -157,31 +157,39 @@ struct TileCopy {
 __device__ __forceinline__ float largest(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
 // What workgroup `blockIdx.x` of a launch works on: a key head, a block of its rows or keys, and a run of the block's loop.
-// Consecutive workgroups land on consecutive XCDs.  Where all blocks cost the same, every XCD takes a run of heads after heads, so that
-// workgroups of one head share an L2.  Causal blocks and the entries of a padded batch differ: there the same block of
-// all heads comes before the next block, so that XCDs share long and short ones (and still keep heads to themselves where their number is
-// a multiple of eight).
+// Consecutive workgroups land on consecutive XCDs.  Where all blocks cost the same, every XCD takes a stretch of heads after heads, so
+// that workgroups of one head share an L2.  Causal blocks and the entries of a padded batch differ: there the same block of all heads
+// comes before the next block, so that XCDs share long and short ones (and still keep heads to themselves where their number is a
+// multiple of eight).
 struct TrainPlace {
-  int bh, block, run;  // bh < 0: no such workgroup
+  int bh, block, run, cut;  // cut: number of the block among those that are cut; -1: a whole block
 };
-__device__ __forceinline__ TrainPlace train_place(const TrainAttnParams& p, int blocks) {
-  const int heads = p.B * p.Hkv, all = heads * blocks;
-  if (p.causal || p.q_lens != nullptr || p.k_lens != nullptr) {
-    const int run = (int)blockIdx.x / all, at = (int)blockIdx.x - run * all, block = at / heads;
-    return run < p.runs ? TrainPlace{at - block * heads, block, run} : TrainPlace{-1, 0, 0};
+__device__ __forceinline__ bool blocks_differ(const TrainAttnParams& p) { return p.causal || p.q_lens != nullptr || p.k_lens != nullptr; }
+__device__ __forceinline__ TrainPlace block_place(const TrainAttnParams& p, int blocks, int i) {
+  if (blocks_differ(p)) {
+    const int heads = p.B * p.Hkv, block = i / heads;
+    return TrainPlace{i - block * heads, block, 0, -1};
   }
-  const int i = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-  if (i >= all * p.runs) return TrainPlace{-1, 0, 0};
-  const int part = i / blocks, bh = part / p.runs;
-  return TrainPlace{bh, i - part * blocks, part - bh * p.runs};
+  const int bh = i / blocks;
+  return TrainPlace{bh, i - bh * blocks, 0, -1};
 }
-// The tiles of a run, of tiles `first` to `last`
+__device__ __forceinline__ TrainPlace train_place(const TrainAttnParams& p, int blocks) {
+  const int at = (int)blockIdx.x;
+  if (at < p.whole) return block_place(p, blocks, (at & 7) * (p.whole >> 3) + (at >> 3));  // (only multiples of eight are left whole)
+  const int run = (at - p.whole) / p.cut, cut = at - p.whole - run * p.cut;
+  TrainPlace place = block_place(p, blocks, p.whole + cut);
+  place.run = run;
+  place.cut = cut;
+  return place;
+}
+// The tiles of a block's run of its tiles `first` to `last`, and how many runs it has
 struct TileRange {
-  int from, to;
+  int from, to, runs;
 };
-__device__ __forceinline__ TileRange run_tiles(int first, int last, int run, int runs) {
-  const int each = (max(0, last - first) + runs - 1) / runs;
-  return TileRange{min(last, first + run * each), min(last, first + (run + 1) * each)};
+__device__ __forceinline__ TileRange run_tiles(const TrainAttnParams& p, const TrainPlace& place, int first, int last) {
+  if (place.cut < 0) return TileRange{first, last, 1};
+  const int runs = max(1, (max(0, last - first) + p.run_tiles - 1) / p.run_tiles), from = first + place.run * p.run_tiles;
+  return TileRange{min(from, last), min(from + p.run_tiles, last), runs};
 }
 
 // A lane's column of a result whose rows are channels (32 dt + 8 g + 4 hh + c): two lanes hold a column's halves and exchange
