@@ -476,6 +476,43 @@ int ksana_sage_train_attn_bwd(const ksana_sage_train_attn* call, const void* q, 
                               const float* lse, const void* d_o, const int64_t do_strides[4], void* dq, void* dk, void* dv,
                               void* scratch, void* stream);
 
+/* What stands between two parts of a block, x [B, L, C] the residual stream and y [B, L, C] the output of the part before:
+ *     u = post(y) post_weight                    post none: u = y
+ *     h = residual_scale x + gate u              without y: h = x
+ *     n = (norm(h) weight + bias) (1 + scale) + shift
+ * norm and post over the C channels of a row: layer norm or rms norm, eps under both roots.  Statistics and all arithmetic in fp32,
+ * n from the unrounded h.  Types: x (and h) bf16 or fp16 with y (and n) of the same type, or fp32 with any y.  C <= 8192. */
+#define KSANA_SAGE_FP32 2
+#define KSANA_SAGE_NORM_NONE 0
+#define KSANA_SAGE_NORM_LAYER 1
+#define KSANA_SAGE_NORM_RMS 2
+typedef struct ksana_sage_vector { /* C channels, in any of the three types; ptr NULL: absent (1 for weights and gate, else 0)   */
+  const void* ptr;                 /* device                                                                                     */
+  int64_t batch_stride;            /* in elements; 0: one for all batch entries (weight, bias, post_weight: always 0)            */
+  int32_t dtype;
+  int32_t reserved;                /* 0 */
+} ksana_sage_vector;
+typedef struct ksana_sage_train_norm {
+  int32_t B, L, C;
+  int32_t x_dtype, y_dtype;
+  int32_t norm, post;              /* KSANA_SAGE_NORM_*; norm is not NONE                                                        */
+  float residual_scale, eps;
+  int32_t reserved;                /* 0 */
+  int64_t x_strides[2], y_strides[2]; /* of B and L, in elements; channels are contiguous                                        */
+  ksana_sage_vector gate, scale, shift, weight, bias, post_weight;
+} ksana_sage_train_norm;
+/* y NULL: no part before (gate, post and post_weight absent, residual_scale 1).  h [B, L, C] of x's type and n of y's,
+ * contiguous; h may be NULL without y.  stats: fp32 [B, L, 4] for the backward call, or NULL. */
+int ksana_sage_train_norm_fwd(const ksana_sage_train_norm* call, const void* x, const void* y, void* h, void* n, float* stats,
+                              void* stream);
+/* Bytes of the backward call's device scratch (256-byte aligned, not kept between calls) */
+int ksana_sage_train_norm_scratch(const ksana_sage_train_norm* call, uint64_t* bytes);
+/* The gradients of everything from those of h (dh, contiguous, or NULL: zeros) and n (dn, contiguous).  dx of x's type, dy of
+ * y's (NULL exactly without y), contiguous.  grads: one pointer per vector in the order of the structure, each contiguous in the
+ * vector's type, [B, C] or [C] as the vector; NULL: not wanted. */
+int ksana_sage_train_norm_bwd(const ksana_sage_train_norm* call, const void* x, const void* y, const float* stats, const void* dh,
+                              const void* dn, void* dx, void* dy, void* const grads[6], void* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libksana_sage_hip.so"
 ABI_VERSION = 25
 
-BF16, FP16 = 0, 1
+BF16, FP16, FP32 = 0, 1, 2
 OK, EINVAL, ENOTSUP, EHIP = 0, -1, -2, -3
 FLAG_PWL_EXP2 = 1
 FLAG_SMOOTH_V = 2
@@ -23,6 +23,7 @@ FLAG_TILE_SKIP = 16
 FLAG_Q_UNSTORED = 32
 FLAG_WS_UNSTORED = 64
 PREP_WAN, PREP_WAN_COMFY, PREP_QWEN = 0, 1, 2
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 KEEP = -(2**63)  # KSANA_SAGE_KEEP
 
 EXPORTS = (
@@ -62,6 +63,9 @@ EXPORTS = (
     "ksana_sage_train_attn_scratch",
     "ksana_sage_train_attn_fwd",
     "ksana_sage_train_attn_bwd",
+    "ksana_sage_train_norm_fwd",
+    "ksana_sage_train_norm_scratch",
+    "ksana_sage_train_norm_bwd",
 )
 
 
@@ -112,6 +116,20 @@ class TrainAttn(C.Structure):
 
     _fields_ = [("shape", Shape), ("dtype", C.c_int32), ("causal", C.c_int32), ("sm_scale", C.c_float), ("reserved", C.c_int32)] + \
         [(n, C.c_int64 * 4) for n in ("q_strides", "k_strides", "v_strides", "o_strides")] + [("q_lens", C.c_void_p), ("k_lens", C.c_void_p)]
+
+
+class Vector(C.Structure):
+    """``ksana_sage_vector``"""
+
+    _fields_ = [("ptr", C.c_void_p), ("batch_stride", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class TrainNorm(C.Structure):
+    """``ksana_sage_train_norm``: a residual norm but for its buffers and its stream."""
+
+    _fields_ = [(n, C.c_int32) for n in ("B", "L", "C", "x_dtype", "y_dtype", "norm", "post")] + \
+        [("residual_scale", C.c_float), ("eps", C.c_float), ("reserved", C.c_int32), ("x_strides", C.c_int64 * 2), ("y_strides", C.c_int64 * 2)] + \
+        [(n, Vector) for n in ("gate", "scale", "shift", "weight", "bias", "post_weight")]
 
 
 class SageLibraryError(RuntimeError):
@@ -180,6 +198,9 @@ def _declare(lib):
     lib.ksana_sage_forward_call.argtypes, lib.ksana_sage_forward_call.restype = [vp] * 7, i
     lib.ksana_sage_train_attn_scratch.argtypes, lib.ksana_sage_train_attn_scratch.restype = [vp] * 3, i
     lib.ksana_sage_train_attn_fwd.argtypes, lib.ksana_sage_train_attn_fwd.restype = [vp] * 8, i
+    lib.ksana_sage_train_norm_fwd.argtypes, lib.ksana_sage_train_norm_fwd.restype = [vp] * 7, i
+    lib.ksana_sage_train_norm_scratch.argtypes, lib.ksana_sage_train_norm_scratch.restype = [vp] * 2, i
+    lib.ksana_sage_train_norm_bwd.argtypes, lib.ksana_sage_train_norm_bwd.restype = [vp] * 11, i
     lib.ksana_sage_train_attn_bwd.argtypes, lib.ksana_sage_train_attn_bwd.restype = [vp] * 13, i
 
 

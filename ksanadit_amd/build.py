@@ -16,7 +16,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libksana_sage_hip.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ("sage_capi.hip", "sage_quant.hip", "sage_attn.hip", "sage_small.hip", "sage_resident.hip", "sage_sla.hip", "sage_probe.hip",
-           "sage_train_attn.hip")
+           "sage_train_attn.hip", "sage_train_norm.hip")
 
 HIPCC_FLAGS = (
     "--offload-arch=gfx950",

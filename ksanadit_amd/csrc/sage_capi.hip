@@ -1149,3 +1149,131 @@ extern "C" int ksana_sage_train_attn_bwd(const ksana_sage_train_attn* call, cons
   const hipError_t e = ksana_sage::launch_train_attn_bwd(p, scratch, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? 0 : hip_fail(e, "training attention, backward");
 }
+
+namespace {
+int train_vector(const char* name, const ksana_sage_vector& v, int B, bool shared, ksana_sage::TrainVector* out) {
+  *out = ksana_sage::TrainVector{};
+  if (!v.ptr) return 0;
+  if (v.dtype < KSANA_SAGE_BF16 || v.dtype > KSANA_SAGE_FP32) return fail(KSANA_SAGE_EINVAL, "%s: dtype %d unknown", name, v.dtype);
+  if (v.reserved != 0) return fail(KSANA_SAGE_EINVAL, "%s: reserved is %d, must be 0", name, v.reserved);
+  if (reinterpret_cast<uintptr_t>(v.ptr) & (v.dtype == KSANA_SAGE_FP32 ? 3u : 1u)) return fail(KSANA_SAGE_EINVAL, "%s is not aligned to its type", name);
+  if (v.batch_stride < 0 || (shared && v.batch_stride != 0)) return fail(KSANA_SAGE_EINVAL, "%s: batch stride %lld", name, (long long)v.batch_stride);
+  *out = ksana_sage::TrainVector{v.ptr, v.batch_stride, v.dtype};
+  return 0;
+}
+bool rows_in_pieces(const void* p, int dtype, int64_t sB, int64_t sL) {
+  const int64_t size = dtype == KSANA_SAGE_FP32 ? 4 : 2;
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && sB * size % 16 == 0 && sL * size % 16 == 0;
+}
+int train_norm_params(const ksana_sage_train_norm* c, const void* x, const void* y, bool has_y, ksana_sage::TrainNormParams* p) {
+  if (!c) return fail(KSANA_SAGE_EINVAL, "call is null");
+  if (c->B < 1 || c->L < 1 || c->C < 1) return fail(KSANA_SAGE_EINVAL, "non-positive extent (B=%d L=%d C=%d)", c->B, c->L, c->C);
+  if (!ksana_sage::train_norm_width_fits(c->C)) return fail(KSANA_SAGE_ENOTSUP, "C=%d exceeds 8192", c->C);
+  if (c->L > (1 << 28) || c->B > (1 << 20)) return fail(KSANA_SAGE_ENOTSUP, "B=%d L=%d exceed the launch grid", c->B, c->L);
+  const bool types = c->x_dtype == KSANA_SAGE_FP32 ? c->y_dtype >= KSANA_SAGE_BF16 && c->y_dtype <= KSANA_SAGE_FP32
+                                                   : (c->x_dtype == KSANA_SAGE_BF16 || c->x_dtype == KSANA_SAGE_FP16) && c->y_dtype == c->x_dtype;
+  if (!types) return fail(KSANA_SAGE_EINVAL, "types %d of x and %d of y do not go together", c->x_dtype, c->y_dtype);
+  if (c->norm != KSANA_SAGE_NORM_LAYER && c->norm != KSANA_SAGE_NORM_RMS) return fail(KSANA_SAGE_EINVAL, "norm %d unknown", c->norm);
+  if (c->post < KSANA_SAGE_NORM_NONE || c->post > KSANA_SAGE_NORM_RMS) return fail(KSANA_SAGE_EINVAL, "post %d unknown", c->post);
+  if (c->reserved != 0) return fail(KSANA_SAGE_EINVAL, "reserved is %d, must be 0", c->reserved);
+  if (!(c->eps >= 0.0f)) return fail(KSANA_SAGE_EINVAL, "eps is negative or not a number");
+  if (c->post == KSANA_SAGE_NORM_NONE && c->post_weight.ptr) return fail(KSANA_SAGE_EINVAL, "post_weight without a norm behind the part");
+  if (!has_y && (c->gate.ptr || c->post != KSANA_SAGE_NORM_NONE || c->residual_scale != 1.0f))
+    return fail(KSANA_SAGE_EINVAL, "gate, post and residual_scale go with y");
+  for (int i = 0; i < 2; ++i)
+    if (c->x_strides[i] < 0 || (has_y && c->y_strides[i] < 0)) return fail(KSANA_SAGE_EINVAL, "negative stride");
+  if (!x) return fail(KSANA_SAGE_EINVAL, "x is null");
+  *p = ksana_sage::TrainNormParams{};
+  if (int rc = train_vector("gate", c->gate, c->B, false, &p->gate)) return rc;
+  if (int rc = train_vector("scale", c->scale, c->B, false, &p->scale)) return rc;
+  if (int rc = train_vector("shift", c->shift, c->B, false, &p->shift)) return rc;
+  if (int rc = train_vector("weight", c->weight, c->B, true, &p->weight)) return rc;
+  if (int rc = train_vector("bias", c->bias, c->B, true, &p->bias)) return rc;
+  if (int rc = train_vector("post_weight", c->post_weight, c->B, true, &p->post_weight)) return rc;
+  const unsigned x_size = c->x_dtype == KSANA_SAGE_FP32 ? 4 : 2, y_size = c->y_dtype == KSANA_SAGE_FP32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(x) % x_size || reinterpret_cast<uintptr_t>(y) % y_size) return fail(KSANA_SAGE_EINVAL, "x or y is not aligned to its type");
+  p->B = c->B;
+  p->L = c->L;
+  p->C = c->C;
+  p->x_dtype = c->x_dtype;
+  p->y_dtype = c->y_dtype;
+  p->norm = c->norm;
+  p->post = c->post;
+  p->residual_scale = c->residual_scale;
+  p->eps = c->eps;
+  p->x = x;
+  p->y = has_y ? y : nullptr;
+  p->x_sB = c->x_strides[0];
+  p->x_sL = c->x_strides[1];
+  p->y_sB = has_y ? c->y_strides[0] : 0;
+  p->y_sL = has_y ? c->y_strides[1] : 0;
+  p->wide = c->C % 8 == 0 && rows_in_pieces(x, c->x_dtype, p->x_sB, p->x_sL) && (!has_y || rows_in_pieces(y, c->y_dtype, p->y_sB, p->y_sL));
+  return 0;
+}
+// Contiguous rows the kernels write or read: 16-byte aligned (they are made of whole pieces where C is)
+int train_rows_given(const char* name, const void* p, bool may_be_null) {
+  if (!p) return may_be_null ? 0 : fail(KSANA_SAGE_EINVAL, "%s is null", name);
+  if (reinterpret_cast<uintptr_t>(p) & 15) return fail(KSANA_SAGE_EINVAL, "%s is not 16-byte aligned", name);
+  return 0;
+}
+}  // namespace
+
+extern "C" int ksana_sage_train_norm_fwd(const ksana_sage_train_norm* call, const void* x, const void* y, void* h, void* n, float* stats, void* stream) {
+  ksana_sage::TrainNormParams p;
+  if (int rc = train_norm_params(call, x, y, y != nullptr, &p)) return rc;
+  if (int rc = train_rows_given("h", h, y == nullptr)) return rc;
+  if (int rc = train_rows_given("n", n, false)) return rc;
+  if (int rc = train_rows_given("stats", stats, true)) return rc;
+  p.h = h;
+  p.n = n;
+  p.stats = stats;
+  const StageRange range("ksana_sage.train_norm_fwd");
+  const hipError_t e = ksana_sage::launch_train_norm_fwd(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "residual norm, forward");
+}
+
+extern "C" int ksana_sage_train_norm_scratch(const ksana_sage_train_norm* call, uint64_t* bytes) {
+  if (!call || !bytes) return fail(KSANA_SAGE_EINVAL, "call or bytes is null");
+  if (call->B < 1 || call->L < 1 || call->C < 1) return fail(KSANA_SAGE_EINVAL, "non-positive extent (B=%d L=%d C=%d)", call->B, call->L, call->C);
+  if (!ksana_sage::train_norm_width_fits(call->C)) return fail(KSANA_SAGE_ENOTSUP, "C=%d exceeds 8192", call->C);
+  if (call->L > (1 << 28) || call->B > (1 << 20)) return fail(KSANA_SAGE_ENOTSUP, "B=%d L=%d exceed the launch grid", call->B, call->L);
+  ksana_sage::TrainNormParams p{};
+  p.B = call->B;
+  p.L = call->L;
+  p.C = call->C;
+  *bytes = ksana_sage::train_norm_scratch(p);
+  return 0;
+}
+
+extern "C" int ksana_sage_train_norm_bwd(const ksana_sage_train_norm* call, const void* x, const void* y, const float* stats, const void* dh,
+                                         const void* dn, void* dx, void* dy, void* const grads[6], void* scratch, void* stream) {
+  ksana_sage::TrainNormParams p;
+  if (int rc = train_norm_params(call, x, y, y != nullptr, &p)) return rc;
+  if (int rc = train_rows_given("stats", stats, false)) return rc;
+  if (int rc = train_rows_given("dh", dh, true)) return rc;
+  if (int rc = train_rows_given("dn", dn, false)) return rc;
+  if (int rc = train_rows_given("dx", dx, false)) return rc;
+  if (int rc = train_rows_given("dy", dy, true)) return rc;
+  if ((y == nullptr) != (dy == nullptr)) return fail(KSANA_SAGE_EINVAL, "dy goes with y");
+  if (!grads) return fail(KSANA_SAGE_EINVAL, "grads is null");
+  const ksana_sage::TrainVector* vectors[6] = {&p.gate, &p.scale, &p.shift, &p.weight, &p.bias, &p.post_weight};
+  for (int i = 0; i < 6; ++i)
+    if (grads[i] && !vectors[i]->ptr) return fail(KSANA_SAGE_EINVAL, "a gradient is wanted of vector %d, which is absent", i);
+  uint64_t bytes = 0;
+  if (int rc = ksana_sage_train_norm_scratch(call, &bytes)) return rc;
+  if (int rc = train_scratch_given(bytes, scratch)) return rc;
+  p.stats = const_cast<float*>(stats);
+  p.dh = dh;
+  p.dn = dn;
+  p.dx = dx;
+  p.dy = dy;
+  p.d_gate = grads[0];
+  p.d_scale = grads[1];
+  p.d_shift = grads[2];
+  p.d_weight = grads[3];
+  p.d_bias = grads[4];
+  p.d_post_weight = grads[5];
+  const StageRange range("ksana_sage.train_norm_bwd");
+  const hipError_t e = ksana_sage::launch_train_norm_bwd(p, scratch, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "residual norm, backward");
+}

@@ -43,4 +43,37 @@ TrainAttnScratch train_attn_scratch(const TrainAttnParams& p, bool backward);
 hipError_t launch_train_attn_fwd(TrainAttnParams p, void* scratch, hipStream_t s);
 hipError_t launch_train_attn_bwd(TrainAttnParams p, void* scratch, hipStream_t s);
 
+
+// ---- residual sum, gate and norms ----
+
+constexpr int kFp32 = 2;                                     // next to KSANA_SAGE_BF16 and _FP16
+constexpr int kNormNone = 0, kNormLayer = 1, kNormRms = 2;
+
+struct TrainVector {  // C channels, for every batch entry (sB elements apart) or for all (sB 0)
+  const void* ptr;    // nullptr: none
+  int64_t sB;
+  int dtype;
+};
+struct TrainNormParams {
+  int B, L, C, x_dtype, y_dtype;  // y_dtype: of y, n and their gradients
+  int norm, post;
+  float residual_scale, eps;
+  const void *x, *y;              // y nullptr: h = x
+  int64_t x_sB, x_sL, y_sB, y_sL; // in elements
+  void *h, *n;                    // contiguous; h may be nullptr
+  float* stats;                   // [B, L, 4]: mean and factor of h's norm and of y's
+  TrainVector gate, scale, shift, weight, bias, post_weight;
+  const void *dh, *dn;            // contiguous; dh may be nullptr
+  void *dx, *dy;                  // contiguous; dy nullptr without y
+  void *d_gate, *d_scale, *d_shift, *d_weight, *d_bias, *d_post_weight;  // of the vectors' types, contiguous [B, C] or [C], or nullptr
+  int wide;                       // all rows are made of whole 16-byte pieces
+  // filled in by the launchers
+  int groups, rows_each;          // workgroups of a batch entry, and their rows
+  float* part;
+};
+bool train_norm_width_fits(int C);
+uint64_t train_norm_scratch(TrainNormParams p);
+hipError_t launch_train_norm_fwd(TrainNormParams p, hipStream_t s);
+hipError_t launch_train_norm_bwd(TrainNormParams p, void* scratch, hipStream_t s);
+
 }  // namespace ksana_sage

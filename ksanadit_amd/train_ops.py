@@ -125,3 +125,153 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
     else:
         o = _attention_forward(q, k, v, bool(is_causal), sm_scale, k_lens, q_lens, False)[0]
     return o.transpose(1, 2) if tensor_layout == "HND" else o
+
+
+_NORMS = {None: _capi.NORM_NONE, "layer": _capi.NORM_LAYER, "rms": _capi.NORM_RMS}
+_NORM_DTYPES = {torch.bfloat16: _capi.BF16, torch.float16: _capi.FP16, torch.float32: _capi.FP32}
+_VECTORS = ("gate", "scale", "shift", "weight", "bias", "post_weight")  # in the order of the library's structure
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``[B, L, C]`` with contiguous channels and strides the kernels take (an expanded tensor has a stride of 0, which they do)."""
+    return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned, as the kernels read gradients."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _NormCall:
+    """The library's structure for one residual norm, and what it points to."""
+
+    __slots__ = ("c", "vectors", "bwd_bytes")
+
+    def __init__(self, x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype):
+        B, L, C_ = x.shape
+        self.vectors = vectors  # (alive as long as the structure points to them)
+        args = []
+        for t in vectors:
+            args.append(_capi.Vector() if t is None else
+                        _capi.Vector(t.data_ptr(), C_ if t.dim() == 2 else 0, _NORM_DTYPES[t.dtype], 0))
+        strides = (0, 0) if y is None else y.stride()[:2]
+        self.c = _capi.TrainNorm(B, L, C_, _NORM_DTYPES[x.dtype], _NORM_DTYPES[n_dtype], _NORMS[norm], _NORMS[post_norm], residual_scale, eps, 0,
+                                 (C.c_int64 * 2)(*x.stride()[:2]), (C.c_int64 * 2)(*strides), *args)
+
+
+def _residual_norm_forward(x, y, call, n_dtype, want_stats: bool):
+    h = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = torch.empty(x.shape, dtype=n_dtype, device=x.device)
+    stats = torch.empty((*x.shape[:2], 4), dtype=torch.float32, device=x.device) if want_stats else None
+    if x.numel() == 0:
+        return h, n, stats
+    with _on(x.device):
+        rc = _capi.load().ksana_sage_train_norm_fwd(C.addressof(call.c), x.data_ptr(), _ptr(y), _ptr(h), n.data_ptr(), _ptr(stats),
+                                                    _stream_ptr(x.device))
+    _capi.check(rc, "train_ops.residual_norm")
+    return h, n, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, scale, shift, weight, bias, post_weight, norm, post_norm, residual_scale, eps, n_dtype):
+        vectors = (gate, scale, shift, weight, bias, post_weight)
+        call = _NormCall(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype)
+        h, n, stats = _residual_norm_forward(x, y, call, n_dtype, True)
+        ctx.save_for_backward(x, y, stats, *vectors)
+        ctx.call, ctx.n_dtype = call, n_dtype
+        ctx.set_materialize_grads(False)
+        return n if y is None else (h, n)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        x, y, stats, *vectors = ctx.saved_tensors
+        dh, dn = grads if y is not None else (None, grads[0])
+        if dh is None and dn is None:
+            return (None,) * 13
+        dn = torch.zeros(x.shape, dtype=ctx.n_dtype, device=x.device) if dn is None else _aligned(dn)
+        dh = None if dh is None else _aligned(dh)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dy = None if y is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        wanted = ctx.needs_input_grad[2:8]
+        d_vectors = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None for t, want in zip(vectors, wanted)]
+        if x.numel() == 0:
+            return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors), *(None,) * 5)
+        lib, call = _capi.load(), ctx.call
+        nbytes = C.c_uint64(0)
+        _capi.check(lib.ksana_sage_train_norm_scratch(C.addressof(call.c), C.addressof(nbytes)), "train_ops.residual_norm, backward")
+        with _on(x.device):
+            scratch = _scratch(nbytes.value, x.device)
+            pointers = (C.c_void_p * 6)(*(_ptr(t) for t in d_vectors))
+            rc = lib.ksana_sage_train_norm_bwd(C.addressof(call.c), x.data_ptr(), _ptr(y), stats.data_ptr(), _ptr(dh), dn.data_ptr(), dx.data_ptr(),
+                                               _ptr(dy), C.addressof(pointers), _ptr(scratch), _stream_ptr(x.device))
+        _capi.check(rc, "train_ops.residual_norm, backward")
+        return (dx, dy, *d_vectors, *(None,) * 5)
+
+
+def _norm_vector(name: str, t: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor | None:
+    """A vector as the kernels read it: ``[C]``, or ``[B, C]`` where every batch entry has its own (also given as ``[B, 1, C]``)."""
+    if t is None:
+        return None
+    B, _, C_ = x.shape
+    if t.device != x.device or t.dtype not in _NORM_DTYPES:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16 on {x.device}, got {t.dtype} on {t.device}")
+    shape = tuple(t.shape)
+    own = name in ("gate", "scale", "shift")
+    if shape == (C_,):
+        return t.contiguous()
+    if own and shape in ((1, C_), (1, 1, C_)):
+        return t.reshape(C_).contiguous()
+    if own and shape in ((B, C_), (B, 1, C_)):
+        return t.reshape(B, C_).contiguous()
+    raise ValueError(f"{name} must be [{C_}]" + (f", [{B}, {C_}] or [{B}, 1, {C_}]" if own else "") + f", got {shape}")
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, residual_scale: float = 1.0, post_norm: str | None = None,
+                  post_weight=None, norm: str = "layer", weight=None, bias=None, scale=None, shift=None, eps: float = 1e-6,
+                  out_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """What stands between two parts of a block, with gradients for every tensor: ``(h, n)`` with
+
+    ``u = post_norm(y) * post_weight``, ``h = residual_scale * x + gate * u``, ``n = (norm(h) * weight + bias) * (1 + scale) + shift``
+
+    for the residual stream ``x`` and the part's output ``y``, both ``[B, L, C]``; h goes on as the residual stream (x's type), n into the next
+    part (y's type).  ``norm`` ("layer" or "rms") and ``post_norm`` (None, "layer" or "rms") run over the channels, ``eps`` under both
+    roots.  ``gate``, ``scale`` and ``shift`` are ``[C]``, ``[B, C]`` or ``[B, 1, C]``; ``weight``, ``bias`` and ``post_weight`` ``[C]``; any of
+    them absent, each in fp32, fp16 or bf16.  Without ``y``, at a block's first part, h is x itself and n of ``out_dtype`` (x's type by
+    default, or a half type under an fp32 stream).  x and y share a type, or x is fp32.  At most 8192 channels.
+
+    Statistics and arithmetic are fp32, n comes from the unrounded h, and every result and gradient is rounded once."""
+    if x.dim() != 3 or (y is not None and y.shape != x.shape):
+        raise ValueError(f"residual_norm expects x and y of one shape [B, L, C], got {tuple(x.shape)}" + ("" if y is None else f" and {tuple(y.shape)}"))
+    if norm not in ("layer", "rms") or post_norm not in _NORMS:
+        raise ValueError(f"norm {norm!r} / post_norm {post_norm!r} unknown")
+    for t in (x,) if y is None else (x, y):
+        if not t.is_cuda:
+            raise RuntimeError(f"residual_norm needs tensors on a HIP device; there is no CPU path (got device {t.device})")
+        if t.dtype not in _NORM_DTYPES or t.device != x.device:
+            raise ValueError(f"x and y must be float32, float16 or bfloat16 on one device, got {t.dtype} on {t.device}")
+    if y is None:
+        if gate is not None or post_norm is not None or post_weight is not None or residual_scale != 1.0:
+            raise ValueError("gate, post_norm, post_weight and residual_scale go with y")
+        n_dtype = x.dtype if out_dtype is None else out_dtype
+    else:
+        n_dtype = y.dtype
+        if out_dtype not in (None, n_dtype):
+            raise ValueError(f"with y the normalised result has its type, {n_dtype}")
+    if n_dtype not in _NORM_DTYPES or n_dtype != x.dtype and x.dtype != torch.float32:
+        raise ValueError(f"x of {x.dtype} does not go with {n_dtype}")
+    if post_weight is not None and post_norm is None:
+        raise ValueError("post_weight goes with post_norm")
+    if x.shape[2] == 0:
+        raise ValueError("residual_norm needs at least one channel")
+    vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, (gate, scale, shift, weight, bias, post_weight))]
+    x_rows, y_rows = _rows(x), None if y is None else _rows(y)
+    residual_scale, eps = float(residual_scale), float(eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *vectors)):
+        out = _ResidualNorm.apply(x_rows, y_rows, *vectors, norm, post_norm, residual_scale, eps, n_dtype)
+        return (x, out) if y is None else out
+    call = _NormCall(x_rows, y_rows, vectors, norm, post_norm, residual_scale, eps, n_dtype)
+    h, n, _ = _residual_norm_forward(x_rows, y_rows, call, n_dtype, False)
+    return (x if y is None else h), n
