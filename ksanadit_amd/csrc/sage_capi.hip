@@ -1161,10 +1161,6 @@ int train_vector(const char* name, const ksana_sage_vector& v, int B, bool share
   *out = ksana_sage::TrainVector{v.ptr, v.batch_stride, v.dtype};
   return 0;
 }
-bool rows_in_pieces(const void* p, int dtype, int64_t sB, int64_t sL) {
-  const int64_t size = dtype == KSANA_SAGE_FP32 ? 4 : 2;
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && sB * size % 16 == 0 && sL * size % 16 == 0;
-}
 int train_norm_params(const ksana_sage_train_norm* c, const void* x, const void* y, bool has_y, ksana_sage::TrainNormParams* p) {
   if (!c) return fail(KSANA_SAGE_EINVAL, "call is null");
   if (c->B < 1 || c->L < 1 || c->C < 1) return fail(KSANA_SAGE_EINVAL, "non-positive extent (B=%d L=%d C=%d)", c->B, c->L, c->C);
@@ -1207,23 +1203,22 @@ int train_norm_params(const ksana_sage_train_norm* c, const void* x, const void*
   p->x_sL = c->x_strides[1];
   p->y_sB = has_y ? c->y_strides[0] : 0;
   p->y_sL = has_y ? c->y_strides[1] : 0;
-  p->wide = c->C % 8 == 0 && rows_in_pieces(x, c->x_dtype, p->x_sB, p->x_sL) && (!has_y || rows_in_pieces(y, c->y_dtype, p->y_sB, p->y_sL));
   return 0;
 }
-// Contiguous rows the kernels write or read: 16-byte aligned (they are made of whole pieces where C is)
-int train_rows_given(const char* name, const void* p, bool may_be_null) {
+int train_rows_given(const char* name, const void* p, unsigned alignment, bool may_be_null) {
   if (!p) return may_be_null ? 0 : fail(KSANA_SAGE_EINVAL, "%s is null", name);
-  if (reinterpret_cast<uintptr_t>(p) & 15) return fail(KSANA_SAGE_EINVAL, "%s is not 16-byte aligned", name);
+  if (reinterpret_cast<uintptr_t>(p) % alignment) return fail(KSANA_SAGE_EINVAL, "%s is not aligned to its type", name);
   return 0;
 }
+unsigned size_of(int dtype) { return dtype == KSANA_SAGE_FP32 ? 4 : 2; }
 }  // namespace
 
 extern "C" int ksana_sage_train_norm_fwd(const ksana_sage_train_norm* call, const void* x, const void* y, void* h, void* n, float* stats, void* stream) {
   ksana_sage::TrainNormParams p;
   if (int rc = train_norm_params(call, x, y, y != nullptr, &p)) return rc;
-  if (int rc = train_rows_given("h", h, y == nullptr)) return rc;
-  if (int rc = train_rows_given("n", n, false)) return rc;
-  if (int rc = train_rows_given("stats", stats, true)) return rc;
+  if (int rc = train_rows_given("h", h, size_of(p.x_dtype), y == nullptr)) return rc;
+  if (int rc = train_rows_given("n", n, size_of(p.y_dtype), false)) return rc;
+  if (int rc = train_rows_given("stats", stats, 16, true)) return rc;
   p.h = h;
   p.n = n;
   p.stats = stats;
@@ -1249,11 +1244,11 @@ extern "C" int ksana_sage_train_norm_bwd(const ksana_sage_train_norm* call, cons
                                          const void* dn, void* dx, void* dy, void* const grads[6], void* scratch, void* stream) {
   ksana_sage::TrainNormParams p;
   if (int rc = train_norm_params(call, x, y, y != nullptr, &p)) return rc;
-  if (int rc = train_rows_given("stats", stats, false)) return rc;
-  if (int rc = train_rows_given("dh", dh, true)) return rc;
-  if (int rc = train_rows_given("dn", dn, false)) return rc;
-  if (int rc = train_rows_given("dx", dx, false)) return rc;
-  if (int rc = train_rows_given("dy", dy, true)) return rc;
+  if (int rc = train_rows_given("stats", stats, 16, false)) return rc;
+  if (int rc = train_rows_given("dh", dh, size_of(p.x_dtype), true)) return rc;
+  if (int rc = train_rows_given("dn", dn, size_of(p.y_dtype), false)) return rc;
+  if (int rc = train_rows_given("dx", dx, size_of(p.x_dtype), false)) return rc;
+  if (int rc = train_rows_given("dy", dy, size_of(p.y_dtype), true)) return rc;
   if ((y == nullptr) != (dy == nullptr)) return fail(KSANA_SAGE_EINVAL, "dy goes with y");
   if (!grads) return fail(KSANA_SAGE_EINVAL, "grads is null");
   const ksana_sage::TrainVector* vectors[6] = {&p.gate, &p.scale, &p.shift, &p.weight, &p.bias, &p.post_weight};

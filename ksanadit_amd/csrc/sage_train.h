@@ -66,7 +66,6 @@ struct TrainNormParams {
   const void *dh, *dn;            // contiguous; dh may be nullptr
   void *dx, *dy;                  // contiguous; dy nullptr without y
   void *d_gate, *d_scale, *d_shift, *d_weight, *d_bias, *d_post_weight;  // of the vectors' types, contiguous [B, C] or [C], or nullptr
-  int wide;                       // all rows are made of whole 16-byte pieces
   // filled in by the launchers
   int groups, rows_each;          // workgroups of a batch entry, and their rows
   float* part;

@@ -32,12 +32,6 @@ template <int DT>
 constexpr int kSize = DT == kFp32 ? 4 : 2;
 
 template <int DT>
-__device__ __forceinline__ float load_one(const void* p, int64_t i) {
-  if constexpr (DT == kFp32) return static_cast<const float*>(p)[i];
-  if constexpr (DT == KSANA_SAGE_BF16) return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
-  return (float)static_cast<const _Float16*>(p)[i];
-}
-template <int DT>
 __device__ __forceinline__ void store_one(void* p, int64_t i, float x) {
   if constexpr (DT == kFp32) static_cast<float*>(p)[i] = x;
   if constexpr (DT == KSANA_SAGE_BF16) static_cast<__bf16*>(p)[i] = (__bf16)x;
@@ -45,7 +39,9 @@ __device__ __forceinline__ void store_one(void* p, int64_t i, float x) {
 }
 __device__ __forceinline__ float load_any(const TrainVector& v, int b, int c) {
   const int64_t i = b * v.sB + c;
-  return v.dtype == kFp32 ? load_one<kFp32>(v.ptr, i) : v.dtype == KSANA_SAGE_BF16 ? load_one<KSANA_SAGE_BF16>(v.ptr, i) : load_one<KSANA_SAGE_FP16>(v.ptr, i);
+  if (v.dtype == kFp32) return static_cast<const float*>(v.ptr)[i];
+  if (v.dtype == KSANA_SAGE_BF16) return __uint_as_float((uint32_t)static_cast<const uint16_t*>(v.ptr)[i] << 16);
+  return (float)static_cast<const _Float16*>(v.ptr)[i];
 }
 __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x) {
   if (dtype == kFp32)
@@ -56,33 +52,38 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x
     store_one<KSANA_SAGE_FP16>(p, i, x);
 }
 
-// A thread's columns of a row.  kWide: 16-byte accesses, column 8 (v T + thread) + e; else one by one, column (8 v + e) T + thread, T the
-// workgroup's threads (rows of a width or at addresses that 16 bytes do not divide).
-template <bool kWide, int kVecs>
+// A thread's columns of a row: 8 (v T + thread) .., T the workgroup's threads, eight at an access whatever the row's address (the GPU takes
+// 16-byte accesses at any).  kWhole: C is a multiple of eight.  Else a row's last eight columns overlap those before: both threads compute and
+// store the same values there, and sums leave out the second one's (`own`).  Value by value instead, 8331 rows of 1153 took 57 us
+// forward and 157 backward where this takes 24 and 55.
+template <bool kWhole, int kVecs>
 struct Columns {
   int C, T, thread;
-  __device__ __forceinline__ int column(int v, int e) const { return kWide ? 8 * (v * T + thread) + e : (8 * v + e) * T + thread; }
-  __device__ __forceinline__ bool has(int v, int e) const { return column(v, e) < C; }  // (kWide: C is a multiple of eight)
+  __device__ __forceinline__ int due(int v) const { return 8 * (v * T + thread); }
+  __device__ __forceinline__ bool some(int v) const { return due(v) < C; }
+  __device__ __forceinline__ int first(int v) const { return kWhole ? due(v) : max(0, min(due(v), C - 8)); }
+  __device__ __forceinline__ bool own(int v, int e) const { return kWhole ? some(v) : some(v) && first(v) + e >= due(v) && first(v) + e < C; }
 
   template <int DT>
   __device__ __forceinline__ void load(const void* row, Raw<DT> (&raw)[kVecs]) const {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
       raw[v] = Raw<DT>{};
-      if constexpr (kWide) {
-        if (!has(v, 0)) continue;
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + (int64_t)column(v, 0) * kSize<DT>);
-        raw[v].w[0] = p[0];
-        if constexpr (DT == kFp32) raw[v].w[1] = p[1];
+      if (!some(v)) continue;
+      const char* p = static_cast<const char*>(row) + (int64_t)first(v) * kSize<DT>;
+      if (kWhole || C >= 8) {
+        __builtin_memcpy(&raw[v].w[0], p, 16);
+        if constexpr (DT == kFp32) __builtin_memcpy(&raw[v].w[1], p + 16, 16);
       } else {
         uint32_t* w = reinterpret_cast<uint32_t*>(&raw[v]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!has(v, e)) continue;
+        for (int e = 0; e < C; ++e) {
+          uint32_t x;
           if constexpr (DT == kFp32)
-            w[e] = static_cast<const uint32_t*>(row)[column(v, e)];
+            x = reinterpret_cast<const uint32_t*>(p)[e];
           else
-            w[e >> 1] |= (uint32_t)static_cast<const uint16_t*>(row)[column(v, e)] << (16 * (e & 1));
+            x = (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+#pragma unroll
+          for (int i = 0; i < (DT == kFp32 ? 8 : 4); ++i) w[i] |= i == (DT == kFp32 ? e : e >> 1) ? x : 0u;
         }
       }
     }
@@ -90,40 +91,79 @@ struct Columns {
   template <int DT>
   static __device__ __forceinline__ void widen(const Raw<DT>& raw, float (&x)[8]) {
     if constexpr (DT == kFp32) {
+      const uint32_t w[8] = {raw.w[0].x, raw.w[0].y, raw.w[0].z, raw.w[0].w, raw.w[1].x, raw.w[1].y, raw.w[1].z, raw.w[1].w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(reinterpret_cast<const uint32_t*>(&raw)[e]);
+      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
     } else {
       widen8<DT>(raw.w[0], x);
     }
   }
-  template <int DT>
+  template <int DT, bool kStream = true>
   __device__ __forceinline__ void store(void* row, int v, const float (&x)[8]) const {
-    if constexpr (kWide) {
-      if (!has(v, 0)) return;
-      char* p = static_cast<char*>(row) + (int64_t)column(v, 0) * kSize<DT>;
-      if constexpr (DT == kFp32) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-      } else {
-        uint32_t w[4];
+    if (!some(v)) return;
+    char* p = static_cast<char*>(row) + (int64_t)first(v) * kSize<DT>;
+    if (kWhole || C >= 8) {
+      uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (DT == KSANA_SAGE_BF16) {
-            typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-            w[i] = __builtin_bit_cast(uint32_t, (b2){(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
-          } else {
-            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-            w[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
-          }
+      for (int i = 0; i < 8 / (4 / kSize<DT>); ++i) {
+        if constexpr (DT == kFp32) {
+          w[i] = __float_as_uint(x[i]);
+        } else if constexpr (DT == KSANA_SAGE_BF16) {
+          typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+          w[i] = __builtin_bit_cast(uint32_t, (b2){(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
+        } else {
+          typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+          w[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      // (past the caches: a gigabyte of other traffic lies between this and its next reader)
+      typedef int Piece __attribute__((ext_vector_type(4), aligned(2)));
+      const Piece lo = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+      if constexpr (kStream)
+        __builtin_nontemporal_store(lo, reinterpret_cast<Piece*>(p));
+      else
+        *reinterpret_cast<Piece*>(p) = lo;
+      if constexpr (DT == kFp32) {
+        const Piece hi = {(int)w[4], (int)w[5], (int)w[6], (int)w[7]};
+        if constexpr (kStream)
+          __builtin_nontemporal_store(hi, reinterpret_cast<Piece*>(p + 16));
+        else
+          *reinterpret_cast<Piece*>(p + 16) = hi;
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (has(v, e)) store_one<DT>(row, column(v, e), x[e]);
+      for (int e = 0; e < 7; ++e)
+        if (e < C) store_one<DT>(p, e, x[e]);
     }
   }
+  // A vector's values, `otherwise` where there is none
+  struct Vector {
+    Raw<kFp32> raw[kVecs];
+    __device__ __forceinline__ void load(const Columns& c, const TrainVector& vec, int b) {
+      if (vec.ptr == nullptr) return;
+      const char* at = static_cast<const char*>(vec.ptr) + b * vec.sB * (vec.dtype == kFp32 ? 4 : 2);
+      if (vec.dtype == kFp32) {
+        c.load<kFp32>(at, raw);
+      } else {
+        Raw<KSANA_SAGE_BF16> half[kVecs];
+        c.load<KSANA_SAGE_BF16>(at, half);
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) raw[v].w[0] = half[v].w[0];
+      }
+    }
+    __device__ __forceinline__ void values(const TrainVector& vec, float otherwise, int v, float (&x)[8]) const {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = otherwise;
+      if (vec.ptr == nullptr) return;
+      if (vec.dtype == kFp32) {
+        widen<kFp32>(raw[v], x);
+      } else if (vec.dtype == KSANA_SAGE_BF16) {
+        widen8<KSANA_SAGE_BF16>(raw[v].w[0], x);
+      } else {
+        widen8<KSANA_SAGE_FP16>(raw[v].w[0], x);
+      }
+    }
+  };
 };
 
 constexpr int kMaxThreads = 512, kMaxWaves = kMaxThreads / 64;
@@ -156,8 +196,8 @@ struct RowStats {
 };
 // Mean (layer) and 1 / sqrt(variance or mean square + eps) of a row.  The variance is the sum of the squares about each wave's own mean
 // and of what the waves' means differ by: no cancellation, and one barrier.
-template <bool kWide, int kVecs>
-__device__ __forceinline__ RowStats row_stats(const Columns<kWide, kVecs>& c, const float (&x)[kVecs][8], int kind, float eps, int waves, int& turn,
+template <bool kWhole, int kVecs>
+__device__ __forceinline__ RowStats row_stats(const Columns<kWhole, kVecs>& c, const float (&x)[kVecs][8], int kind, float eps, int waves, int& turn,
                                               float (*lds)[kMaxWaves][2]) {
   const float n = (float)c.C;
   if (kind == kNormRms) {
@@ -165,7 +205,7 @@ __device__ __forceinline__ RowStats row_stats(const Columns<kWide, kVecs>& c, co
 #pragma unroll
     for (int v = 0; v < kVecs; ++v)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) square = __fmaf_rn(x[v][e], x[v][e], square);
+      for (int e = 0; e < 8; ++e) square = c.own(v, e) ? __fmaf_rn(x[v][e], x[v][e], square) : square;
     const float all = workgroup_sums(Sums{square, 0.0f}, waves, turn, lds).a;
     return RowStats{0.0f, 1.0f / sqrtf(all / n + eps)};
   }
@@ -175,8 +215,8 @@ __device__ __forceinline__ RowStats row_stats(const Columns<kWide, kVecs>& c, co
   for (int v = 0; v < kVecs; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      sum += x[v][e];  // (columns that do not exist hold zeros)
-      own += c.has(v, e) ? 1 : 0;
+      sum += c.own(v, e) ? x[v][e] : 0.0f;
+      own += c.own(v, e) ? 1 : 0;
     }
   sum = over_lanes<Sum>(sum);
   const float count = over_lanes<Sum>((float)own);
@@ -186,7 +226,7 @@ __device__ __forceinline__ RowStats row_stats(const Columns<kWide, kVecs>& c, co
   for (int v = 0; v < kVecs; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = c.has(v, e) ? x[v][e] - wave_mean : 0.0f;
+      const float d = c.own(v, e) ? x[v][e] - wave_mean : 0.0f;
       square = __fmaf_rn(d, d, square);
     }
   square = over_lanes<Sum>(square);
@@ -220,10 +260,10 @@ __device__ __forceinline__ RowRange row_range(const TrainNormParams& p) {
   return RowRange{b, from, min(p.L, from + p.rows_each)};
 }
 
-template <int XT, int YT, bool kWide, int kVecs>
+template <int XT, int YT, bool kWhole, int kVecs>
 __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_fwd_kernel(const TrainNormParams p) {
   __shared__ float lds[2][kMaxWaves][2];
-  const Columns<kWide, kVecs> c{p.C, (int)blockDim.x, (int)threadIdx.x};
+  const Columns<kWhole, kVecs> c{p.C, (int)blockDim.x, (int)threadIdx.x};
   const int waves = (int)blockDim.x >> 6;
   int turn = 0;
   const RowRange rows = row_range(p);
@@ -231,64 +271,64 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_fwd_kernel(const 
   const char* x_at = static_cast<const char*>(p.x) + (rows.b * p.x_sB + rows.from * p.x_sL) * kSize<XT>;
   const char* y_at = static_cast<const char*>(p.y) + (rows.b * p.y_sB + rows.from * p.y_sL) * kSize<YT>;
   const bool has_y = p.y != nullptr;
-  Raw<XT> x_raw[kVecs];
-  Raw<YT> y_raw[kVecs];
-  c.template load<XT>(x_at, x_raw);
-  if (has_y) c.template load<YT>(y_at, y_raw);
-  float a[kVecs][8], t[kVecs][8], g[kVecs][8];
-#pragma unroll
-  for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      a[v][e] = 1.0f;
-      t[v][e] = 0.0f;
-      g[v][e] = has_y ? 1.0f : 0.0f;
-    }
-  auto each = [&](const TrainVector& vec, auto&& f) {
-    if (vec.ptr == nullptr) return;
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c.has(v, e)) f(v, e, load_any(vec, rows.b, c.column(v, e)));
+  // Two rows on their way while one is worked on: with one, 32760 rows of 5120 bf16 channels took 383 us, 3.5 TB/s.
+  struct Rows {
+    Raw<XT> x[kVecs];
+    Raw<YT> y[kVecs];
+  } raw[2] = {};
+  int fetched = rows.from;
+  auto fetch = [&](Rows& into) {
+    if (fetched >= rows.to) return;
+    c.template load<XT>(x_at, into.x);
+    if (has_y) c.template load<YT>(y_at, into.y);
+    x_at += p.x_sL * kSize<XT>;
+    y_at += p.y_sL * kSize<YT>;
+    ++fetched;
   };
-  each(p.weight, [&](int v, int e, float w) { a[v][e] = w; });
-  each(p.bias, [&](int v, int e, float w) { t[v][e] = w; });
-  each(p.scale, [&](int v, int e, float s) {
-    a[v][e] *= 1.0f + s;
-    t[v][e] *= 1.0f + s;
-  });
-  each(p.shift, [&](int v, int e, float s) { t[v][e] += s; });
-  each(p.gate, [&](int v, int e, float s) { g[v][e] = s; });
-  each(p.post_weight, [&](int v, int e, float s) { g[v][e] *= s; });
+  fetch(raw[0]);
+  fetch(raw[1]);
+  float a[kVecs][8], t[kVecs][8], g[kVecs][8];
+  {
+    typename Columns<kWhole, kVecs>::Vector weight, bias, scale, shift, gate, post_weight;  // (all on their way before the first is used)
+    weight.load(c, p.weight, rows.b);
+    scale.load(c, p.scale, rows.b);
+    bias.load(c, p.bias, rows.b);
+    shift.load(c, p.shift, rows.b);
+    gate.load(c, p.gate, rows.b);
+    post_weight.load(c, p.post_weight, rows.b);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      float w[8], bs[8], sc[8], sh[8], ga[8], po[8];
+      weight.values(p.weight, 1.0f, v, w);
+      scale.values(p.scale, 0.0f, v, sc);
+      bias.values(p.bias, 0.0f, v, bs);
+      shift.values(p.shift, 0.0f, v, sh);
+      gate.values(p.gate, 1.0f, v, ga);
+      post_weight.values(p.post_weight, 1.0f, v, po);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a[v][e] = w[e] * (1.0f + sc[e]);
+        t[v][e] = bs[e] * (1.0f + sc[e]) + sh[e];
+        g[v][e] = has_y ? ga[e] * po[e] : 0.0f;
+      }
+    }
+  }
   const int64_t first = (int64_t)rows.b * p.L;
-  for (int row = rows.from; row < rows.to; ++row) {
+  auto work = [&](int row, Rows& from) {
     float h[kVecs][8], y[kVecs][8];
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      c.template widen<XT>(x_raw[v], h[v]);
-      if (has_y) c.template widen<YT>(y_raw[v], y[v]);
+      c.template widen<XT>(from.x[v], h[v]);
+      c.template widen<YT>(from.y[v], y[v]);
     }
-    if (row + 1 < rows.to) {
-      x_at += p.x_sL * kSize<XT>;
-      y_at += p.y_sL * kSize<YT>;
-      c.template load<XT>(x_at, x_raw);
-      if (has_y) c.template load<YT>(y_at, y_raw);
-    }
+    fetch(from);
+    // (no norm behind the part: mean 0 and factor 1, no y: a gate of 0)
     RowStats of_y{0.0f, 1.0f};
-    if (has_y) {
-      if (p.post != kNormNone) {
-        of_y = row_stats(c, y, p.post, p.eps, waves, turn, lds);
+    if (p.post != kNormNone) of_y = row_stats(c, y, p.post, p.eps, waves, turn, lds);
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v)
+    for (int v = 0; v < kVecs; ++v)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[v][e] = c.has(v, e) ? (y[v][e] - of_y.mean) * of_y.inv : 0.0f;
-      }
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[v][e] = __fmaf_rn(g[v][e], y[v][e], p.residual_scale * h[v][e]);
-    }
+      for (int e = 0; e < 8; ++e) h[v][e] = __fmaf_rn(g[v][e], (y[v][e] - of_y.mean) * of_y.inv, p.residual_scale * h[v][e]);
     const RowStats of_h = row_stats(c, h, p.norm, p.eps, waves, turn, lds);
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -300,13 +340,17 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_fwd_kernel(const 
     }
     if (p.stats != nullptr && threadIdx.x == 0)
       *reinterpret_cast<float4*>(p.stats + 4 * (first + row)) = make_float4(of_h.mean, of_h.inv, of_y.mean, of_y.inv);
+  };
+  for (int row = rows.from; row < rows.to; row += 2) {
+    work(row, raw[0]);
+    if (row + 1 < rows.to) work(row + 1, raw[1]);
   }
 }
 
-template <int XT, int YT, bool kWide, int kVecs>
+template <int XT, int YT, bool kWhole, int kVecs>
 __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const TrainNormParams p) {
   __shared__ float lds[2][kMaxWaves][2];
-  const Columns<kWide, kVecs> c{p.C, (int)blockDim.x, (int)threadIdx.x};
+  const Columns<kWhole, kVecs> c{p.C, (int)blockDim.x, (int)threadIdx.x};
   const int waves = (int)blockDim.x >> 6;
   int turn = 0;
   const RowRange rows = row_range(p);
@@ -322,33 +366,34 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
     const char* y_at = static_cast<const char*>(p.y) + (rows.b * p.y_sB + rows.from * p.y_sL) * kSize<YT>;
     const char* dh_at = static_cast<const char*>(p.dh) + (first + rows.from) * p.C * kSize<XT>;
     const char* dn_at = static_cast<const char*>(p.dn) + (first + rows.from) * p.C * kSize<YT>;
-    Raw<XT> x_raw[kVecs], dh_raw[kVecs];
-    Raw<YT> y_raw[kVecs], dn_raw[kVecs];
+    Raw<XT> x_raw[kVecs], dh_raw[kVecs] = {};
+    Raw<YT> y_raw[kVecs] = {}, dn_raw[kVecs];
     c.template load<XT>(x_at, x_raw);
     if (has_y) c.template load<YT>(y_at, y_raw);
     if (has_dh) c.template load<XT>(dh_at, dh_raw);
     c.template load<YT>(dn_at, dn_raw);
     float4 stats = *reinterpret_cast<const float4*>(p.stats + 4 * (first + rows.from));
     float a[kVecs][8], g[kVecs][8];
+    {
+      typename Columns<kWhole, kVecs>::Vector weight, scale, gate, post_weight;
+      weight.load(c, p.weight, rows.b);
+      scale.load(c, p.scale, rows.b);
+      gate.load(c, p.gate, rows.b);
+      post_weight.load(c, p.post_weight, rows.b);
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v)
+      for (int v = 0; v < kVecs; ++v) {
+        float w[8], sc[8], ga[8], po[8];
+        weight.values(p.weight, 1.0f, v, w);
+        scale.values(p.scale, 0.0f, v, sc);
+        gate.values(p.gate, 1.0f, v, ga);
+        post_weight.values(p.post_weight, 1.0f, v, po);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        a[v][e] = 1.0f;
-        g[v][e] = has_y ? 1.0f : 0.0f;
+        for (int e = 0; e < 8; ++e) {
+          a[v][e] = w[e] * (1.0f + sc[e]);
+          g[v][e] = has_y ? ga[e] * po[e] : 0.0f;
+        }
       }
-    auto each = [&](const TrainVector& vec, auto&& f) {
-      if (vec.ptr == nullptr) return;
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c.has(v, e)) f(v, e, load_any(vec, rows.b, c.column(v, e)));
-    };
-    each(p.weight, [&](int v, int e, float w) { a[v][e] = w; });
-    each(p.scale, [&](int v, int e, float s) { a[v][e] *= 1.0f + s; });
-    each(p.gate, [&](int v, int e, float s) { g[v][e] = s; });
-    each(p.post_weight, [&](int v, int e, float s) { g[v][e] *= s; });
+    }
     const float n = (float)p.C;
     for (int row = rows.from; row < rows.to; ++row) {
       const RowStats of_h{stats.x, stats.y}, of_y{stats.z, stats.w};
@@ -357,18 +402,8 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
       for (int v = 0; v < kVecs; ++v) {
         c.template widen<XT>(x_raw[v], hat[v]);
         c.template widen<YT>(dn_raw[v], m[v]);
-        if (has_dh) {
-          c.template widen<XT>(dh_raw[v], d[v]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[v][e] = 0.0f;
-        }
-        if (has_y) {
-          c.template widen<YT>(y_raw[v], y[v]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[v][e] = 0.0f;
-        }
+        c.template widen<XT>(dh_raw[v], d[v]);
+        c.template widen<YT>(y_raw[v], y[v]);
       }
       if (row + 1 < rows.to) {
         x_at += p.x_sL * kSize<XT>;
@@ -386,16 +421,13 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
       for (int v = 0; v < kVecs; ++v)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          if (has_y) {
-            if (p.post != kNormNone) y[v][e] = c.has(v, e) ? (y[v][e] - of_y.mean) * of_y.inv : 0.0f;
-            hat[v][e] = __fmaf_rn(g[v][e], y[v][e], p.residual_scale * hat[v][e]);
-          }
-          hat[v][e] = c.has(v, e) ? (hat[v][e] - of_h.mean) * of_h.inv : 0.0f;
+          y[v][e] = (y[v][e] - of_y.mean) * of_y.inv;
+          hat[v][e] = (__fmaf_rn(g[v][e], y[v][e], p.residual_scale * hat[v][e]) - of_h.mean) * of_h.inv;
           s0[v][e] += m[v][e];
           s1[v][e] = __fmaf_rn(m[v][e], hat[v][e], s1[v][e]);
           m[v][e] *= a[v][e];
-          sums.a = __fmaf_rn(m[v][e], hat[v][e], sums.a);
-          sums.b += m[v][e];
+          sums.a = c.own(v, e) ? __fmaf_rn(m[v][e], hat[v][e], sums.a) : sums.a;
+          sums.b += c.own(v, e) ? m[v][e] : 0.0f;
         }
       sums = workgroup_sums(sums, waves, turn, lds);
       const float along = sums.a / n, mean = p.norm == kNormLayer ? sums.b / n : 0.0f;
@@ -409,7 +441,7 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
           const float through = d[v][e] * g[v][e];
           hat[v][e] = d[v][e] * p.residual_scale;
           d[v][e] = through;
-          if (c.has(v, e)) {
+          if (c.own(v, e)) {
             of_post.a = __fmaf_rn(through, y[v][e], of_post.a);
             of_post.b += through;
           }
@@ -425,10 +457,8 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
       }
 #pragma unroll
       for (int v = 0; v < kVecs; ++v) {
-        if (p.post != kNormNone) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[v][e] = of_y.inv * (d[v][e] - y_mean - y[v][e] * y_along);
-        }
+        for (int e = 0; e < 8; ++e) d[v][e] = of_y.inv * (d[v][e] - y_mean - y[v][e] * y_along);
         c.template store<YT>(static_cast<char*>(p.dy) + (first + row) * p.C * kSize<YT>, v, d[v]);
       }
     }
@@ -436,57 +466,71 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
   float* part = p.part + (int64_t)blockIdx.x * 3 * p.C;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
-    c.template store<kFp32>(part, v, s0[v]);
-    c.template store<kFp32>(part + p.C, v, s1[v]);
-    c.template store<kFp32>(part + 2 * p.C, v, kk[v]);
+    c.template store<kFp32, false>(part, v, s0[v]);
+    c.template store<kFp32, false>(part + p.C, v, s1[v]);
+    c.template store<kFp32, false>(part + 2 * p.C, v, kk[v]);
   }
 }
 
-// The workgroups' sums added up, 64 columns to a workgroup, its threads sharing the parts; and what follows from them
-constexpr int kSlots = 16;
+// The workgroups' sums added up, 16 columns to a workgroup, its 64 groups of threads sharing the parts; and what follows from the sums.
+// Bound by latency: everything a thread reads of an entry (24 values of up to 512 parts) is on its way before the first is added.
+constexpr int kJoinColumns = 16, kSlots = 64, kAtOnce = 8;
 __global__ __launch_bounds__(1024) void sage_train_norm_vectors_kernel(const TrainNormParams p) {
-  __shared__ float lds[3][kSlots][64];
-  const int lane = threadIdx.x & 63, slot = threadIdx.x >> 6, column = (int)blockIdx.x * 64 + lane;
-  const bool here = column < p.C;
+  constexpr int kWaves = kJoinColumns * kSlots / 64;
+  __shared__ float lds[2][3][kWaves][kJoinColumns];
+  const int lane = threadIdx.x % kJoinColumns, slot = threadIdx.x / kJoinColumns, column = min((int)blockIdx.x * kJoinColumns + lane, p.C - 1);
+  const bool writes = slot == 0 && (int)blockIdx.x * kJoinColumns + lane < p.C;
   float d_gate = 0.0f, d_scale = 0.0f, d_shift = 0.0f, d_weight = 0.0f, d_bias = 0.0f, d_post = 0.0f;
   for (int b = 0; b < p.B; ++b) {
+    float w = 1.0f, bias = 0.0f, s = 1.0f, gate = 1.0f, post = 1.0f;
+    if (slot == 0) {
+      if (p.weight.ptr != nullptr) w = load_any(p.weight, b, column);
+      if (p.bias.ptr != nullptr) bias = load_any(p.bias, b, column);
+      if (p.scale.ptr != nullptr) s = 1.0f + load_any(p.scale, b, column);
+      if (p.gate.ptr != nullptr) gate = load_any(p.gate, b, column);
+      if (p.post_weight.ptr != nullptr) post = load_any(p.post_weight, b, column);
+    }
+    const float* part = p.part + (int64_t)b * p.groups * 3 * p.C + column;
     float sum[3] = {};
-    if (here) {
-      const float* part = p.part + (int64_t)b * p.groups * 3 * p.C + column;
-#pragma unroll 4
-      for (int g = slot; g < p.groups; g += kSlots)
+    for (int first = slot; first < p.groups; first += kSlots * kAtOnce) {
+      float x[kAtOnce][3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) sum[i] += part[((int64_t)g * 3 + i) * p.C];
+      for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[j][i] = part[((int64_t)min(first + j * kSlots, p.groups - 1) * 3 + i) * p.C];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) sum[i] += first + j * kSlots < p.groups ? x[j][i] : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) lds[i][slot][lane] = sum[i];
-    __syncthreads();
-    if (slot == 0 && here) {
+    for (int i = 0; i < 3; ++i) {
+      sum[i] += __shfl_xor(sum[i], 16);
+      sum[i] += __shfl_xor(sum[i], 32);
+      if ((threadIdx.x & 63) < kJoinColumns) lds[b & 1][i][threadIdx.x >> 6][lane] = sum[i];
+    }
+    __syncthreads();  // (the two places alternate: one barrier an entry)
+    if (slot != 0) continue;
+    float all[3] = {};
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        sum[i] = 0.0f;
-        for (int j = 0; j < kSlots; ++j) sum[i] += lds[i][j][lane];
-      }
-      const float w = p.weight.ptr != nullptr ? load_any(p.weight, b, column) : 1.0f, bias = p.bias.ptr != nullptr ? load_any(p.bias, b, column) : 0.0f;
-      const float s = p.scale.ptr != nullptr ? 1.0f + load_any(p.scale, b, column) : 1.0f;
-      const float gate = p.gate.ptr != nullptr ? load_any(p.gate, b, column) : 1.0f;
-      const float post = p.post_weight.ptr != nullptr ? load_any(p.post_weight, b, column) : 1.0f;
-      const float of_scale = __fmaf_rn(w, sum[1], bias * sum[0]), of_gate = post * sum[2];
-      d_weight = __fmaf_rn(s, sum[1], d_weight);
-      d_bias = __fmaf_rn(s, sum[0], d_bias);
-      d_post = __fmaf_rn(gate, sum[2], d_post);
-      const int64_t at = (int64_t)b * p.C + column;
-      d_gate += of_gate;
-      d_scale += of_scale;
-      d_shift += sum[0];
-      // a vector of every batch entry's own: its gradient is complete
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) all[i] += lds[b & 1][i][v][lane];
+    const float of_gate = post * all[2], of_scale = __fmaf_rn(w, all[1], bias * all[0]);
+    const int64_t at = (int64_t)b * p.C + column;
+    if (writes) {  // vectors of every entry's own
       if (p.d_gate != nullptr && p.gate.sB != 0) store_any(p.d_gate, p.gate.dtype, at, of_gate);
       if (p.d_scale != nullptr && p.scale.sB != 0) store_any(p.d_scale, p.scale.dtype, at, of_scale);
-      if (p.d_shift != nullptr && p.shift.sB != 0) store_any(p.d_shift, p.shift.dtype, at, sum[0]);
+      if (p.d_shift != nullptr && p.shift.sB != 0) store_any(p.d_shift, p.shift.dtype, at, all[0]);
     }
-    __syncthreads();
+    d_gate += of_gate;
+    d_scale += of_scale;
+    d_shift += all[0];
+    d_weight = __fmaf_rn(s, all[1], d_weight);
+    d_bias = __fmaf_rn(s, all[0], d_bias);
+    d_post = __fmaf_rn(gate, all[2], d_post);
   }
-  if (slot != 0 || !here) return;
+  if (!writes) return;
   if (p.d_gate != nullptr && p.gate.sB == 0) store_any(p.d_gate, p.gate.dtype, column, d_gate);
   if (p.d_scale != nullptr && p.scale.sB == 0) store_any(p.d_scale, p.scale.dtype, column, d_scale);
   if (p.d_shift != nullptr && p.shift.sB == 0) store_any(p.d_shift, p.shift.dtype, column, d_shift);
@@ -508,26 +552,27 @@ NormShape norm_shape(int C) {
   return NormShape{0, 0};
 }
 
-// Workgroups of a batch entry and their rows: about `places` workgroups in all, which the GPU holds at once
-void deal_rows(TrainNormParams& p, int places) {
+// Workgroups of a batch entry and their rows: about as many workgroups in all as the GPU holds at once.  Its 256 compute units hold 16
+// and 12 waves each of the forward kernels with one and two pieces to a thread, 12 and 8 of the backward kernels.
+void deal_rows(TrainNormParams& p, bool backward) {
+  const NormShape shape = norm_shape(p.C);
+  const int waves = shape.threads / 64, room = (shape.vecs == 1 ? 16 : 12) - (backward ? 4 : 0), places = 256 * std::max(1, room / waves);
   const int groups = std::max(1, std::min(p.L, places / p.B));
   p.rows_each = (p.L + groups - 1) / groups;
   p.groups = (p.L + p.rows_each - 1) / p.rows_each;
 }
-int fwd_places(const TrainNormParams& p) { return 256 * std::max(1, 1024 / norm_shape(p.C).threads); }
-int bwd_places(const TrainNormParams& p) { return 256 * std::max(1, 512 / norm_shape(p.C).threads); }
 
-template <int XT, int YT, bool kWide, int kVecs>
+template <int XT, int YT, bool kWhole, int kVecs>
 void start(const TrainNormParams& p, bool backward, hipStream_t s) {
   const dim3 grid((unsigned)(p.B * p.groups)), block(norm_shape(p.C).threads);
   if (backward)
-    sage_train_norm_bwd_kernel<XT, YT, kWide, kVecs><<<grid, block, 0, s>>>(p);
+    sage_train_norm_bwd_kernel<XT, YT, kWhole, kVecs><<<grid, block, 0, s>>>(p);
   else
-    sage_train_norm_fwd_kernel<XT, YT, kWide, kVecs><<<grid, block, 0, s>>>(p);
+    sage_train_norm_fwd_kernel<XT, YT, kWhole, kVecs><<<grid, block, 0, s>>>(p);
 }
 template <int XT, int YT>
 void start(const TrainNormParams& p, bool backward, hipStream_t s) {
-  switch (norm_shape(p.C).vecs + (p.wide ? 0 : 4)) {
+  switch (norm_shape(p.C).vecs + (p.C % 8 == 0 ? 0 : 4)) {
     case 1: return start<XT, YT, true, 1>(p, backward, s);
     case 2: return start<XT, YT, true, 2>(p, backward, s);
     case 5: return start<XT, YT, false, 1>(p, backward, s);
@@ -553,21 +598,21 @@ hipError_t launch(const TrainNormParams& p, bool backward, hipStream_t s) {
 bool train_norm_width_fits(int C) { return norm_shape(C).vecs != 0; }
 
 uint64_t train_norm_scratch(TrainNormParams p) {
-  deal_rows(p, bwd_places(p));
+  deal_rows(p, true);
   return (uint64_t)p.B * p.groups * 3 * p.C * 4;
 }
 
 hipError_t launch_train_norm_fwd(TrainNormParams p, hipStream_t s) {
-  deal_rows(p, fwd_places(p));
+  deal_rows(p, false);
   return launch(p, false, s);
 }
 
 hipError_t launch_train_norm_bwd(TrainNormParams p, void* scratch, hipStream_t s) {
-  deal_rows(p, bwd_places(p));
+  deal_rows(p, true);
   p.part = static_cast<float*>(scratch);
   const hipError_t e = launch(p, true, s);
   if (e != hipSuccess) return e;
-  sage_train_norm_vectors_kernel<<<(p.C + 63) / 64, 64 * kSlots, 0, s>>>(p);
+  sage_train_norm_vectors_kernel<<<(p.C + kJoinColumns - 1) / kJoinColumns, kJoinColumns * kSlots, 0, s>>>(p);
   return hipGetLastError();
 }
 

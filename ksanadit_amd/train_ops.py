@@ -129,18 +129,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
 
 _NORMS = {None: _capi.NORM_NONE, "layer": _capi.NORM_LAYER, "rms": _capi.NORM_RMS}
 _NORM_DTYPES = {torch.bfloat16: _capi.BF16, torch.float16: _capi.FP16, torch.float32: _capi.FP32}
+_NO_VECTOR = _capi.Vector()
 _VECTORS = ("gate", "scale", "shift", "weight", "bias", "post_weight")  # in the order of the library's structure
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``[B, L, C]`` with contiguous channels and strides the kernels take (an expanded tensor has a stride of 0, which they do)."""
     return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned, as the kernels read gradients."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class _NormCall:
@@ -153,8 +148,8 @@ class _NormCall:
         self.vectors = vectors  # (alive as long as the structure points to them)
         args = []
         for t in vectors:
-            args.append(_capi.Vector() if t is None else
-                        _capi.Vector(t.data_ptr(), C_ if t.dim() == 2 else 0, _NORM_DTYPES[t.dtype], 0))
+            args.append(_NO_VECTOR if t is None else
+                        _capi.Vector(t.data_ptr(), t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else 0, _NORM_DTYPES[t.dtype], 0))
         strides = (0, 0) if y is None else y.stride()[:2]
         self.c = _capi.TrainNorm(B, L, C_, _NORM_DTYPES[x.dtype], _NORM_DTYPES[n_dtype], _NORMS[norm], _NORMS[post_norm], residual_scale, eps, 0,
                                  (C.c_int64 * 2)(*x.stride()[:2]), (C.c_int64 * 2)(*strides), *args)
@@ -191,8 +186,8 @@ class _ResidualNorm(torch.autograd.Function):
         dh, dn = grads if y is not None else (None, grads[0])
         if dh is None and dn is None:
             return (None,) * 13
-        dn = torch.zeros(x.shape, dtype=ctx.n_dtype, device=x.device) if dn is None else _aligned(dn)
-        dh = None if dh is None else _aligned(dh)
+        dn = torch.zeros(x.shape, dtype=ctx.n_dtype, device=x.device) if dn is None else dn.contiguous()
+        dh = None if dh is None else dh.contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dy = None if y is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
         wanted = ctx.needs_input_grad[2:8]
@@ -212,7 +207,8 @@ class _ResidualNorm(torch.autograd.Function):
 
 
 def _norm_vector(name: str, t: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor | None:
-    """A vector as the kernels read it: ``[C]``, or ``[B, C]`` where every batch entry has its own (also given as ``[B, 1, C]``)."""
+    """A vector as the kernels read it, its channels contiguous: ``[C]``, or ``[B, C]`` / ``[B, 1, C]`` with one for every batch entry or
+    one for all of them (also slices of such a tensor, whose entries lie further apart)."""
     if t is None:
         return None
     B, _, C_ = x.shape
@@ -220,13 +216,11 @@ def _norm_vector(name: str, t: torch.Tensor | None, x: torch.Tensor) -> torch.Te
         raise ValueError(f"{name} must be float32, float16 or bfloat16 on {x.device}, got {t.dtype} on {t.device}")
     shape = tuple(t.shape)
     own = name in ("gate", "scale", "shift")
-    if shape == (C_,):
+    if shape != (C_,) and not (own and shape in ((B, C_), (1, C_), (B, 1, C_), (1, 1, C_))):
+        raise ValueError(f"{name} must be [{C_}]" + (f", [{B}, {C_}] or [{B}, 1, {C_}]" if own else "") + f", got {shape}")
+    if (C_ > 1 and t.stride(-1) != 1) or (len(shape) > 1 and shape[0] > 1 and t.stride(0) <= 0):
         return t.contiguous()
-    if own and shape in ((1, C_), (1, 1, C_)):
-        return t.reshape(C_).contiguous()
-    if own and shape in ((B, C_), (B, 1, C_)):
-        return t.reshape(B, C_).contiguous()
-    raise ValueError(f"{name} must be [{C_}]" + (f", [{B}, {C_}] or [{B}, 1, {C_}]" if own else "") + f", got {shape}")
+    return t
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, residual_scale: float = 1.0, post_norm: str | None = None,
