@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace ksana_sage {
 
@@ -68,153 +69,177 @@ __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + 
 
 // ------------------------------------------------------------------------------------------------------------ forward
 
-template <int DT, int D, int kCols>
-__global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_fwd_kernel(const TrainAttnParams p) {
+// A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys, two waves to a SIMD.  While the
+// probabilities of tile t are formed and multiplied with its values, the scores of tile t + 1 are: a few vector instructions stand behind
+// every matrix instruction and run beside it.  So values are wanted a step after their keys; each have two places in LDS.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void sage_train_fwd_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
-  constexpr int kWaves = 4, kRowsWg = kWaves * 32 * kCols, kStages = 2;
+  constexpr int kWaves = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
-  const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
+  const int all_rows = p.Lq * p.group, blocks = (all_rows + kTrainBlock - 1) / kTrainBlock;
   const TrainPlace place = train_place(p, blocks);
   const int bh = place.bh, block = blocks - 1 - place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
-  const int row0 = block * kRowsWg;
+  const int row0 = block * kTrainBlock;
   const TileRange range = run_tiles(p, place, 0, key_tiles_of(p, e, row0));
   if (place.run >= range.runs) return;
 
-  const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
-  const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
   const unsigned lds = lds_base();
-  v16f acc[kCols][T::kBlocks];
-  float top[kCols], minus[kCols], sum[kCols];  // reference point of the row (unscaled), what is added to its scaled scores, its sum
+  v16f acc[T::kBlocks];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    top[n] = -INFINITY;
-    minus[n] = kForwardShift<DT>;
-    sum[n] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < T::kBlocks; ++d) acc[n][d] = v16f{};
-  }
-  int row[kCols], limit[kCols];
-#pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    row[n] = row0 + (wave * kCols + n) * 32 + m;
-    limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
-  }
+  for (int d = 0; d < T::kBlocks; ++d) acc[d] = v16f{};
+  float top = -INFINITY, minus = kForwardShift<DT>, sum = 0.0f;  // reference point (unscaled), what is added to scaled scores, the row's sum
+  const int row = row0 + wave * 32 + m;
   if (range.from < range.to) {
-    const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
-    auto copy = [&](int t) {
-      const int at = min(t, range.to - 1) * kTrainTile;
-      const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
-      k_copy.start(at, e.keys, stage, wave, lane);
-      v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
-    };
-    copy(range.from);
-    v4i q[kCols][T::kSteps];
-#pragma unroll
-    for (int n = 0; n < kCols; ++n)
-      load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, min(row[n], e.rows - 1)), hh, p.flip, q[n]);
+    const TileCopy<D, kWaves> k_copy(p.k + b * p.ks.sB + hk * p.ks.sH, p.ks.sL, wave, lane), v_copy(p.v + b * p.vs.sB + hk * p.vs.sH, p.vs.sL, wave, lane);
+    auto k_tile = [&](int t) { return lds + (t & 1) * T::kBytes; };
+    auto v_tile = [&](int t) { return lds + (2 + (t & 1)) * T::kBytes; };
+    auto copy_keys = [&](int t) { k_copy.start(min(t, range.to - 1) * kTrainTile, e.keys, k_tile(t), wave, lane); };
+    auto copy_values = [&](int t) { v_copy.start(min(t, range.to - 1) * kTrainTile, e.keys, v_tile(t), wave, lane); };
+    copy_keys(range.from);
+    v4i q[T::kSteps];
+    load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, min(row, e.rows - 1)), hh, p.flip, q);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
-    // keys that every row of the wave sees
-    const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
-    const bool idle = row0 + wave * 32 * kCols >= e.rows;  // a wave without rows copies its share
-    const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
-#pragma unroll 1
-    for (int t = range.from; t < range.to; ++t) {
+    const int limit = p.causal ? min(e.keys, row_position(p, row) + 1) : e.keys;  // keys that the row sees, and that all of the wave see
+    const int all_see = p.causal ? min(e.keys, row_position(p, min(row0 + wave * 32, e.rows - 1)) + 1) : e.keys;
+    const bool idle = row0 + wave * 32 >= e.rows;  // a wave without rows copies its share
+    float most = -INFINITY;
+    auto hide = [&](int t, v16f (&s)[2]) {
+      if ((t + 1) * kTrainTile <= all_see) return;
+      int left = limit - t * kTrainTile - 4 * hh;
+      pin(left);  // (a branch that stays one: 64 instructions for every tile otherwise)
+      float x = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[h][i] = 32 * h + acc_row(i) < left ? s[h][i] : -INFINITY;
+        x = largest(x, s[0][i], s[1][i]);
+      }
+      most = x;
+    };
+    // Tile t: its scores in s, the largest of the lane's in `most`; forms the scores of tile t + 1 in `next` unless `last`.
+    auto step = [&](int t, v16f (&s)[2], v16f (&next)[2], auto last) {
       tile_ready<0>();
-      copy(t + 1);
-      if (idle) continue;
-      const unsigned k_tile = lds + (t % kStages) * 2 * T::kBytes, v_tile = k_tile + T::kBytes;
-      v16f s[kCols][2];
+      copy_values(t + 1);
+      if constexpr (!last.value) copy_keys(t + 2);
+      if (idle) return;
+      const float here = over_halves<Max>(most);
+      if (__any(here * p.c > kLazy + kForwardShift<DT> - minus || (top == -INFINITY && here > -INFINITY))) {
+        const float at = fmaxf(top, here);
+        const float factor = top == -INFINITY ? 0.0f : fast_exp2((top - at) * p.c);
+        top = at;
+        minus = at == -INFINITY ? kForwardShift<DT> : kForwardShift<DT> - at * p.c;
+        sum *= factor;
 #pragma unroll
-      for (int n = 0; n < kCols; ++n) s[n][0] = s[n][1] = v16f{};
+        for (int d = 0; d < T::kBlocks; ++d)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = read_row<D>(k_tile + row_at, h, st);
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) s[n][h] = mfma16<DT>(a, q[n][st], s[n][h]);
-        }
-      if ((t + 1) * kTrainTile > all_see) {
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-          int left = limit[n] - t * kTrainTile - 4 * hh;
-          pin(left);  // (a branch that stays one: 64 instructions for every tile otherwise)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[n][h][i] = 32 * h + acc_row(i) < left ? s[n][h][i] : -INFINITY;
-        }
+          for (int i = 0; i < 16; ++i) acc[d][i] *= factor;
       }
-      float most[kCols];
-      bool move = false;
+      unsigned k_at = k_tile(t + 1) + row_at, v_at = v_tile(t) + column_at;
+      pin(k_at);  // (one address and constants, not sixteen)
+      pin(v_at);
+      v4i pr[4];
+      {
+        constexpr int kParts = 2 * T::kSteps, kEach = 32 / kParts, kAhead = 3;
+        v4i a[kAhead];
+        if constexpr (!last.value) {
 #pragma unroll
-      for (int n = 0; n < kCols; ++n) {
-        float x = s[n][0][0];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x = largest(x, s[n][0][i], s[n][1][i]);
-        most[n] = over_halves<Max>(x);
-        move = move || most[n] * p.c > kLazy + kForwardShift<DT> - minus[n] || (top[n] == -INFINITY && most[n] > -INFINITY);
-      }
-      if (__any(move)) {
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-          const float next = fmaxf(top[n], most[n]);
-          const float factor = next == -INFINITY ? 1.0f : fast_exp2((top[n] - next) * p.c);
-          top[n] = next;
-          minus[n] = next == -INFINITY ? kForwardShift<DT> : kForwardShift<DT> - next * p.c;
-          sum[n] *= factor;
-#pragma unroll
-          for (int d = 0; d < T::kBlocks; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[n][d][i] *= factor;
+          for (int i = 0; i < kAhead; ++i) a[i] = read_row<D>(k_at, i / T::kSteps, i % T::kSteps);
+          next[0] = next[1] = v16f{};
         }
-      }
-      v4i pr[kCols][4];
+        float x[32];
 #pragma unroll
-      for (int n = 0; n < kCols; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            x[i] = fast_exp2(__fmaf_rn(s[n][h][i], p.c, minus[n]));
-            sum[n] += x[i];
+        for (int i = 0; i < kParts; ++i) {
+          if constexpr (!last.value) {
+            const int h = i / T::kSteps, j = i + kAhead;
+            next[h] = mfma16<DT>(a[i % kAhead], q[i % T::kSteps], next[h]);
+            if (j < kParts) a[i % kAhead] = read_row<D>(k_at, j / T::kSteps, j % T::kSteps);
           }
-          pr[n][2 * h] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
-          pr[n][2 * h + 1] = pack8<DT>(x[8], x[9], x[10], x[11], x[12], x[13], x[14], x[15]);
+#pragma unroll
+          for (int j = i * kEach; j < (i + 1) * kEach; ++j) x[j] = fast_exp2(__fmaf_rn(s[j / 16][j % 16], p.c, minus));
+#pragma unroll
+          for (int j = (i - 1) * kEach; j < i * kEach; ++j)
+            if (j >= 0) sum += x[j];
+          pin(sum);  // (added up here, not later with all of x held for it)
+          if (i * kEach % 8 == 0 && i > 0) {
+            const int f = i * kEach / 8 - 1;
+            pr[f] = pack8<DT>(x[8 * f], x[8 * f + 1], x[8 * f + 2], x[8 * f + 3], x[8 * f + 4], x[8 * f + 5], x[8 * f + 6], x[8 * f + 7]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-      for (int st = 0; st < 4; ++st)
+        for (int j = 32 - kEach; j < 32; ++j) sum += x[j];
+        pr[3] = pack8<DT>(x[24], x[25], x[26], x[27], x[28], x[29], x[30], x[31]);
+      }
+      {
+        constexpr int kParts = 4 * T::kBlocks, kEach = 16 / kParts, kAhead = 3;
+        v4i a[kAhead];
 #pragma unroll
-        for (int d = 0; d < T::kBlocks; ++d) {
-          const v4i a = read_column<D>(v_tile + column_at, d, st);
+        for (int i = 0; i < kAhead; ++i) a[i] = read_column<D>(v_at, i % T::kBlocks, i / T::kBlocks);
+        float x = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < kCols; ++n) acc[n][d] = mfma16<DT>(a, pr[n][st], acc[n][d]);
+        for (int i = 0; i < kParts; ++i) {
+          const int j = i + kAhead;
+          acc[i % T::kBlocks] = mfma16<DT>(a[i % kAhead], pr[i / T::kBlocks], acc[i % T::kBlocks]);
+          if (j < kParts) a[i % kAhead] = read_column<D>(v_at, j % T::kBlocks, j / T::kBlocks);
+          if constexpr (!last.value) {
+#pragma unroll
+            for (int l = i * kEach; l < (i + 1) * kEach; ++l) x = largest(x, next[0][l], next[1][l]);
+            pin(x);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
+        most = x;
+      }
+      if constexpr (!last.value) hide(t + 1, next);
+    };
+    typedef std::integral_constant<bool, false> More;
+    typedef std::integral_constant<bool, true> Last;
+    v16f s0[2], s1[2];
+    tile_ready<0>();
+    copy_keys(range.from + 1);
+    copy_values(range.from);
+    if (!idle) {
+      s0[0] = s0[1] = v16f{};
+#pragma unroll
+      for (int i = 0; i < 2 * T::kSteps; ++i)
+        s0[i / T::kSteps] = mfma16<DT>(read_row<D>(k_tile(range.from) + row_at, i / T::kSteps, i % T::kSteps), q[i % T::kSteps], s0[i / T::kSteps]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = largest(most, s0[0][i], s0[1][i]);
+      hide(range.from, s0);
+    }
+    int t = range.from;
+#pragma unroll 1
+    for (; t + 2 < range.to; t += 2) {
+      step(t, s0, s1, More{});
+      step(t + 1, s1, s0, More{});
+    }
+    if (t + 1 < range.to) {
+      step(t, s0, s1, More{});
+      step(t + 1, s1, s0, Last{});
+    } else {
+      step(t, s0, s1, Last{});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup's LDS
   }
-#pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    const bool takes_part = row[n] < e.rows, exists = row[n] < all_rows;
-    const float total = over_halves<Sum>(sum[n]);
-    const float factor = !takes_part || total == 0.0f ? 0.0f : 1.0f / total;
-    const int r = min(row[n], all_rows - 1), l = row_position(p, r), h = hk * p.group + r - l * p.group;
-    if (range.runs > 1) {
-      const int64_t at = ((int64_t)place.cut * p.runs + place.run) * kTrainBlock + row[n] - row0;
-      store_column_part<D>(acc[n], 1.0f, p.part + at * D, hh, takes_part);
-      if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.cut * p.runs * kTrainBlock * D + 2 * at) = make_float2(minus[n], total);
-      continue;
-    }
-    if (!takes_part) {
-#pragma unroll
-      for (int d = 0; d < T::kBlocks; ++d) acc[n][d] = v16f{};
-    }
-    store_column<DT, D>(acc[n], factor, p.o + b * p.os.sB + l * p.os.sL + h * p.os.sH, hh, exists);
-    if (exists && hh == 0 && p.lse != nullptr)
-      p.lse[((int64_t)b * p.Hq + h) * p.Lq + l] = factor == 0.0f ? -INFINITY : (log2f(total) - minus[n]) * kLn2;
+  const bool takes_part = row < e.rows, exists = row < all_rows;
+  const float total = over_halves<Sum>(sum);
+  const float factor = !takes_part || total == 0.0f ? 0.0f : 1.0f / total;
+  const int r = min(row, all_rows - 1), l = row_position(p, r), h = hk * p.group + r - l * p.group;
+  if (range.runs > 1) {
+    const int64_t at = ((int64_t)place.cut * p.runs + place.run) * kTrainBlock + row - row0;
+    store_column_part<D>(acc, 1.0f, p.part + at * D, hh, takes_part);
+    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.cut * p.runs * kTrainBlock * D + 2 * at) = make_float2(minus, total);
+    return;
   }
+  if (!takes_part) {
+#pragma unroll
+    for (int d = 0; d < T::kBlocks; ++d) acc[d] = v16f{};
+  }
+  store_column<DT, D>(acc, factor, p.o + b * p.os.sB + l * p.os.sL + h * p.os.sH, hh, exists);
+  if (exists && hh == 0 && p.lse != nullptr)
+    p.lse[((int64_t)b * p.Hq + h) * p.Lq + l] = factor == 0.0f ? -INFINITY : (log2f(total) - minus) * kLn2;
 }
 
 // ------------------------------------------------------------------------------------------------------------ backward
@@ -737,7 +762,7 @@ struct LdsRequest {
 void fill_in(TrainAttnParams& p) {
   p.group = p.Hq / p.Hkv;
   p.group_inv = (unsigned)((UINT64_C(0x100000000) + p.group - 1) / p.group);
-  p.c = fabsf(p.sm_scale) * kLog2e;
+  p.c = std::max(fabsf(p.sm_scale) * kLog2e, 1.2e-38f);  // (times -infinity, where a score is hidden, still that)
   p.flip = p.sm_scale < 0.0f ? 0x80008000u : 0u;
   p.row_pad = (p.Lq * p.group + kTrainTile - 1) / kTrainTile * kTrainTile;
   p.norm_q_blocks = (p.row_pad + kNormRows - 1) / kNormRows;
@@ -799,12 +824,11 @@ constexpr int kManyRuns = 16;  // from here on lanes share a row's runs
 
 template <int DT, int D>
 hipError_t fwd(TrainAttnParams p, hipStream_t s) {
-  constexpr int kCols = 1, kLds = 2 * 2 * Tile<D>::kBytes;
-  static_assert(kTrainBlock == 128 * kCols);
+  constexpr int kLds = 4 * Tile<D>::kBytes;
   static LdsRequest request;
-  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D, kCols>), kLds);
+  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_train_fwd_kernel<DT, D>), kLds);
   if (e != hipSuccess) return e;
-  sage_train_fwd_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+  sage_train_fwd_kernel<DT, D><<<workgroups(p), 256, kLds, s>>>(p);
   if (p.runs > 1) {
     constexpr int kLanes = D / 8;
     const int rows = joined_rows((int64_t)p.Lq * p.group), groups = (rows * kLanes + 255) / 256;  // workgroups of a block
