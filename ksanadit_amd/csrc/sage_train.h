@@ -22,6 +22,7 @@ struct TrainAttnParams {
   // filled in by the launchers
   int group;            // Hq / Hkv
   unsigned group_inv;   // ceil(2^32 / group)
+  int group_shift;      // log2(group) for powers of two up to 16, else -1
   float c;              // |sm_scale| log2(e)
   uint32_t flip;        // sign bits of two 16-bit values where sm_scale is negative
   int row_pad;          // rows of row_l and row_d of a key head: Lq * group up to a multiple of 64

@@ -244,6 +244,10 @@ __global__ __launch_bounds__(256, 2) void sage_train_fwd_kernel(const TrainAttnP
 
 // ------------------------------------------------------------------------------------------------------------ backward
 
+template <int DT>
+__device__ __forceinline__ float row_minus(float lse) {
+  return lse == -INFINITY ? -INFINITY : kBackwardShift<DT> - lse * kLog2e;
+}
 constexpr int kNormRows = 64;  // rows of a workgroup (256 and a loop: 18.8 us of 40 heads of 1560 rows where this takes 8)
 
 // Per query row -log2(e) lse (plus the shift) and -sum(dO o); in fp16 besides the largest squared norms of rows of dO and of v per block of rows.
@@ -285,7 +289,7 @@ __global__ __launch_bounds__(256) void sage_train_rows_kernel(const TrainAttnPar
         if (r < e.rows) {
           const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
           const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + l];
-          minus = lse == -INFINITY ? -INFINITY : kBackwardShift<DT> - lse * kLog2e;
+          minus = row_minus<DT>(lse);
         }
         p.row_l[(int64_t)bh * p.row_pad + r] = minus;
         p.row_d[(int64_t)bh * p.row_pad + r] = -d;
@@ -370,14 +374,14 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
   if (range.from < range.to) {
     const uint16_t* q_heads = p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH;
     const uint16_t* do_heads = p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH;
-    const TileCopy<D, kWaves> q_copy(q_heads, p.qs.sL, wave, lane), do_copy(do_heads, p.dos.sL, wave, lane);
+    const QueryCopy<D, kWaves> q_copy(p, q_heads, p.qs, lane), do_copy(p, do_heads, p.dos, lane);
     const float* row_l = p.row_l + (int64_t)bh * p.row_pad;
     const float* row_d = p.row_d + (int64_t)bh * p.row_pad;
     auto copy = [&](int t) {
       const int at = min(t, range.to - 1) * kTrainTile;
       const unsigned stage = lds + (t % kStages) * kStage;
-      q_copy.start_grouped(p, p.qs, at, e.rows, stage, wave, lane);
-      do_copy.start_grouped(p, p.dos, at, e.rows, stage + T::kBytes, wave, lane);
+      q_copy.start(p, at, e.rows, stage, wave, lane);
+      do_copy.start(p, at, e.rows, stage + T::kBytes, wave, lane);
       // (two waves each, so that every wave has as many copies in flight)
       lds_copy4_at((wave & 1 ? row_d : row_l) + at, lane * 4, stage + 2 * T::kBytes + (wave & 1) * kTrainTile * 4);
     };
@@ -528,6 +532,10 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
   for (int n = 0; n < kCols; ++n) {
     row[n] = row0 + (wave * kCols + n) * 32 + m;
     limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
+    if (!kHalf && place.run == 0 && row[n] >= e.rows && row[n] < p.row_pad && hh == 0) {
+      p.row_l[(int64_t)bh * p.row_pad + row[n]] = -INFINITY;
+      p.row_d[(int64_t)bh * p.row_pad + row[n]] = 0.0f;
+    }
   }
   if (range.from < range.to) {
     const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
@@ -545,8 +553,30 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(
       const int r = min(row[n], e.rows - 1);
       load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, r), hh, p.flip, q[n]);
       load_row<D>(p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH + row_offset(p, p.dos, r), hh, 0, g[n]);
-      l[n] = p.row_l[(int64_t)bh * p.row_pad + r];
-      d[n] = p.row_d[(int64_t)bh * p.row_pad + r];
+      if constexpr (kHalf) {
+        l[n] = p.row_l[(int64_t)bh * p.row_pad + r];
+        d[n] = p.row_d[(int64_t)bh * p.row_pad + r];
+      } else {
+        // dO is here: what sage_train_rows_kernel would have to read it once more for is formed on the way, and kept for dk and dv
+        const int at = row_position(p, r), h = hk * p.group + r - at * p.group;
+        const uint16_t* o = p.o_in + b * p.os.sB + at * p.os.sL + h * p.os.sH + 8 * hh;
+        const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + at];
+        float sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < T::kSteps; ++s) {
+          float x[8], y[8];
+          widen8<DT>(*reinterpret_cast<const uint4*>(o + 16 * s), x);
+          widen8<DT>(__builtin_bit_cast(uint4, g[n][s]), y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum = __fmaf_rn(x[j], y[j], sum);
+        }
+        l[n] = row_minus<DT>(lse);
+        d[n] = -over_halves<Sum>(sum);
+        if (place.run == 0 && hh == 0 && row[n] < e.rows) {
+          p.row_l[(int64_t)bh * p.row_pad + row[n]] = l[n];
+          p.row_d[(int64_t)bh * p.row_pad + row[n]] = d[n];
+        }
+      }
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
@@ -762,6 +792,7 @@ struct LdsRequest {
 void fill_in(TrainAttnParams& p) {
   p.group = p.Hq / p.Hkv;
   p.group_inv = (unsigned)((UINT64_C(0x100000000) + p.group - 1) / p.group);
+  p.group_shift = p.group <= 16 && (p.group & (p.group - 1)) == 0 ? __builtin_ctz((unsigned)p.group) : -1;
   p.c = std::max(fabsf(p.sm_scale) * kLog2e, 1.2e-38f);  // (times -infinity, where a score is hidden, still that)
   p.flip = p.sm_scale < 0.0f ? 0x80008000u : 0u;
   p.row_pad = (p.Lq * p.group + kTrainTile - 1) / kTrainTile * kTrainTile;
@@ -853,29 +884,33 @@ void join_bwd(const TrainAttnParams& p, int64_t all, hipStream_t s) {
 
 template <int DT, int D>
 hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
-  sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, p.B * p.Hkv), 256, 0, s>>>(p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
   constexpr int kCols = 1;
-  if (p.dk != nullptr) {
-    constexpr int kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
-    static LdsRequest request;
-    e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
-    if (e != hipSuccess) return e;
-    take_cut(p, cuts.dkv);
-    sage_train_dkv_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
-    join_bwd<DT, D, true>(p, p.Lk, s);
+  hipError_t e = hipSuccess;
+  // in bf16 the rows' numbers come along with dq, where that is wanted
+  if (DT == KSANA_SAGE_FP16 || p.dq == nullptr) {
+    sage_train_rows_kernel<DT, D><<<dim3(p.norm_blocks, p.B * p.Hkv), 256, 0, s>>>(p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  if (p.dq == nullptr) return hipSuccess;
-  constexpr int kLds = 2 * 2 * Tile<D>::kBytes;
+  if (p.dq != nullptr) {
+    constexpr int kLds = 2 * 2 * Tile<D>::kBytes;
+    static LdsRequest request;
+    e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);
+    if (e != hipSuccess) return e;
+    take_cut(p, cuts.dq);
+    sage_train_dq_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+    join_bwd<DT, D, false>(p, (int64_t)p.Lq * p.group, s);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (p.dk == nullptr) return hipSuccess;
+  constexpr int kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
   static LdsRequest request;
-  e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);
+  e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
   if (e != hipSuccess) return e;
-  take_cut(p, cuts.dq);
-  sage_train_dq_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
-  join_bwd<DT, D, false>(p, (int64_t)p.Lq * p.group, s);
+  take_cut(p, cuts.dkv);
+  sage_train_dkv_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+  join_bwd<DT, D, true>(p, p.Lk, s);
   return hipGetLastError();
 }
 
