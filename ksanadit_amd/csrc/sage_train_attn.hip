@@ -504,159 +504,161 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
   }
 }
 
-template <int DT, int D, int kCols>
-__global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dq_kernel(const TrainAttnParams p) {
+// A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
+// k^T dS^T.  A half's vector work stands behind matrix instructions of the other half.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
-  constexpr int kWaves = 4, kRowsWg = kWaves * 32 * kCols, kStages = 2;
+  constexpr int kWaves = 4;
   constexpr bool kHalf = DT == KSANA_SAGE_FP16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
-  const int all_rows = p.Lq * p.group, blocks = (all_rows + kRowsWg - 1) / kRowsWg;
+  const int all_rows = p.Lq * p.group, blocks = (all_rows + kTrainBlock - 1) / kTrainBlock;
   const TrainPlace place = train_place(p, blocks);
   const int bh = place.bh, block = blocks - 1 - place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
-  const int row0 = block * kRowsWg;
+  const int row0 = block * kTrainBlock;
   const TileRange range = run_tiles(p, place, 0, key_tiles_of(p, e, row0));
   if (place.run >= range.runs) return;
 
-  const uint16_t* k_head = p.k + b * p.ks.sB + hk * p.ks.sH;
-  const uint16_t* v_head = p.v + b * p.vs.sB + hk * p.vs.sH;
   const unsigned lds = lds_base();
-  v16f dq[kCols][T::kBlocks];
+  v16f dq[T::kBlocks];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n)
-#pragma unroll
-    for (int c = 0; c < T::kBlocks; ++c) dq[n][c] = v16f{};
+  for (int c = 0; c < T::kBlocks; ++c) dq[c] = v16f{};
   float scale = 1.0f;
-  int row[kCols], limit[kCols];
-#pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    row[n] = row0 + (wave * kCols + n) * 32 + m;
-    limit[n] = p.causal ? min(e.keys, row_position(p, row[n]) + 1) : e.keys;
-    if (!kHalf && place.run == 0 && row[n] >= e.rows && row[n] < p.row_pad && hh == 0) {
-      p.row_l[(int64_t)bh * p.row_pad + row[n]] = -INFINITY;
-      p.row_d[(int64_t)bh * p.row_pad + row[n]] = 0.0f;
-    }
+  const int row = row0 + wave * 32 + m;
+  if (!kHalf && place.run == 0 && row >= e.rows && row < p.row_pad && hh == 0) {
+    p.row_l[(int64_t)bh * p.row_pad + row] = -INFINITY;
+    p.row_d[(int64_t)bh * p.row_pad + row] = 0.0f;
   }
   if (range.from < range.to) {
-    const TileCopy<D, kWaves> k_copy(k_head, p.ks.sL, wave, lane), v_copy(v_head, p.vs.sL, wave, lane);
+    const TileCopy<D, kWaves> k_copy(p.k + b * p.ks.sB + hk * p.ks.sH, p.ks.sL, wave, lane), v_copy(p.v + b * p.vs.sB + hk * p.vs.sH, p.vs.sL, wave, lane);
     auto copy = [&](int t) {
       const int at = min(t, range.to - 1) * kTrainTile;
-      const unsigned stage = lds + (t % kStages) * 2 * T::kBytes;
+      const unsigned stage = lds + (t & 1) * 2 * T::kBytes;
       k_copy.start(at, e.keys, stage, wave, lane);
       v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
     };
     copy(range.from);
-    v4i q[kCols][T::kSteps], g[kCols][T::kSteps];
-    float l[kCols], d[kCols];
+    v4i q[T::kSteps], g[T::kSteps];
+    const int r = min(row, e.rows - 1);
+    load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, r), hh, p.flip, q);
+    load_row<D>(p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH + row_offset(p, p.dos, r), hh, 0, g);
+    float l, d;
+    if constexpr (kHalf) {
+      l = p.row_l[(int64_t)bh * p.row_pad + r];
+      d = p.row_d[(int64_t)bh * p.row_pad + r];
+      scale = ds_scale(p, bh, lane);
+    } else {
+      // dO is here: what sage_train_rows_kernel would have to read it once more for is formed on the way, and kept for dk and dv
+      const int at = row_position(p, r), h = hk * p.group + r - at * p.group;
+      const uint16_t* o = p.o_in + b * p.os.sB + at * p.os.sL + h * p.os.sH + 8 * hh;
+      const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + at];
+      float sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      const int r = min(row[n], e.rows - 1);
-      load_row<D>(p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH + row_offset(p, p.qs, r), hh, p.flip, q[n]);
-      load_row<D>(p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH + row_offset(p, p.dos, r), hh, 0, g[n]);
-      if constexpr (kHalf) {
-        l[n] = p.row_l[(int64_t)bh * p.row_pad + r];
-        d[n] = p.row_d[(int64_t)bh * p.row_pad + r];
-      } else {
-        // dO is here: what sage_train_rows_kernel would have to read it once more for is formed on the way, and kept for dk and dv
-        const int at = row_position(p, r), h = hk * p.group + r - at * p.group;
-        const uint16_t* o = p.o_in + b * p.os.sB + at * p.os.sL + h * p.os.sH + 8 * hh;
-        const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + at];
-        float sum = 0.0f;
+      for (int s = 0; s < T::kSteps; ++s) {
+        float x[8], y[8];
+        widen8<DT>(*reinterpret_cast<const uint4*>(o + 16 * s), x);
+        widen8<DT>(__builtin_bit_cast(uint4, g[s]), y);
 #pragma unroll
-        for (int s = 0; s < T::kSteps; ++s) {
-          float x[8], y[8];
-          widen8<DT>(*reinterpret_cast<const uint4*>(o + 16 * s), x);
-          widen8<DT>(__builtin_bit_cast(uint4, g[n][s]), y);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) sum = __fmaf_rn(x[j], y[j], sum);
-        }
-        l[n] = row_minus<DT>(lse);
-        d[n] = -over_halves<Sum>(sum);
-        if (place.run == 0 && hh == 0 && row[n] < e.rows) {
-          p.row_l[(int64_t)bh * p.row_pad + row[n]] = l[n];
-          p.row_d[(int64_t)bh * p.row_pad + row[n]] = d[n];
-        }
+        for (int j = 0; j < 8; ++j) sum = __fmaf_rn(x[j], y[j], sum);
+      }
+      l = row_minus<DT>(lse);
+      d = -over_halves<Sum>(sum);
+      if (place.run == 0 && hh == 0 && row < e.rows) {
+        p.row_l[(int64_t)bh * p.row_pad + row] = l;
+        p.row_d[(int64_t)bh * p.row_pad + row] = d;
       }
     }
-    if constexpr (kHalf) scale = ds_scale(p, bh, lane);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
-    const int first = min(row0 + wave * 32 * kCols, e.rows - 1);
-    const bool idle = row0 + wave * 32 * kCols >= e.rows;  // a wave without rows copies its share
-    const int all_see = p.causal ? min(e.keys, row_position(p, first) + 1) : e.keys;
+    const int limit = p.causal ? min(e.keys, row_position(p, row) + 1) : e.keys;
+    const int all_see = p.causal ? min(e.keys, row_position(p, min(row0 + wave * 32, e.rows - 1)) + 1) : e.keys;
+    const bool idle = row0 + wave * 32 >= e.rows;  // a wave without rows copies its share
 #pragma unroll 1
     for (int t = range.from; t < range.to; ++t) {
       tile_ready<0>();
       copy(t + 1);
       if (idle) continue;
-      const unsigned k_tile = lds + (t % kStages) * 2 * T::kBytes, v_tile = k_tile + T::kBytes;
-      const bool edge = (t + 1) * kTrainTile > all_see;
+      unsigned k_rows = lds + (t & 1) * 2 * T::kBytes + row_at, v_rows = k_rows + T::kBytes, k_columns = lds + (t & 1) * 2 * T::kBytes + column_at;
+      pin(k_rows);  // (one address and constants each)
+      pin(v_rows);
+      pin(k_columns);
+      // A step of the tile: an operand read ahead, a matrix instruction, and vector work of a part of the 16 elements of a half
+      constexpr int kSteps = T::kSteps, kEach = 16 / kSteps, kAhead = 3;
+      v16f s[2], dp[2];
+      v4i ds[2][2], a[kAhead];
+      auto rows_product = [&](unsigned rows, int h, const v4i(&other)[kSteps], v16f& to, auto&& beside) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v16f s[kCols], dp[kCols];
+        for (int i = 0; i < kAhead; ++i) a[i] = read_row<D>(rows, h, i);
 #pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-          s[n] = v16f{};
-#pragma unroll
-          for (int i = 0; i < 16; ++i) dp[n][i] = d[n];
+        for (int i = 0; i < kSteps; ++i) {
+          to = mfma16<DT>(a[i % kAhead], other[i], to);
+          if (i + kAhead < kSteps) a[i % kAhead] = read_row<D>(rows, h, i + kAhead);
+          beside(i);
+          __builtin_amdgcn_sched_barrier(0);
         }
+      };
+      auto columns_product = [&](int h, auto&& beside) {
 #pragma unroll
-        for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = read_row<D>(k_tile + row_at, h, st);
+        for (int i = 0; i < kAhead; ++i) a[i] = read_column<D>(k_columns, i % T::kBlocks, 2 * h + i / T::kBlocks);
 #pragma unroll
-          for (int n = 0; n < kCols; ++n) s[n] = mfma16<DT>(a, q[n][st], s[n]);
+        for (int i = 0; i < kSteps; ++i) {
+          const int j = i + kAhead;
+          dq[i % T::kBlocks] = mfma16<DT>(a[i % kAhead], ds[h][i / T::kBlocks], dq[i % T::kBlocks]);
+          if (j < kSteps) a[i % kAhead] = read_column<D>(k_columns, j % T::kBlocks, 2 * h + j / T::kBlocks);
+          beside(i);
+          __builtin_amdgcn_sched_barrier(0);
         }
+      };
+      auto probabilities = [&](int h) {
+        return [&, h](int i) {
 #pragma unroll
-        for (int st = 0; st < T::kSteps; ++st) {
-          const v4i a = read_row<D>(v_tile + row_at, h, st);
+          for (int j = i * kEach; j < (i + 1) * kEach; ++j) s[h][j] = fast_exp2(__fmaf_rn(s[h][j], p.c, l));
+        };
+      };
+      auto gradients = [&](int h) {
+        return [&, h](int i) {
 #pragma unroll
-          for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, g[n][st], dp[n]);
-        }
-        v4i ds[kCols][2];
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) {
-          float y[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[n]));
-          if (edge) {
-            int left = limit[n] - t * kTrainTile - 32 * h - 4 * hh;
-            pin(left);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = acc_row(i) < left ? y[i] : 0.0f;
+          for (int j = i * kEach; j < (i + 1) * kEach; ++j) s[h][j] *= kHalf ? dp[h][j] * scale : dp[h][j];
+          if ((i + 1) * kEach % 8 == 0) {
+            const int f = (i + 1) * kEach / 8 - 1;
+            ds[h][f] = pack8<DT>(s[h][8 * f], s[h][8 * f + 1], s[h][8 * f + 2], s[h][8 * f + 3], s[h][8 * f + 4], s[h][8 * f + 5], s[h][8 * f + 6], s[h][8 * f + 7]);
           }
+        };
+      };
+      auto hide = [&](int h) {
+        if ((t + 1) * kTrainTile <= all_see) return;
+        int left = limit - t * kTrainTile - 32 * h - 4 * hh;
+        pin(left);  // (a branch that stays one)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] *= kHalf ? dp[n][i] * scale : dp[n][i];
+        for (int i = 0; i < 16; ++i) s[h][i] = acc_row(i) < left ? s[h][i] : 0.0f;
+      };
+      auto nothing = [](int) {};
+      s[0] = s[1] = v16f{};
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            ds[n][j] = pack8<DT>(y[8 * j], y[8 * j + 1], y[8 * j + 2], y[8 * j + 3], y[8 * j + 4], y[8 * j + 5], y[8 * j + 6], y[8 * j + 7]);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int c = 0; c < T::kBlocks; ++c) {
-            const v4i a = read_column<D>(k_tile + column_at, c, 2 * h + j);
-#pragma unroll
-            for (int n = 0; n < kCols; ++n) dq[n][c] = mfma16<DT>(a, ds[n][j], dq[n][c]);
-          }
-      }
+      for (int i = 0; i < 16; ++i) dp[0][i] = dp[1][i] = d;
+      rows_product(k_rows, 0, q, s[0], nothing);
+      rows_product(v_rows, 0, g, dp[0], probabilities(0));
+      hide(0);
+      rows_product(k_rows, 1, q, s[1], gradients(0));
+      rows_product(v_rows, 1, g, dp[1], probabilities(1));
+      hide(1);
+      columns_product(0, gradients(1));
+      columns_product(1, nothing);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   const float unshift = fast_exp2(-kBackwardShift<DT>);
+  const bool exists = row < all_rows;
+  const int r = min(row, all_rows - 1), at = row_position(p, r), h = hk * p.group + r - at * p.group;
+  if (row >= e.rows) {
 #pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    const bool exists = row[n] < all_rows;
-    const int r = min(row[n], all_rows - 1), at = row_position(p, r), h = hk * p.group + r - at * p.group;
-    if (row[n] >= e.rows) {
-#pragma unroll
-      for (int c = 0; c < T::kBlocks; ++c) dq[n][c] = v16f{};
-    }
-    if (range.runs > 1) {
-      store_column_part<D>(dq[n], p.sm_scale * unshift / scale, p.part + (((int64_t)place.cut * p.runs + place.run) * kTrainBlock + row[n] - row0) * D, hh,
-                           exists);
-      continue;
-    }
-    store_column<DT, D>(dq[n], p.sm_scale * unshift / scale, p.dq + (((int64_t)b * p.Lq + at) * p.Hq + h) * D, hh, exists);
+    for (int c = 0; c < T::kBlocks; ++c) dq[c] = v16f{};
   }
+  if (range.runs > 1) {
+    store_column_part<D>(dq, p.sm_scale * unshift / scale, p.part + (((int64_t)place.cut * p.runs + place.run) * kTrainBlock + row - row0) * D, hh, exists);
+    return;
+  }
+  store_column<DT, D>(dq, p.sm_scale * unshift / scale, p.dq + (((int64_t)b * p.Lq + at) * p.Hq + h) * D, hh, exists);
 }
 
 // ------------------------------------------------------------------------------------------------------------ runs joined
@@ -895,10 +897,10 @@ hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
   if (p.dq != nullptr) {
     constexpr int kLds = 2 * 2 * Tile<D>::kBytes;
     static LdsRequest request;
-    e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D, kCols>), kLds);
+    e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D>), kLds);
     if (e != hipSuccess) return e;
     take_cut(p, cuts.dq);
-    sage_train_dq_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+    sage_train_dq_kernel<DT, D><<<workgroups(p), 256, kLds, s>>>(p);
     join_bwd<DT, D, false>(p, (int64_t)p.Lq * p.group, s);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
