@@ -19,6 +19,8 @@ Differences, all deliberate:
   folds the cast the Wan block applies before its output projection (wan_model.py:197-204) into the kernel;
 * ``smooth_v`` (constructor argument, opt-in): V is quantized around its channel means, which the kernel adds back to
   the output - the option of the same name of the library behind the reference's call;
+* ``trainable`` (constructor argument, opt-in): calls whose inputs require gradients, with gradients enabled, run the 16-bit attention
+  that has a backward pass (``train_ops.attention``) in place of the quantized one, which has none; all other calls are as ever;
 * ``pwl_exp2`` (constructor argument, opt-in): a form of exp2 without the transcendental, 1.06-1.12x the speed at
   27 000 keys and more (head size 128; no gain at 4 400 and below) at a cosine similarity lower by ~1.5e-4;
 * availability: no HIP device -> ``supports()`` is False and the selector moves on, like the
@@ -30,7 +32,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _capi, platform
+from .. import _capi, platform, train_ops
 from ..config import KsanaAttentionBackend, KsanaAttentionConfig
 from ..sage_ops import sageattn
 from .base import KsanaAttentionBackendImpl
@@ -75,6 +77,8 @@ class SageAttentionImpl(KsanaAttentionBackendImpl):
         self.pwl_exp2 = bool(extra_impl_args.get("pwl_exp2", False))
         # opt-in: V quantized around its channel means (see sage_ops.sageattn)
         self.smooth_v = bool(extra_impl_args.get("smooth_v", False))
+        # opt-in: attention with a backward pass where gradients are wanted (see train_ops.attention)
+        self.trainable = bool(extra_impl_args.get("trainable", False))
         self.attention_config = attention_config
         self.check_config()
 
@@ -84,6 +88,9 @@ class SageAttentionImpl(KsanaAttentionBackendImpl):
             query, key, value = (t.to(torch.bfloat16) for t in (query, key, value))
         k_lens = kwargs.get("k_lens") if self.honor_k_lens else None
         q_lens = kwargs.get("q_lens") if self.honor_k_lens else None
+        if self.trainable and torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+            output = train_ops.attention(query, key, value, is_causal=self.causal, sm_scale=self.softmax_scale, k_lens=k_lens, q_lens=q_lens)
+            return output.to(original_dtype if self.out_dtype is None else self.out_dtype)
         output = sageattn(query, key, value, tensor_layout="NHD", is_causal=self.causal, sm_scale=self.softmax_scale,
                           k_lens=k_lens, out_dtype=self.out_dtype, pwl_exp2=self.pwl_exp2,
                           smooth_v=self.smooth_v, q_lens=q_lens)

@@ -1056,7 +1056,7 @@ int train_attn_params(const ksana_sage_train_attn* c, ksana_sage::TrainAttnParam
     return fail(KSANA_SAGE_ENOTSUP, "Lq=%d with %lld query heads to a key head: too many rows", s.Lq, (long long)group);
   if ((int64_t)s.B * s.Hkv > 65535) return fail(KSANA_SAGE_ENOTSUP, "B*Hkv = %lld exceeds the launch grid (65535)", (long long)s.B * s.Hkv);
   const int64_t most = (s.Lq * group > s.Lk ? s.Lq * group : s.Lk) / 64 + 2;
-  if ((int64_t)s.B * s.Hkv * most > (INT64_C(1) << 30)) return fail(KSANA_SAGE_ENOTSUP, "the call's workgroups exceed the launch grid");
+  if ((int64_t)s.B * s.Hkv * most > (INT64_C(1) << 23)) return fail(KSANA_SAGE_ENOTSUP, "the call's workgroups exceed the launch grid");
   if (reinterpret_cast<uintptr_t>(c->q_lens) & 3) return fail(KSANA_SAGE_EINVAL, "q_lens is not 4-byte aligned");
   if (reinterpret_cast<uintptr_t>(c->k_lens) & 3) return fail(KSANA_SAGE_EINVAL, "k_lens is not 4-byte aligned");
   *p = ksana_sage::TrainAttnParams{};

@@ -818,7 +818,8 @@ TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double sha
   const int64_t rest = blocks - whole;
   double least = 1e30;
   int best = tiles;  // of a run
-  for (int n = 1; n <= 128 && n <= tiles; ++n) {
+  const int most = rest > (1 << 19) ? 1 : std::min(tiles, 128);  // (a launch holds 2^24 workgroups)
+  for (int n = 1; n <= most; ++n) {
     const int each = (tiles + n - 1) / n;
     const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * rest * bytes * share / kBytesPerTile;
     const double cost = differ ? std::max((double)blocks * tiles * share / kPlaces * (1.0 + kSetup / each) + 0.5 * each, each + kSetup) + join
@@ -854,6 +855,7 @@ unsigned workgroups(const TrainAttnParams& p) { return (unsigned)(p.whole + (int
 // Rows of a block that the joins look at
 int joined_rows(int64_t all) { return (int)std::min<int64_t>(all, kTrainBlock); }
 constexpr int kManyRuns = 16;  // from here on lanes share a row's runs
+constexpr int64_t kMostGroups = 1 << 23;
 
 template <int DT, int D>
 hipError_t fwd(TrainAttnParams p, hipStream_t s) {
@@ -865,7 +867,7 @@ hipError_t fwd(TrainAttnParams p, hipStream_t s) {
   if (p.runs > 1) {
     constexpr int kLanes = D / 8;
     const int rows = joined_rows((int64_t)p.Lq * p.group), groups = (rows * kLanes + 255) / 256;  // workgroups of a block
-    if (p.runs >= kManyRuns)
+    if (p.runs >= kManyRuns && (int64_t)rows * p.cut <= kMostGroups)
       sage_train_join_fwd_kernel<DT, D, 256 / kLanes><<<(unsigned)((int64_t)rows * p.cut), 256, 0, s>>>(p, rows);
     else
       sage_train_join_fwd_kernel<DT, D, 1><<<(unsigned)((int64_t)groups * p.cut), 256, 0, s>>>(p, groups);
@@ -878,7 +880,7 @@ void join_bwd(const TrainAttnParams& p, int64_t all, hipStream_t s) {
   if (p.runs == 1) return;
   constexpr int kLanes = (kKeys ? 2 : 1) * D / 8;
   const int rows = joined_rows(all), groups = (rows * kLanes + 255) / 256;
-  if (p.runs >= kManyRuns)
+  if (p.runs >= kManyRuns && (int64_t)rows * p.cut <= kMostGroups)
     sage_train_join_bwd_kernel<DT, D, kKeys, 256 / kLanes><<<(unsigned)((int64_t)rows * p.cut), 256, 0, s>>>(p, rows);
   else
     sage_train_join_bwd_kernel<DT, D, kKeys, 1><<<(unsigned)((int64_t)groups * p.cut), 256, 0, s>>>(p, groups);

@@ -25,6 +25,12 @@ def _on(device: torch.device):
     return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """The tensor as the kernels read it (``_usable``), a contiguous one at an address that 16 does not divide included."""
+    t = _usable(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _scratch(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -36,11 +42,11 @@ def _ptr(t: torch.Tensor | None):
 class _AttentionCall:
     """The library's structure for tensors ``[B, L, H, D]`` as the kernels read them, and its scratch sizes."""
 
-    __slots__ = ("c", "lens", "fwd_bytes", "bwd_bytes")
+    __slots__ = ("c", "strides", "fwd_bytes", "bwd_bytes")
 
     def __init__(self, q, k, v, o, is_causal: bool, sm_scale: float | None, k_lens, q_lens):
         B, Lq, Hq, D = q.shape
-        self.lens = (k_lens, q_lens)  # (alive as long as the structure points to them)
+        self.strides = (q.stride(), k.stride(), v.stride(), o.stride())
         self.c = _capi.TrainAttn(_capi.Shape(B, Hq, k.shape[2], Lq, k.shape[1], D), _DTYPES[q.dtype], int(is_causal),
                                  D**-0.5 if sm_scale is None else float(sm_scale), 0, _strides(q), _strides(k), _strides(v), _strides(o),
                                  _ptr(q_lens), _ptr(k_lens))
@@ -73,15 +79,23 @@ def _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, want_lse: b
     return o, lse, call
 
 
-def _attention_backward(do, q, k, v, o, lse, call, want_q: bool, want_kv: bool):
+def _attention_backward(do, q, k, v, o, lse, call, is_causal, sm_scale, k_lens, q_lens, want_q: bool, want_kv: bool):
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if want else None
                   for t, want in ((q, want_q), (k, want_kv), (v, want_kv)))
     if q.numel() == 0 or k.numel() == 0:
         return tuple(None if t is None else t.zero_() for t in (dq, dk, dv))
-    do = _usable(do)
+    do = _readable(do)
+    # hooks that keep saved tensors elsewhere may give them back laid out and placed otherwise
+    c = call.c
+    if call.strides != (q.stride(), k.stride(), v.stride(), o.stride()):
+        q, k, v, o = (_readable(t) for t in (q, k, v, o))
+        call = _AttentionCall(q, k, v, o, is_causal, sm_scale, k_lens, q_lens)
+        c = call.c
+    else:
+        c.q_lens, c.k_lens = _ptr(q_lens), _ptr(k_lens)
     with _on(q.device):
         scratch = _scratch(call.bwd_bytes, q.device)
-        rc = _capi.load().ksana_sage_train_attn_bwd(C.addressof(call.c), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
+        rc = _capi.load().ksana_sage_train_attn_bwd(C.addressof(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
                                                     do.data_ptr(), _strides(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(scratch), _stream_ptr(q.device))
     _capi.check(rc, "train_ops.attention, backward")
     return dq, dk, dv
@@ -91,15 +105,16 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, is_causal, sm_scale, k_lens, q_lens):
         o, lse, call = _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, True)
-        ctx.save_for_backward(q, k, v, o, lse)
-        ctx.call = call
+        ctx.save_for_backward(q, k, v, o, lse, k_lens, q_lens)
+        ctx.call, ctx.is_causal, ctx.sm_scale = call, is_causal, sm_scale
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
-        dq, dk, dv = _attention_backward(do, *ctx.saved_tensors, ctx.call, want_q, want_k or want_v)
+        q, k, v, o, lse, k_lens, q_lens = ctx.saved_tensors
+        dq, dk, dv = _attention_backward(do, q, k, v, o, lse, ctx.call, ctx.is_causal, ctx.sm_scale, k_lens, q_lens, want_q, want_k or want_v)
         return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
 
 
@@ -110,8 +125,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
 
     ``k_lens``, ``q_lens``, ``is_causal`` and ``sm_scale`` mean what they mean for ``sageattn``; rows that see no key are zeros
     and give no gradient; keys and values behind ``k_lens[b]``, query rows and their gradients behind ``q_lens[b]`` are not
-    read.  Counts on the device are taken as they are when the kernels run, also in the backward pass: they must not be
-    written between the two.  Scores, softmax statistics and sums are fp32; probabilities and their gradients are rounded to the tensors' type
+    read.  Int32 counts on the device are read by the kernels, in the backward pass again (writing to them in between is an
+    error, as for the tensors).  Scores, softmax statistics and sums are fp32; probabilities and their gradients are rounded to the tensors' type
     where they are multiplied on, in fp16 scaled by powers of two that keep small gradients representable."""
     if tensor_layout not in ("NHD", "HND"):
         raise ValueError(f"tensor_layout {tensor_layout!r} unknown")
@@ -119,7 +134,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
         q, k, v = (t.transpose(1, 2) if t.dim() == 4 else t for t in (q, k, v))
     _check_attention(q, k, v)
     k_lens, q_lens = (_k_lens_arg(n, q.shape[0], q.device, name) for n, name in ((k_lens, "k_lens"), (q_lens, "q_lens")))
-    q, k, v = _usable(q), _usable(k), _usable(v)
+    q, k, v = _readable(q), _readable(k), _readable(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         o = _Attention.apply(q, k, v, bool(is_causal), sm_scale, k_lens, q_lens)
     else:
@@ -141,11 +156,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 class _NormCall:
     """The library's structure for one residual norm, and what it points to."""
 
-    __slots__ = ("c", "vectors", "bwd_bytes")
+    __slots__ = ("c",)
 
     def __init__(self, x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype):
         B, L, C_ = x.shape
-        self.vectors = vectors  # (alive as long as the structure points to them)
         args = []
         for t in vectors:
             args.append(_NO_VECTOR if t is None else
@@ -175,7 +189,7 @@ class _ResidualNorm(torch.autograd.Function):
         call = _NormCall(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype)
         h, n, stats = _residual_norm_forward(x, y, call, n_dtype, True)
         ctx.save_for_backward(x, y, stats, *vectors)
-        ctx.call, ctx.n_dtype = call, n_dtype
+        ctx.options = (norm, post_norm, residual_scale, eps, n_dtype)
         ctx.set_materialize_grads(False)
         return n if y is None else (h, n)
 
@@ -186,7 +200,11 @@ class _ResidualNorm(torch.autograd.Function):
         dh, dn = grads if y is not None else (None, grads[0])
         if dh is None and dn is None:
             return (None,) * 13
-        dn = torch.zeros(x.shape, dtype=ctx.n_dtype, device=x.device) if dn is None else dn.contiguous()
+        n_dtype = ctx.options[-1]
+        x, y = _rows(x), None if y is None else _rows(y)
+        # (made from the saved tensors as they are now: hooks may have moved them and laid them out anew)
+        call = _NormCall(x, y, [None if t is None else _vector_rows(t) for t in vectors], *ctx.options)
+        dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dy = None if y is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
@@ -194,7 +212,7 @@ class _ResidualNorm(torch.autograd.Function):
         d_vectors = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None for t, want in zip(vectors, wanted)]
         if x.numel() == 0:
             return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors), *(None,) * 5)
-        lib, call = _capi.load(), ctx.call
+        lib = _capi.load()
         nbytes = C.c_uint64(0)
         _capi.check(lib.ksana_sage_train_norm_scratch(C.addressof(call.c), C.addressof(nbytes)), "train_ops.residual_norm, backward")
         with _on(x.device):
@@ -218,7 +236,12 @@ def _norm_vector(name: str, t: torch.Tensor | None, x: torch.Tensor) -> torch.Te
     own = name in ("gate", "scale", "shift")
     if shape != (C_,) and not (own and shape in ((B, C_), (1, C_), (B, 1, C_), (1, 1, C_))):
         raise ValueError(f"{name} must be [{C_}]" + (f", [{B}, {C_}] or [{B}, 1, {C_}]" if own else "") + f", got {shape}")
-    if (C_ > 1 and t.stride(-1) != 1) or (len(shape) > 1 and shape[0] > 1 and t.stride(0) <= 0):
+    return _vector_rows(t)
+
+
+def _vector_rows(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous channels; entries of their own any positive stride apart."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1 or t.dim() > 1 and t.shape[0] > 1 and t.stride(0) <= 0:
         return t.contiguous()
     return t
 

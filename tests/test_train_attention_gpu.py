@@ -120,3 +120,205 @@ def test_counts_of_padded_batches(hip_device, k_lens, q_lens, causal):
         if q_lens is not None:
             n = max(0, q_lens[b])
             assert not o[b, n:].any() and not dq[b, n:].any()
+
+
+# ------------------------------------------------------------------------------------------------ scales and magnitudes
+@gpu
+@pytest.mark.parametrize("scale", [-0.09, 0.0, 1.0])
+def test_any_scale(hip_device, scale):
+    _check(*_draw(1, 1, 2, 1, 70, 130, 64, torch.float16, std=0.5), hip_device, scale=scale, causal=True)
+
+
+@gpu
+@pytest.mark.parametrize("do_std", [1e-6, 300.0])
+def test_gradients_of_any_size_in_fp16(hip_device, do_std):
+    """Loss-scaled and vanishing gradients: nothing inside overflows or vanishes that the result can hold."""
+    _check(*_draw(2, 1, 2, 2, 150, 400, 128, torch.float16, do_std=do_std), hip_device)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_reference_points_that_move(hip_device, dtype):
+    """Scores that grow from tile to tile, by less and by more than the points may lag, and rows that only see small ones."""
+    q, k, v, do = _draw(4, 1, 1, 1, 64, 640, 128, dtype)
+    k *= (0.2 + torch.arange(640).view(1, -1, 1, 1) / 200).to(dtype)
+    _check(q, k, v, do, hip_device, causal=False)
+
+
+# ------------------------------------------------------------------------------------------------ layouts
+def _attend(q, k, v, do, **kw):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = train_ops.attention(*leaves, **kw)
+    return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+def test_layouts_give_the_same_bits(hip_device):
+    q, k, v, do = (t.to(hip_device) for t in _draw(6, 2, 6, 3, 150, 170, 64, torch.bfloat16))
+    want = _attend(q, k, v, do)
+    assert _same(_attend(q, k, v, do), want)  # and repeated calls
+    # slices of a fused projection, heads before positions, a base that is not aligned, gradients with strides of zero
+    fused = torch.empty(2, 170, 12, 64, dtype=q.dtype, device=hip_device)
+    fused[:, :150, :6], fused[:, :, 6:9], fused[:, :, 9:] = q, k, v
+    assert _same(_attend(fused[:, :150, :6], fused[:, :, 6:9], fused[:, :, 9:], do), want)
+    first = [t.transpose(1, 2).contiguous() for t in (q, k, v, do)]
+    got = _attend(*first, tensor_layout="HND")
+    assert _same([t.transpose(1, 2) for t in got], want)
+    odd = [torch.empty(t.numel() + 1, dtype=t.dtype, device=hip_device)[1:].view(t.shape).copy_(t) for t in (q, k, v, do)]
+    assert _same(_attend(*odd), want)
+    ones = torch.ones((), dtype=q.dtype, device=hip_device).expand(do.shape)
+    assert _same(_attend(q, k, v, ones), _attend(q, k, v, ones.contiguous()))
+
+
+@gpu
+def test_counts_of_any_kind(hip_device):
+    q, k, v, do = (t.to(hip_device) for t in _draw(7, 2, 2, 2, 90, 100, 128, torch.float16))
+    want = _attend(q, k, v, do, k_lens=torch.tensor([60, 100], dtype=torch.int32, device=hip_device), q_lens=torch.tensor([90, 33], device=hip_device))
+    assert _same(_attend(q, k, v, do, k_lens=[60, 100], q_lens=torch.tensor([90, 33])), want)
+    with pytest.raises(ValueError, match="k_lens"):
+        train_ops.attention(q, k, v, k_lens=[3])
+
+
+@gpu
+def test_only_wanted_gradients(hip_device):
+    q, k, v, do = (t.to(hip_device) for t in _draw(8, 1, 2, 2, 100, 140, 128, torch.bfloat16))
+    _, dq, dk, dv = _attend(q, k, v, do)
+    for wanted in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        leaves = [t.detach().requires_grad_(i in wanted) for i, t in enumerate((q, k, v))]
+        got = torch.autograd.grad(train_ops.attention(*leaves), [leaves[i] for i in wanted], do)
+        assert _same(got, [(dq, dk, dv)[i] for i in wanted])
+    assert not train_ops.attention(q, k, v).requires_grad
+    with torch.no_grad():
+        assert not train_ops.attention(*[t.detach().requires_grad_() for t in (q, k, v)]).requires_grad
+
+
+@gpu
+def test_saved_tensors_may_be_kept_elsewhere(hip_device):
+    q, k, v, do = (t.to(hip_device) for t in _draw(9, 2, 4, 2, 100, 140, 64, torch.bfloat16))
+    want = _attend(q, k, v, do, k_lens=[140, 31])
+    wide = [torch.zeros(*t.shape[:2], 2 * t.shape[2], t.shape[3], dtype=t.dtype, device=hip_device)[:, :, ::2].copy_(t) for t in (q, k, v)]
+    with torch.autograd.graph.save_on_cpu():  # they come back contiguous
+        got = _attend(*wide, do, k_lens=[140, 31])
+    assert _same(got, want)
+
+
+@gpu
+def test_what_cannot_be_differentiated_is_refused(hip_device):
+    q = torch.randn(1, 20, 1, 64, device=hip_device, dtype=torch.float16, requires_grad=True)
+    lens = torch.tensor([15], dtype=torch.int32, device=hip_device)
+    o = train_ops.attention(q, q, q, k_lens=lens)
+    (g,) = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), q)
+    o = train_ops.attention(q, q, q, k_lens=lens)
+    lens.fill_(3)  # after the forward pass has used it
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with pytest.raises(ValueError, match="dtype"):
+        train_ops.attention(*[q.float()] * 3)
+    with pytest.raises(ValueError, match="one device and one dtype"):
+        train_ops.attention(q, q.bfloat16(), q)
+    with pytest.raises(NotImplementedError, match="head size"):
+        train_ops.attention(*[torch.zeros(1, 4, 1, 96, device=hip_device, dtype=torch.float16)] * 3)
+    with pytest.raises(ValueError, match="not a multiple"):
+        train_ops.attention(q.expand(1, 20, 3, 64), q.expand(1, 20, 2, 64), q.expand(1, 20, 2, 64))
+
+
+@gpu
+def test_nothing_to_attend_from_or_to(hip_device):
+    def t(*shape):
+        return torch.randn(shape, device=hip_device, dtype=torch.bfloat16, requires_grad=True)
+
+    for q, k, v in ((t(1, 0, 2, 64), t(1, 5, 2, 64), t(1, 5, 2, 64)), (t(1, 5, 2, 64), t(1, 0, 2, 64), t(1, 0, 2, 64)), (t(0, 5, 2, 64),) * 3):
+        o = train_ops.attention(q, k, v)
+        assert o.shape == q.shape and not o.any()
+        o.sum().backward()
+        assert not q.grad.any() and not k.grad.any() and not v.grad.any()
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs, sizes
+@gpu
+def test_streams_and_graphs(hip_device):
+    """The same bits from another stream, and from graphs with the backward pass in them: replayed several times with other inputs and
+    with eager work between the replays; two graphs side by side share nothing."""
+    sets = [[t.to(hip_device) for t in _draw(20 + i, 1, 4, 2, 200, 900, 128, torch.float16)] for i in range(3)]
+    want = [_attend(*s, is_causal=True) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert _same(_attend(*sets[0], is_causal=True), want[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        inputs = [torch.empty_like(t) for t in sets[0]]
+        for a, b in zip(inputs, sets[0]):
+            a.copy_(b)
+        with torch.cuda.stream(side):  # (warmed up on the capturing stream, as torch asks)
+            side.wait_stream(torch.cuda.current_stream())
+            _attend(*inputs, is_causal=True)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outputs = _attend(*inputs, is_causal=True)
+        graphs.append((graph, inputs, outputs))
+    for turn in range(4):
+        for at, (graph, inputs, outputs) in enumerate(graphs):
+            s = (turn + at) % 3
+            for a, b in zip(inputs, sets[s]):
+                a.copy_(b)
+            graph.replay()
+            _attend(*sets[(s + 1) % 3])  # eager work of the same kind
+            torch.cuda.synchronize()
+            assert _same(outputs, want[s])
+
+
+@gpu
+def test_offsets_beyond_32_bits(hip_device):
+    """Keys and values of 2.3 billion elements each, by heads of the last batch entry against the formula."""
+    B, L, H, D = 2, 70000, 128, 128
+    g = torch.Generator(device=hip_device).manual_seed(1)
+    k, v = (torch.randn((B, L, H, D), generator=g, device=hip_device, dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    q, do = (torch.randn((B, 3, H, D), generator=g, device=hip_device, dtype=torch.bfloat16) for _ in range(2))
+    q.requires_grad_()
+    assert k.numel() > 2**31
+    got = (o := train_ops.attention(q, k, v), *torch.autograd.grad(o, (q, k, v), do))
+    for h in (0, H - 1):
+        part = [t.detach()[1:, :, h : h + 1].cpu() for t in (q, k, v, do)]
+        want = _formula(*part)
+        for x, y, most in zip(got, want[::2], want[1::2]):
+            assert ((x.detach()[1:, :, h : h + 1].cpu().double() - y).abs() <= most).all()
+
+
+@gpu
+@pytest.mark.parametrize("Hq,Hkv,Lq,Lk,causal", [(16, 4, 1500, 1500, True), (40, 40, 1560, 1560, False), (2, 2, 5000, 77, False), (3, 3, 64, 9000, False)])
+def test_cut_loops_against_uncut_ones(hip_device, Hq, Hkv, Lq, Lk, causal):
+    """Blocks whose loops are cut into runs, and the same heads among enough others that nothing is cut: results that differ by their
+    roundings only, each within what the formula allows."""
+    q, k, v, do = _draw(11, 1, Hq, Hkv, Lq, Lk, 128, torch.bfloat16)
+    got = _attend(*(t.to(hip_device) for t in (q, k, v, do)), is_causal=causal)
+    h, hk = Hq - 1, Hkv - 1
+    rep = Hq // Hkv
+    part = (q[:, :, h - rep + 1 :], k[:, :, hk:], v[:, :, hk:], do[:, :, h - rep + 1 :])
+    want = _formula(*part, causal=causal)
+    for x, y, most in zip(got, want[::2], want[1::2]):
+        x = x[:, :, -y.shape[2] :].cpu().double()
+        assert ((x - y).abs() <= most).all()
+
+
+# ------------------------------------------------------------------------------------------------ where the package offers it
+@gpu
+def test_the_backend_trains_where_it_is_asked_to(hip_device):
+    from ksanadit_amd import KsanaAttentionBackend, KsanaAttentionConfig
+    from ksanadit_amd.backends.sage_attn import SageAttentionImpl
+
+    q, k, v, do = (t.to(hip_device) for t in _draw(12, 1, 2, 2, 100, 120, 128, torch.bfloat16))
+    make = lambda **kw: SageAttentionImpl(KsanaAttentionConfig(backend=KsanaAttentionBackend.SAGE_ATTN), 2, 128, False, 128**-0.5, **kw)  # noqa: E731
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = make(trainable=True).forward(*leaves)
+    assert _same((o.detach(), *torch.autograd.grad(o, leaves, do)), _attend(q, k, v, do))
+    assert torch.equal(make(trainable=True).forward(q, k, v), make().forward(q, k, v))  # without gradients: as ever
+    assert make(trainable=True, out_dtype=torch.float16).forward(*leaves).dtype == torch.float16

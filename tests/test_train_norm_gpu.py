@@ -154,3 +154,128 @@ def test_vectors_for_all_entries_sum_their_gradients(hip_device):
     t, dh, dn = make(1, 3, 50, 264, bf16, bf16, fp32, ALL, shared=True)
     want = definition({k: v.double() for k, v in t.items()}, dh.double(), dn.double(), "layer", "rms", 1.0, 1e-6)
     _check(_run(t, dh, dn, hip_device, "layer", "rms", 1.0), want, _types(t, dn))
+
+
+def _same(a, b):
+    return a.keys() == b.keys() and all(torch.equal(a[k], b[k]) for k in a)
+
+
+@gpu
+def test_layouts_give_the_same_bits(hip_device):
+    t, dh, dn = make(3, 2, 40, 264, bf16, bf16, fp32, ALL)
+    want = _run(t, dh, dn, hip_device, "layer", "rms", 0.5)
+    assert _same(_run(t, dh, dn, hip_device, "layer", "rms", 0.5), want)
+
+    def apart(x):  # every other row, column and entry of something larger, at an odd address
+        big = torch.zeros([2 * n for n in x.shape[:-1]] + [x.shape[-1] + 3], dtype=x.dtype, device=x.device)
+        view = big[tuple(slice(None, None, 2) for _ in x.shape[:-1])][..., 1 : x.shape[-1] + 1]
+        return view.copy_(x).detach()
+
+    assert _same(_run(t, dh, dn, hip_device, "layer", "rms", 0.5, wrap=apart), want)
+    # a chunk of a modulation table, vectors without their middle dimension, a tensor whose rows are one row
+    table = torch.stack([t["gate"], t["scale"], t["shift"]], 1).flatten(1, 2).to(hip_device)
+    u = {k: v.to(hip_device) for k, v in t.items()}
+    h, n = train_ops.residual_norm(**{**u, "gate": table[:, :1], "scale": table[:, 1:2], "shift": table[:, 2]}, norm="layer", post_norm="rms",
+                                   residual_scale=0.5)
+    assert torch.equal(h, want["h"]) and torch.equal(n, want["n"])
+    row = u["x"][:, :1].expand(-1, 40, -1)
+    got, ref = (train_ops.residual_norm(x, u["y"]) for x in (row, row.contiguous()))
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+@gpu
+def test_only_some_results_or_gradients_are_wanted(hip_device):
+    t, dh, dn = make(4, 2, 30, 520, fp32, bf16, fp32, ALL)
+    u = {k: v.to(hip_device) for k, v in t.items()}
+    full = _run(t, dh, dn, hip_device, "rms", "layer", 1.0)
+    none = {k: v.double() for k, v in t.items()}
+    for use in ("h", "n"):
+        leaves = {k: v.clone().requires_grad_() for k, v in u.items()}
+        h, n = train_ops.residual_norm(**leaves, norm="rms", post_norm="layer")
+        d = torch.autograd.grad(h if use == "h" else n, list(leaves.values()), (dh if use == "h" else dn).to(hip_device), allow_unused=True)
+        want = definition(none, dh.double() * (use == "h"), dn.double() * (use == "n"), "rms", "layer", 1.0, 1e-6)
+        _check(dict(zip(leaves, d)), want, _types(t, dn))
+    leaves = {k: v.clone().requires_grad_(k in ("gate", "weight")) for k, v in u.items()}
+    h, n = train_ops.residual_norm(**leaves, norm="rms", post_norm="layer")
+    d = torch.autograd.grad((h, n), (leaves["gate"], leaves["weight"]), (dh.to(hip_device), dn.to(hip_device)))
+    assert torch.equal(d[0], full["gate"]) and torch.equal(d[1], full["weight"])
+    with torch.no_grad():
+        h, n = train_ops.residual_norm(**u, norm="rms", post_norm="layer")
+    assert torch.equal(h, full["h"]) and torch.equal(n, full["n"])
+
+
+@gpu
+def test_saved_tensors_may_be_kept_elsewhere(hip_device):
+    t, dh, dn = make(5, 2, 30, 128, bf16, bf16, bf16, ALL)
+    want = _run(t, dh, dn, hip_device, "layer", "layer", 1.0)
+    wide = lambda x: torch.zeros(*x.shape[:-1], 2 * x.shape[-1], dtype=x.dtype, device=x.device)[..., : x.shape[-1]].copy_(x)  # noqa: E731
+    with torch.autograd.graph.save_on_cpu():
+        assert _same(_run(t, dh, dn, hip_device, "layer", "layer", 1.0, wrap=wide), want)
+
+
+@gpu
+def test_rows_far_from_zero_keep_their_variance(hip_device):
+    """Values around 1e4 that differ by 1: squares minus the squared mean would lose them."""
+    x = (1e4 + torch.randn(1, 3, 4096, generator=torch.Generator().manual_seed(1))).float()
+    t, zero = {"x": x}, torch.zeros_like(x)
+    want = definition({"x": x.double()}, zero.double(), zero.double(), "layer", None, 1.0, 1e-6)
+    h, n = train_ops.residual_norm(x.to(hip_device))
+    assert h.data_ptr() and h.shape == x.shape
+    _check({"n": n}, want, _types(t, zero))
+
+
+@gpu
+def test_refusals_and_empty_tensors(hip_device):
+    x = torch.randn(2, 3, 16, device=hip_device)
+    with pytest.raises(ValueError, match="go with y"):
+        train_ops.residual_norm(x, gate=x[0, 0])
+    with pytest.raises(ValueError, match="post_weight"):
+        train_ops.residual_norm(x, x, post_weight=x[0, 0])
+    with pytest.raises(ValueError, match="does not go with"):
+        train_ops.residual_norm(x.half(), x)
+    with pytest.raises(ValueError, match="its type"):
+        train_ops.residual_norm(x, x, out_dtype=torch.float16)
+    with pytest.raises(NotImplementedError, match="8192"):
+        train_ops.residual_norm(torch.zeros(1, 1, 8200, device=hip_device))
+    for shape in ((0, 3, 16), (2, 0, 16)):
+        e, w = torch.zeros(shape, device=hip_device, requires_grad=True), torch.ones(16, device=hip_device, requires_grad=True)
+        h, n = train_ops.residual_norm(e, e, weight=w)
+        (h.sum() + n.sum()).backward()
+        assert n.shape == shape and e.grad.shape == shape and not w.grad.any()
+    y = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(train_ops.residual_norm(y)[1].square().sum(), y, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@gpu
+def test_streams_and_graphs(hip_device):
+    sets = [make(30 + i, 2, 64, 776, bf16, bf16, fp32, ALL) for i in range(3)]
+    want = [_run(*s, hip_device, "layer", "rms", 1.0) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    held = {k: v.to(hip_device) for k, v in sets[0][0].items()}
+    grads = [g.to(hip_device) for g in sets[0][1:]]
+
+    def step():
+        leaves = {k: v.detach().requires_grad_() for k, v in held.items()}
+        h, n = train_ops.residual_norm(**leaves, norm="layer", post_norm="rms")
+        return {"h": h.detach(), "n": n.detach(), **dict(zip(leaves, torch.autograd.grad((h, n), list(leaves.values()), grads)))}
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        assert _same(step(), want[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step()
+    for turn in range(5):
+        t, dh, dn = sets[turn % 3]
+        for name, v in t.items():
+            held[name].copy_(v)
+        grads[0].copy_(dh)
+        grads[1].copy_(dn)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert _same(out, want[turn % 3])
+        _run(*sets[(turn + 1) % 3], hip_device, "rms", "layer", 0.5)  # eager work of the same kind

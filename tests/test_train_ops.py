@@ -1,0 +1,166 @@
+"""The operators with gradients where no GPU is needed: what they refuse, and the tests' own formulas against differences."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+from ksanadit_amd import _capi, train_ops
+from tests.test_train_attention_gpu import HALF_STEP, _draw, _formula
+from tests.test_train_norm_gpu import ALL, definition, make
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(shape, dtype=dtype)
+
+
+# ------------------------------------------------------------------------------------------------ the formulas
+def _directional(f, inputs, directions, step):
+    plus, minus = (f([x + sign * step * d for x, d in zip(inputs, directions)]) for sign in (1, -1))
+    return (plus - minus) / (2 * step)
+
+
+@pytest.mark.parametrize("causal,lens", [(False, None), (True, None), (True, ([5, 0], [9, 7]))])
+def test_the_attention_formula_against_differences(causal, lens):
+    """Central differences of sum(o * do): off by step^2 / 6 times a third derivative (below 1e3 for these sizes) and 2^-52 / step."""
+    k_lens, q_lens = lens if lens else (None, None)
+    q, k, v, do = _draw(3, 2, 4, 2, 9, 11, 8, torch.float32)
+    HALF_STEP[torch.float64] = 0.0
+    try:
+        q, k, v, do = (t.double() for t in (q, k, v, do))
+        kw = dict(causal=causal, k_lens=k_lens, q_lens=q_lens)
+        o, _, dq, _, dk, _, dv, _ = _formula(q, k, v, do, **kw)
+        g = torch.Generator().manual_seed(1)
+        directions = [torch.randn(t.shape, generator=g, dtype=torch.float64) for t in (q, k, v)]
+        got = _directional(lambda x: (_formula(*x, do, **kw)[0] * do).sum(), (q, k, v), directions, 1e-5)
+    finally:
+        del HALF_STEP[torch.float64]
+    want = sum((a * b).sum() for a, b in zip((dq, dk, dv), directions))
+    assert abs(got - want) <= 1e-6 * max(1.0, abs(want))
+
+
+@pytest.mark.parametrize("norm,post,names", [("layer", None, ALL[:4]), ("rms", "layer", ALL), ("layer", "rms", ALL), ("rms", None, ("weight",))])
+def test_the_norm_definition_against_differences(norm, post, names):
+    t, dh, dn = make(2, 2, 5, 12, torch.float32, torch.float32, torch.float32, names)
+    t = {k: v.double() for k, v in t.items()}
+    dh, dn = dh.double() * ("y" in names), dn.double()
+    r = 0.7 if "y" in names else 1.0
+    full = definition(t, dh, dn, norm, post, r, 1e-6)
+    g = torch.Generator().manual_seed(1)
+    directions = [torch.randn(v.shape, generator=g, dtype=torch.float64) for v in t.values()]
+
+    def value(x):
+        d = definition(dict(zip(t, x)), dh, dn, norm, post, r, 1e-6)
+        return (d["h"][0] * dh).sum() + (d["n"][0] * dn).sum()
+
+    got = _directional(value, list(t.values()), directions, 1e-5)
+    want = sum((full[k][0] * d).sum() for k, d in zip(t, directions))
+    assert abs(got - want) <= 1e-6 * max(1.0, abs(want))
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_tensors_off_the_gpu_are_refused():
+    q = _meta(1, 4, 2, 64)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        train_ops.attention(q, q, q)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        train_ops.residual_norm(_meta(1, 4, 64))
+
+
+def test_arguments_of_the_attention():
+    q = _meta(1, 4, 2, 64)
+    with pytest.raises(ValueError, match="4-D"):
+        train_ops.attention(q[0], q, q)
+    with pytest.raises(ValueError, match="tensor_layout"):
+        train_ops.attention(q, q, q, tensor_layout="LHD")
+
+
+def test_arguments_of_the_norm():
+    x = _meta(2, 4, 64)
+    for kw, what in (({"norm": "batch"}, "unknown"), ({"post_norm": "l2", "y": x}, "unknown"), ({"y": x[:, :3]}, "one shape")):
+        with pytest.raises(ValueError, match=what):
+            train_ops.residual_norm(x, **kw)
+    with pytest.raises(ValueError, match="one shape"):
+        train_ops.residual_norm(x[0])
+    for name, shape in (("gate", (3, 64)), ("weight", (2, 64)), ("shift", (2, 4, 64)), ("scale", (63,))):
+        with pytest.raises(ValueError, match=name):
+            train_ops._norm_vector(name, torch.empty(shape), x)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        train_ops._norm_vector("gate", torch.empty(64, dtype=torch.float64), x)
+
+
+def _attn_call(**kw):
+    B, Hq, Hkv, Lq, Lk, D = (kw.pop(n, d) for n, d in zip(("B", "Hq", "Hkv", "Lq", "Lk", "D"), (1, 4, 2, 16, 16, 128)))
+
+    def strides(L, H):
+        return _capi.Strides(L * H * D, H * D, D, 1)
+
+    c = _capi.TrainAttn(_capi.Shape(B, Hq, Hkv, Lq, Lk, D), 0, 0, 0.1, 0, strides(Lq, Hq), strides(Lk, Hkv), strides(Lk, Hkv), strides(Lq, Hq), None, None)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+@pytest.mark.parametrize("kw,rc", [
+    ({}, 0), ({"B": 0}, -1), ({"Hkv": 3}, -1), ({"D": 96}, -2), ({"Lk": 0}, -1), ({"dtype": 2}, -1), ({"reserved": 1}, -1), ({"sm_scale": float("inf")}, -1),
+    ({"sm_scale": float("nan")}, -1), ({"Lq": 1 << 25}, -2), ({"Lk": (1 << 24) + 1}, -2), ({"Hq": 8192, "Hkv": 1, "Lq": 1 << 10}, -2),
+    ({"Hq": 70000, "Hkv": 70000}, -2), ({"q_lens": 2}, -1), ({"k_lens": 3}, -1), ({"B": 1024, "Hq": 60, "Hkv": 60, "Lk": 1 << 20}, -2)])
+def test_calls_of_the_attention_are_checked(kw, rc):
+    lib, n = _capi.load(), C.c_uint64(0)
+    assert lib.ksana_sage_train_attn_scratch(C.addressof(_attn_call(**kw)), C.addressof(n), C.addressof(n)) == rc, lib.ksana_sage_last_error()
+    assert lib.ksana_sage_train_attn_scratch(None, None, None) == -1
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(q=None), b"q is null"), (dict(k=0x1008), b"not 16-byte"), (dict(lse=0x1002), b"lse"), (dict(c=dict(q_strides=_capi.Strides(1, 2, 3, 1))), b"stride"),
+    (dict(c=dict(v_strides=_capi.Strides(4096, 256, 128, 2))), b"D stride"), (dict(scratch=None), b"scratch is null"), (dict(scratch=0x1010), b"256-byte"),
+    (dict(c=dict(k_strides=_capi.Strides(1 << 40, 1 << 33, 128, 1))), b"beyond"),
+    (dict(bwd=True, dk=None), b"together"), (dict(bwd=True, dq=0x1008), b"gradient"), (dict(bwd=True, lse=None), b"lse"), (dict(bwd=True, do=None), b"d_o is null")])
+def test_buffers_of_the_attention_are_checked(change, what):
+    """Nothing here reaches a device: the library looks at addresses, never through them."""
+    lib = _capi.load()
+    # (keys for many runs, so that scratch is needed)
+    c = _attn_call(Lk=4096, **change.get("c", {}))
+    a = {n: 0x1000 for n in ("q", "k", "v", "o", "lse", "scratch", "do", "dq", "dk", "dv")}
+    a.update({k: v for k, v in change.items() if k in a})
+    if change.get("bwd"):
+        st = _capi.Strides(*c.q_strides)
+        rc = lib.ksana_sage_train_attn_bwd(C.addressof(c), a["q"], a["k"], a["v"], a["o"], a["lse"], a["do"], C.addressof(st), a["dq"], a["dk"], a["dv"],
+                                           a["scratch"], None)
+    else:
+        rc = lib.ksana_sage_train_attn_fwd(C.addressof(c), a["q"], a["k"], a["v"], a["o"], a["lse"], a["scratch"], None)
+    assert rc in (-1, -2) and what in lib.ksana_sage_last_error(), lib.ksana_sage_last_error()
+
+
+def _norm_call(vectors=None, **kw):
+    v = {n: _capi.Vector() for n in train_ops._VECTORS} | (vectors or {})
+    d = dict(B=2, L=3, C=64, x_dtype=0, y_dtype=0, norm=1, post=0, residual_scale=1.0, eps=1e-6, reserved=0) | kw
+    return _capi.TrainNorm(*d.values(), (C.c_int64 * 2)(192, 64), (C.c_int64 * 2)(192, 64), *v.values())
+
+
+@pytest.mark.parametrize("kw,rc,what", [
+    ({"C": 8193}, -2, b"8192"), ({"L": 0}, -1, b"extent"), ({"x_dtype": 0, "y_dtype": 1}, -1, b"types"), ({"x_dtype": 3}, -1, b"types"), ({"norm": 0}, -1, b"norm"),
+    ({"norm": 3}, -1, b"norm"), ({"post": -1}, -1, b"post"), ({"eps": -1.0}, -1, b"eps"), ({"eps": float("nan")}, -1, b"eps"), ({"reserved": 5}, -1, b"reserved"),
+    ({"vectors": {"post_weight": _capi.Vector(0x1000, 0, 2, 0)}}, -1, b"post_weight"), ({"vectors": {"gate": _capi.Vector(0x1000, 0, 5, 0)}}, -1, b"dtype"),
+    ({"vectors": {"weight": _capi.Vector(0x1000, 64, 2, 0)}}, -1, b"batch stride"), ({"vectors": {"shift": _capi.Vector(0x1001, 0, 0, 0)}}, -1, b"aligned")])
+def test_calls_of_the_norm_are_checked(kw, rc, what):
+    lib = _capi.load()
+    assert lib.ksana_sage_train_norm_fwd(C.addressof(_norm_call(**kw)), 0x1000, 0x1000, 0x1000, 0x1000, None, None) == rc
+    assert what in lib.ksana_sage_last_error()
+
+
+def test_buffers_of_the_norm_are_checked():
+    lib, call = _capi.load(), _norm_call()
+    good = C.addressof(call)
+    fwd = lib.ksana_sage_train_norm_fwd
+    assert fwd(good, None, 0x1000, 0x1000, 0x1000, None, None) == -1 and b"x is null" in lib.ksana_sage_last_error()
+    assert fwd(good, 0x1000, 0x1000, None, 0x1000, None, None) == -1 and b"h is null" in lib.ksana_sage_last_error()
+    assert fwd(good, 0x1001, 0x1000, 0x1000, 0x1000, None, None) == -1
+    scaled = _norm_call(residual_scale=0.5)
+    assert fwd(C.addressof(scaled), 0x1000, None, None, 0x1000, None, None) == -1 and b"go with y" in lib.ksana_sage_last_error()
+    grads = (C.c_void_p * 6)(None, 0x1000, None, None, None, None)
+    bwd = lib.ksana_sage_train_norm_bwd
+    assert bwd(good, 0x1000, 0x1000, 0x1000, None, 0x1000, 0x1000, 0x1000, C.addressof(grads), 0x1000, None) == -1 and b"absent" in lib.ksana_sage_last_error()
+    none = (C.c_void_p * 6)()
+    assert bwd(good, 0x1000, 0x1000, 0x1000, None, 0x1000, 0x1000, None, C.addressof(none), 0x1000, None) == -1 and b"dy" in lib.ksana_sage_last_error()
+    assert bwd(good, 0x1000, 0x1000, 0x1000, None, 0x1000, 0x1000, 0x1000, C.addressof(none), None, None) == -1 and b"scratch" in lib.ksana_sage_last_error()
