@@ -11,6 +11,7 @@ allocator.  Repeated calls give the same bits.  Gradients of gradients are refus
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from contextlib import nullcontext
 
 import torch
@@ -31,6 +32,10 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _scratch(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -39,20 +44,16 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-class _AttentionCall:
-    """The library's structure for tensors ``[B, L, H, D]`` as the kernels read them, and its scratch sizes."""
+# The library's structures, packed (ctypes takes three times as long to build one; a call of few tokens costs what its host work does)
+_ATTENTION = struct.Struct("=8ifi16q2Q")  # ksana_sage_train_attn
+_NORM = struct.Struct("=7i2fi4q" + 6 * "Qqii")  # ksana_sage_train_norm
 
-    __slots__ = ("c", "strides", "fwd_bytes", "bwd_bytes")
 
-    def __init__(self, q, k, v, o, is_causal: bool, sm_scale: float | None, k_lens, q_lens):
-        B, Lq, Hq, D = q.shape
-        self.strides = (q.stride(), k.stride(), v.stride(), o.stride())
-        self.c = _capi.TrainAttn(_capi.Shape(B, Hq, k.shape[2], Lq, k.shape[1], D), _DTYPES[q.dtype], int(is_causal),
-                                 D**-0.5 if sm_scale is None else float(sm_scale), 0, _strides(q), _strides(k), _strides(v), _strides(o),
-                                 _ptr(q_lens), _ptr(k_lens))
-        fwd, bwd = C.c_uint64(0), C.c_uint64(0)
-        _capi.check(_capi.load().ksana_sage_train_attn_scratch(C.addressof(self.c), C.addressof(fwd), C.addressof(bwd)), "train_ops.attention")
-        self.fwd_bytes, self.bwd_bytes = fwd.value, bwd.value
+def _attention_call(q, k, v, o, is_causal: bool, sm_scale: float | None, k_lens, q_lens) -> bytes:
+    B, Lq, Hq, D = q.shape
+    return _ATTENTION.pack(B, Hq, k.shape[2], Lq, k.shape[1], D, _DTYPES[q.dtype], is_causal, D**-0.5 if sm_scale is None else sm_scale, 0,
+                           *q.stride(), *k.stride(), *v.stride(), *o.stride(), 0 if q_lens is None else q_lens.data_ptr(),
+                           0 if k_lens is None else k_lens.data_ptr())
 
 
 def _check_attention(q, k, v) -> None:
@@ -64,49 +65,48 @@ def _check_attention(q, k, v) -> None:
 
 
 def _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, want_lse: bool):
-    """(o, lse or None, the call) of ``[B, L, H, D]`` tensors the kernels can read."""
+    """(o, lse or None, bytes of the backward pass's scratch) of ``[B, L, H, D]`` tensors the kernels can read."""
     B, Lq, Hq, D = q.shape
-    o = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    o = _contiguous_like(q)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device) if want_lse else None
     if q.numel() == 0 or k.numel() == 0:
-        return o.zero_(), None if lse is None else lse.fill_(-torch.inf), None
-    call = _AttentionCall(q, k, v, o, is_causal, sm_scale, k_lens, q_lens)
+        return o.zero_(), None if lse is None else lse.fill_(-torch.inf), 0
+    lib, call = _capi.load(), _attention_call(q, k, v, o, is_causal, sm_scale, k_lens, q_lens)
+    nbytes = (C.c_uint64 * 2)()
+    rc = lib.ksana_sage_train_attn_scratch(call, C.addressof(nbytes), C.addressof(nbytes) + 8)
+    if rc != _capi.OK:
+        _capi.check(rc, "train_ops.attention")
     with _on(q.device):
-        scratch = _scratch(call.fwd_bytes, q.device)
-        rc = _capi.load().ksana_sage_train_attn_fwd(C.addressof(call.c), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse),
-                                                    _ptr(scratch), _stream_ptr(q.device))
-    _capi.check(rc, "train_ops.attention")
-    return o, lse, call
+        scratch = _scratch(nbytes[0], q.device)
+        rc = lib.ksana_sage_train_attn_fwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), _ptr(scratch), _stream_ptr(q.device))
+    if rc != _capi.OK:
+        _capi.check(rc, "train_ops.attention")
+    return o, lse, nbytes[1]
 
 
-def _attention_backward(do, q, k, v, o, lse, call, is_causal, sm_scale, k_lens, q_lens, want_q: bool, want_kv: bool):
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if want else None
-                  for t, want in ((q, want_q), (k, want_kv), (v, want_kv)))
+def _attention_backward(do, q, k, v, o, lse, scratch_bytes, is_causal, sm_scale, k_lens, q_lens, want_q: bool, want_kv: bool):
+    dq = _contiguous_like(q) if want_q else None
+    dk, dv = (_contiguous_like(k), _contiguous_like(k)) if want_kv else (None, None)
     if q.numel() == 0 or k.numel() == 0:
         return tuple(None if t is None else t.zero_() for t in (dq, dk, dv))
-    do = _readable(do)
-    # hooks that keep saved tensors elsewhere may give them back laid out and placed otherwise
-    c = call.c
-    if call.strides != (q.stride(), k.stride(), v.stride(), o.stride()):
-        q, k, v, o = (_readable(t) for t in (q, k, v, o))
-        call = _AttentionCall(q, k, v, o, is_causal, sm_scale, k_lens, q_lens)
-        c = call.c
-    else:
-        c.q_lens, c.k_lens = _ptr(q_lens), _ptr(k_lens)
+    # (the saved tensors too: hooks that keep them elsewhere may give them back laid out and placed otherwise)
+    do, q, k, v, o = (_readable(t) for t in (do, q, k, v, o))
+    call, strides = _attention_call(q, k, v, o, is_causal, sm_scale, k_lens, q_lens), _strides(do)
     with _on(q.device):
-        scratch = _scratch(call.bwd_bytes, q.device)
-        rc = _capi.load().ksana_sage_train_attn_bwd(C.addressof(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(),
-                                                    do.data_ptr(), _strides(do), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(scratch), _stream_ptr(q.device))
-    _capi.check(rc, "train_ops.attention, backward")
+        scratch = _scratch(scratch_bytes, q.device)
+        rc = _capi.load().ksana_sage_train_attn_bwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), do.data_ptr(),
+                                                    C.addressof(strides), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(scratch), _stream_ptr(q.device))
+    if rc != _capi.OK:
+        _capi.check(rc, "train_ops.attention, backward")
     return dq, dk, dv
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, is_causal, sm_scale, k_lens, q_lens):
-        o, lse, call = _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, True)
+        o, lse, scratch_bytes = _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, True)
         ctx.save_for_backward(q, k, v, o, lse, k_lens, q_lens)
-        ctx.call, ctx.is_causal, ctx.sm_scale = call, is_causal, sm_scale
+        ctx.options = (scratch_bytes, is_causal, sm_scale)
         return o
 
     @staticmethod
@@ -114,7 +114,7 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, do):
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
         q, k, v, o, lse, k_lens, q_lens = ctx.saved_tensors
-        dq, dk, dv = _attention_backward(do, q, k, v, o, lse, ctx.call, ctx.is_causal, ctx.sm_scale, k_lens, q_lens, want_q, want_k or want_v)
+        dq, dk, dv = _attention_backward(do, q, k, v, o, lse, *ctx.options, k_lens, q_lens, want_q, want_k or want_v)
         return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
 
 
@@ -133,6 +133,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
     if tensor_layout == "HND":
         q, k, v = (t.transpose(1, 2) if t.dim() == 4 else t for t in (q, k, v))
     _check_attention(q, k, v)
+    if sm_scale is not None and not abs(sm_scale) < 3.4e38:
+        raise ValueError(f"sm_scale {sm_scale} is not a finite fp32 number")
     k_lens, q_lens = (_k_lens_arg(n, q.shape[0], q.device, name) for n, name in ((k_lens, "k_lens"), (q_lens, "q_lens")))
     q, k, v = _readable(q), _readable(k), _readable(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -144,7 +146,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
 
 _NORMS = {None: _capi.NORM_NONE, "layer": _capi.NORM_LAYER, "rms": _capi.NORM_RMS}
 _NORM_DTYPES = {torch.bfloat16: _capi.BF16, torch.float16: _capi.FP16, torch.float32: _capi.FP32}
-_NO_VECTOR = _capi.Vector()
 _VECTORS = ("gate", "scale", "shift", "weight", "bias", "post_weight")  # in the order of the library's structure
 
 
@@ -153,32 +154,28 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
 
 
-class _NormCall:
-    """The library's structure for one residual norm, and what it points to."""
-
-    __slots__ = ("c",)
-
-    def __init__(self, x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype):
-        B, L, C_ = x.shape
-        args = []
-        for t in vectors:
-            args.append(_NO_VECTOR if t is None else
-                        _capi.Vector(t.data_ptr(), t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else 0, _NORM_DTYPES[t.dtype], 0))
-        strides = (0, 0) if y is None else y.stride()[:2]
-        self.c = _capi.TrainNorm(B, L, C_, _NORM_DTYPES[x.dtype], _NORM_DTYPES[n_dtype], _NORMS[norm], _NORMS[post_norm], residual_scale, eps, 0,
-                                 (C.c_int64 * 2)(*x.stride()[:2]), (C.c_int64 * 2)(*strides), *args)
+def _norm_call(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype) -> bytes:
+    B, L, C_ = x.shape
+    args = []
+    for t in vectors:
+        if t is None:
+            args += (0, 0, 0, 0)
+        else:
+            args += (t.data_ptr(), t.stride(0) if t.dim() > 1 and t.shape[0] > 1 else 0, _NORM_DTYPES[t.dtype], 0)
+    return _NORM.pack(B, L, C_, _NORM_DTYPES[x.dtype], _NORM_DTYPES[n_dtype], _NORMS[norm], _NORMS[post_norm], residual_scale, eps, 0,
+                      *x.stride()[:2], *((0, 0) if y is None else y.stride()[:2]), *args)
 
 
 def _residual_norm_forward(x, y, call, n_dtype, want_stats: bool):
-    h = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = torch.empty(x.shape, dtype=n_dtype, device=x.device)
+    h = None if y is None else _contiguous_like(x)
+    n = _contiguous_like(x) if n_dtype == x.dtype else torch.empty(x.shape, dtype=n_dtype, device=x.device)
     stats = torch.empty((*x.shape[:2], 4), dtype=torch.float32, device=x.device) if want_stats else None
     if x.numel() == 0:
         return h, n, stats
     with _on(x.device):
-        rc = _capi.load().ksana_sage_train_norm_fwd(C.addressof(call.c), x.data_ptr(), _ptr(y), _ptr(h), n.data_ptr(), _ptr(stats),
-                                                    _stream_ptr(x.device))
-    _capi.check(rc, "train_ops.residual_norm")
+        rc = _capi.load().ksana_sage_train_norm_fwd(call, x.data_ptr(), _ptr(y), _ptr(h), n.data_ptr(), _ptr(stats), _stream_ptr(x.device))
+    if rc != _capi.OK:
+        _capi.check(rc, "train_ops.residual_norm")
     return h, n, stats
 
 
@@ -186,8 +183,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, shift, weight, bias, post_weight, norm, post_norm, residual_scale, eps, n_dtype):
         vectors = (gate, scale, shift, weight, bias, post_weight)
-        call = _NormCall(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype)
-        h, n, stats = _residual_norm_forward(x, y, call, n_dtype, True)
+        h, n, stats = _residual_norm_forward(x, y, _norm_call(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype), n_dtype, True)
         ctx.save_for_backward(x, y, stats, *vectors)
         ctx.options = (norm, post_norm, residual_scale, eps, n_dtype)
         ctx.set_materialize_grads(False)
@@ -201,26 +197,26 @@ class _ResidualNorm(torch.autograd.Function):
         if dh is None and dn is None:
             return (None,) * 13
         n_dtype = ctx.options[-1]
+        # (hooks may have laid the saved tensors out anew)
         x, y = _rows(x), None if y is None else _rows(y)
-        # (made from the saved tensors as they are now: hooks may have moved them and laid them out anew)
-        call = _NormCall(x, y, [None if t is None else _vector_rows(t) for t in vectors], *ctx.options)
+        call = _norm_call(x, y, [None if t is None else _vector_rows(t) for t in vectors], *ctx.options)
         dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
         dh = None if dh is None else dh.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dy = None if y is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        dx, dy = _contiguous_like(x), None if y is None else _contiguous_like(y)
         wanted = ctx.needs_input_grad[2:8]
-        d_vectors = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None for t, want in zip(vectors, wanted)]
+        d_vectors = [_contiguous_like(t) if t is not None and want else None for t, want in zip(vectors, wanted)]
         if x.numel() == 0:
             return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors), *(None,) * 5)
         lib = _capi.load()
-        nbytes = C.c_uint64(0)
-        _capi.check(lib.ksana_sage_train_norm_scratch(C.addressof(call.c), C.addressof(nbytes)), "train_ops.residual_norm, backward")
-        with _on(x.device):
-            scratch = _scratch(nbytes.value, x.device)
-            pointers = (C.c_void_p * 6)(*(_ptr(t) for t in d_vectors))
-            rc = lib.ksana_sage_train_norm_bwd(C.addressof(call.c), x.data_ptr(), _ptr(y), stats.data_ptr(), _ptr(dh), dn.data_ptr(), dx.data_ptr(),
-                                               _ptr(dy), C.addressof(pointers), _ptr(scratch), _stream_ptr(x.device))
-        _capi.check(rc, "train_ops.residual_norm, backward")
+        nbytes, pointers = C.c_uint64(0), (C.c_void_p * 6)(*[_ptr(t) for t in d_vectors])
+        rc = lib.ksana_sage_train_norm_scratch(call, C.addressof(nbytes))
+        if rc == _capi.OK:
+            with _on(x.device):
+                scratch = _scratch(nbytes.value, x.device)
+                rc = lib.ksana_sage_train_norm_bwd(call, x.data_ptr(), _ptr(y), stats.data_ptr(), _ptr(dh), dn.data_ptr(), dx.data_ptr(), _ptr(dy),
+                                                   C.addressof(pointers), _ptr(scratch), _stream_ptr(x.device))
+        if rc != _capi.OK:
+            _capi.check(rc, "train_ops.residual_norm, backward")
         return (dx, dy, *d_vectors, *(None,) * 5)
 
 
@@ -289,6 +285,6 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, 
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *vectors)):
         out = _ResidualNorm.apply(x_rows, y_rows, *vectors, norm, post_norm, residual_scale, eps, n_dtype)
         return (x, out) if y is None else out
-    call = _NormCall(x_rows, y_rows, vectors, norm, post_norm, residual_scale, eps, n_dtype)
+    call = _norm_call(x_rows, y_rows, vectors, norm, post_norm, residual_scale, eps, n_dtype)
     h, n, _ = _residual_norm_forward(x_rows, y_rows, call, n_dtype, False)
     return (x if y is None else h), n

@@ -164,3 +164,24 @@ def test_buffers_of_the_norm_are_checked():
     none = (C.c_void_p * 6)()
     assert bwd(good, 0x1000, 0x1000, 0x1000, None, 0x1000, 0x1000, None, C.addressof(none), 0x1000, None) == -1 and b"dy" in lib.ksana_sage_last_error()
     assert bwd(good, 0x1000, 0x1000, 0x1000, None, 0x1000, 0x1000, 0x1000, C.addressof(none), None, None) == -1 and b"scratch" in lib.ksana_sage_last_error()
+
+
+def test_packed_structures_are_the_librarys():
+    """Byte by byte what the ctypes structures hold."""
+    q, k = torch.empty(2, 7, 6, 64, dtype=torch.float16), torch.empty(2, 9, 3, 128, dtype=torch.float16)[..., :64]
+    lens = torch.zeros(2, dtype=torch.int32)
+    c = _capi.TrainAttn(_capi.Shape(2, 6, 3, 7, 9, 64), 1, 1, 0.25, 0, *(_capi.Strides(*t.stride()) for t in (q, k, k, q)), None, lens.data_ptr())
+    assert bytes(c) == train_ops._attention_call(q, k, k, q, True, 0.25, lens, None)
+    x, g, w = torch.empty(2, 5, 48), torch.empty(2, 3, 48, dtype=torch.bfloat16)[:, 1:2], torch.empty(48, dtype=torch.float16)
+    none = _capi.Vector()
+    n = _capi.TrainNorm(2, 5, 48, 2, 0, 2, 1, 0.5, 1e-5, 0, (C.c_int64 * 2)(240, 48), (C.c_int64 * 2)(240, 48), _capi.Vector(g.data_ptr(), 144, 0, 0), none, none,
+                        _capi.Vector(w.data_ptr(), 0, 1, 0), none, none)
+    assert bytes(n) == train_ops._norm_call(x, x.bfloat16(), [g, None, None, w, None, None], "rms", "layer", 0.5, 1e-5, torch.bfloat16)
+
+
+def test_scales_that_fp32_cannot_hold(monkeypatch):
+    monkeypatch.setattr(train_ops, "_check_attention", lambda *a: None)
+    q = _meta(1, 4, 2, 64)
+    for scale in (float("nan"), float("inf"), -1e39):
+        with pytest.raises(ValueError, match="sm_scale"):
+            train_ops.attention(q, q, q, sm_scale=scale)
