@@ -344,33 +344,31 @@ __device__ __forceinline__ float ds_scale(const TrainAttnParams& p, int bh, int 
   return ldexpf(1.0f, max(-100, min(100, -ex)));
 }
 
-template <int DT, int D, int kCols>
-__global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel(const TrainAttnParams p) {
+// A wave keeps 32 keys and walks tiles of 64 query rows in halves: S = q k^T and dP = dO v^T (a lane holds scores of one key; dP's
+// accumulators start at -d), dv^T += dO^T P, dk^T += q^T dS.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
-  constexpr int kWaves = 4, kKeysWg = kWaves * 32 * kCols, kStages = 2;
+  constexpr int kWaves = 4;
   constexpr int kStage = 2 * T::kBytes + 2 * kTrainTile * 4;  // q, dO, row_l, row_d
   constexpr bool kHalf = DT == KSANA_SAGE_FP16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
-  const int blocks = (p.Lk + kKeysWg - 1) / kKeysWg;
+  const int blocks = (p.Lk + kTrainBlock - 1) / kTrainBlock;
   const TrainPlace place = train_place(p, blocks);
   const int bh = place.bh, block = place.block, b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
-  const int key0 = block * kKeysWg;
+  const int key0 = block * kTrainBlock;
   int first_tile;
   const int tiles = row_tiles_of(p, e, key0, first_tile);
   const TileRange range = run_tiles(p, place, first_tile, tiles);
   if (place.run >= range.runs) return;
 
   const unsigned lds = lds_base();
-  v16f dk[kCols][T::kBlocks], dv[kCols][T::kBlocks];
+  v16f dk[T::kBlocks], dv[T::kBlocks];
 #pragma unroll
-  for (int n = 0; n < kCols; ++n)
-#pragma unroll
-    for (int d = 0; d < T::kBlocks; ++d) dk[n][d] = dv[n][d] = v16f{};
+  for (int d = 0; d < T::kBlocks; ++d) dk[d] = dv[d] = v16f{};
   float scale = 1.0f;
-  int key[kCols];
-#pragma unroll
-  for (int n = 0; n < kCols; ++n) key[n] = key0 + (wave * kCols + n) * 32 + m;
+  const int key = key0 + wave * 32 + m;
   if (range.from < range.to) {
     const uint16_t* q_heads = p.q + b * p.qs.sB + (int64_t)hk * p.group * p.qs.sH;
     const uint16_t* do_heads = p.d_o + b * p.dos.sB + (int64_t)hk * p.group * p.dos.sH;
@@ -379,129 +377,109 @@ __global__ __launch_bounds__(256, kCols == 1 ? 2 : 1) void sage_train_dkv_kernel
     const float* row_d = p.row_d + (int64_t)bh * p.row_pad;
     auto copy = [&](int t) {
       const int at = min(t, range.to - 1) * kTrainTile;
-      const unsigned stage = lds + (t % kStages) * kStage;
+      const unsigned stage = lds + (t & 1) * kStage;
       q_copy.start(p, at, e.rows, stage, wave, lane);
       do_copy.start(p, at, e.rows, stage + T::kBytes, wave, lane);
       // (two waves each, so that every wave has as many copies in flight)
       lds_copy4_at((wave & 1 ? row_d : row_l) + at, lane * 4, stage + 2 * T::kBytes + (wave & 1) * kTrainTile * 4);
     };
     copy(range.from);
-    v4i k[kCols][T::kSteps], v[kCols][T::kSteps];
-#pragma unroll
-    for (int n = 0; n < kCols; ++n) {
-      const int at = min(key[n], e.keys - 1);
-      load_row<D>(p.k + b * p.ks.sB + at * p.ks.sL + hk * p.ks.sH, hh, p.flip, k[n]);
-      load_row<D>(p.v + b * p.vs.sB + at * p.vs.sL + hk * p.vs.sH, hh, 0, v[n]);
+    v4i k[T::kSteps], v[T::kSteps];
+    {
+      const int at = min(key, e.keys - 1);
+      load_row<D>(p.k + b * p.ks.sB + at * p.ks.sL + hk * p.ks.sH, hh, p.flip, k);
+      load_row<D>(p.v + b * p.vs.sB + at * p.vs.sL + hk * p.vs.sH, hh, 0, v);
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
-    const bool idle = key0 + wave * 32 * kCols >= e.keys;  // a wave without keys copies its share
-    const int64_t sees_all = (int64_t)(key0 + (wave + 1) * 32 * kCols - 1) * p.group;  // the first row that sees every key of the wave
+    const bool idle = key0 + wave * 32 >= e.keys;  // a wave without keys copies its share
+    const int64_t sees_all = (int64_t)(key0 + (wave + 1) * 32 - 1) * p.group;  // the first row that sees every key of the wave
 #pragma unroll 1
     for (int t = range.from; t < range.to; ++t) {
       tile_ready<0>();
       copy(t + 1);
       if (idle) continue;
-      const unsigned q_tile = lds + (t % kStages) * kStage, do_tile = q_tile + T::kBytes, stats = do_tile + T::kBytes;
+      const unsigned q_tile = lds + (t & 1) * kStage, do_tile = q_tile + T::kBytes, stats = do_tile + T::kBytes;
       const bool diagonal = p.causal && (int64_t)t * kTrainTile < sees_all;
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        // S, P, dv += P^T dO, dP, dS, dk += dS^T q in turn: what one part leaves is used up by the next, or the
-        // accumulators and the keys and values would not fit the registers of two waves
-        v16f s[kCols], dp[kCols];
-#pragma unroll
-        for (int n = 0; n < kCols; ++n) s[n] = v16f{};
+        // S, P, dv, dP, dS, dk in turn: what one part leaves is used up by the next.  The two results and the wave's keys and values take 192 of
+        // 256 registers; with a half's probabilities formed behind dP's matrix instructions and dS behind those of dv, keys are
+        // read back from memory: 1971 us for 8 heads of 16384 tokens of 128 channels, where this takes 1788.
+        v16f s = v16f{}, dp;
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
           const v4i a = read_row<D>(q_tile + row_at, h, st);
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) s[n] = mfma16<DT>(a, k[n][st], s[n]);
+          s = mfma16<DT>(a, k[st], s);
         }
-        float x[kCols][16];
+        float x[16];
         {
           v4f l[4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) l[g] = *(LdsF4)(uintptr_t)(stats + (32 * h + 8 * g + 4 * hh) * 4);
 #pragma unroll
-          for (int n = 0; n < kCols; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[n][i] = fast_exp2(__fmaf_rn(s[n][i], p.c, l[i >> 2][i & 3]));
+          for (int i = 0; i < 16; ++i) x[i] = fast_exp2(__fmaf_rn(s[i], p.c, l[i >> 2][i & 3]));
         }
         if (diagonal) {
+          int from = (int)min((int64_t)key * p.group - t * kTrainTile - 32 * h - 4 * hh, (int64_t)kTrainTile);
+          pin(from);  // (a branch that stays one)
 #pragma unroll
-          for (int n = 0; n < kCols; ++n) {
-            int from = (int)min((int64_t)key[n] * p.group - t * kTrainTile - 32 * h - 4 * hh, (int64_t)kTrainTile);
-            pin(from);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[n][i] = acc_row(i) < from ? 0.0f : x[n][i];
-          }
+          for (int i = 0; i < 16; ++i) x[i] = acc_row(i) < from ? 0.0f : x[i];
         }
-        v4i pr[kCols][2];
+        v4i pr[2];
 #pragma unroll
-        for (int n = 0; n < kCols; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            pr[n][j] = pack8<DT>(x[n][8 * j], x[n][8 * j + 1], x[n][8 * j + 2], x[n][8 * j + 3], x[n][8 * j + 4], x[n][8 * j + 5], x[n][8 * j + 6], x[n][8 * j + 7]);
+        for (int j = 0; j < 2; ++j)
+          pr[j] = pack8<DT>(x[8 * j], x[8 * j + 1], x[8 * j + 2], x[8 * j + 3], x[8 * j + 4], x[8 * j + 5], x[8 * j + 6], x[8 * j + 7]);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
             const v4i a = read_column<D>(do_tile + column_at, c, 2 * h + j);
-#pragma unroll
-            for (int n = 0; n < kCols; ++n) dv[n][c] = mfma16<DT>(a, pr[n][j], dv[n][c]);
+dv[c] = mfma16<DT>(a, pr[j], dv[c]);
           }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const v4f d = *(LdsF4)(uintptr_t)(stats + (kTrainTile + 32 * h + 8 * g + 4 * hh) * 4);
 #pragma unroll
-          for (int n = 0; n < kCols; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dp[n][4 * g + i] = d[i];
+          for (int i = 0; i < 4; ++i) dp[4 * g + i] = d[i];
         }
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
           const v4i a = read_row<D>(do_tile + row_at, h, st);
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) dp[n] = mfma16<DT>(a, v[n][st], dp[n]);
+dp = mfma16<DT>(a, v[st], dp);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (what the next product reads early stands in registers that are not there)
 #pragma unroll
-        for (int n = 0; n < kCols; ++n) {
+        for (int i = 0; i < 16; ++i) x[i] *= kHalf ? dp[i] * scale : dp[i];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[n][i] *= kHalf ? dp[n][i] * scale : dp[n][i];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            pr[n][j] = pack8<DT>(x[n][8 * j], x[n][8 * j + 1], x[n][8 * j + 2], x[n][8 * j + 3], x[n][8 * j + 4], x[n][8 * j + 5], x[n][8 * j + 6], x[n][8 * j + 7]);
-        }
+        for (int j = 0; j < 2; ++j)
+          pr[j] = pack8<DT>(x[8 * j], x[8 * j + 1], x[8 * j + 2], x[8 * j + 3], x[8 * j + 4], x[8 * j + 5], x[8 * j + 6], x[8 * j + 7]);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
             const v4i a = read_column<D>(q_tile + column_at, c, 2 * h + j);
-#pragma unroll
-            for (int n = 0; n < kCols; ++n) dk[n][c] = mfma16<DT>(a, pr[n][j], dk[n][c]);
+dk[c] = mfma16<DT>(a, pr[j], dk[c]);
           }
       }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   const float unshift = fast_exp2(-kBackwardShift<DT>);
+  const bool exists = key < p.Lk;
+  if (key >= e.keys) {
 #pragma unroll
-  for (int n = 0; n < kCols; ++n) {
-    const bool exists = key[n] < p.Lk;
-    if (key[n] >= e.keys) {
-#pragma unroll
-      for (int c = 0; c < T::kBlocks; ++c) dk[n][c] = dv[n][c] = v16f{};
-    }
-    if (range.runs > 1) {
-      float* at = p.part + (((int64_t)place.cut * p.runs + place.run) * kTrainBlock + key[n] - key0) * 2 * D;
-      store_column_part<D>(dk[n], p.sm_scale * unshift / scale, at, hh, exists);
-      store_column_part<D>(dv[n], unshift, at + D, hh, exists);
-      continue;
-    }
-    const int64_t at = (((int64_t)b * p.Lk + min(key[n], p.Lk - 1)) * p.Hkv + hk) * D;
-    store_column<DT, D>(dk[n], p.sm_scale * unshift / scale, p.dk + at, hh, exists);
-    store_column<DT, D>(dv[n], unshift, p.dv + at, hh, exists);
+    for (int c = 0; c < T::kBlocks; ++c) dk[c] = dv[c] = v16f{};
   }
+  if (range.runs > 1) {
+    float* at = p.part + (((int64_t)place.cut * p.runs + place.run) * kTrainBlock + key - key0) * 2 * D;
+    store_column_part<D>(dk, p.sm_scale * unshift / scale, at, hh, exists);
+    store_column_part<D>(dv, unshift, at + D, hh, exists);
+    return;
+  }
+  const int64_t at = (((int64_t)b * p.Lk + min(key, p.Lk - 1)) * p.Hkv + hk) * D;
+  store_column<DT, D>(dk, p.sm_scale * unshift / scale, p.dk + at, hh, exists);
+  store_column<DT, D>(dv, unshift, p.dv + at, hh, exists);
 }
 
 // A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
@@ -888,7 +866,6 @@ void join_bwd(const TrainAttnParams& p, int64_t all, hipStream_t s) {
 
 template <int DT, int D>
 hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
-  constexpr int kCols = 1;
   hipError_t e = hipSuccess;
   // in bf16 the rows' numbers come along with dq, where that is wanted
   if (DT == KSANA_SAGE_FP16 || p.dq == nullptr) {
@@ -910,10 +887,10 @@ hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
   if (p.dk == nullptr) return hipSuccess;
   constexpr int kLds = 2 * (2 * Tile<D>::kBytes + 2 * kTrainTile * 4);
   static LdsRequest request;
-  e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D, kCols>), kLds);
+  e = request.make(reinterpret_cast<const void*>(&sage_train_dkv_kernel<DT, D>), kLds);
   if (e != hipSuccess) return e;
   take_cut(p, cuts.dkv);
-  sage_train_dkv_kernel<DT, D, kCols><<<workgroups(p), 256, kLds, s>>>(p);
+  sage_train_dkv_kernel<DT, D><<<workgroups(p), 256, kLds, s>>>(p);
   join_bwd<DT, D, true>(p, p.Lk, s);
   return hipGetLastError();
 }

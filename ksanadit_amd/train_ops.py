@@ -33,7 +33,7 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
 
 
 def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t) if t.is_contiguous() and not t.has_names() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _scratch(nbytes: int, device) -> torch.Tensor | None:
