@@ -780,19 +780,22 @@ void fill_in(TrainAttnParams& p) {
   p.norm_blocks = p.norm_q_blocks + (p.dtype == KSANA_SAGE_FP16 ? (p.Lk + kNormRows - 1) / kNormRows : 0);
 }
 
-// How a launch of `blocks` blocks that walk at most `tiles` tiles each is cut, with `bytes` of results to a block.  Two workgroups to each of
-// 256 compute units; in units of a tile's time (about 2 us with both there), a workgroup costs kSetup besides its tiles, a launch
-// that joins runs kJoin and what its bytes take, written and read.  Blocks that cost the same: as many as fill whole rounds are
-// left whole, the others are cut so that they fill one more.  Others (`differ`, `share` of the tiles being there at all): runs of one
-// length, which even out what a workgroup has to do.
+// How a launch of `blocks` blocks that walk at most `tiles` tiles each is cut, with `bytes` of results to a block.  `places`: two
+// workgroups to each of 256 compute units, three of dk and dv of 64 channels (12 heads of 4096 tokens: 113 + 11 us, counted as two 142).
+// In units of a tile's time (about 2 us with all there), a workgroup costs kSetup besides its tiles, a launch that joins runs kJoin and
+// what its bytes take, written and read.  Blocks that cost the same: as many as fill whole rounds are
+// left whole, the others are cut so that they fill one more.  Others (`differ`; of a causal call's tiles half are there): all whole or all in
+// runs of one length.  Whole ones come with the longest first, so that the short ones fill up what those leave of the last round, unless
+// there are so few that two long ones share a place; runs need whole rounds, or half a run's time besides their mean.  (16 heads of 8192
+// causal tokens: rows whole 276 + 372 us, forward and dq, in two runs 291 + 387 and 34 for the joins; on 4 key heads, dk and dv: keys whole
+// 1120, in 3 runs 594 + 12, in 5 618 + 17, in 7 587 + 21.)
 struct TrainCut {
   int whole, cut, runs, run_tiles;
   uint64_t part(int width) const { return runs > 1 ? (uint64_t)cut * runs * kTrainBlock * width * 4 : 0; }
 };
-TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double share) {
+TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double share, int places) {
   constexpr double kSetup = 2.0, kJoin = 2.0, kBytesPerTile = 4e12 * 2e-6;
-  constexpr int kPlaces = 512;
-  const int whole = differ ? 0 : (int)(blocks / kPlaces * kPlaces);
+  const int whole = differ ? 0 : (int)(blocks / places * places);
   const int64_t rest = blocks - whole;
   double least = 1e30;
   int best = tiles;  // of a run
@@ -800,8 +803,16 @@ TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double sha
   for (int n = 1; n <= most; ++n) {
     const int each = (tiles + n - 1) / n;
     const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * rest * bytes * share / kBytesPerTile;
-    const double cost = differ ? std::max((double)blocks * tiles * share / kPlaces * (1.0 + kSetup / each) + 0.5 * each, each + kSetup) + join
-                               : (double)((rest * n + kPlaces - 1) / kPlaces) * (each + kSetup) + join;
+    const double number = rest * (share < 1.0 && n > 1 ? share * tiles / each + 0.5 : (double)((tiles + each - 1) / each));  // of runs that are there
+    double cost = std::ceil(number / places) * (each + kSetup);
+    if (differ && n == 1 && share < 1.0) {
+      cost = std::max(tiles + kSetup, rest * (share * tiles + kSetup) / places);
+      // (the (i places + 1)-th longest block is one of i + 1 in its place)
+      for (int i = 1; i < 8 && (int64_t)i * places < rest; ++i) cost = std::max(cost, (i + 1) * (tiles * (1.0 - (double)i * places / rest) + kSetup));
+    } else if (differ) {
+      cost = std::min(cost, std::max(number * (each + kSetup) / places + 0.5 * each, each + kSetup));
+    }
+    cost += join;
     if (cost < 0.97 * least) {
       least = cost;
       best = each;
@@ -820,8 +831,8 @@ TrainCuts train_cuts(const TrainAttnParams& p) {
   const int key_tiles = (p.Lk + kTrainTile - 1) / kTrainTile, row_tiles = (int)((rows + kTrainTile - 1) / kTrainTile);
   const bool differ = p.causal || p.q_lens != nullptr || p.k_lens != nullptr;
   const double share = p.causal && p.Lq > 1 ? 0.5 : 1.0, row_bytes = 4.0 * std::min<int64_t>(rows, kTrainBlock) * p.D;
-  const TrainCut of_rows = cut_of(row_blocks, key_tiles, row_bytes, differ, share);
-  return TrainCuts{of_rows, cut_of(key_blocks, row_tiles, 8.0 * std::min(p.Lk, kTrainBlock) * p.D, differ, share), of_rows};
+  const TrainCut of_rows = cut_of(row_blocks, key_tiles, row_bytes, differ, share, 512);
+  return TrainCuts{of_rows, cut_of(key_blocks, row_tiles, 8.0 * std::min(p.Lk, kTrainBlock) * p.D, differ, share, p.D == 64 ? 768 : 512), of_rows};
 }
 void take_cut(TrainAttnParams& p, const TrainCut& c) {
   p.whole = c.whole;
