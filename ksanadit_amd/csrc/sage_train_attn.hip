@@ -526,6 +526,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       l = p.row_l[(int64_t)bh * p.row_pad + r];
       d = p.row_d[(int64_t)bh * p.row_pad + r];
       scale = ds_scale(p, bh, lane);
+      l += (float)__builtin_amdgcn_frexp_expf(scale) - 1.0f;  // (a power of two: P takes dS's scale along)
     } else {
       // dO is here: what sage_train_rows_kernel would have to read it once more for is formed on the way, and kept for dk and dv
       const int at = row_position(p, r), h = hk * p.group + r - at * p.group;
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       auto gradients = [&](int h) {
         return [&, h](int i) {
 #pragma unroll
-          for (int j = i * kEach; j < (i + 1) * kEach; ++j) s[h][j] *= kHalf ? dp[h][j] * scale : dp[h][j];
+          for (int j = i * kEach; j < (i + 1) * kEach; ++j) s[h][j] *= dp[h][j];
           if ((i + 1) * kEach % 8 == 0) {
             const int f = (i + 1) * kEach / 8 - 1;
             ds[h][f] = pack8<DT>(s[h][8 * f], s[h][8 * f + 1], s[h][8 * f + 2], s[h][8 * f + 3], s[h][8 * f + 4], s[h][8 * f + 5], s[h][8 * f + 6], s[h][8 * f + 7]);
