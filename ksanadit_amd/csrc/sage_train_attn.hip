@@ -64,6 +64,14 @@ __device__ __forceinline__ void load_row(const uint16_t* row, int hh, uint32_t f
   }
 }
 
+// The lane's row is here from now on.  Without this the compiler waits where its values are used, for every load under way: in a loop
+// that is the next tile, in every turn.
+template <int N>
+__device__ __forceinline__ void row_ready(v4i (&row)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(row[s]));
+}
+
 // Numbers of the keys of accumulator i of 32-key block t: 32 t + 8 (i / 4) + 4 hh + i % 4
 __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
@@ -198,6 +206,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_fwd_kernel(const TrainAttnP
     typedef std::integral_constant<bool, true> Last;
     v16f s0[2], s1[2];
     tile_ready<0>();
+    row_ready(q);
     copy_keys(range.from + 1);
     copy_values(range.from);
     if (!idle) {
@@ -391,6 +400,8 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
       load_row<D>(p.v + b * p.vs.sB + at * p.vs.sL + hk * p.vs.sH, hh, 0, v);
     }
     if constexpr (kHalf) scale = ds_scale(p, bh, lane);
+    row_ready(k);
+    row_ready(v);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     const bool idle = key0 + wave * 32 >= e.keys;  // a wave without keys copies its share
     const int64_t sees_all = (int64_t)(key0 + (wave + 1) * 32 - 1) * p.group;  // the first row that sees every key of the wave
@@ -548,6 +559,8 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
         p.row_d[(int64_t)bh * p.row_pad + row] = d;
       }
     }
+    row_ready(q);
+    row_ready(g);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
     const int limit = p.causal ? min(e.keys, row_position(p, row) + 1) : e.keys;
     const int all_see = p.causal ? min(e.keys, row_position(p, min(row0 + wave * 32, e.rows - 1)) + 1) : e.keys;
