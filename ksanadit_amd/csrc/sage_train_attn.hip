@@ -9,6 +9,11 @@
 // atomic additions of all workgroups: their order would change the result from call to call.
 //
 // P and dS are rounded to the tensors' type where they become matrix operands; S, dP, all sums and accumulators are fp32.
+//
+// Long sequences are bound by what the matrix pipes draw: with them busy 63 % (forward), 76 % (dq) and 67 % (dk and dv) of the time the
+// clock falls from 2.4 to 1.7 - 1.8 GHz.  20 heads of 32760 bf16 tokens of 128 channels: forward 9.4 ms, dq 12.6, dk and dv 17.2, that
+// is 1170, 1310 and 1280 TFLOP/s of the products that they form (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
+// and what a workgroup does besides its loop, 32760 rows on 512 keys, 40 heads: 420, 580 and 640 us; a few rows by a chain of latencies.
 #include "sage_train_device.h"
 
 #include <algorithm>
@@ -80,6 +85,7 @@ __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + 
 // A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys, two waves to a SIMD.  While the
 // probabilities of tile t are formed and multiplied with its values, the scores of tile t + 1 are: a few vector instructions stand behind
 // every matrix instruction and run beside it.  So values are wanted a step after their keys; each have two places in LDS.
+// 8 heads of 16384 tokens: bf16 1004 us, 1095 TFLOP/s, fp16 1063; of 64 channels 669 us, where exponentials count twice as much.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_fwd_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -257,7 +263,7 @@ template <int DT>
 __device__ __forceinline__ float row_minus(float lse) {
   return lse == -INFINITY ? -INFINITY : kBackwardShift<DT> - lse * kLog2e;
 }
-constexpr int kNormRows = 64;  // rows of a workgroup (256 and a loop: 18.8 us of 40 heads of 1560 rows where this takes 8)
+constexpr int kNormRows = 64;  // rows of a workgroup (256 and a loop: 18.8 us of 40 heads of 1560 rows where this takes 10)
 
 // Per query row -log2(e) lse (plus the shift) and -sum(dO o); in fp16 besides the largest squared norms of rows of dO and of v per block of rows.
 template <int DT, int D>
@@ -354,7 +360,8 @@ __device__ __forceinline__ float ds_scale(const TrainAttnParams& p, int bh, int 
 }
 
 // A wave keeps 32 keys and walks tiles of 64 query rows in halves: S = q k^T and dP = dO v^T (a lane holds scores of one key; dP's
-// accumulators start at -d), dv^T += dO^T P, dk^T += q^T dS.
+// accumulators start at -d), dv^T += dO^T P, dk^T += q^T dS.  The other wave of the SIMD works beside a wave's vector instructions.
+// 8 heads of 16384 tokens: bf16 1853 us, 1190 TFLOP/s, fp16 1995; of 64 channels 1029 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -416,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
       for (int h = 0; h < 2; ++h) {
         // S, P, dv, dP, dS, dk in turn: what one part leaves is used up by the next.  The two results and the wave's keys and values take 192 of
         // 256 registers; with a half's probabilities formed behind dP's matrix instructions and dS behind those of dv, keys are
-        // read back from memory: 1971 us for 8 heads of 16384 tokens of 128 channels, where this takes 1788.
+        // read back from memory: 8 % longer for 8 heads of 16384 tokens of 128 channels.  (A loop over the halves for the same reason.)
         v16f s = v16f{}, dp;
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
@@ -446,7 +453,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
             const v4i a = read_column<D>(do_tile + column_at, c, 2 * h + j);
-dv[c] = mfma16<DT>(a, pr[j], dv[c]);
+            dv[c] = mfma16<DT>(a, pr[j], dv[c]);
           }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -457,7 +464,7 @@ dv[c] = mfma16<DT>(a, pr[j], dv[c]);
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) {
           const v4i a = read_row<D>(do_tile + row_at, h, st);
-dp = mfma16<DT>(a, v[st], dp);
+          dp = mfma16<DT>(a, v[st], dp);
         }
         __builtin_amdgcn_sched_barrier(0);  // (what the next product reads early stands in registers that are not there)
 #pragma unroll
@@ -470,7 +477,7 @@ dp = mfma16<DT>(a, v[st], dp);
 #pragma unroll
           for (int c = 0; c < T::kBlocks; ++c) {
             const v4i a = read_column<D>(q_tile + column_at, c, 2 * h + j);
-dk[c] = mfma16<DT>(a, pr[j], dk[c]);
+            dk[c] = mfma16<DT>(a, pr[j], dk[c]);
           }
       }
     }
@@ -494,7 +501,8 @@ dk[c] = mfma16<DT>(a, pr[j], dk[c]);
 }
 
 // A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
-// k^T dS^T.  A half's vector work stands behind matrix instructions of the other half.
+// k^T dS^T.  A half's vector work stands behind matrix instructions of the other half (in front of them: 1371 us where this takes 1308).
+// 8 heads of 16384 tokens: bf16 1332 us, 1240 TFLOP/s, fp16 1433; of 64 channels 816 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -655,7 +663,8 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
 
 // ------------------------------------------------------------------------------------------------------------ runs joined
 
-// Eight channels per lane; kSlots groups of lanes share a row's runs and add their sums up in a fixed order.
+// Bound by the bytes of the runs and, of few rows, by latency.  Eight channels per lane; kSlots groups of lanes share a row's runs and
+// add their sums up in a fixed order (from kManyRuns runs on; 64 runs of one row, 40 heads: 6 us).
 template <int kSlots>
 __device__ __forceinline__ void add_slots(float (&x)[9], int slot, int lanes, int lane) {
   if constexpr (kSlots > 1) {
@@ -857,7 +866,7 @@ void take_cut(TrainAttnParams& p, const TrainCut& c) {
 unsigned workgroups(const TrainAttnParams& p) { return (unsigned)(p.whole + (int64_t)p.cut * p.runs); }
 // Rows of a block that the joins look at
 int joined_rows(int64_t all) { return (int)std::min<int64_t>(all, kTrainBlock); }
-constexpr int kManyRuns = 16;  // from here on lanes share a row's runs
+constexpr int kManyRuns = 16;  // from here on lanes share a row's runs: one lane after the other, 64 runs take 20 us where this takes 6
 constexpr int64_t kMostGroups = 1 << 23;
 
 template <int DT, int D>

@@ -55,7 +55,7 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float x
 // A thread's columns of a row: 8 (v T + thread) .., T the workgroup's threads, eight at an access whatever the row's address (the GPU takes
 // 16-byte accesses at any).  kWhole: C is a multiple of eight.  Else a row's last eight columns overlap those before: both threads compute and
 // store the same values there, and sums leave out the second one's (`own`).  Value by value instead, 8331 rows of 1153 took 57 us
-// forward and 157 backward where this takes 24 and 55.
+// forward and 157 backward where this takes 25 and 45.
 template <bool kWhole, int kVecs>
 struct Columns {
   int C, T, thread;
@@ -116,7 +116,9 @@ struct Columns {
           w[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
         }
       }
-      // (past the caches: a gigabyte of other traffic lies between this and its next reader)
+      // First out of the caches: the rows that come next and the next call's are worth more of them.  8704 rows of 5120 fp32 channels 102 us,
+      // kept like others 113; 32760 bf16 rows backward 402 and 416; with a reader of both results right behind, 1560 rows 34.0 and
+      // 34.9, 8192 rows 119 and 113, 16384 rows 230 and 237.
       typedef int Piece __attribute__((ext_vector_type(4), aligned(2)));
       const Piece lo = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
       if constexpr (kStream)
@@ -271,7 +273,9 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_fwd_kernel(const 
   const char* x_at = static_cast<const char*>(p.x) + (rows.b * p.x_sB + rows.from * p.x_sL) * kSize<XT>;
   const char* y_at = static_cast<const char*>(p.y) + (rows.b * p.y_sB + rows.from * p.y_sL) * kSize<YT>;
   const bool has_y = p.y != nullptr;
-  // Two rows on their way while one is worked on: with one, 32760 rows of 5120 bf16 channels took 383 us, 3.5 TB/s.
+  // Two rows on their way while one is worked on: 32760 rows of 5120 bf16 channels 276 us, 4.9 TB/s, with one row on its way 383.  (A copy
+  // reaches 5.0.)  fp32 rows beside bf16 ones, 8704 of 5120: 97 us, 5.5 TB/s: more than a copy's, part of what
+  // is read is in the last-level cache still when a call follows another on the same rows.
   struct Rows {
     Raw<XT> x[kVecs];
     Raw<YT> y[kVecs];
@@ -347,6 +351,7 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_fwd_kernel(const 
   }
 }
 
+// Reads x, y, dh and dn again rather than keep normalised rows: 32760 rows of 5120 bf16 channels 400 us, 5.0 TB/s.
 template <int XT, int YT, bool kWhole, int kVecs>
 __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const TrainNormParams p) {
   __shared__ float lds[2][kMaxWaves][2];
@@ -473,7 +478,8 @@ __global__ __launch_bounds__(kMaxThreads) void sage_train_norm_bwd_kernel(const 
 }
 
 // The workgroups' sums added up, 16 columns to a workgroup, its 64 groups of threads sharing the parts; and what follows from the sums.
-// Bound by latency: everything a thread reads of an entry (24 values of up to 512 parts) is on its way before the first is added.
+// Bound by latency: everything a thread reads of an entry (24 values of up to 512 parts) is on its way before the first is added.  One entry of
+// 5120 columns 10 us, three of 1153 12 us.
 constexpr int kJoinColumns = 16, kSlots = 64, kAtOnce = 8;
 __global__ __launch_bounds__(1024) void sage_train_norm_vectors_kernel(const TrainNormParams p) {
   constexpr int kWaves = kJoinColumns * kSlots / 64;
