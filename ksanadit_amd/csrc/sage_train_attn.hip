@@ -851,7 +851,7 @@ struct TrainCuts {
 TrainCuts train_cuts(const TrainAttnParams& p) {
   const int64_t heads = (int64_t)p.B * p.Hkv, rows = (int64_t)p.Lq * p.group;
   const int64_t row_blocks = heads * ((rows + kTrainBlock - 1) / kTrainBlock), key_blocks = heads * ((p.Lk + kTrainBlock - 1) / kTrainBlock);
-  const int key_tiles = (p.Lk + kTrainTile - 1) / kTrainTile, row_tiles = (int)((rows + kTrainTile - 1) / kTrainTile);
+  const int key_tiles = ((p.causal ? std::min(p.Lk, p.Lq) : p.Lk) + kTrainTile - 1) / kTrainTile, row_tiles = (int)((rows + kTrainTile - 1) / kTrainTile);
   const bool differ = p.causal || p.q_lens != nullptr || p.k_lens != nullptr;
   const double share = p.causal && p.Lq > 1 ? 0.5 : 1.0, row_bytes = 4.0 * std::min<int64_t>(rows, kTrainBlock) * p.D;
   const TrainCut of_rows = cut_of(row_blocks, key_tiles, row_bytes, differ, share, 512);

@@ -127,7 +127,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
     and give no gradient; keys and values behind ``k_lens[b]``, query rows and their gradients behind ``q_lens[b]`` are not
     read.  Int32 counts on the device are read by the kernels, in the backward pass again (writing to them in between is an
     error, as for the tensors).  Scores, softmax statistics and sums are fp32; probabilities and their gradients are rounded to the tensors' type
-    where they are multiplied on, in fp16 scaled by powers of two that keep small gradients representable."""
+    where they are multiplied on, in fp16 scaled by powers of two that keep small gradients representable.  Keys that only causal masking
+    hides have the weight 0, as in a product of matrices: not-a-numbers and infinities among them may show in the rows before."""
     if tensor_layout not in ("NHD", "HND"):
         raise ValueError(f"tensor_layout {tensor_layout!r} unknown")
     if tensor_layout == "HND":

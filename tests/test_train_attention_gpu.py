@@ -309,6 +309,16 @@ def test_cut_loops_against_uncut_ones(hip_device, Hq, Hkv, Lq, Lk, causal):
         assert ((x - y).abs() <= most).all()
 
 
+@gpu
+@pytest.mark.parametrize("B,Hq,Hkv,Lq,Lk,D,dtype,k_lens,q_lens", [
+    (1, 8, 2, 1500, 1500, 64, torch.bfloat16, None, None), (2, 6, 2, 600, 2300, 64, torch.float16, None, None), (1, 5, 1, 1900, 700, 128, torch.bfloat16, None, None),
+    (1, 3, 1, 40, 9000, 128, torch.float16, None, None), (4, 48, 48, 290, 290, 128, torch.bfloat16, None, None),
+    (4, 48, 16, 290, 270, 64, torch.float16, [270, 0, 131, 64], [290, 5, 129, 1]), (2, 4, 4, 200, 6000, 64, torch.bfloat16, [6000, 77], None)])
+def test_causal_blocks_whole_and_in_runs(hip_device, B, Hq, Hkv, Lq, Lk, D, dtype, k_lens, q_lens):
+    """Blocks of which later ones see more: more of them than the card holds at once, and few, with runs that some do not have."""
+    _check(*_draw(13, B, Hq, Hkv, Lq, Lk, D, dtype), hip_device, causal=True, k_lens=k_lens, q_lens=q_lens)
+
+
 # ------------------------------------------------------------------------------------------------ where the package offers it
 @gpu
 def test_the_backend_trains_where_it_is_asked_to(hip_device):
