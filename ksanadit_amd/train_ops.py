@@ -28,6 +28,8 @@ def _on(device: torch.device):
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """The tensor as the kernels read it (``_usable``), a contiguous one at an address that 16 does not divide included."""
+    if t.is_contiguous() and t.shape[3] % 8 == 0 and t.data_ptr() % 16 == 0:  # (looking at strides costs more than a kernel of few tokens leaves)
+        return t
     t = _usable(t)
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -152,7 +154,7 @@ _VECTORS = ("gate", "scale", "shift", "weight", "bias", "post_weight")  # in the
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``[B, L, C]`` with contiguous channels and strides the kernels take (an expanded tensor has a stride of 0, which they do)."""
-    return t if t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(2) == 1 and t.stride(0) >= 0 and t.stride(1) >= 0 else t.contiguous()
 
 
 def _norm_call(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype) -> bytes:
@@ -221,19 +223,27 @@ class _ResidualNorm(torch.autograd.Function):
         return (dx, dy, *d_vectors, *(None,) * 5)
 
 
+def _wants_gradient(*tensors) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
 def _norm_vector(name: str, t: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor | None:
     """A vector as the kernels read it, its channels contiguous: ``[C]``, or ``[B, C]`` / ``[B, 1, C]`` with one for every batch entry or
     one for all of them (also slices of such a tensor, whose entries lie further apart)."""
     if t is None:
         return None
     B, _, C_ = x.shape
-    if t.device != x.device or t.dtype not in _NORM_DTYPES:
+    if t.get_device() != x.get_device() or t.dtype not in _NORM_DTYPES:
         raise ValueError(f"{name} must be float32, float16 or bfloat16 on {x.device}, got {t.dtype} on {t.device}")
-    shape = tuple(t.shape)
-    own = name in ("gate", "scale", "shift")
-    if shape != (C_,) and not (own and shape in ((B, C_), (1, C_), (B, 1, C_), (1, 1, C_))):
-        raise ValueError(f"{name} must be [{C_}]" + (f", [{B}, {C_}] or [{B}, 1, {C_}]" if own else "") + f", got {shape}")
-    return _vector_rows(t)
+    shape = t.shape
+    if shape != (C_,):
+        own = name in ("gate", "scale", "shift")
+        if not (own and shape in ((B, C_), (1, C_), (B, 1, C_), (1, 1, C_))):
+            raise ValueError(f"{name} must be [{C_}]" + (f", [{B}, {C_}] or [{B}, 1, {C_}]" if own else "") + f", got {tuple(shape)}")
+    return t if t.is_contiguous() else _vector_rows(t)
 
 
 def _vector_rows(t: torch.Tensor) -> torch.Tensor:
@@ -264,7 +274,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, 
     for t in (x,) if y is None else (x, y):
         if not t.is_cuda:
             raise RuntimeError(f"residual_norm needs tensors on a HIP device; there is no CPU path (got device {t.device})")
-        if t.dtype not in _NORM_DTYPES or t.device != x.device:
+        if t.dtype not in _NORM_DTYPES or t.get_device() != x.get_device():
             raise ValueError(f"x and y must be float32, float16 or bfloat16 on one device, got {t.dtype} on {t.device}")
     if y is None:
         if gate is not None or post_norm is not None or post_weight is not None or residual_scale != 1.0:
@@ -283,7 +293,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, 
     vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, (gate, scale, shift, weight, bias, post_weight))]
     x_rows, y_rows = _rows(x), None if y is None else _rows(y)
     residual_scale, eps = float(residual_scale), float(eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, *vectors)):
+    if torch.is_grad_enabled() and _wants_gradient(x, y, *vectors):
         out = _ResidualNorm.apply(x_rows, y_rows, *vectors, norm, post_norm, residual_scale, eps, n_dtype)
         return (x, out) if y is None else out
     call = _norm_call(x_rows, y_rows, vectors, norm, post_norm, residual_scale, eps, n_dtype)
