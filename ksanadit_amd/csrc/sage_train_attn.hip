@@ -29,6 +29,7 @@ extern __shared__ __align__(1024) char train_lds[];
 __device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)train_lds; }
 
 constexpr int kTrainBlock = 128;  // query rows, or keys, of a workgroup
+constexpr int kMostRuns = 128;    // of a block
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // Rounded to fp16, probabilities relative to a row's largest would lose bits from 2^-14 on and vanish at 2^-25; scaled up as far as
 // the format goes, they do so a factor of 2^6 (forward, where the reference point may lag by 2^kLazy) or 2^15 (backward) later.
@@ -681,7 +682,8 @@ __device__ __forceinline__ void add_slots(float (&x)[9], int slot, int lanes, in
   }
 }
 
-// A run's sums stand against a reference point of its own.
+// A run's sums stand against a reference point of its own.  With slots a row has a workgroup, which asks for all it reads before it looks at any
+// of it (reference points one load after the other, then sums: 6.3 us for the 64 runs of a row of 40 heads, this 4).
 template <int DT, int D, int kSlots>
 __global__ __launch_bounds__(256) void sage_train_join_fwd_kernel(const TrainAttnParams p, const int groups) {
   constexpr int kLanes = D / 8, kRows = 256 / (kLanes * kSlots);
@@ -697,33 +699,64 @@ __global__ __launch_bounds__(256) void sage_train_join_fwd_kernel(const TrainAtt
   if (runs == 1 || r >= all_rows) return;  // (with slots, of the whole workgroup)
   const int64_t first = (int64_t)place.cut * p.runs * kTrainBlock + i;
   const float2* ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.cut * p.runs * kTrainBlock * D);
+  auto point = [&](int j) { return ml[first + (int64_t)j * kTrainBlock]; };
+  auto values = [&](int j) { return reinterpret_cast<const float4*>(p.part + (first + (int64_t)j * kTrainBlock) * D + 8 * lane); };
   float sum[9] = {}, top = -INFINITY;
-  if (r < e.rows) {
-    for (int j = lane; j < runs; j += kLanes) {  // (a lane after the other: 20 us for the 64 runs of one row, 4 so)
-      const float2 x = ml[first + (int64_t)j * kTrainBlock];
-      top = x.y != 0.0f ? fmaxf(top, -x.x) : top;  // (a run whose keys are all hidden has no reference point)
+  auto add = [&](const float4& lo, const float4& hi, float factor) {
+    sum[0] = __fmaf_rn(lo.x, factor, sum[0]);
+    sum[1] = __fmaf_rn(lo.y, factor, sum[1]);
+    sum[2] = __fmaf_rn(lo.z, factor, sum[2]);
+    sum[3] = __fmaf_rn(lo.w, factor, sum[3]);
+    sum[4] = __fmaf_rn(hi.x, factor, sum[4]);
+    sum[5] = __fmaf_rn(hi.y, factor, sum[5]);
+    sum[6] = __fmaf_rn(hi.z, factor, sum[6]);
+    sum[7] = __fmaf_rn(hi.w, factor, sum[7]);
+  };
+  if constexpr (kSlots > 1) {
+    constexpr int kOwn = (kMostRuns + kSlots - 1) / kSlots;
+    static_assert(kMostRuns <= 256);
+    __shared__ float factors[kMostRuns], of_wave[2][4];
+    if (r < e.rows) {  // (the whole workgroup)
+      const int j = threadIdx.x;
+      const float2 x = j < runs ? point(j) : make_float2(0.0f, 0.0f);
+      float4 lo[kOwn], hi[kOwn];
+#pragma unroll
+      for (int n = 0; n < kOwn; ++n) {
+        const float4* o = values(min(slot + n * kSlots, runs - 1));
+        lo[n] = o[0];
+        hi[n] = o[1];
+      }
+      const float most = over_lanes<Max>(x.y != 0.0f ? -x.x : -INFINITY);  // (a run whose keys are all hidden has no reference point)
+      if ((j & 63) == 0) of_wave[0][j >> 6] = most;
+      __syncthreads();
+      top = fmaxf(fmaxf(of_wave[0][0], of_wave[0][1]), fmaxf(of_wave[0][2], of_wave[0][3]));
+      const float factor = x.y != 0.0f ? fast_exp2(-x.x - top) : 0.0f;
+      if (j < kMostRuns) factors[j] = factor;
+      const float total = over_lanes<Sum>(x.y * factor);
+      if ((j & 63) == 0) of_wave[1][j >> 6] = total;
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < kOwn; ++n)
+        if (slot + n * kSlots < runs) add(lo[n], hi[n], factors[slot + n * kSlots]);
+    }
+    add_slots<kSlots>(sum, slot, kLanes, lane);
+    if (slot != 0) return;
+    sum[8] = r < e.rows ? of_wave[1][0] + of_wave[1][1] + of_wave[1][2] + of_wave[1][3] : 0.0f;
+  } else if (r < e.rows) {
+    for (int j = lane; j < runs; j += kLanes) {
+      const float2 x = point(j);
+      top = x.y != 0.0f ? fmaxf(top, -x.x) : top;
     }
 #pragma unroll
     for (int j = kLanes / 2; j > 0; j >>= 1) top = fmaxf(top, __shfl_xor(top, j));
 #pragma unroll 4
-    for (int j = slot; j < runs; j += kSlots) {
-      const float2 x = ml[first + (int64_t)j * kTrainBlock];
+    for (int j = 0; j < runs; ++j) {
+      const float2 x = point(j);
       const float factor = x.y != 0.0f ? fast_exp2(-x.x - top) : 0.0f;
-      const float4* o = reinterpret_cast<const float4*>(p.part + (first + (int64_t)j * kTrainBlock) * D + 8 * lane);
-      const float4 lo = o[0], hi = o[1];
       sum[8] = __fmaf_rn(x.y, factor, sum[8]);
-      sum[0] = __fmaf_rn(lo.x, factor, sum[0]);
-      sum[1] = __fmaf_rn(lo.y, factor, sum[1]);
-      sum[2] = __fmaf_rn(lo.z, factor, sum[2]);
-      sum[3] = __fmaf_rn(lo.w, factor, sum[3]);
-      sum[4] = __fmaf_rn(hi.x, factor, sum[4]);
-      sum[5] = __fmaf_rn(hi.y, factor, sum[5]);
-      sum[6] = __fmaf_rn(hi.z, factor, sum[6]);
-      sum[7] = __fmaf_rn(hi.w, factor, sum[7]);
+      add(values(j)[0], values(j)[1], factor);
     }
   }
-  add_slots<kSlots>(sum, slot, kLanes, lane);
-  if (slot != 0) return;
   const int l = row_position(p, r), h = hk * p.group + r - l * p.group;
   const float factor = sum[8] == 0.0f ? 0.0f : 1.0f / sum[8];
   *reinterpret_cast<v4i*>(p.o + b * p.os.sB + l * p.os.sL + h * p.os.sH + 8 * lane) =
@@ -822,7 +855,7 @@ TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double sha
   const int64_t rest = blocks - whole;
   double least = 1e30;
   int best = tiles;  // of a run
-  const int most = rest > (1 << 19) ? 1 : std::min(tiles, 128);  // (a launch holds 2^24 workgroups)
+  const int most = rest > (1 << 19) ? 1 : std::min(tiles, kMostRuns);  // (a launch holds 2^24 workgroups)
   for (int n = 1; n <= most; ++n) {
     const int each = (tiles + n - 1) / n;
     const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * rest * bytes * share / kBytesPerTile;
