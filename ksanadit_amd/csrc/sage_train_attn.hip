@@ -899,8 +899,9 @@ void take_cut(TrainAttnParams& p, const TrainCut& c) {
 unsigned workgroups(const TrainAttnParams& p) { return (unsigned)(p.whole + (int64_t)p.cut * p.runs); }
 // Rows of a block that the joins look at
 int joined_rows(int64_t all) { return (int)std::min<int64_t>(all, kTrainBlock); }
-constexpr int kManyRuns = 16;  // from here on lanes share a row's runs: one lane after the other, 64 runs take 20 us where this takes 6
-constexpr int64_t kMostGroups = 1 << 23;
+// Many runs of few rows (of all blocks): lanes share a row's.  Forward and dq, 64 runs of 40 rows: 4 and 4 us, one lane after the other 20 and more; 22 of
+// 960 rows: 7.3 and 7.3, 8.9 and 10.8; 16 of 4096: 15.8 and 11.2, 7.3 and 6.6; 24 of 1200 rows of 64 channels: 15.8 and 13.0, 5.4 and 5.6.
+constexpr int kManyRuns = 16, kFewJoined = 1024;
 
 template <int DT, int D>
 hipError_t fwd(TrainAttnParams p, hipStream_t s) {
@@ -912,7 +913,7 @@ hipError_t fwd(TrainAttnParams p, hipStream_t s) {
   if (p.runs > 1) {
     constexpr int kLanes = D / 8;
     const int rows = joined_rows((int64_t)p.Lq * p.group), groups = (rows * kLanes + 255) / 256;  // workgroups of a block
-    if (p.runs >= kManyRuns && (int64_t)rows * p.cut <= kMostGroups)
+    if (p.runs >= kManyRuns && (int64_t)rows * p.cut <= kFewJoined)
       sage_train_join_fwd_kernel<DT, D, 256 / kLanes><<<(unsigned)((int64_t)rows * p.cut), 256, 0, s>>>(p, rows);
     else
       sage_train_join_fwd_kernel<DT, D, 1><<<(unsigned)((int64_t)groups * p.cut), 256, 0, s>>>(p, groups);
@@ -925,7 +926,7 @@ void join_bwd(const TrainAttnParams& p, int64_t all, hipStream_t s) {
   if (p.runs == 1) return;
   constexpr int kLanes = (kKeys ? 2 : 1) * D / 8;
   const int rows = joined_rows(all), groups = (rows * kLanes + 255) / 256;
-  if (p.runs >= kManyRuns && (int64_t)rows * p.cut <= kMostGroups)
+  if (p.runs >= kManyRuns && (int64_t)rows * p.cut <= kFewJoined)
     sage_train_join_bwd_kernel<DT, D, kKeys, 256 / kLanes><<<(unsigned)((int64_t)rows * p.cut), 256, 0, s>>>(p, rows);
   else
     sage_train_join_bwd_kernel<DT, D, kKeys, 1><<<(unsigned)((int64_t)groups * p.cut), 256, 0, s>>>(p, groups);
