@@ -665,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
 // ------------------------------------------------------------------------------------------------------------ runs joined
 
 // Bound by the bytes of the runs and, of few rows, by latency.  Eight channels per lane; kSlots groups of lanes share a row's runs and
-// add their sums up in a fixed order (from kManyRuns runs on; 64 runs of one row, 40 heads: 6 us).
+// add their sums up in a fixed order (many runs of few rows; 64 runs of one row, 40 heads: 4 us).
 template <int kSlots>
 __device__ __forceinline__ void add_slots(float (&x)[9], int slot, int lanes, int lane) {
   if constexpr (kSlots > 1) {
