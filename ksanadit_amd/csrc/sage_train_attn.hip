@@ -504,6 +504,11 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 // A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
 // k^T dS^T.  A half's vector work stands behind matrix instructions of the other half (in front of them: 1371 us where this takes 1308).
 // 8 heads of 16384 tokens: bf16 1332 us, 1240 TFLOP/s, fp16 1433; of 64 channels 816 us.
+//
+// A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and keys
+// that are off zero by as much as they vary, or by more, would carry that into dq.  m is the mean of the head's first tile of keys (one m for all
+// runs of a row), subtracted at the end as the rounded dS's sum times m: relative error against 64 bits, bf16, keys N(0, 1) off zero by
+// N(0, 1) per channel 0.0037 without it, DQERR with it; by N(0, 4) 0.010 and DQERR4.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -568,6 +573,28 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
         p.row_d[(int64_t)bh * p.row_pad + row] = d;
       }
     }
+    float* sums_of_keys = reinterpret_cast<float*>(train_lds + 2 * 2 * T::kBytes);  // [kWaves][D], of the first tile
+    const int first_keys = min(kTrainTile, e.keys);
+    {
+      constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+      const int piece = threadIdx.x % kLanes;
+      float sum[8] = {};
+#pragma unroll
+      for (int i = 0; i < kTrainTile / kRows; ++i) {
+        const int key = i * kRows + threadIdx.x / kLanes;
+        float x[8];
+        widen8<DT>(*reinterpret_cast<const uint4*>(p.k + b * p.ks.sB + min(key, first_keys - 1) * p.ks.sL + hk * p.ks.sH + 8 * piece), x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += key < first_keys ? x[j] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int n = kLanes; n < 64; n <<= 1) sum[j] += __shfl_xor(sum[j], n);
+        if (lane < kLanes) sums_of_keys[wave * D + 8 * piece + j] = sum[j];
+      }
+    }
+    float sum_ds = 0.0f;
     row_ready(q);
     row_ready(g);
     const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
@@ -623,6 +650,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
           if ((i + 1) * kEach % 8 == 0) {
             const int f = (i + 1) * kEach / 8 - 1;
             ds[h][f] = pack8<DT>(s[h][8 * f], s[h][8 * f + 1], s[h][8 * f + 2], s[h][8 * f + 3], s[h][8 * f + 4], s[h][8 * f + 5], s[h][8 * f + 6], s[h][8 * f + 7]);
+            sum_ds = add8<DT>(ds[h][f], sum_ds);
           }
         };
       };
@@ -647,6 +675,17 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       columns_product(1, nothing);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const bool sees = limit >= first_keys;  // (a causal row that does not see all of that tile does without)
+    sum_ds = over_halves<Sum>(sum_ds) / -(float)first_keys;
+#pragma unroll
+    for (int c = 0; c < T::kBlocks; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        v4f m{};
+        for (int w = 0; w < kWaves; ++w) m += *reinterpret_cast<const v4f*>(sums_of_keys + w * D + 32 * c + 8 * g + 4 * hh);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dq[c][4 * g + i] = sees ? __fmaf_rn(sum_ds, m[i], dq[c][4 * g + i]) : dq[c][4 * g + i];
+      }
   }
   const float unshift = fast_exp2(-kBackwardShift<DT>);
   const bool exists = row < all_rows;
@@ -942,7 +981,7 @@ hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   if (p.dq != nullptr) {
-    constexpr int kLds = 2 * 2 * Tile<D>::kBytes;
+    constexpr int kLds = 2 * 2 * Tile<D>::kBytes + 4 * D * 4;
     static LdsRequest request;
     e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D>), kLds);
     if (e != hipSuccess) return e;

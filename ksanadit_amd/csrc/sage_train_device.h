@@ -36,6 +36,23 @@ __device__ __forceinline__ v4i pack8(float a, float b, float c, float d, float e
   return v4i{(int)lo.x, (int)lo.y, (int)hi.x, (int)hi.y};
 }
 
+// sum + the eight values of an operand, as they are rounded
+template <int DT>
+__device__ __forceinline__ float add8(const v4i& x, float sum) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int pair = x[i];  // (a vector's element is no operand of a bit cast: the first is taken)
+    if constexpr (DT == KSANA_SAGE_BF16) {
+      typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, pair), __builtin_bit_cast(v2, 0x3f803f80), sum, false);
+    } else {
+      typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, pair), __builtin_bit_cast(v2, 0x3c003c00), sum, false);
+    }
+  }
+  return sum;
+}
+
 // A tile: 64 rows of D 16-bit channels.  A copy instruction of a wave fills 1 KiB in a row with 64 pieces of 16 bytes: whole rows, that
 // are not neighbours.  Which rows share a copy and how far apart the copies lie is chosen so that row r starts 64 (r % 4) + 16 (r / 4 % 4)
 // bytes into the 256 that the banks hold side by side: sixteen lanes that read one piece of sixteen rows, and 32 lanes that read 64 bytes

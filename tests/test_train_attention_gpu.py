@@ -8,7 +8,12 @@ far below u here.  Every bound below is that: factor u |terms| summed, with the 
 fp16 is a fixed-point format below 2^-14: its values are multiples of 2^-24 there, and rounding to nearest is off by up to 2^-25 however
 small the value.  That is added once per rounding: to a result as it is; to a probability, which is scaled by 2^15 in the backward
 pass and by 2^6 against the row's largest one (at most 1) in the forward pass, 2^-40 and 2^-31; to a gradient of a score, scaled by 2^15
-and a power of two of at least half of 1 / (2 max|dO| max|v|), 2^-40 times 4 max|dO| max|v|.  (bf16 has fp32's exponents: nothing.)"""
+and a power of two of at least half of 1 / (2 max|dO| max|v|), 2^-40 times 4 max|dO| max|v|.  (bf16 has fp32's exponents: nothing.)
+
+dq.  A row's exact dS sum to zero, so c sum dS k = c sum dS (k - m) whatever m is.  The kernel forms c (sum dS' k - (sum dS') m) with its own dS' =
+dS + e, which is c sum (dS + e) (k - m): off by c sum e (k - m), so |k - m| stands in the bound where |k| would without m - more for a key that
+is smaller than the mean, less where keys share an offset.  m is the mean of the entry's first min(64, count) keys for rows that see them all, and 0
+for others.  Sums, the mean and the product with it are fp32: at most 2^-20 of sum |dS| (|k| + |m|) besides."""
 
 import math
 
@@ -71,8 +76,14 @@ def _formula(q, k, v, do, *, causal=False, scale=None, k_lens=None, q_lens=None)
     def pair(value, error):
         return value.permute(0, 2, 1, 3), (error + u * value.abs()).permute(0, 2, 1, 3) * 1.01 + (2.0**-25 if half else 1e-30)
 
-    ks, qs = abs(scale) * kd.abs(), abs(scale) * qd.abs()
-    return (*pair(o, e_fwd @ vd.abs() + soft.amax(-1, keepdim=True) * o.abs()), *pair(ds @ kd * scale, e_ds @ ks),
+    qs = abs(scale) * qd.abs()
+    # of dq: rows that see all of the entry's first keys, and those that do not
+    counts = torch.full((B,), Lk) if k_lens is None else torch.as_tensor(k_lens).clamp(0, Lk)
+    first = [min(64, int(n)) for n in counts]
+    m = torch.stack([kd[b, :, : max(1, n)].mean(1, keepdim=True) for b, n in enumerate(first)])
+    with_m = torch.stack([seen[b, :, :, max(0, n - 1)] for b, n in enumerate(first)]).unsqueeze(-1)
+    e_dq = abs(scale) * (torch.where(with_m, e_ds @ (kd - m).abs(), e_ds @ kd.abs()) + 2.0**-20 * (ds.abs() @ (kd.abs() + m.abs())))
+    return (*pair(o, e_fwd @ vd.abs() + soft.amax(-1, keepdim=True) * o.abs()), *pair(ds @ kd * scale, e_dq),
             *pair(heads(ds.transpose(2, 3) @ qd) * scale, heads(e_ds.transpose(2, 3) @ qs)),
             *pair(heads(p.transpose(2, 3) @ dod), heads(e_p.transpose(2, 3) @ dod.abs())))
 
