@@ -673,9 +673,27 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       hide(1);
       columns_product(0, gradients(1));
       columns_product(1, nothing);
+      if (t == 0 && all_see < first_keys) {
+        // rows that see a part of the first tile, and nothing else: m is the mean of that
+        float share = limit < first_keys ? over_halves<Sum>(sum_ds) / -(float)limit : 0.0f;
+        int left = limit - 4 * hh;
+        pin(share);
+        pin(left);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 32 * h + acc_row(8 * f + j) < left ? share : 0.0f;
+            ds[h][f] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+          }
+        columns_product(0, nothing);
+        columns_product(1, nothing);
+      }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool sees = limit >= first_keys;  // (a causal row that does not see all of that tile does without)
+    const bool sees = limit >= first_keys;
     sum_ds = over_halves<Sum>(sum_ds) / -(float)first_keys;
 #pragma unroll
     for (int c = 0; c < T::kBlocks; ++c)

@@ -12,8 +12,9 @@ and a power of two of at least half of 1 / (2 max|dO| max|v|), 2^-40 times 4 max
 
 dq.  A row's exact dS sum to zero, so c sum dS k = c sum dS (k - m) whatever m is.  The kernel forms c (sum dS' k - (sum dS') m) with its own dS' =
 dS + e, which is c sum (dS + e) (k - m): off by c sum e (k - m), so |k - m| stands in the bound where |k| would without m - more for a key that
-is smaller than the mean, less where keys share an offset.  m is the mean of the entry's first min(64, count) keys for rows that see them all, and 0
-for others.  Sums, the mean and the product with it are fp32: at most 2^-20 of sum |dS| (|k| + |m|) besides."""
+is smaller than the mean, less where keys share an offset.  m is the mean of the entry's first min(64, count) keys for rows that see them all, and of
+what they see for others.  There the sum of dS', which is one of e, goes into a product once more, its share of each key rounded to the tensors' type: u
+(and in fp16 the step below 2^-14, scaled as for dS) times the sum of e over the keys' number, on every key.  Sums, the mean and the product with it are fp32: at most 2^-20 of sum |dS| (|k| + |m|) besides."""
 
 import math
 
@@ -81,8 +82,14 @@ def _formula(q, k, v, do, *, causal=False, scale=None, k_lens=None, q_lens=None)
     counts = torch.full((B,), Lk) if k_lens is None else torch.as_tensor(k_lens).clamp(0, Lk)
     first = [min(64, int(n)) for n in counts]
     m = torch.stack([kd[b, :, : max(1, n)].mean(1, keepdim=True) for b, n in enumerate(first)])
-    with_m = torch.stack([seen[b, :, :, max(0, n - 1)] for b, n in enumerate(first)]).unsqueeze(-1)
-    e_dq = abs(scale) * (torch.where(with_m, e_ds @ (kd - m).abs(), e_ds @ kd.abs()) + 2.0**-20 * (ds.abs() @ (kd.abs() + m.abs())))
+    e_dq = e_ds @ (kd - m).abs()
+    for b, n in enumerate(first):
+        for r in range(min(n - 1, Lq) if causal else 0):  # row r sees keys 0 to r
+            own = kd[b, :, : r + 1]
+            e = e_ds[b, :, r, : r + 1].unsqueeze(1)
+            again = u * e.mean(2, keepdim=True) + (2.0**-40 * most if half else 0.0)
+            e_dq[b, :, r] = (e @ (own - own.mean(1, keepdim=True)).abs() + again * own.abs().sum(1, keepdim=True)).squeeze(1)
+    e_dq = abs(scale) * (e_dq + 2.0**-20 * (ds.abs() @ (kd.abs() + m.abs())))
     return (*pair(o, e_fwd @ vd.abs() + soft.amax(-1, keepdim=True) * o.abs()), *pair(ds @ kd * scale, e_dq),
             *pair(heads(ds.transpose(2, 3) @ qd) * scale, heads(e_ds.transpose(2, 3) @ qs)),
             *pair(heads(p.transpose(2, 3) @ dod), heads(e_p.transpose(2, 3) @ dod.abs())))
