@@ -573,7 +573,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
         p.row_d[(int64_t)bh * p.row_pad + row] = d;
       }
     }
-    float* sums_of_keys = reinterpret_cast<float*>(train_lds + 2 * 2 * T::kBytes);  // [kWaves][D], of the first tile
+    float* sums_of_keys = reinterpret_cast<float*>(train_lds + 2 * 2 * T::kBytes);  // of the first tile, [D], and of each wave's part of it
     const int first_keys = min(kTrainTile, e.keys);
     {
       constexpr int kLanes = D / 8, kRows = 256 / kLanes;
@@ -589,9 +589,24 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        if constexpr (kLanes == 8) {
+          sum[j] = over_slots<Sum>(sum[j]);
+        } else {
+          const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[j]), __float_as_uint(sum[j]), false, false);
+          sum[j] = over_halves<Sum>(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+        }
+      }
+      float* of_wave = sums_of_keys + D + wave * D + 8 * piece;
+      if (lane < kLanes) {
+        *reinterpret_cast<float4*>(of_wave) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        *reinterpret_cast<float4*>(of_wave + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the copies under way are not waited for)
+      if (threadIdx.x < D) {
+        float all = 0.0f;
 #pragma unroll
-        for (int n = kLanes; n < 64; n <<= 1) sum[j] += __shfl_xor(sum[j], n);
-        if (lane < kLanes) sums_of_keys[wave * D + 8 * piece + j] = sum[j];
+        for (int w = 1; w <= kWaves; ++w) all += sums_of_keys[w * D + threadIdx.x];
+        sums_of_keys[threadIdx.x] = all;
       }
     }
     float sum_ds = 0.0f;
@@ -699,8 +714,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
     for (int c = 0; c < T::kBlocks; ++c)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        v4f m{};
-        for (int w = 0; w < kWaves; ++w) m += *reinterpret_cast<const v4f*>(sums_of_keys + w * D + 32 * c + 8 * g + 4 * hh);
+        const v4f m = *reinterpret_cast<const v4f*>(sums_of_keys + 32 * c + 8 * g + 4 * hh);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dq[c][4 * g + i] = sees ? __fmaf_rn(sum_ds, m[i], dq[c][4 * g + i]) : dq[c][4 * g + i];
       }
@@ -999,7 +1013,7 @@ hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   if (p.dq != nullptr) {
-    constexpr int kLds = 2 * 2 * Tile<D>::kBytes + 4 * D * 4;
+    constexpr int kLds = 2 * 2 * Tile<D>::kBytes + 5 * D * 4;
     static LdsRequest request;
     e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D>), kLds);
     if (e != hipSuccess) return e;
