@@ -10,10 +10,10 @@
 //
 // P and dS are rounded to the tensors' type where they become matrix operands; S, dP, all sums and accumulators are fp32.
 //
-// Long sequences are bound by what the matrix pipes draw: with them busy 63 % (forward), 76 % (dq) and 67 % (dk and dv) of the time the
-// clock falls from 2.4 to 1.7 - 1.8 GHz.  20 heads of 32760 bf16 tokens of 128 channels: forward 9.4 ms, dq 12.6, dk and dv 17.2, that
-// is 1170, 1310 and 1280 TFLOP/s of the products that they form (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
-// and what a workgroup does besides its loop, 32760 rows on 512 keys, 40 heads: 420, 580 and 640 us; a few rows by a chain of latencies.
+// Long sequences are bound by what the matrix pipes draw: with them busy 64 % (forward), 69 % (dq) and 65 % (dk and dv) of the time the
+// clock falls from 2.4 to 1.7 - 1.8 GHz.  20 heads of 32760 bf16 tokens of 128 channels: forward 10.0 ms, dq 13.8, dk and dv 18.5, that
+// is 1100, 1200 and 1190 TFLOP/s of the products that they form (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
+// and what a workgroup does besides its loop, 32760 rows on 512 keys, 40 heads: 426, 621 and 662 us; a few rows by a chain of latencies.
 #include "sage_train_device.h"
 
 #include <algorithm>
@@ -86,7 +86,7 @@ __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + 
 // A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys, two waves to a SIMD.  While the
 // probabilities of tile t are formed and multiplied with its values, the scores of tile t + 1 are: a few vector instructions stand behind
 // every matrix instruction and run beside it.  So values are wanted a step after their keys; each have two places in LDS.
-// 8 heads of 16384 tokens: bf16 1004 us, 1095 TFLOP/s, fp16 1063; of 64 channels 669 us, where exponentials count twice as much.
+// 8 heads of 16384 tokens: bf16 1024 us, 1075 TFLOP/s, fp16 1086; of 64 channels 670 us, where exponentials count twice as much.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_fwd_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -362,7 +362,7 @@ __device__ __forceinline__ float ds_scale(const TrainAttnParams& p, int bh, int 
 
 // A wave keeps 32 keys and walks tiles of 64 query rows in halves: S = q k^T and dP = dO v^T (a lane holds scores of one key; dP's
 // accumulators start at -d), dv^T += dO^T P, dk^T += q^T dS.  The other wave of the SIMD works beside a wave's vector instructions.
-// 8 heads of 16384 tokens: bf16 1853 us, 1190 TFLOP/s, fp16 1995; of 64 channels 1029 us.
+// 8 heads of 16384 tokens: bf16 1899 us, 1160 TFLOP/s, fp16 2053; of 64 channels 1055 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -503,12 +503,13 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 
 // A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
 // k^T dS^T.  A half's vector work stands behind matrix instructions of the other half (in front of them: 1371 us where this takes 1308).
-// 8 heads of 16384 tokens: bf16 1332 us, 1240 TFLOP/s, fp16 1433; of 64 channels 816 us.
+// 8 heads of 16384 tokens: bf16 1416 us, 1165 TFLOP/s, fp16 1508; of 64 channels 861 us.
 //
 // A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and keys
-// that are off zero by as much as they vary, or by more, would carry that into dq.  m is the mean of the head's first tile of keys (one m for all
-// runs of a row), subtracted at the end as the rounded dS's sum times m: relative error against 64 bits, bf16, keys N(0, 1) off zero by
-// N(0, 1) per channel 0.0037 without it, DQERR with it; by N(0, 4) 0.010 and DQERR4.
+// that are off zero by as much as they vary, or by more, would carry that into dq.  m is the mean of the head's first tile of keys, or of
+// what the row sees of it (one m for all runs of a row), and the rounded dS's sum times m is subtracted at the end.  Relative error against 64
+// bits, bf16, keys N(0, 1) off zero by N(0, 1) per channel: 0.0024, 0.0037 without; off by N(0, 16) 0.0024 and 0.010.  It costs 4 % of the kernel's time,
+// 6 % with 8 tiles to a block.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -914,7 +915,7 @@ void fill_in(TrainAttnParams& p) {
 // left whole, the others are cut so that they fill one more.  Others (`differ`; of a causal call's tiles half are there): all whole or all in
 // runs of one length.  Whole ones come with the longest first, so that the short ones fill up what those leave of the last round, unless
 // there are so few that two long ones share a place; runs need whole rounds, or half a run's time besides their mean.  (16 heads of 8192
-// causal tokens: rows whole 276 + 372 us, forward and dq, in two runs 291 + 387 and 34 for the joins; on 4 key heads, dk and dv: keys whole
+// causal tokens: rows whole 276 + 372 us, forward and dq (without what it does about m), in two runs 291 + 387 and 34 for the joins; on 4 key heads, dk and dv: keys whole
 // 1120, in 3 runs 594 + 12, in 5 618 + 17, in 7 587 + 21.)
 struct TrainCut {
   int whole, cut, runs, run_tiles;
