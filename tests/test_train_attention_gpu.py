@@ -328,6 +328,17 @@ def test_cut_loops_against_uncut_ones(hip_device, Hq, Hkv, Lq, Lk, causal):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("B,Hq,Hkv,Lq,Lk,D,causal,k_lens", [
+    (1, 2, 2, 300, 700, 128, False, None), (1, 4, 2, 300, 300, 64, True, None), (1, 6, 2, 5, 4000, 128, False, None), (2, 2, 2, 150, 200, 128, True, [200, 33])])
+def test_keys_that_share_an_offset(hip_device, dtype, B, Hq, Hkv, Lq, Lk, D, causal, k_lens):
+    """Off zero by eight times what they vary: the bound of dq, which counts |k - m|, knows nothing of it."""
+    q, k, v, do = _draw(17, B, Hq, Hkv, Lq, Lk, D, dtype)
+    off = 8 * torch.randn((1, 1, Hkv, D), generator=torch.Generator().manual_seed(18))
+    _check(q * 0.25, (k.float() + off).to(dtype), v, do, hip_device, causal=causal, k_lens=k_lens)
+
+
+@gpu
 @pytest.mark.parametrize("B,Hq,Hkv,Lq,Lk,D,dtype,k_lens,q_lens", [
     (1, 8, 2, 1500, 1500, 64, torch.bfloat16, None, None), (2, 6, 2, 600, 2300, 64, torch.float16, None, None), (1, 5, 1, 1900, 700, 128, torch.bfloat16, None, None),
     (1, 3, 1, 40, 9000, 128, torch.float16, None, None), (4, 48, 48, 290, 290, 128, torch.bfloat16, None, None),
