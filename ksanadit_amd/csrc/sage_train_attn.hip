@@ -30,6 +30,7 @@ __device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__
 
 constexpr int kTrainBlock = 128;  // query rows, or keys, of a workgroup
 constexpr int kMostRuns = 128;    // of a block
+constexpr int kSpread = 32, kFewKeys = 128;  // keys that dq estimates a row's mean key by; rows that see fewer than kFewKeys take the first kSpread besides
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // Rounded to fp16, probabilities relative to a row's largest would lose bits from 2^-14 on and vanish at 2^-25; scaled up as far as
 // the format goes, they do so a factor of 2^6 (forward, where the reference point may lag by 2^kLazy) or 2^15 (backward) later.
@@ -505,11 +506,17 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 // k^T dS^T.  A half's vector work stands behind matrix instructions of the other half (in front of them: 1371 us where this takes 1308).
 // 8 heads of 16384 tokens: bf16 1416 us, 1165 TFLOP/s, fp16 1508; of 64 channels 861 us.
 //
-// A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and keys
-// that are off zero by as much as they vary, or by more, would carry that into dq.  m is the mean of the head's first tile of keys, or of
-// what the row sees of it (one m for all runs of a row), and the rounded dS's sum times m is subtracted at the end.  Relative error against 64
-// bits, bf16, keys N(0, 1) off zero by N(0, 1) per channel: 0.0024, 0.0037 without; off by N(0, 16) 0.0024 and 0.010.  It costs 4 % of the kernel's time,
-// 6 % with 8 tiles to a block.
+// A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and that
+// carries the mean of the keys that the row attends to into dq wherever this is off zero.  The m that takes most of it away is that mean, sum P k.  It is
+// estimated: the row's own probabilities on kSpread keys, spread evenly over those that the block sees; where its first row sees few, on the first kSpread and
+// as many spread over the others, each of these weighted with the keys it stands for.  As a last tile the sum of the rounded dS times their shares is
+// subtracted from dS, so keys of one kind or of several, text in front of an image or a whole sequence, leave the same error.  Relative error against 64
+// bits, bf16, 4352 keys N(0, 1): 0.0025; without m 0.0024, and 0.0039, 0.012, 0.024 with all keys off zero by 1, 4, 8 times N(0, 1) per channel, where
+// 0.0025 remain with it; the first 64, or half of them, off by 4 and not attended to: 0.0025 and 0.0026 (with the mean of the first 64 for m 0.013 and
+// 0.011); an eighth of them attended to, or half: 0.0030 and 0.0026 (without 0.012).  Rows that attend to a single key are worse off with an
+// estimate, 0.0058 for 0.0045 where scores vary by 16, and a key far off that carries most of a row and is not in the sample stays as without (0.0097).  The mean
+// itself, one more product, leaves 0.0019 - 0.0024 in all of these and takes a third more work.  64 keys leave 0.0024 - 0.0028 and take 1.6 % of the pass
+// of 32760 rows on 512 keys; 32 take 0 - 1 %.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -536,11 +543,17 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
   }
   if (range.from < range.to) {
     const TileCopy<D, kWaves> k_copy(p.k + b * p.ks.sB + hk * p.ks.sH, p.ks.sL, wave, lane), v_copy(p.v + b * p.vs.sB + hk * p.vs.sH, p.vs.sL, wave, lane);
+    const int block_sees = p.causal ? min(e.keys, row_position(p, min(row0 + kTrainBlock, all_rows) - 1) + 1) : e.keys;
+    const bool few = (p.causal ? min(e.keys, row_position(p, row0) + 1) : e.keys) < kFewKeys;  // that the block's first row sees
+    const int spread_from = few ? kSpread : 0;
     auto copy = [&](int t) {
-      const int at = min(t, range.to - 1) * kTrainTile;
       const unsigned stage = lds + (t & 1) * 2 * T::kBytes;
-      k_copy.start(at, e.keys, stage, wave, lane);
-      v_copy.start(at, e.keys, stage + T::kBytes, wave, lane);
+      if (t < range.to) {
+        k_copy.start(t * kTrainTile, e.keys, stage, wave, lane);
+        v_copy.start(t * kTrainTile, e.keys, stage + T::kBytes, wave, lane);
+      } else {
+        k_copy.template start_spread<kSpread>(spread_from, block_sees, stage, wave, lane);
+      }
     };
     copy(range.from);
     v4i q[T::kSteps], g[T::kSteps];
@@ -574,42 +587,6 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
         p.row_d[(int64_t)bh * p.row_pad + row] = d;
       }
     }
-    float* sums_of_keys = reinterpret_cast<float*>(train_lds + 2 * 2 * T::kBytes);  // of the first tile, [D], and of each wave's part of it
-    const int first_keys = min(kTrainTile, e.keys);
-    {
-      constexpr int kLanes = D / 8, kRows = 256 / kLanes;
-      const int piece = threadIdx.x % kLanes;
-      float sum[8] = {};
-#pragma unroll
-      for (int i = 0; i < kTrainTile / kRows; ++i) {
-        const int key = i * kRows + threadIdx.x / kLanes;
-        float x[8];
-        widen8<DT>(*reinterpret_cast<const uint4*>(p.k + b * p.ks.sB + min(key, first_keys - 1) * p.ks.sL + hk * p.ks.sH + 8 * piece), x);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += key < first_keys ? x[j] : 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (kLanes == 8) {
-          sum[j] = over_slots<Sum>(sum[j]);
-        } else {
-          const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[j]), __float_as_uint(sum[j]), false, false);
-          sum[j] = over_halves<Sum>(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-        }
-      }
-      float* of_wave = sums_of_keys + D + wave * D + 8 * piece;
-      if (lane < kLanes) {
-        *reinterpret_cast<float4*>(of_wave) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-        *reinterpret_cast<float4*>(of_wave + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (the copies under way are not waited for)
-      if (threadIdx.x < D) {
-        float all = 0.0f;
-#pragma unroll
-        for (int w = 1; w <= kWaves; ++w) all += sums_of_keys[w * D + threadIdx.x];
-        sums_of_keys[threadIdx.x] = all;
-      }
-    }
     float sum_ds = 0.0f;
     row_ready(q);
     row_ready(g);
@@ -617,6 +594,37 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
     const int limit = p.causal ? min(e.keys, row_position(p, row) + 1) : e.keys;
     const int all_see = p.causal ? min(e.keys, row_position(p, min(row0 + wave * 32, e.rows - 1)) + 1) : e.keys;
     const bool idle = row0 + wave * 32 >= e.rows;  // a wave without rows copies its share
+    // A step of the tile: an operand read ahead, a matrix instruction, and vector work of a part of the 16 elements of a half
+    constexpr int kSteps = T::kSteps, kEach = 16 / kSteps, kAhead = 3;
+    v16f s[2], dp[2];
+    v4i ds[2][2], a[kAhead];
+    auto rows_product = [&](unsigned rows, int h, const v4i(&other)[kSteps], v16f& to, auto&& beside) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) a[i] = read_row<D>(rows, h, i);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        to = mfma16<DT>(a[i % kAhead], other[i], to);
+        if (i + kAhead < kSteps) a[i % kAhead] = read_row<D>(rows, h, i + kAhead);
+        beside(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto columns_product = [&](unsigned columns, int h, auto&& beside) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) a[i] = read_column<D>(columns, i % T::kBlocks, 2 * h + i / T::kBlocks);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int j = i + kAhead;
+        dq[i % T::kBlocks] = mfma16<DT>(a[i % kAhead], ds[h][i / T::kBlocks], dq[i % T::kBlocks]);
+        if (j < kSteps) a[i % kAhead] = read_column<D>(columns, j % T::kBlocks, 2 * h + j / T::kBlocks);
+        beside(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto pack = [&](int h, int f) {
+      return pack8<DT>(s[h][8 * f], s[h][8 * f + 1], s[h][8 * f + 2], s[h][8 * f + 3], s[h][8 * f + 4], s[h][8 * f + 5], s[h][8 * f + 6], s[h][8 * f + 7]);
+    };
+    auto nothing = [](int) {};
 #pragma unroll 1
     for (int t = range.from; t < range.to; ++t) {
       tile_ready<0>();
@@ -626,33 +634,6 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       pin(k_rows);  // (one address and constants each)
       pin(v_rows);
       pin(k_columns);
-      // A step of the tile: an operand read ahead, a matrix instruction, and vector work of a part of the 16 elements of a half
-      constexpr int kSteps = T::kSteps, kEach = 16 / kSteps, kAhead = 3;
-      v16f s[2], dp[2];
-      v4i ds[2][2], a[kAhead];
-      auto rows_product = [&](unsigned rows, int h, const v4i(&other)[kSteps], v16f& to, auto&& beside) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) a[i] = read_row<D>(rows, h, i);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          to = mfma16<DT>(a[i % kAhead], other[i], to);
-          if (i + kAhead < kSteps) a[i % kAhead] = read_row<D>(rows, h, i + kAhead);
-          beside(i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      };
-      auto columns_product = [&](int h, auto&& beside) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) a[i] = read_column<D>(k_columns, i % T::kBlocks, 2 * h + i / T::kBlocks);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int j = i + kAhead;
-          dq[i % T::kBlocks] = mfma16<DT>(a[i % kAhead], ds[h][i / T::kBlocks], dq[i % T::kBlocks]);
-          if (j < kSteps) a[i % kAhead] = read_column<D>(k_columns, j % T::kBlocks, 2 * h + j / T::kBlocks);
-          beside(i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      };
       auto probabilities = [&](int h) {
         return [&, h](int i) {
 #pragma unroll
@@ -665,7 +646,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
           for (int j = i * kEach; j < (i + 1) * kEach; ++j) s[h][j] *= dp[h][j];
           if ((i + 1) * kEach % 8 == 0) {
             const int f = (i + 1) * kEach / 8 - 1;
-            ds[h][f] = pack8<DT>(s[h][8 * f], s[h][8 * f + 1], s[h][8 * f + 2], s[h][8 * f + 3], s[h][8 * f + 4], s[h][8 * f + 5], s[h][8 * f + 6], s[h][8 * f + 7]);
+            ds[h][f] = pack(h, f);
             sum_ds = add8<DT>(ds[h][f], sum_ds);
           }
         };
@@ -677,7 +658,6 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[h][i] = acc_row(i) < left ? s[h][i] : 0.0f;
       };
-      auto nothing = [](int) {};
       s[0] = s[1] = v16f{};
 #pragma unroll
       for (int i = 0; i < 16; ++i) dp[0][i] = dp[1][i] = d;
@@ -687,38 +667,58 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       rows_product(k_rows, 1, q, s[1], gradients(0));
       rows_product(v_rows, 1, g, dp[1], probabilities(1));
       hide(1);
-      columns_product(0, gradients(1));
-      columns_product(1, nothing);
-      if (t == 0 && all_see < first_keys) {
-        // rows that see a part of the first tile, and nothing else: m is the mean of that
-        float share = limit < first_keys ? over_halves<Sum>(sum_ds) / -(float)limit : 0.0f;
-        int left = limit - 4 * hh;
-        pin(share);
-        pin(left);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = 32 * h + acc_row(8 * f + j) < left ? share : 0.0f;
-            ds[h][f] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
-          }
-        columns_product(0, nothing);
-        columns_product(1, nothing);
-      }
+      columns_product(k_columns, 0, gradients(1));
+      columns_product(k_columns, 1, nothing);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool sees = limit >= first_keys;
-    sum_ds = over_halves<Sum>(sum_ds) / -(float)first_keys;
+    tile_ready<0>();  // (and no copy outlives the workgroup's LDS)
+    if (!idle) {
+      const unsigned tile = lds + (range.to & 1) * 2 * T::kBytes;
+      float most = -INFINITY, total = 0.0f;
+      auto scores = [&](int h, int left) {  // of the half's first `left` keys
+        s[h] = v16f{};
+        rows_product(tile + row_at, h, q, s[h], nothing);
 #pragma unroll
-    for (int c = 0; c < T::kBlocks; ++c)
+        for (int i = 0; i < 16; ++i) {
+          s[h][i] = acc_row(i) < left - 4 * hh ? s[h][i] : -INFINITY;
+          most = fmaxf(most, s[h][i]);
+        }
+      };
+      const int spread = block_sees - spread_from, seen = limit - spread_from;  // key j of the first half is key j spread / kSpread of those
+      scores(0, spread >= kSpread ? (kSpread * seen + spread - 1) / spread : seen);
+      if (few) scores(1, limit);
+      most = over_halves<Max>(most) * p.c;
+      auto probabilities = [&](int h, float weight) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const v4f m = *reinterpret_cast<const v4f*>(sums_of_keys + 32 * c + 8 * g + 4 * hh);
+        for (int i = 0; i < 16; ++i) {
+          s[h][i] = fast_exp2(__fmaf_rn(s[h][i], p.c, -most)) * weight;
+          total += s[h][i];
+        }
+      };
+      probabilities(0, fmaxf(1.0f, (float)spread / kSpread));  // (one key for so many)
+      if (few) probabilities(1, 1.0f);
+      total = over_halves<Sum>(total);
+      const float share = total > 0.0f ? over_halves<Sum>(sum_ds) / -total : 0.0f;  // (not a number: nor is the row's dq)
+      auto subtract = [&](int h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dq[c][4 * g + i] = sees ? __fmaf_rn(sum_ds, m[i], dq[c][4 * g + i]) : dq[c][4 * g + i];
-      }
+        for (int i = 0; i < 16; ++i) s[h][i] *= share;
+#pragma unroll
+        for (int f = 0; f < 2; ++f) ds[h][f] = pack(h, f);
+        columns_product(tile + column_at, h, nothing);
+        if (range.runs == 1) return;
+        // a run's dS sum to more than roundings: what is left of the shares when they are rounded counts too
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          float x[8];
+          widen8<DT>(__builtin_bit_cast(uint4, ds[h][f]), x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[h][8 * f + j] -= x[j];
+          ds[h][f] = pack(h, f);
+        }
+        columns_product(tile + column_at, h, nothing);
+      };
+      subtract(0);
+      if (few) subtract(1);
+    }
   }
   const float unshift = fast_exp2(-kBackwardShift<DT>);
   const bool exists = row < all_rows;
@@ -1014,7 +1014,7 @@ hipError_t bwd(TrainAttnParams p, const TrainCuts& cuts, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   if (p.dq != nullptr) {
-    constexpr int kLds = 2 * 2 * Tile<D>::kBytes + 5 * D * 4;
+    constexpr int kLds = 2 * 2 * Tile<D>::kBytes;
     static LdsRequest request;
     e = request.make(reinterpret_cast<const void*>(&sage_train_dq_kernel<DT, D>), kLds);
     if (e != hipSuccess) return e;

@@ -86,6 +86,10 @@ __device__ __forceinline__ void lds_copy16_at(const void* base, unsigned lane_of
 __device__ __forceinline__ void lds_copy4_at(const void* base, unsigned lane_off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(lane_off), "s"(base) : "memory", "m0");
 }
+// .. from an address of each lane's own
+__device__ __forceinline__ void lds_copy16_from(const void* lane_at, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(lane_at) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 // All copies of this wave but the youngest kLater are in LDS, its LDS reads are done, and so are the other waves'.
 template <int kLater>
@@ -153,6 +157,17 @@ struct TileCopy {
       for (int c = 0; c < T::kCopies / kWaves; ++c)
         lds_copy16_at(at, (unsigned)min(T::row_of(c * kWaves + wave, lane), rows - row - 1) * (unsigned)row_bytes + lane % T::kPieces * 16,
                       tile + T::copy_at(c * kWaves + wave));
+    }
+  }
+  // A tile of single rows: kCount spread evenly over rows `from` to `to`, number i is from + i (to - from) / kCount, or as many as there are; then the first kCount rows.
+  // Those that do not exist are copies of others.
+  template <int kCount>
+  __device__ __forceinline__ void start_spread(int from, int to, unsigned tile, int wave, int lane) const {
+#pragma unroll
+    for (int c = 0; c < T::kCopies / kWaves; ++c) {
+      const int i = T::row_of(c * kWaves + wave, lane);
+      const int row = i >= kCount ? i - kCount : from + (to - from >= kCount ? i * (to - from) / kCount : i);
+      lds_copy16_from(base + min(row, to - 1) * row_bytes + lane % T::kPieces * 16, tile + T::copy_at(c * kWaves + wave));
     }
   }
 };

@@ -14,7 +14,10 @@ dq.  A row's exact dS sum to zero, so c sum dS k = c sum dS (k - m) whatever m i
 dS + e, which is c sum (dS + e) (k - m): off by c sum e (k - m), so |k - m| stands in the bound where |k| would without m - more for a key that
 is smaller than the mean, less where keys share an offset.  m is the mean of the entry's first min(64, count) keys for rows that see them all, and of
 what they see for others.  There the sum of dS', which is one of e, goes into a product once more, its share of each key rounded to the tensors' type: u
-(and in fp16 the step below 2^-14, scaled as for dS) times the sum of e over the keys' number, on every key.  Sums, the mean and the product with it are fp32: at most 2^-20 of sum |dS| (|k| + |m|) besides."""
+(and in fp16 the step below 2^-14, scaled as for dS) times the sum of e over the keys' number, on every key.  Sums, the mean and the product with it are fp32: at most 2^-20 of sum |dS| (|k| + |m|) besides.
+
+So much for any kernel with that m, and these bounds stand.  The kernel's own m is nearer to what a row attends to (an estimate of sum P k), for which its first
+term, P times what d is off by, nearly vanishes: it keeps to about a third of them, and ``test_keys_of_two_kinds`` says what it keeps to that a first tile's mean does not."""
 
 import math
 
@@ -336,6 +339,58 @@ def test_keys_that_share_an_offset(hip_device, dtype, B, Hq, Hkv, Lq, Lk, D, cau
     q, k, v, do = _draw(17, B, Hq, Hkv, Lq, Lk, D, dtype)
     off = 8 * torch.randn((1, 1, Hkv, D), generator=torch.Generator().manual_seed(18))
     _check(q * 0.25, (k.float() + off).to(dtype), v, do, hip_device, causal=causal, k_lens=k_lens)
+
+
+def _kinds(seed, dtype, Hq, Hkv, Lq, Lk, D, first, attended):
+    """Keys of which the first ones are off the others by four times what these vary, and queries that lean to one kind or to neither"""
+    q, k, v, do = _draw(seed, 1, Hq, Hkv, Lq, Lk, D, dtype)
+    off = torch.randn((1, 1, Hkv, D), generator=torch.Generator().manual_seed(seed + 1))
+    k = torch.cat((k[:, :first].float() + 4 * off, k[:, first:].float()), 1).to(dtype)
+    return (q.float() + 0.5 * attended * off.repeat_interleave(Hq // Hkv, 2)).to(dtype), k, v, do
+
+
+def _dq_rms(q, k, v, do, causal):
+    """dq in 64 bits and the root of the sum of squares that its roundings leave, whatever keys are there.
+
+    The kernel forms c sum (dS + e) (k - m).  e holds each dS' rounding, of variance at most u^2 / 3 dS^2, and P times what d is off by, whose sum
+    over P (k - m) vanishes where m is the row's own mean key sum P k.  So with it the variance is at most c^2 sum u^2 / 3 dS^2 |k - m|^2, plus u^2 / 3 dq^2 for
+    the result.  d is off by the roundings of o (dO^2 o^2) and of P (P^2 dP^2), in sum of about twice the variance of e without it (o^2 has the size of sum P^2 in
+    each channel, dP^2 that of |dO|^2): with m from a sample, that is by |m' - m|^2 <= |k - m|^2 off, at most 1 + 2 + 1 times the variance.  (fp16: 2^-40 of
+    4 max|dO| max|v| at most besides, its values' spacing, and 2^-25 of a result.)"""
+    B, Lq, Hq, D = q.shape
+    rep, u = Hq // k.shape[2], HALF_STEP[q.dtype]
+    qd, dod = (t.double().transpose(1, 2) for t in (q, do))
+    kd, vd = (t.double().transpose(1, 2).repeat_interleave(rep, 1) for t in (k, v))
+    s = qd @ kd.transpose(2, 3) * D**-0.5
+    if causal:
+        s = s.masked_fill(torch.ones(s.shape[2:], dtype=torch.bool).triu(1), -math.inf)
+    p = s.softmax(-1)
+    dp = dod @ vd.transpose(2, 3)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    mean = p @ kd
+    spread = (kd * kd).sum(-1).unsqueeze(2) - 2 * mean @ kd.transpose(2, 3) + (mean * mean).sum(-1, keepdim=True)  # |k - m|^2
+    half = q.dtype == torch.float16
+    fixed = 2.0**-40 * 4 * dod.norm(dim=-1).max() * vd.norm(dim=-1).max() if half else 0.0
+    dq = ds @ kd * D**-0.5
+    variance = ((u * u / 3 * ds * ds + fixed**2 * (p > 0)) * spread).sum() / D + u * u / 3 * (dq * dq).sum() + (2.0**-50 * dq.numel() if half else 0.0)
+    return dq.transpose(1, 2), variance.sqrt()
+
+
+_KINDS = [  # Hq, Hkv, Lq, Lk, D, of the first kind, queries lean to it, causal
+    (2, 2, 300, 1024, 128, 64, -1, False), (4, 2, 200, 1000, 64, 500, -1, False), (4, 2, 200, 1000, 128, 500, 1, False), (2, 2, 150, 2000, 128, 250, 0, False),
+    (2, 1, 100, 9000, 128, 64, -1, False), (2, 2, 800, 800, 128, 400, -1, True), (2, 2, 30, 40, 64, 20, -1, False)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("Hq,Hkv,Lq,Lk,D,first,attended,causal", _KINDS)
+def test_keys_of_two_kinds(hip_device, dtype, Hq, Hkv, Lq, Lk, D, first, attended, causal):
+    """A few keys in front or half of them off the others, as text in front of an image: twice (four times the variance) what roundings leave."""
+    t = _kinds(19, dtype, Hq, Hkv, Lq, Lk, D, first, attended)
+    want, rms = _dq_rms(*t, causal)
+    got = _attend(*(x.to(hip_device) for x in t), is_causal=causal)[1].cpu().double()
+    off = ((got - want).norm() / rms).item()
+    assert off <= 2.0, f"dq {off:.2f} times what roundings leave (relative error {((got - want).norm() / want.norm()).item():.5f})"
 
 
 @gpu
