@@ -200,9 +200,10 @@ class _ResidualNorm(torch.autograd.Function):
         if dh is None and dn is None:
             return (None,) * 13
         n_dtype = ctx.options[-1]
-        # (hooks may have laid the saved tensors out anew)
+        # (hooks may have laid the saved tensors out anew; all copies are held until the launches are made)
         x, y = _rows(x), None if y is None else _rows(y)
-        call = _norm_call(x, y, [None if t is None else _vector_rows(t) for t in vectors], *ctx.options)
+        vectors = [None if t is None else _vector_rows(t) for t in vectors]
+        call = _norm_call(x, y, vectors, *ctx.options)
         dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
         dh = None if dh is None else dh.contiguous()
         dx, dy = _contiguous_like(x), None if y is None else _contiguous_like(y)

@@ -1,6 +1,7 @@
 """The operators with gradients where no GPU is needed: what they refuse, and the tests' own formulas against differences."""
 
 import ctypes as C
+import weakref
 
 import pytest
 import torch
@@ -185,3 +186,70 @@ def test_scales_that_fp32_cannot_hold(monkeypatch):
     for scale in (float("nan"), float("inf"), -1e39):
         with pytest.raises(ValueError, match="sm_scale"):
             train_ops.attention(q, q, q, sm_scale=scale)
+
+
+# ------------------------------------------------------------------------------------------------ saved tensors that hooks lay out anew
+class _Library:
+    """Stands for the compiled library on tensors of the CPU: forward passes write what is given, backward passes are looked at."""
+
+    def __init__(self, fwd, bwd):
+        self.ksana_sage_train_attn_fwd = self.ksana_sage_train_norm_fwd = fwd
+        self.ksana_sage_train_attn_bwd = self.ksana_sage_train_norm_bwd = bwd
+
+    def ksana_sage_train_attn_scratch(self, *a):
+        return 0
+
+    def ksana_sage_train_norm_scratch(self, *a):
+        return 0
+
+
+def _memory(address, dtype, n):
+    return torch.frombuffer((C.c_char * (n * dtype.itemsize)).from_address(address), dtype=dtype).clone()
+
+
+def _write(address, t):
+    C.memmove(address, t.data_ptr(), t.numel() * t.element_size())
+
+
+def _laid_out_anew(t):
+    """The same values a stride of two apart"""
+    return t if t.dim() == 0 else torch.stack((t, torch.full_like(t, 7)), -1)[..., 0]
+
+
+@pytest.fixture
+def on_the_cpu(monkeypatch):
+    monkeypatch.setattr(train_ops, "_on", lambda device: train_ops.nullcontext())
+    monkeypatch.setattr(train_ops, "_stream_ptr", lambda device: 0)
+    return lambda *functions: monkeypatch.setattr(train_ops._capi, "load", lambda: _Library(*functions))
+
+
+def test_vectors_that_hooks_lay_out_anew(monkeypatch, on_the_cpu):
+    """The backward call reads the vectors that the forward pass saved, from memory that nothing else has been given meanwhile."""
+    B, L, Ch = 2, 3, 16
+    x, y = torch.randn(B, L, Ch), torch.randn(B, L, Ch)
+    vectors = [torch.randn(B, 1, Ch) for _ in range(3)] + [torch.randn(Ch) for _ in range(3)]
+    copies, seen = [], []
+    rows = train_ops._vector_rows
+
+    def watched(t):
+        out = rows(t)
+        copies.append(weakref.ref(out))
+        return out
+
+    monkeypatch.setattr(train_ops, "_vector_rows", watched)
+
+    def bwd(call, *a):
+        seen.append(all(c() is not None for c in copies))
+        fields = train_ops._NORM.unpack(call)[14:]
+        for i, t in enumerate(vectors):
+            at, stride = fields[4 * i : 4 * i + 2]
+            for b in range(B if t.dim() > 1 else 1):
+                seen.append(torch.equal(_memory(at + 4 * b * stride, torch.float32, Ch), t[b, 0] if t.dim() > 1 else t))
+        return 0
+
+    on_the_cpu(lambda *a: 0, bwd)
+    leaves = [t.requires_grad_() for t in (x, y, *vectors)]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _laid_out_anew):
+        h, n = train_ops._ResidualNorm.apply(*leaves, "layer", "rms", 1.0, 1e-6, torch.float32)
+    torch.autograd.grad((h, n), leaves, (torch.zeros_like(h), torch.zeros_like(n)))
+    assert len(copies) == 6 and len(seen) == 1 + 3 * B + 3 and all(seen), seen
