@@ -42,6 +42,17 @@ def _scratch(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _kept(t: torch.Tensor | None, dtype: torch.dtype, shape) -> torch.Tensor | None:
+    """What a forward pass saved for the kernels, contiguous and at an address they read: hooks that keep saved tensors elsewhere may give them back laid
+    out and placed otherwise, but not as other tensors."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape:
+        raise RuntimeError(f"a saved tensor came back from its hooks as {t.dtype} {tuple(t.shape)}, it was {dtype} {tuple(shape)}")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
@@ -86,13 +97,17 @@ def _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, want_lse: b
     return o, lse, nbytes[1]
 
 
-def _attention_backward(do, q, k, v, o, lse, scratch_bytes, is_causal, sm_scale, k_lens, q_lens, want_q: bool, want_kv: bool):
+def _attention_backward(do, q, k, v, o, lse, scratch_bytes, k_shape, is_causal, sm_scale, k_lens, q_lens, want_q: bool, want_kv: bool):
     dq = _contiguous_like(q) if want_q else None
     dk, dv = (_contiguous_like(k), _contiguous_like(k)) if want_kv else (None, None)
     if q.numel() == 0 or k.numel() == 0:
         return tuple(None if t is None else t.zero_() for t in (dq, dk, dv))
-    # (the saved tensors too: hooks that keep them elsewhere may give them back laid out and placed otherwise)
+    if not (q.shape == o.shape == do.shape and k.shape == v.shape == k_shape and q.dtype == k.dtype == v.dtype == o.dtype == do.dtype):
+        raise RuntimeError("a saved tensor came back from its hooks with another shape or type")
+    # (the saved tensors too: see _kept)
     do, q, k, v, o = (_readable(t) for t in (do, q, k, v, o))
+    B, Lq, Hq = q.shape[:3]
+    lse, k_lens, q_lens = _kept(lse, torch.float32, (B, Hq, Lq)), _kept(k_lens, torch.int32, (B,)), _kept(q_lens, torch.int32, (B,))
     call, strides = _attention_call(q, k, v, o, is_causal, sm_scale, k_lens, q_lens), _strides(do)
     with _on(q.device):
         scratch = _scratch(scratch_bytes, q.device)
@@ -108,7 +123,7 @@ class _Attention(torch.autograd.Function):
     def forward(ctx, q, k, v, is_causal, sm_scale, k_lens, q_lens):
         o, lse, scratch_bytes = _attention_forward(q, k, v, is_causal, sm_scale, k_lens, q_lens, True)
         ctx.save_for_backward(q, k, v, o, lse, k_lens, q_lens)
-        ctx.options = (scratch_bytes, is_causal, sm_scale)
+        ctx.options = (scratch_bytes, k.shape, is_causal, sm_scale)
         return o
 
     @staticmethod
@@ -200,9 +215,13 @@ class _ResidualNorm(torch.autograd.Function):
         if dh is None and dn is None:
             return (None,) * 13
         n_dtype = ctx.options[-1]
-        # (hooks may have laid the saved tensors out anew; all copies are held until the launches are made)
+        # (hooks may have laid the saved tensors out anew: see _kept.  All copies are held until the launches are made.)
+        like = dn if dh is None else dh
+        if x.shape != like.shape or (dh is not None and x.dtype != dh.dtype) or (y is not None and (y.shape != x.shape or y.dtype != n_dtype)):
+            raise RuntimeError("a saved tensor came back from its hooks with another shape or type")
         x, y = _rows(x), None if y is None else _rows(y)
-        vectors = [None if t is None else _vector_rows(t) for t in vectors]
+        vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, vectors)]
+        stats = _kept(stats, torch.float32, (*x.shape[:2], 4))
         call = _norm_call(x, y, vectors, *ctx.options)
         dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
         dh = None if dh is None else dh.contiguous()

@@ -228,6 +228,16 @@ def test_saved_tensors_may_be_kept_elsewhere(hip_device):
 
 
 @gpu
+def test_saved_tensors_may_be_laid_out_anew(hip_device):
+    """Statistics and counts too: each comes back with its last dimension a stride of two apart."""
+    q, k, v, do = (t.to(hip_device) for t in _draw(10, 2, 4, 2, 100, 140, 64, torch.float16))
+    want = _attend(q, k, v, do, k_lens=[140, 31], q_lens=[7, 100])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack((t, torch.full_like(t, 7)), -1)[..., 0]):
+        got = _attend(q, k, v, do, k_lens=[140, 31], q_lens=[7, 100])
+    assert _same(got, want)
+
+
+@gpu
 def test_what_cannot_be_differentiated_is_refused(hip_device):
     q = torch.randn(1, 20, 1, 64, device=hip_device, dtype=torch.float16, requires_grad=True)
     lens = torch.tensor([15], dtype=torch.int32, device=hip_device)

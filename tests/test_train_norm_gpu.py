@@ -279,3 +279,13 @@ def test_streams_and_graphs(hip_device):
         torch.cuda.synchronize()
         assert _same(out, want[turn % 3])
         _run(*sets[(turn + 1) % 3], hip_device, "rms", "layer", 0.5)  # eager work of the same kind
+
+
+@gpu
+def test_saved_tensors_may_be_laid_out_anew(hip_device):
+    """.. with channels a stride of two apart: each is copied, and the copies stay while the kernels read them."""
+    t, dh, dn = make(6, 2, 30, 264, bf16, bf16, fp32, ALL)
+    want = _run(t, dh, dn, hip_device, "rms", "layer", 0.5)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: torch.stack((x, torch.full_like(x, 7)), -1)[..., 0]):
+        got = _run(t, dh, dn, hip_device, "rms", "layer", 0.5)
+    assert _same(got, want)

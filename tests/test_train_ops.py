@@ -253,3 +253,61 @@ def test_vectors_that_hooks_lay_out_anew(monkeypatch, on_the_cpu):
         h, n = train_ops._ResidualNorm.apply(*leaves, "layer", "rms", 1.0, 1e-6, torch.float32)
     torch.autograd.grad((h, n), leaves, (torch.zeros_like(h), torch.zeros_like(n)))
     assert len(copies) == 6 and len(seen) == 1 + 3 * B + 3 and all(seen), seen
+
+
+def test_a_norms_statistics_that_hooks_lay_out_anew(on_the_cpu):
+    stats, seen = torch.randn(2, 3, 4), []
+
+    def fwd(call, x, y, h, n, stats_at, stream):
+        _write(stats_at, stats)
+        return 0
+
+    def bwd(call, x, y, stats_at, *a):
+        seen.append(torch.equal(_memory(stats_at, torch.float32, stats.numel()), stats.flatten()))
+        return 0
+
+    on_the_cpu(fwd, bwd)
+    x = torch.randn(2, 3, 16, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _laid_out_anew):
+        h, n = train_ops._ResidualNorm.apply(x, x, *[None] * 6, "layer", None, 1.0, 1e-6, torch.float32)
+    torch.autograd.grad((h, n), x, (torch.zeros_like(h), torch.zeros_like(n)))
+    assert seen == [True]
+
+
+def test_statistics_and_counts_that_hooks_lay_out_anew(on_the_cpu):
+    B, Lq, H, D = 2, 5, 3, 64
+    q = torch.randn(B, Lq, H, D).bfloat16()
+    lse, lens, seen = torch.randn(B, H, Lq), [torch.tensor([4, 5], dtype=torch.int32), torch.tensor([3, 1], dtype=torch.int32)], []
+
+    def fwd(call, q, k, v, o, lse_at, *a):
+        _write(lse_at, lse)
+        return 0
+
+    def bwd(call, q, k, v, o, lse_at, *a):
+        q_lens, k_lens = train_ops._ATTENTION.unpack(call)[-2:]
+        seen.extend((torch.equal(_memory(lse_at, torch.float32, lse.numel()), lse.flatten()), torch.equal(_memory(k_lens, torch.int32, B), lens[0]),
+                     torch.equal(_memory(q_lens, torch.int32, B), lens[1])))
+        return 0
+
+    on_the_cpu(fwd, bwd)
+    leaf = q.requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _laid_out_anew):
+        o = train_ops._Attention.apply(leaf, leaf, leaf, False, None, *lens)
+    torch.autograd.grad(o, leaf, torch.zeros_like(o))
+    assert seen == [True] * 3
+
+
+def test_saved_tensors_that_hooks_make_others_of_are_refused(on_the_cpu):
+    on_the_cpu(lambda *a: 0, lambda *a: pytest.fail("called"))
+    for change in (lambda t: t.half() if t.dtype == torch.float32 else t, lambda t: t[:1], lambda t: t.long() if t.dtype == torch.int32 else t):
+        q = torch.zeros(2, 5, 3, 64, dtype=torch.bfloat16, requires_grad=True)
+        x, w = torch.zeros(2, 3, 16, requires_grad=True), torch.zeros(2, 16, requires_grad=True)
+        lens = torch.tensor([4, 5], dtype=torch.int32)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            o = train_ops._Attention.apply(q, q, q, False, None, lens, None)
+            h, n = train_ops._ResidualNorm.apply(x, x, None, w, None, None, None, None, "layer", None, 1.0, 1e-6, torch.float32)
+        with pytest.raises(RuntimeError, match="came back"):
+            torch.autograd.grad(o, q, torch.zeros_like(o))
+        if change(torch.zeros(2, dtype=torch.int32)).dtype == torch.int32:
+            with pytest.raises(RuntimeError, match="came back"):
+                torch.autograd.grad((h, n), (x, w), (torch.zeros_like(h), torch.zeros_like(n)))
