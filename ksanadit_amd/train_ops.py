@@ -15,7 +15,9 @@ import struct
 from contextlib import nullcontext
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _capi
 from .sage_ops import _DTYPES, _k_lens_arg, _require_hip, _stream_ptr, _strides, _usable
@@ -24,6 +26,15 @@ from .sage_ops import _DTYPES, _k_lens_arg, _require_hip, _stream_ptr, _strides,
 def _on(device: torch.device):
     """The device made current where it is not: kernels start on the current one."""
     return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _refuse_unseen(name: str, *tensors: torch.Tensor | None) -> None:
+    """The kernels are started past torch's dispatcher: what records its operators, or carries tangents through them, would go on with memory that nothing
+    has been written to, or without the tangent."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative (a dual tensor was given)")
+    if torch._C._get_tracing_state() is not None or get_proxy_mode() is not None:
+        raise NotImplementedError(f"{name} cannot be traced (torch.jit.trace, make_fx): its kernels are not operators of torch")
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -129,6 +140,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
+        _refuse_unseen("attention's backward pass", do)
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
         q, k, v, o, lse, k_lens, q_lens = ctx.saved_tensors
         dq, dk, dv = _attention_backward(do, q, k, v, o, lse, *ctx.options, k_lens, q_lens, want_q, want_k or want_v)
@@ -151,6 +163,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
     if tensor_layout == "HND":
         q, k, v = (t.transpose(1, 2) if t.dim() == 4 else t for t in (q, k, v))
     _check_attention(q, k, v)
+    _refuse_unseen("attention", q, k, v)
     if sm_scale is not None and not abs(sm_scale) < 3.4e38:
         raise ValueError(f"sm_scale {sm_scale} is not a finite fp32 number")
     k_lens, q_lens = (_k_lens_arg(n, q.shape[0], q.device, name) for n, name in ((k_lens, "k_lens"), (q_lens, "q_lens")))
@@ -210,6 +223,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
+        _refuse_unseen("residual_norm's backward pass", *grads)
         x, y, stats, *vectors = ctx.saved_tensors
         dh, dn = grads if y is not None else (None, grads[0])
         if dh is None and dn is None:
@@ -310,6 +324,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, 
         raise ValueError("post_weight goes with post_norm")
     if x.shape[2] == 0:
         raise ValueError("residual_norm needs at least one channel")
+    _refuse_unseen("residual_norm", x, y, gate, scale, shift, weight, bias, post_weight)
     vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, (gate, scale, shift, weight, bias, post_weight))]
     x_rows, y_rows = _rows(x), None if y is None else _rows(y)
     residual_scale, eps = float(residual_scale), float(eps)

@@ -5,6 +5,7 @@ import weakref
 
 import pytest
 import torch
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from ksanadit_amd import _capi, train_ops
 from tests.test_train_attention_gpu import HALF_STEP, _draw, _formula
@@ -186,6 +187,42 @@ def test_scales_that_fp32_cannot_hold(monkeypatch):
     for scale in (float("nan"), float("inf"), -1e39):
         with pytest.raises(ValueError, match="sm_scale"):
             train_ops.attention(q, q, q, sm_scale=scale)
+
+
+def _forward_dual(f, t):
+    with torch.autograd.forward_ad.dual_level():
+        f(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+@pytest.mark.parametrize("wants_gradient", [False, True])
+@pytest.mark.parametrize("through", [
+    _forward_dual, lambda f, t: torch.func.jvp(f, (t,), (t,)), lambda f, t: torch.jit.trace(f, t, check_trace=False), lambda f, t: make_fx(f)(t),
+    lambda f, t: make_fx(f, tracing_mode="symbolic")(t), lambda f, t: make_fx(f, pre_dispatch=True)(t)],
+    ids=["dual", "jvp", "jit", "fx", "fx_symbolic", "fx_pre_dispatch"])
+def test_what_goes_past_the_kernels_is_refused(monkeypatch, on_the_cpu, through, wants_gradient):
+    """Forward mode and tracing see torch's own operators only: the result would be without its tangent, the trace without the kernels."""
+    on_the_cpu(lambda *a: 0, lambda *a: 0)
+    monkeypatch.setattr(train_ops, "_require_hip", lambda *t: None)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    q, x, w = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 4, 16), torch.zeros(16)
+    train_ops.attention(q, q, q)
+    train_ops.residual_norm(x)
+    for f, t in ((lambda t: train_ops.attention(t, q, q), q), (lambda t: train_ops.attention(q, q, t), q), (lambda t: train_ops.residual_norm(t)[1], x),
+                 (lambda t: train_ops.residual_norm(x, t)[0], x), (lambda t: train_ops.residual_norm(x, bias=t)[1], w)):
+        with pytest.raises(NotImplementedError, match="forward-mode|cannot be traced"):
+            through(f, t.clone().requires_grad_(wants_gradient))
+
+
+@pytest.mark.parametrize("through", [_forward_dual, lambda f, t: make_fx(f)(t)], ids=["dual", "fx"])
+def test_backward_passes_that_go_past_the_kernels_are_refused(on_the_cpu, through):
+    on_the_cpu(lambda *a: 0, lambda *a: 0)
+    q, x = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16, requires_grad=True), torch.zeros(1, 4, 16, requires_grad=True)
+    o = train_ops._Attention.apply(q, q, q, False, None, None, None)
+    h, n = train_ops._ResidualNorm.apply(x, x, *[None] * 6, "layer", None, 1.0, 1e-6, torch.float32)
+    for out, leaf in ((o, q), (h, x), (n, x)):
+        torch.autograd.grad(out, leaf, torch.zeros_like(out), retain_graph=True)
+        with pytest.raises(NotImplementedError, match="forward-mode|cannot be traced"):
+            through(lambda t: torch.autograd.grad(out, leaf, t, retain_graph=True), torch.zeros_like(out))
 
 
 # ------------------------------------------------------------------------------------------------ saved tensors that hooks lay out anew
