@@ -16,7 +16,6 @@ from contextlib import nullcontext
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _capi
@@ -129,6 +128,27 @@ def _attention_backward(do, q, k, v, o, lse, scratch_bytes, k_shape, is_causal, 
     return dq, dk, dv
 
 
+class _Once(torch.autograd.Function):
+    """Gradients on their way out of a backward pass that is itself recorded, and what they were formed from: differentiating them is refused.
+    (torch's once_differentiable cuts them off from what they depend on: ``torch.autograd.functional.jvp`` then gives zeros.)"""
+
+    @staticmethod
+    def forward(ctx, number: int, *tensors):
+        return tuple(t.view_as(t) for t in tensors[:number])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("train_ops: gradients of gradients are not available")
+
+
+def _not_twice(grads: tuple, *sources: torch.Tensor | None) -> tuple:
+    if not torch.is_grad_enabled():
+        return grads
+    given = [t for t in grads if t is not None]
+    out = iter(_Once.apply(len(given), *given, *(t for t in sources if t is not None)))
+    return tuple(None if t is None else next(out) for t in grads)
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, is_causal, sm_scale, k_lens, q_lens):
@@ -138,13 +158,13 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
         _refuse_unseen("attention's backward pass", do)
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
         q, k, v, o, lse, k_lens, q_lens = ctx.saved_tensors
-        dq, dk, dv = _attention_backward(do, q, k, v, o, lse, *ctx.options, k_lens, q_lens, want_q, want_k or want_v)
-        return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
+        with torch.no_grad():
+            dq, dk, dv = _attention_backward(do, q, k, v, o, lse, *ctx.options, k_lens, q_lens, want_q, want_k or want_v)
+        return *_not_twice((dq, dk if want_k else None, dv if want_v else None), do, q, k, v), None, None, None, None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: str = "NHD", is_causal: bool = False,
@@ -210,6 +230,38 @@ def _residual_norm_forward(x, y, call, n_dtype, want_stats: bool):
     return h, n, stats
 
 
+def _residual_norm_backward(grads, saved, options, wanted) -> tuple:
+    """Gradients of x, y and the six vectors from those of the results, None where there is nothing or nothing is wanted"""
+    x, y, stats, *vectors = saved
+    dh, dn = grads if y is not None else (None, grads[0])
+    n_dtype = options[-1]
+    # (hooks may have laid the saved tensors out anew: see _kept.  All copies are held until the launches are made.)
+    like = dn if dh is None else dh
+    if x.shape != like.shape or (dh is not None and x.dtype != dh.dtype) or (y is not None and (y.shape != x.shape or y.dtype != n_dtype)):
+        raise RuntimeError("a saved tensor came back from its hooks with another shape or type")
+    x, y = _rows(x), None if y is None else _rows(y)
+    vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, vectors)]
+    stats = _kept(stats, torch.float32, (*x.shape[:2], 4))
+    call = _norm_call(x, y, vectors, *options)
+    dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
+    dh = None if dh is None else dh.contiguous()
+    dx, dy = _contiguous_like(x), None if y is None else _contiguous_like(y)
+    d_vectors = [_contiguous_like(t) if t is not None and want else None for t, want in zip(vectors, wanted)]
+    if x.numel() == 0:
+        return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors))
+    lib = _capi.load()
+    nbytes, pointers = C.c_uint64(0), (C.c_void_p * 6)(*[_ptr(t) for t in d_vectors])
+    rc = lib.ksana_sage_train_norm_scratch(call, C.addressof(nbytes))
+    if rc == _capi.OK:
+        with _on(x.device):
+            scratch = _scratch(nbytes.value, x.device)
+            rc = lib.ksana_sage_train_norm_bwd(call, x.data_ptr(), _ptr(y), stats.data_ptr(), _ptr(dh), dn.data_ptr(), dx.data_ptr(), _ptr(dy),
+                                               C.addressof(pointers), _ptr(scratch), _stream_ptr(x.device))
+    if rc != _capi.OK:
+        _capi.check(rc, "train_ops.residual_norm, backward")
+    return (dx, dy, *d_vectors)
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, shift, weight, bias, post_weight, norm, post_norm, residual_scale, eps, n_dtype):
@@ -221,40 +273,14 @@ class _ResidualNorm(torch.autograd.Function):
         return n if y is None else (h, n)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
         _refuse_unseen("residual_norm's backward pass", *grads)
-        x, y, stats, *vectors = ctx.saved_tensors
-        dh, dn = grads if y is not None else (None, grads[0])
-        if dh is None and dn is None:
+        if all(g is None for g in grads):
             return (None,) * 13
-        n_dtype = ctx.options[-1]
-        # (hooks may have laid the saved tensors out anew: see _kept.  All copies are held until the launches are made.)
-        like = dn if dh is None else dh
-        if x.shape != like.shape or (dh is not None and x.dtype != dh.dtype) or (y is not None and (y.shape != x.shape or y.dtype != n_dtype)):
-            raise RuntimeError("a saved tensor came back from its hooks with another shape or type")
-        x, y = _rows(x), None if y is None else _rows(y)
-        vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, vectors)]
-        stats = _kept(stats, torch.float32, (*x.shape[:2], 4))
-        call = _norm_call(x, y, vectors, *ctx.options)
-        dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
-        dh = None if dh is None else dh.contiguous()
-        dx, dy = _contiguous_like(x), None if y is None else _contiguous_like(y)
-        wanted = ctx.needs_input_grad[2:8]
-        d_vectors = [_contiguous_like(t) if t is not None and want else None for t, want in zip(vectors, wanted)]
-        if x.numel() == 0:
-            return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors), *(None,) * 5)
-        lib = _capi.load()
-        nbytes, pointers = C.c_uint64(0), (C.c_void_p * 6)(*[_ptr(t) for t in d_vectors])
-        rc = lib.ksana_sage_train_norm_scratch(call, C.addressof(nbytes))
-        if rc == _capi.OK:
-            with _on(x.device):
-                scratch = _scratch(nbytes.value, x.device)
-                rc = lib.ksana_sage_train_norm_bwd(call, x.data_ptr(), _ptr(y), stats.data_ptr(), _ptr(dh), dn.data_ptr(), dx.data_ptr(), _ptr(dy),
-                                                   C.addressof(pointers), _ptr(scratch), _stream_ptr(x.device))
-        if rc != _capi.OK:
-            _capi.check(rc, "train_ops.residual_norm, backward")
-        return (dx, dy, *d_vectors, *(None,) * 5)
+        saved = ctx.saved_tensors
+        with torch.no_grad():
+            d = _residual_norm_backward(grads, saved, ctx.options, ctx.needs_input_grad[2:8])
+        return *_not_twice(d, *grads, saved[0], saved[1], *saved[3:]), *(None,) * 5
 
 
 def _wants_gradient(*tensors) -> bool:

@@ -225,6 +225,26 @@ def test_backward_passes_that_go_past_the_kernels_are_refused(on_the_cpu, throug
             through(lambda t: torch.autograd.grad(out, leaf, t, retain_graph=True), torch.zeros_like(out))
 
 
+def test_gradients_of_gradients_are_refused_however_they_are_asked_for(on_the_cpu):
+    """With respect to the tensors and to the results' gradients, by which ``torch.autograd.functional.jvp`` gets at a forward derivative."""
+    on_the_cpu(lambda *a: 0, lambda *a: 0)
+    attend = lambda q: train_ops._Attention.apply(q, q, q, False, None, None, None)  # noqa: E731
+    norm = lambda w: train_ops._ResidualNorm.apply(x, x, None, w, None, None, None, None, "layer", None, 1.0, 1e-6, torch.float32)  # noqa: E731
+    x = torch.zeros(1, 4, 16)
+    for f, t in ((attend, torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)), (norm, torch.zeros(16))):
+        with pytest.raises(RuntimeError, match="gradients of gradients"):
+            torch.autograd.functional.jvp(f, t, torch.ones_like(t))
+        leaf = t.clone().requires_grad_()
+        out = f(leaf)
+        outs = out if isinstance(out, tuple) else (out,)
+        dos = [torch.zeros_like(o).requires_grad_() for o in outs]
+        (d,) = torch.autograd.grad(outs, leaf, dos, create_graph=True)
+        assert d.shape == leaf.shape
+        for other in (leaf, *dos):
+            with pytest.raises(RuntimeError, match="gradients of gradients"):
+                torch.autograd.grad(d.sum(), other, retain_graph=True)
+
+
 # ------------------------------------------------------------------------------------------------ saved tensors that hooks lay out anew
 class _Library:
     """Stands for the compiled library on tensors of the CPU: forward passes write what is given, backward passes are looked at."""
