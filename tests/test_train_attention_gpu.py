@@ -426,3 +426,33 @@ def test_the_backend_trains_where_it_is_asked_to(hip_device):
     assert _same((o.detach(), *torch.autograd.grad(o, leaves, do)), _attend(q, k, v, do))
     assert torch.equal(make(trainable=True).forward(q, k, v), make().forward(q, k, v))  # without gradients: as ever
     assert make(trainable=True, out_dtype=torch.float16).forward(*leaves).dtype == torch.float16
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_the_op_trains_where_it_is_asked_to(hip_device, causal):
+    from ksanadit_amd import KsanaAttentionConfig, pick_attn_op
+
+    q, k, v, do = (t.to(hip_device) for t in _draw(21, 1, 4, 2, 100, 120, 128, torch.bfloat16))
+    make = pick_attn_op(KsanaAttentionConfig(backend="sage_attention"))
+    op, plain = (make(num_heads=4, head_size=128, num_kv_heads=2, causal=causal, **kw) for kw in ({"trainable": True}, {}))
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = op(*leaves)
+    assert _same((o.detach(), *torch.autograd.grad(o, leaves, do)), _attend(q, k, v, do, is_causal=causal))
+    assert torch.equal(op(q, k, v), plain(q, k, v))  # without gradients: the quantized attention, as ever
+    leaves = [t.float().requires_grad_() for t in (q, k, v)]  # (cast to bf16, as for the quantized attention)
+    o = op(*leaves)
+    assert o.dtype == torch.float32 and _same([t.bfloat16() for t in torch.autograd.grad(o, leaves, do.float())], _attend(q, k, v, do, is_causal=causal)[1:])
+
+
+@gpu
+def test_a_compiled_function_calls_it(hip_device):
+    """The kernels are no operators of torch: a compiled function leaves its graph for them, in the forward and the backward pass, in every call."""
+    q, k, v, do = (t.to(hip_device) for t in _draw(22, 1, 2, 2, 60, 70, 64, torch.bfloat16))
+    f = torch.compile(lambda q, k, v: train_ops.attention(q * 2, k, v) * 2, backend="aot_eager")
+    for scale in (1, 3):
+        leaves = [(t * scale).requires_grad_() for t in (q, k, v)]
+        o = f(*leaves)
+        got = (o.detach(), *torch.autograd.grad(o, leaves, do))
+        want = _attend(leaves[0].detach() * 2, leaves[1].detach(), leaves[2].detach(), do * 2)
+        assert _same(got, (want[0] * 2, want[1] * 2, *want[2:]))

@@ -368,3 +368,18 @@ def test_saved_tensors_that_hooks_make_others_of_are_refused(on_the_cpu):
         if change(torch.zeros(2, dtype=torch.int32)).dtype == torch.int32:
             with pytest.raises(RuntimeError, match="came back"):
                 torch.autograd.grad((h, n), (x, w), (torch.zeros_like(h), torch.zeros_like(n)))
+
+
+# ------------------------------------------------------------------------------------------------ through the attention op
+def test_the_op_takes_trainable(monkeypatch):
+    """torch's SDPA trains as it is (here the backend that a CPU has); a backend that has no backward pass is refused."""
+    from ksanadit_amd import KsanaAttentionBackend, KsanaAttentionConfig, attention_op, pick_attn_op
+    from ksanadit_amd.backends.radial_sage_attn import RadialSageAttentionImpl
+
+    make = pick_attn_op(KsanaAttentionConfig(backend=KsanaAttentionBackend.TORCH_SDPA))
+    q = torch.randn(1, 5, 2, 64, requires_grad=True)
+    (g,) = torch.autograd.grad(make(num_heads=2, head_size=64, trainable=True)(q, q, q).square().sum(), q)
+    assert g.abs().max() > 0
+    monkeypatch.setattr(attention_op, "get_attention_backend_impl", lambda **kw: RadialSageAttentionImpl)
+    with pytest.raises(ValueError, match="no backward pass"):
+        make(num_heads=2, head_size=64, trainable=True)(q, q, q)
