@@ -571,17 +571,22 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       const int at = row_position(p, r), h = hk * p.group + r - at * p.group;
       const uint16_t* o = p.o_in + b * p.os.sB + at * p.os.sL + h * p.os.sH + 8 * hh;
       const float lse = p.lse[((int64_t)b * p.Hq + h) * p.Lq + at];
-      float sum = 0.0f;
+      float sum[T::kSteps] = {};
 #pragma unroll
       for (int s = 0; s < T::kSteps; ++s) {
         float x[8], y[8];
         widen8<DT>(*reinterpret_cast<const uint4*>(o + 16 * s), x);
         widen8<DT>(__builtin_bit_cast(uint4, g[s]), y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = __fmaf_rn(x[j], y[j], sum);
+        for (int j = 0; j < 8; ++j) sum[s] = __fmaf_rn(x[j], y[j], sum[s]);
       }
+      // (added up in the order of that kernel's lanes: dk and dv have the same bits whether dq is wanted or not)
+#pragma unroll
+      for (int n = T::kSteps / 2; n > 0; n /= 2)
+#pragma unroll
+        for (int s = 0; s < n; ++s) sum[s] += sum[s + n];
       l = row_minus<DT>(lse);
-      d = -over_halves<Sum>(sum);
+      d = -over_halves<Sum>(sum[0]);
       if (place.run == 0 && hh == 0 && row < e.rows) {
         p.row_l[(int64_t)bh * p.row_pad + row] = l;
         p.row_d[(int64_t)bh * p.row_pad + row] = d;

@@ -218,6 +218,18 @@ def test_only_wanted_gradients(hip_device):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("B,Hq,Hkv,Lq,Lk,D,causal", [(1, 8, 8, 700, 300, 128, False), (2, 8, 4, 333, 500, 64, True), (1, 4, 1, 64, 3000, 128, False)])
+def test_gradients_of_keys_do_not_hang_on_who_else_wants_one(hip_device, dtype, B, Hq, Hkv, Lq, Lk, D, causal):
+    """Rows' numbers come along with dq where that is wanted, and from a kernel of their own where it is not: the same bits, in every row."""
+    for seed in range(4):
+        q, k, v, do = (t.to(hip_device) for t in _draw(40 + seed, B, Hq, Hkv, Lq, Lk, D, dtype))
+        _, _, dk, dv = _attend(q, k, v, do, is_causal=causal)
+        leaves = [k.detach().requires_grad_(), v.detach().requires_grad_()]
+        assert _same(torch.autograd.grad(train_ops.attention(q, *leaves, is_causal=causal), leaves, do), (dk, dv))
+
+
+@gpu
 def test_saved_tensors_may_be_kept_elsewhere(hip_device):
     q, k, v, do = (t.to(hip_device) for t in _draw(9, 2, 4, 2, 100, 140, 64, torch.bfloat16))
     want = _attend(q, k, v, do, k_lens=[140, 31])
