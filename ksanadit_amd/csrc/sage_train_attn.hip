@@ -503,8 +503,8 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 }
 
 // A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
-// k^T dS^T.  A half's vector work stands behind matrix instructions of the other half (in front of them: 1371 us where this takes 1308).
-// 8 heads of 16384 tokens: bf16 1416 us, 1165 TFLOP/s, fp16 1508; of 64 channels 861 us.
+// k^T dS^T.  A half's vector work stands behind matrix instructions of the other half: the matrix pipes
+// are busy 69 - 76 % of the time.  8 heads of 16384 tokens: bf16 1416 us, 1165 TFLOP/s, fp16 1508; of 64 channels 861 us.
 //
 // A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and that
 // carries the mean of the keys that the row attends to into dq wherever this is off zero.  The m that takes most of it away is that mean, sum P k.  It is
@@ -932,7 +932,8 @@ TrainCut cut_of(int64_t blocks, int tiles, double bytes, bool differ, double sha
   const int64_t rest = blocks - whole;
   double least = 1e30;
   int best = tiles;  // of a run
-  const int most = rest > (1 << 19) ? 1 : std::min(tiles, kMostRuns);  // (a launch holds 2^24 workgroups)
+  // a launch holds fewer than 2^24 workgroups, and a join has up to 16 of them to a block
+  const int most = rest > (1 << 19) ? 1 : (int)std::min<int64_t>(std::min(tiles, kMostRuns), ((1 << 24) - 1 - whole) / std::max<int64_t>(rest, 1));
   for (int n = 1; n <= most; ++n) {
     const int each = (tiles + n - 1) / n;
     const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * rest * bytes * share / kBytesPerTile;

@@ -113,6 +113,20 @@ def test_calls_of_the_attention_are_checked(kw, rc):
     assert lib.ksana_sage_train_attn_scratch(None, None, None) == -1
 
 
+def test_cut_loops_stay_within_a_launch():
+    """Workgroups of a launch, 256 threads each, as the scratch of the runs tells them: fewer than 2^24, whatever is asked for."""
+    lib, g = _capi.load(), torch.Generator().manual_seed(3)
+    n, cut = C.c_uint64(0), 0
+    for _ in range(4000):
+        B, heads, group, Lq, Lk = (int(2 ** (torch.rand((), generator=g) * bits)) for bits in (10, 9, 4, 24, 24))
+        c = _attn_call(B=B, Hq=heads * group, Hkv=heads, Lq=Lq, Lk=Lk, D=64 * int(torch.randint(1, 3, (), generator=g)), causal=int(torch.randint(2, (), generator=g)))
+        if lib.ksana_sage_train_attn_scratch(C.addressof(c), C.addressof(n), None) == 0:
+            workgroups = n.value // (128 * (c.shape.D + 2) * 4)  # cut blocks times their runs
+            assert workgroups < 2**24
+            cut += workgroups > 0
+    assert cut > 500
+
+
 @pytest.mark.parametrize("change,what", [
     (dict(q=None), b"q is null"), (dict(k=0x1008), b"not 16-byte"), (dict(lse=0x1002), b"lse"), (dict(c=dict(q_strides=_capi.Strides(1, 2, 3, 1))), b"stride"),
     (dict(c=dict(v_strides=_capi.Strides(4096, 256, 128, 2))), b"D stride"), (dict(scratch=None), b"scratch is null"), (dict(scratch=0x1010), b"256-byte"),
