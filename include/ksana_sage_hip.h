@@ -456,7 +456,7 @@ typedef struct ksana_sage_train_attn {
   ksana_sage_shape shape;
   int32_t dtype;          /* of q, k, v, o and all gradients                                                       */
   int32_t causal;         /* row i sees keys 0 .. i                                                                */
-  float sm_scale;
+  float sm_scale;         /* at most 2e38 in size                                                                  */
   int32_t reserved;       /* 0                                                                                     */
   int64_t q_strides[4], k_strides[4], v_strides[4], o_strides[4];
   const int32_t* q_lens;  /* device, [B] or NULL: only the first q_lens[b] query rows are computed, the others are zeros */

@@ -1048,7 +1048,8 @@ int train_attn_params(const ksana_sage_train_attn* c, ksana_sage::TrainAttnParam
   if (s.D != 128 && s.D != 64) return fail(KSANA_SAGE_ENOTSUP, "head size %d not supported (128 or 64)", s.D);
   if (c->dtype != KSANA_SAGE_BF16 && c->dtype != KSANA_SAGE_FP16) return fail(KSANA_SAGE_EINVAL, "dtype %d unknown", c->dtype);
   if (c->reserved != 0) return fail(KSANA_SAGE_EINVAL, "reserved is %d, must be 0", c->reserved);
-  if (!(c->sm_scale > -INFINITY && c->sm_scale < INFINITY)) return fail(KSANA_SAGE_EINVAL, "sm_scale is not finite");
+  // (times log2(e) it has to be a number still)
+  if (!(c->sm_scale >= -2e38f && c->sm_scale <= 2e38f)) return fail(KSANA_SAGE_EINVAL, "sm_scale is not a number of at most 2e38 in size");
   if (s.Lq > (1 << 24) || s.Lk > (1 << 24)) return fail(KSANA_SAGE_ENOTSUP, "Lq=%d Lk=%d: at most %d", s.Lq, s.Lk, 1 << 24);
   // query rows of the heads of a key head are numbered together: their number in an int, its division by a product of 32 x 32 bits
   const int64_t group = s.Hq / s.Hkv;

@@ -184,8 +184,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: 
         q, k, v = (t.transpose(1, 2) if t.dim() == 4 else t for t in (q, k, v))
     _check_attention(q, k, v)
     _refuse_unseen("attention", q, k, v)
-    if sm_scale is not None and not abs(sm_scale) < 3.4e38:
-        raise ValueError(f"sm_scale {sm_scale} is not a finite fp32 number")
+    if sm_scale is not None and not abs(sm_scale) <= 2e38:
+        raise ValueError(f"sm_scale {sm_scale} is not a number of at most 2e38 in size")
     k_lens, q_lens = (_k_lens_arg(n, q.shape[0], q.device, name) for n, name in ((k_lens, "k_lens"), (q_lens, "q_lens")))
     q, k, v = _readable(q), _readable(k), _readable(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -397,3 +397,14 @@ def test_the_op_takes_trainable(monkeypatch):
     monkeypatch.setattr(attention_op, "get_attention_backend_impl", lambda **kw: RadialSageAttentionImpl)
     with pytest.raises(ValueError, match="no backward pass"):
         make(num_heads=2, head_size=64, trainable=True)(q, q, q)
+
+
+def test_scales_whose_product_with_log2_e_fp32_cannot_hold(monkeypatch):
+    """Scores are scaled by sm_scale log2(e): infinite, it made not-a-numbers of scores of zero."""
+    monkeypatch.setattr(train_ops, "_check_attention", lambda *a: None)
+    q, lib, n = _meta(1, 4, 2, 64), _capi.load(), C.c_uint64(0)
+    for scale, rc in ((2.4e38, -1), (-3.3e38, -1), (1.9e38, 0), (-1.9e38, 0)):
+        assert lib.ksana_sage_train_attn_scratch(C.addressof(_attn_call(sm_scale=scale)), C.addressof(n), C.addressof(n)) == rc
+        if rc != 0:
+            with pytest.raises(ValueError, match="sm_scale"):
+                train_ops.attention(q, q, q, sm_scale=scale)
