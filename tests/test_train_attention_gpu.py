@@ -19,12 +19,13 @@ what they see for others.  There the sum of dS', which is one of e, goes into a 
 So much for any kernel with that m, and these bounds stand.  The kernel's own m is nearer to what a row attends to (an estimate of sum P k), for which its first
 term, P times what d is off by, nearly vanishes: it keeps to about a third of them, and ``test_keys_of_two_kinds`` says what it keeps to that a first tile's mean does not."""
 
+import ctypes as C
 import math
 
 import pytest
 import torch
 
-from ksanadit_amd import train_ops
+from ksanadit_amd import _capi, train_ops
 
 gpu = pytest.mark.gpu
 HALF_STEP = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
@@ -350,6 +351,39 @@ def test_cut_loops_against_uncut_ones(hip_device, Hq, Hkv, Lq, Lk, causal):
     for x, y, most in zip(got, want[::2], want[1::2]):
         x = x[:, :, -y.shape[2] :].cpu().double()
         assert ((x - y).abs() <= most).all()
+
+
+def _runs_scratch(q, k, causal, k_lens):
+    """Bytes that the runs of a call's cut loops need, forward and backward: none where every block is walked whole"""
+    lib, n = _capi.load(), (C.c_uint64 * 2)()
+    call = train_ops._attention_call(q, k, k, q, causal, None, k_lens, None)
+    assert lib.ksana_sage_train_attn_scratch(call, C.addressof(n), C.addressof(n) + 8) == 0
+    B, Lq, Hq, _ = q.shape
+    Lk, Hkv = k.shape[1:3]
+    tiles = -(-Lq * Hq // Hkv // 64)
+    rows = 2 * (-(-B * Hkv * tiles * 64 * 4 // 256) * 256) + -(-B * Hkv * (tiles + (-(-Lk // 64) if q.dtype == torch.float16 else 0)) * 4 // 256) * 256
+    return n[0], n[1] - rows
+
+
+@gpu
+@pytest.mark.parametrize("B,Hq,Hkv,Lq,Lk,D,dtype,causal,k_lens,copies,forward_too", [
+    (1, 4, 4, 1024, 1024, 128, torch.bfloat16, False, None, 16, True), (1, 4, 4, 1024, 1024, 64, torch.float16, False, None, 48, True),
+    (1, 4, 2, 1000, 900, 128, torch.bfloat16, True, None, 32, True), (1, 8, 8, 8192, 100, 128, torch.bfloat16, False, None, 64, False),
+    (1, 6, 2, 5, 4000, 128, torch.float16, False, None, 256, True), (2, 4, 4, 600, 700, 64, torch.bfloat16, False, [700, 333], 96, True)])
+def test_the_same_heads_cut_and_whole(hip_device, B, Hq, Hkv, Lq, Lk, D, dtype, causal, k_lens, copies, forward_too):
+    """Few heads, whose loops are cut into runs (of the keys alone where queries are many), and copies of them that fill the card, none of which is."""
+    t = _draw(23, B, Hq, Hkv, Lq, Lk, D, dtype)
+    want = _formula(*t, causal=causal, k_lens=k_lens)
+    for n in (1, copies):
+        q, k, v, do = (x.to(hip_device).repeat(n, 1, 1, 1) for x in t)
+        lens = None if k_lens is None else torch.tensor(k_lens * n, dtype=torch.int32, device=hip_device)
+        fwd, bwd = _runs_scratch(q, k, causal, lens)
+        assert (fwd > 0, bwd > 0) == (n == 1 and forward_too, n == 1)
+        got = _attend(q, k, v, do, is_causal=causal, k_lens=lens)
+        for name, x, y, most in zip(("o", "dq", "dk", "dv"), got, want[::2], want[1::2]):
+            assert torch.equal(x[:B], x[-B:]), name
+            off = ((x[:B].cpu().double() - y).abs() / most).max().item()
+            assert off <= 1.0, f"{name}: {off:.2f} of what roundings allow, {n} copies"
 
 
 @gpu
