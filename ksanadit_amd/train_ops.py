@@ -19,7 +19,7 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _capi
-from .sage_ops import _DTYPES, _k_lens_arg, _require_hip, _stream_ptr, _strides, _usable
+from .sage_ops import _DTYPES, _k_lens_arg, _require_hip, _stream_ptr, _usable
 
 
 def _on(device: torch.device):
@@ -52,15 +52,14 @@ def _scratch(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _kept(t: torch.Tensor | None, dtype: torch.dtype, shape) -> torch.Tensor | None:
+def _kept(t: torch.Tensor | None, dtype: torch.dtype, shape, device: int) -> torch.Tensor | None:
     """What a forward pass saved for the kernels, contiguous and at an address they read: hooks that keep saved tensors elsewhere may give them back laid
     out and placed otherwise, but not as other tensors."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape:
-        raise RuntimeError(f"a saved tensor came back from its hooks as {t.dtype} {tuple(t.shape)}, it was {dtype} {tuple(shape)}")
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+        raise RuntimeError(f"a saved tensor came back from its hooks as {t.dtype} {tuple(t.shape)} on {t.device}, it was {dtype} {tuple(shape)}")
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -70,6 +69,7 @@ def _ptr(t: torch.Tensor | None):
 # The library's structures, packed (ctypes takes three times as long to build one; a call of few tokens costs what its host work does)
 _ATTENTION = struct.Struct("=8ifi16q2Q")  # ksana_sage_train_attn
 _NORM = struct.Struct("=7i2fi4q" + 6 * "Qqii")  # ksana_sage_train_norm
+_STRIDES, _POINTERS = struct.Struct("=4q"), struct.Struct("=6Q")
 
 
 def _attention_call(q, k, v, o, is_causal: bool, sm_scale: float | None, k_lens, q_lens) -> bytes:
@@ -112,17 +112,20 @@ def _attention_backward(do, q, k, v, o, lse, scratch_bytes, k_shape, is_causal, 
     dk, dv = (_contiguous_like(k), _contiguous_like(k)) if want_kv else (None, None)
     if q.numel() == 0 or k.numel() == 0:
         return tuple(None if t is None else t.zero_() for t in (dq, dk, dv))
-    if not (q.shape == o.shape == do.shape and k.shape == v.shape == k_shape and q.dtype == k.dtype == v.dtype == o.dtype == do.dtype):
-        raise RuntimeError("a saved tensor came back from its hooks with another shape or type")
+    shape, dtype, device = do.shape, do.dtype, do.get_device()
+    if not (q.shape == shape and o.shape == shape and k.shape == k_shape and v.shape == k_shape
+            and q.dtype is dtype and k.dtype is dtype and v.dtype is dtype and o.dtype is dtype
+            and q.get_device() == device and k.get_device() == device and v.get_device() == device and o.get_device() == device):
+        raise RuntimeError("a saved tensor came back from its hooks with another shape, type or device")
     # (the saved tensors too: see _kept)
-    do, q, k, v, o = (_readable(t) for t in (do, q, k, v, o))
-    B, Lq, Hq = q.shape[:3]
-    lse, k_lens, q_lens = _kept(lse, torch.float32, (B, Hq, Lq)), _kept(k_lens, torch.int32, (B,)), _kept(q_lens, torch.int32, (B,))
-    call, strides = _attention_call(q, k, v, o, is_causal, sm_scale, k_lens, q_lens), _strides(do)
+    do, q, k, v, o = _readable(do), _readable(q), _readable(k), _readable(v), _readable(o)
+    lse = _kept(lse, torch.float32, (shape[0], shape[2], shape[1]), device)
+    k_lens, q_lens = _kept(k_lens, torch.int32, shape[:1], device), _kept(q_lens, torch.int32, shape[:1], device)
+    call = _attention_call(q, k, v, o, is_causal, sm_scale, k_lens, q_lens)
     with _on(q.device):
         scratch = _scratch(scratch_bytes, q.device)
         rc = _capi.load().ksana_sage_train_attn_bwd(call, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), do.data_ptr(),
-                                                    C.addressof(strides), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(scratch), _stream_ptr(q.device))
+                                                    _STRIDES.pack(*do.stride()), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(scratch), _stream_ptr(q.device))
     if rc != _capi.OK:
         _capi.check(rc, "train_ops.attention, backward")
     return dq, dk, dv
@@ -142,9 +145,9 @@ class _Once(torch.autograd.Function):
 
 
 def _not_twice(grads: tuple, *sources: torch.Tensor | None) -> tuple:
-    if not torch.is_grad_enabled():
-        return grads
     given = [t for t in grads if t is not None]
+    if not given:
+        return grads
     out = iter(_Once.apply(len(given), *given, *(t for t in sources if t is not None)))
     return tuple(None if t is None else next(out) for t in grads)
 
@@ -160,11 +163,18 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         _refuse_unseen("attention's backward pass", do)
+        if torch.is_grad_enabled():
+            with torch.no_grad():
+                d = _Attention.gradients(ctx, do)
+            return _not_twice(d, do, *ctx.saved_tensors[:3])
+        return _Attention.gradients(ctx, do)
+
+    @staticmethod
+    def gradients(ctx, do):
         want_q, want_k, want_v = ctx.needs_input_grad[:3]
         q, k, v, o, lse, k_lens, q_lens = ctx.saved_tensors
-        with torch.no_grad():
-            dq, dk, dv = _attention_backward(do, q, k, v, o, lse, *ctx.options, k_lens, q_lens, want_q, want_k or want_v)
-        return *_not_twice((dq, dk if want_k else None, dv if want_v else None), do, q, k, v), None, None, None, None
+        dq, dk, dv = _attention_backward(do, q, k, v, o, lse, *ctx.options, k_lens, q_lens, want_q, want_k or want_v)
+        return dq, dk if want_k else None, dv if want_v else None, None, None, None, None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tensor_layout: str = "NHD", is_causal: bool = False,
@@ -230,36 +240,39 @@ def _residual_norm_forward(x, y, call, n_dtype, want_stats: bool):
     return h, n, stats
 
 
-def _residual_norm_backward(grads, saved, options, wanted) -> tuple:
-    """Gradients of x, y and the six vectors from those of the results, None where there is nothing or nothing is wanted"""
-    x, y, stats, *vectors = saved
+def _residual_norm_backward(ctx, grads) -> tuple:
+    x, y, stats, *vectors = ctx.saved_tensors
     dh, dn = grads if y is not None else (None, grads[0])
-    n_dtype = options[-1]
+    if dh is None and dn is None:
+        return (None,) * 13
+    options, like = ctx.options, dn if dh is None else dh
+    n_dtype, shape, device = options[-1], like.shape, like.get_device()
     # (hooks may have laid the saved tensors out anew: see _kept.  All copies are held until the launches are made.)
-    like = dn if dh is None else dh
-    if x.shape != like.shape or (dh is not None and x.dtype != dh.dtype) or (y is not None and (y.shape != x.shape or y.dtype != n_dtype)):
-        raise RuntimeError("a saved tensor came back from its hooks with another shape or type")
+    if x.shape != shape or x.get_device() != device or (dh is not None and x.dtype is not dh.dtype) or (
+            y is not None and (y.shape != shape or y.dtype is not n_dtype or y.get_device() != device)):
+        raise RuntimeError("a saved tensor came back from its hooks with another shape, type or device")
     x, y = _rows(x), None if y is None else _rows(y)
-    vectors = [_norm_vector(name, t, x) for name, t in zip(_VECTORS, vectors)]
-    stats = _kept(stats, torch.float32, (*x.shape[:2], 4))
+    vectors = [t if t is None or (t.is_contiguous() and t.shape == s and t.get_device() == device) else _norm_vector(name, t, x)
+               for name, t, s in zip(_VECTORS, vectors, ctx.shapes)]
+    stats = _kept(stats, torch.float32, (shape[0], shape[1], 4), device)
     call = _norm_call(x, y, vectors, *options)
     dn = torch.zeros(x.shape, dtype=n_dtype, device=x.device) if dn is None else dn.contiguous()
     dh = None if dh is None else dh.contiguous()
     dx, dy = _contiguous_like(x), None if y is None else _contiguous_like(y)
-    d_vectors = [_contiguous_like(t) if t is not None and want else None for t, want in zip(vectors, wanted)]
+    d_vectors = [_contiguous_like(t) if t is not None and want else None for t, want in zip(vectors, ctx.needs_input_grad[2:8])]
     if x.numel() == 0:
-        return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors))
+        return (dx, dy, *(None if t is None else t.zero_() for t in d_vectors), *(None,) * 5)
     lib = _capi.load()
-    nbytes, pointers = C.c_uint64(0), (C.c_void_p * 6)(*[_ptr(t) for t in d_vectors])
+    nbytes, pointers = C.c_uint64(0), _POINTERS.pack(*[0 if t is None else t.data_ptr() for t in d_vectors])
     rc = lib.ksana_sage_train_norm_scratch(call, C.addressof(nbytes))
     if rc == _capi.OK:
         with _on(x.device):
             scratch = _scratch(nbytes.value, x.device)
             rc = lib.ksana_sage_train_norm_bwd(call, x.data_ptr(), _ptr(y), stats.data_ptr(), _ptr(dh), dn.data_ptr(), dx.data_ptr(), _ptr(dy),
-                                               C.addressof(pointers), _ptr(scratch), _stream_ptr(x.device))
+                                               pointers, _ptr(scratch), _stream_ptr(x.device))
     if rc != _capi.OK:
         _capi.check(rc, "train_ops.residual_norm, backward")
-    return (dx, dy, *d_vectors)
+    return (dx, dy, *d_vectors, *(None,) * 5)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -269,18 +282,19 @@ class _ResidualNorm(torch.autograd.Function):
         h, n, stats = _residual_norm_forward(x, y, _norm_call(x, y, vectors, norm, post_norm, residual_scale, eps, n_dtype), n_dtype, True)
         ctx.save_for_backward(x, y, stats, *vectors)
         ctx.options = (norm, post_norm, residual_scale, eps, n_dtype)
+        ctx.shapes = [None if t is None else t.shape for t in vectors]
         ctx.set_materialize_grads(False)
         return n if y is None else (h, n)
 
     @staticmethod
     def backward(ctx, *grads):
         _refuse_unseen("residual_norm's backward pass", *grads)
-        if all(g is None for g in grads):
-            return (None,) * 13
-        saved = ctx.saved_tensors
-        with torch.no_grad():
-            d = _residual_norm_backward(grads, saved, ctx.options, ctx.needs_input_grad[2:8])
-        return *_not_twice(d, *grads, saved[0], saved[1], *saved[3:]), *(None,) * 5
+        if torch.is_grad_enabled():
+            with torch.no_grad():
+                d = _residual_norm_backward(ctx, grads)
+            x, y, _, *vectors = ctx.saved_tensors
+            return _not_twice(d, *grads, x, y, *vectors)
+        return _residual_norm_backward(ctx, grads)
 
 
 def _wants_gradient(*tensors) -> bool:

@@ -251,6 +251,18 @@ def test_saved_tensors_may_be_laid_out_anew(hip_device):
 
 
 @gpu
+@pytest.mark.parametrize("of", ["q", "lse", "lens"])
+def test_saved_tensors_left_elsewhere_are_refused(hip_device, of):
+    """What a hook gives back on the host is no address that a kernel reads."""
+    q = torch.zeros(1, 20, 2, 64, device=hip_device, dtype=torch.float16, requires_grad=True)
+    kind = {"q": torch.float16, "lse": torch.float32, "lens": torch.int32}[of]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu() if t.dtype == kind else t):
+        o = train_ops.attention(q, q, q, k_lens=torch.tensor([15], dtype=torch.int32, device=hip_device))
+    with pytest.raises(RuntimeError, match="came back"):
+        o.backward(torch.zeros_like(o))
+
+
+@gpu
 def test_what_cannot_be_differentiated_is_refused(hip_device):
     q = torch.randn(1, 20, 1, 64, device=hip_device, dtype=torch.float16, requires_grad=True)
     lens = torch.tensor([15], dtype=torch.int32, device=hip_device)

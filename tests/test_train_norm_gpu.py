@@ -289,3 +289,13 @@ def test_saved_tensors_may_be_laid_out_anew(hip_device):
     with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: torch.stack((x, torch.full_like(x, 7)), -1)[..., 0]):
         got = _run(t, dh, dn, hip_device, "rms", "layer", 0.5)
     assert _same(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("of", [bf16, fp32, fp16], ids=["rows", "statistics", "vectors"])
+def test_saved_tensors_left_elsewhere_are_refused(hip_device, of):
+    x, w = torch.zeros(2, 3, 16, device=hip_device, dtype=bf16, requires_grad=True), torch.ones(16, device=hip_device, dtype=fp16, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu() if t.dtype == of else t):
+        h, n = train_ops.residual_norm(x, x, weight=w)
+    with pytest.raises((RuntimeError, ValueError), match="came back|weight must be"):
+        torch.autograd.grad((h, n), (x, w), (torch.zeros_like(h), torch.zeros_like(n)))

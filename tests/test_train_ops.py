@@ -253,7 +253,7 @@ def test_gradients_of_gradients_are_refused_however_they_are_asked_for(on_the_cp
         outs = out if isinstance(out, tuple) else (out,)
         dos = [torch.zeros_like(o).requires_grad_() for o in outs]
         (d,) = torch.autograd.grad(outs, leaf, dos, create_graph=True)
-        assert d.shape == leaf.shape
+        assert d.shape == leaf.shape and train_ops._not_twice((None, None), leaf) == (None, None)
         for other in (leaf, *dos):
             with pytest.raises(RuntimeError, match="gradients of gradients"):
                 torch.autograd.grad(d.sum(), other, retain_graph=True)
