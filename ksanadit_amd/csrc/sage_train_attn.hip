@@ -8,12 +8,14 @@
 // keeps query rows and walks the keys).  That is seven products of the backward pass where five would do with dq summed by
 // atomic additions of all workgroups: their order would change the result from call to call.
 //
-// P and dS are rounded to the tensors' type where they become matrix operands; S, dP, all sums and accumulators are fp32.
+// P and dS are rounded to the tensors' type where they become matrix operands, which have 16 bits where they are to run at this rate; S, dP, all
+// sums and accumulators are fp32.  d is formed from the result as it is rounded: an unrounded one, as much memory again, leaves dq the same error
+// (0.0024 in bf16), since P's roundings are in it too.
 //
-// Long sequences are bound by what the matrix pipes draw: with them busy 64 % (forward), 69 % (dq) and 65 % (dk and dv) of the time the
-// clock falls from 2.4 to 1.7 - 1.8 GHz.  20 heads of 32760 bf16 tokens of 128 channels: forward 10.0 ms, dq 13.8, dk and dv 18.5, that
-// is 1100, 1200 and 1190 TFLOP/s of the products that they form (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
-// and what a workgroup does besides its loop, 32760 rows on 512 keys, 40 heads: 426, 621 and 662 us; a few rows by a chain of latencies.
+// Long sequences are bound by what the matrix pipes draw: with them busy 65 % (forward), 70 % (dq) and 66 % (dk and dv) of the time the
+// clock falls from 2.4 to 1.7 - 1.8 GHz.  20 heads of 32760 bf16 tokens of 128 channels: forward 9.2 ms, dq 12.7, dk and dv 17.0, that
+// is 1200, 1290 and 1290 TFLOP/s of the products that they form, 8 % less on slow boxes (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
+// and what a workgroup does besides its loop, 32760 rows on 512 keys, 40 heads: 422, 642 and 666 us; a few rows by a chain of latencies.
 #include "sage_train_device.h"
 
 #include <algorithm>
@@ -87,7 +89,8 @@ __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + 
 // A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys, two waves to a SIMD.  While the
 // probabilities of tile t are formed and multiplied with its values, the scores of tile t + 1 are: a few vector instructions stand behind
 // every matrix instruction and run beside it.  So values are wanted a step after their keys; each have two places in LDS.
-// 8 heads of 16384 tokens: bf16 1024 us, 1075 TFLOP/s, fp16 1086; of 64 channels 670 us, where exponentials count twice as much.
+// 8 heads of 16384 tokens: bf16 981 us, 1121 TFLOP/s, fp16 1030; of 64 channels 667 us, where exponentials count twice as much.  Of 128 channels 14 or 16
+// registers go through memory, before the loop and behind it.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_fwd_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -363,7 +366,7 @@ __device__ __forceinline__ float ds_scale(const TrainAttnParams& p, int bh, int 
 
 // A wave keeps 32 keys and walks tiles of 64 query rows in halves: S = q k^T and dP = dO v^T (a lane holds scores of one key; dP's
 // accumulators start at -d), dv^T += dO^T P, dk^T += q^T dS.  The other wave of the SIMD works beside a wave's vector instructions.
-// 8 heads of 16384 tokens: bf16 1899 us, 1160 TFLOP/s, fp16 2053; of 64 channels 1055 us.
+// 8 heads of 16384 tokens: bf16 1826 us, 1205 TFLOP/s, fp16 1947; of 64 channels 1011 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -504,17 +507,17 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 
 // A wave keeps 32 query rows and walks tiles of 64 keys in halves: S^T = k q^T, dP^T = v dO^T (their accumulators start at -d), dq^T +=
 // k^T dS^T.  A half's vector work stands behind matrix instructions of the other half: the matrix pipes
-// are busy 69 - 76 % of the time.  8 heads of 16384 tokens: bf16 1416 us, 1165 TFLOP/s, fp16 1508; of 64 channels 861 us.
+// are busy 70 % of the time.  8 heads of 16384 tokens: bf16 1347 us, 1224 TFLOP/s, fp16 1421; of 64 channels 850 us.
 //
 // A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and that
 // carries the mean of the keys that the row attends to into dq wherever this is off zero.  The m that takes most of it away is that mean, sum P k.  It is
 // estimated: the row's own probabilities on kSpread keys, spread evenly over those that the block sees; where its first row sees few, on the first kSpread and
 // as many spread over the others, each of these weighted with the keys it stands for.  As a last tile the sum of the rounded dS times their shares is
 // subtracted from dS, so keys of one kind or of several, text in front of an image or a whole sequence, leave the same error.  Relative error against 64
-// bits, bf16, 4352 keys N(0, 1): 0.0025; without m 0.0024, and 0.0039, 0.012, 0.024 with all keys off zero by 1, 4, 8 times N(0, 1) per channel, where
-// 0.0025 remain with it; the first 64, or half of them, off by 4 and not attended to: 0.0025 and 0.0026 (with the mean of the first 64 for m 0.013 and
-// 0.011); an eighth of them attended to, or half: 0.0030 and 0.0026 (without 0.012).  Rows that attend to a single key are worse off with an
-// estimate, 0.0058 for 0.0045 where scores vary by 16, and a key far off that carries most of a row and is not in the sample stays as without (0.0097).  The mean
+// bits, bf16, 512 rows on 4352 keys N(0, 1): 0.0025, without m 0.0024.  All keys off zero by 1, 4, 8 times N(0, 1) per channel: 0.0025, without 0.0036, 0.012,
+// 0.021.  The first 64, or half of them, off by 4 and not attended to: 0.0025 and 0.0026 (with the mean of the first 64 for m 0.012 in both); an eighth of
+// them attended to, or half: 0.0029 and 0.0026 (without 0.011).  Rows that attend to one key or two are worse off with an estimate, 0.0039 for 0.0031 where
+// scores vary by 4 and 0.0074 for 0.0058 where by 16, and a key far off that carries most of a row and is not in the sample stays as without (0.0073).  The mean
 // itself, one more product, leaves 0.0019 - 0.0024 in all of these and takes a third more work.  64 keys leave 0.0024 - 0.0028 and take 1.6 % of the pass
 // of 32760 rows on 512 keys; 32 take 0 - 1 %.
 template <int DT, int D>

@@ -551,7 +551,7 @@ struct NormShape {
   int vecs, threads;
 };
 NormShape norm_shape(int C) {
-  for (int vecs = 1; vecs <= 2; ++vecs) {  // (with three, the backward kernel's sums and rows do not fit the registers)
+  for (int vecs = 1; vecs <= 2; ++vecs) {  // (with three, the backward kernel's sums and rows do not fit the registers; with two, 2 - 10 of fp32 streams of odd width go through memory)
     const int threads = (C + 512 * vecs - 1) / (512 * vecs) * 64;
     if (threads <= kMaxThreads) return NormShape{vecs, threads};
   }

@@ -4,8 +4,9 @@
 masking, 16-bit products without quantization, and a backward pass that recomputes the probabilities.
 ``residual_norm`` is what stands between two parts of a block: gate, residual sum, norm and modulation in one pass.
 
-Both run on the tensors' HIP device, on torch's current stream there, without synchronising; scratch comes from torch's caching
-allocator.  Repeated calls give the same bits.  Gradients of gradients are refused.
+Both run on the tensors' HIP device, on torch's current stream there; scratch comes from torch's caching allocator.  They do not synchronise and may be
+captured into a graph, with counts, if any, as int32 tensors on that device (others are copied there in the call, which waits for the copy and cannot be captured).
+Repeated calls give the same bits.  Gradients of gradients, forward-mode derivatives and tracing are refused; ``torch.compile`` leaves its graph for them.
 """
 
 from __future__ import annotations

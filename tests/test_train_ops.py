@@ -208,6 +208,7 @@ def _forward_dual(f, t):
         f(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
 
 
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 @pytest.mark.parametrize("wants_gradient", [False, True])
 @pytest.mark.parametrize("through", [
     _forward_dual, lambda f, t: torch.func.jvp(f, (t,), (t,)), lambda f, t: torch.jit.trace(f, t, check_trace=False), lambda f, t: make_fx(f)(t),
