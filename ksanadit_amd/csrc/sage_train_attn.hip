@@ -694,7 +694,7 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       const int spread = block_sees - spread_from, seen = limit - spread_from;  // key j of the first half is key j spread / kSpread of those
       scores(0, spread >= kSpread ? (kSpread * seen + spread - 1) / spread : seen);
       if (few) scores(1, limit);
-      most = over_halves<Max>(most) * p.c;
+      most = fmaxf(over_halves<Max>(most) * p.c, -3e38f);  // (scores that are all out of fp32's range: no shares)
       auto probabilities = [&](int h, float weight) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {

@@ -365,6 +365,22 @@ def test_cut_loops_against_uncut_ones(hip_device, Hq, Hkv, Lq, Lk, causal):
         assert ((x - y).abs() <= most).all()
 
 
+@gpu
+@pytest.mark.parametrize("Lk", [60, 256, 2048])
+def test_keys_whose_scores_leave_the_range_of_fp32(hip_device, Lk):
+    """Every eighth key (and with it all that dq estimates the mean key by, of 256 and more) has a score of minus infinity, finite as it is itself: it
+    weighs nothing, and the others' gradients are what they are without it, to the roundings of dS and of the result (u each, of sums of a few hundred
+    terms in no order: four of their root mean squares)."""
+    q, k, v, do = _draw(24, 1, 2, 2, 100, Lk, 128, torch.bfloat16)
+    q, k = ((q.float().abs() + 0.1) * 1e19).bfloat16(), (k.float() * 1e-19).bfloat16()
+    k[:, ::8] = -1e20
+    others = torch.arange(Lk) % 8 != 0
+    got = [t.cpu().double() for t in _attend(*(t.to(hip_device) for t in (q, k, v, do)))]
+    assert all(t.isfinite().all() for t in got) and not got[2][:, ~others].any() and not got[3][:, ~others].any()
+    want, rms = _dq_rms(q, k[:, others], v[:, others], do, False)
+    assert (got[1] - want).norm() <= 4 * rms
+
+
 def _runs_scratch(q, k, causal, k_lens):
     """Bytes that the runs of a call's cut loops need, forward and backward: none where every block is walked whole"""
     lib, n = _capi.load(), (C.c_uint64 * 2)()
