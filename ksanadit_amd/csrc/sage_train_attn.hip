@@ -14,7 +14,7 @@
 //
 // Long sequences are bound by what the matrix pipes draw: with them busy 65 % (forward), 70 % (dq) and 66 % (dk and dv) of the time the
 // clock falls from 2.4 to 1.7 - 1.8 GHz.  20 heads of 32760 bf16 tokens of 128 channels: forward 9.2 ms, dq 12.7, dk and dv 17.0, that
-// is 1200, 1290 and 1290 TFLOP/s of the products that they form, 8 % less on slow boxes (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
+// is 1200, 1290 and 1290 TFLOP/s of the products that they form, 8 % less on slower cards (a library's product of 16384^3: 1400).  Few keys under many rows are bound by the rows' bytes
 // and what a workgroup does besides its loop, 32760 rows on 512 keys, 40 heads: 422, 642 and 666 us; a few rows by a chain of latencies.
 #include "sage_train_device.h"
 
@@ -32,7 +32,7 @@ __device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__
 
 constexpr int kTrainBlock = 128;  // query rows, or keys, of a workgroup
 constexpr int kMostRuns = 128;    // of a block
-constexpr int kSpread = 32, kFewKeys = 128;  // keys that dq estimates a row's mean key by; rows that see fewer than kFewKeys take the first kSpread besides
+constexpr int kSpread = 32, kFewKeys = 128;  // keys that dq estimates a row's mean key by; blocks whose first row sees fewer than kFewKeys take the first kSpread besides
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // Rounded to fp16, probabilities relative to a row's largest would lose bits from 2^-14 on and vanish at 2^-25; scaled up as far as
 // the format goes, they do so a factor of 2^6 (forward, where the reference point may lag by 2^kLazy) or 2^15 (backward) later.
@@ -511,15 +511,16 @@ __global__ __launch_bounds__(256, 2) void sage_train_dkv_kernel(const TrainAttnP
 //
 // A row's dS sum to zero, so dq = c sum dS (k - m) for any m.  Rounded, and with d formed from the rounded result, they do not quite, and that
 // carries the mean of the keys that the row attends to into dq wherever this is off zero.  The m that takes most of it away is that mean, sum P k.  It is
-// estimated: the row's own probabilities on kSpread keys, spread evenly over those that the block sees; where its first row sees few, on the first kSpread and
-// as many spread over the others, each of these weighted with the keys it stands for.  As a last tile the sum of the rounded dS times their shares is
-// subtracted from dS, so keys of one kind or of several, text in front of an image or a whole sequence, leave the same error.  Relative error against 64
-// bits, bf16, 512 rows on 4352 keys N(0, 1): 0.0025, without m 0.0024.  All keys off zero by 1, 4, 8 times N(0, 1) per channel: 0.0025, without 0.0036, 0.012,
-// 0.021.  The first 64, or half of them, off by 4 and not attended to: 0.0025 and 0.0026 (with the mean of the first 64 for m 0.012 in both); an eighth of
-// them attended to, or half: 0.0029 and 0.0026 (without 0.011).  Rows that attend to one key or two are worse off with an estimate, 0.0039 for 0.0031 where
-// scores vary by 4 and 0.0074 for 0.0058 where by 16, and a key far off that carries most of a row and is not in the sample stays as without (0.0073).  The mean
-// itself, one more product, leaves 0.0019 - 0.0024 in all of these and takes a third more work.  64 keys leave 0.0024 - 0.0028 and take 1.6 % of the pass
-// of 32760 rows on 512 keys; 32 take 0 - 1 %.
+// estimated from kSpread keys, spread evenly over those that the block sees (where its first row sees few, from the first kSpread and as many spread over the
+// others): each with its own probability, and what these leave of one shared out by the probabilities' roots, weighted with the keys that each stands for.
+// (By the probabilities themselves a row of few large ones would have one key of the sample for its mean.)  As a last tile the sum of the rounded dS times their
+// shares is subtracted from dS, so keys of one kind or of several, text in front of an image or a whole sequence, leave about the same error.  Relative
+// error against 64 bits, bf16, 512 rows on 4352 keys N(0, 1): 0.0024, as without m.  All keys off zero by 1, 4, 8 times N(0, 1) per channel: 0.0024, without
+// 0.0036, 0.012, 0.021.  The first 64, or half of them, off by 4 and not attended to: 0.0024 and 0.0025 (with the mean of the first 64 for m 0.012 in both); an
+// eighth of them attended to, or half: 0.0028 and 0.0025 (without 0.011).  Rows that attend to one key or two are worse off with an estimate, 0.0034 for
+// 0.0031 where scores vary by 4 and 0.0071 for 0.0058 where by 16, and a key far off that carries most of a row and is not in the sample stays as without
+// (0.0073).  The mean itself, one more product, leaves 0.0019 - 0.0024 in all of these and takes a third more work.  The estimate costs 1.4 % of the pass of 32760
+// rows on 512 keys; where loops have 25 tiles and more nothing shows.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnParams p) {
   using T = Tile<D>;
@@ -695,20 +696,27 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
       scores(0, spread >= kSpread ? (kSpread * seen + spread - 1) / spread : seen);
       if (few) scores(1, limit);
       most = fmaxf(over_halves<Max>(most) * p.c, -3e38f);  // (scores that are all out of fp32's range: no shares)
-      auto probabilities = [&](int h, float weight) {
+      // roots of the probabilities relative to the largest: their sum, and what the keys have of the row
+      float mass = 0.0f;
+      auto roots = [&](int h, float weight) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[h][i] = fast_exp2(__fmaf_rn(s[h][i], p.c, -most)) * weight;
-          total += s[h][i];
+          s[h][i] = fast_exp2(0.5f * __fmaf_rn(s[h][i], p.c, -most));
+          total = __fmaf_rn(s[h][i], weight, total);
+          mass = __fmaf_rn(s[h][i], s[h][i], mass);
         }
       };
-      probabilities(0, fmaxf(1.0f, (float)spread / kSpread));  // (one key for so many)
-      if (few) probabilities(1, 1.0f);
+      const float weight = fmaxf(1.0f, (float)spread / kSpread);  // (one key for so many)
+      roots(0, weight);
+      if (few) roots(1, 1.0f);
       total = over_halves<Sum>(total);
-      const float share = total > 0.0f ? over_halves<Sum>(sum_ds) / -total : 0.0f;  // (not a number: nor is the row's dq)
-      auto subtract = [&](int h) {
+      sum_ds = -over_halves<Sum>(sum_ds);
+      const float minus = kHalf ? l - kBackwardShift<DT> - ((float)__builtin_amdgcn_frexp_expf(scale) - 1.0f) : l;  // -log2(e) lse
+      const float largest_one = fast_exp2(most + minus), rest = fmaxf(0.0f, 1.0f - over_halves<Sum>(mass) * largest_one);
+      const float own = sum_ds * largest_one, share = total > 0.0f ? sum_ds * rest / total : 0.0f;  // (not a number: nor is the row's dq)
+      auto subtract = [&](int h, float weight) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[h][i] *= share;
+        for (int i = 0; i < 16; ++i) s[h][i] *= __fmaf_rn(s[h][i], own, weight * share);
 #pragma unroll
         for (int f = 0; f < 2; ++f) ds[h][f] = pack(h, f);
         columns_product(tile + column_at, h, nothing);
@@ -724,8 +732,8 @@ __global__ __launch_bounds__(256, 2) void sage_train_dq_kernel(const TrainAttnPa
         }
         columns_product(tile + column_at, h, nothing);
       };
-      subtract(0);
-      if (few) subtract(1);
+      subtract(0, weight);
+      if (few) subtract(1, 1.0f);
     }
   }
   const float unshift = fast_exp2(-kBackwardShift<DT>);

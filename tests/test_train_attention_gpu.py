@@ -17,7 +17,7 @@ what they see for others.  There the sum of dS', which is one of e, goes into a 
 (and in fp16 the step below 2^-14, scaled as for dS) times the sum of e over the keys' number, on every key.  Sums, the mean and the product with it are fp32: at most 2^-20 of sum |dS| (|k| + |m|) besides.
 
 So much for any kernel with that m, and these bounds stand.  The kernel's own m is nearer to what a row attends to (an estimate of sum P k), for which its first
-term, P times what d is off by, nearly vanishes: it keeps to about a third of them, and ``test_keys_of_two_kinds`` says what it keeps to that a first tile's mean does not."""
+term, P times what d is off by, nearly vanishes: it keeps to half of them, and ``test_keys_of_two_kinds`` says what it keeps to that a first tile's mean does not."""
 
 import ctypes as C
 import math
