@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define KSANA_SAGE_ABI_VERSION 25
+#define KSANA_SAGE_ABI_VERSION 26
 
 /* element types of q/k/v/o */
 #define KSANA_SAGE_BF16 0
@@ -512,6 +512,65 @@ int ksana_sage_train_norm_scratch(const ksana_sage_train_norm* call, uint64_t* b
  * vector's type, [B, C] or [C] as the vector; NULL: not wanted. */
 int ksana_sage_train_norm_bwd(const ksana_sage_train_norm* call, const void* x, const void* y, const float* stats, const void* dh,
                               const void* dn, void* dx, void* dy, void* const grads[6], void* scratch, void* stream);
+
+/* ---- Rotary positions and a paged cache of keys and values: what a block needs that generates chunk by chunk.  No counterpart
+ * in the reference, which has no cache and applies its rotation ahead of a whole sequence. ---- */
+
+/* Rows [B, L, H, D] whose first `width` channels turn in pairs (a, b), channels 2 i and 2 i + 1 or i and i + width / 2, by the angle
+ * t = position * frequency i: a' = m (a cos t - b sin t), b' = m (a sin t + b cos t), m the magnitude.  The others are copied.  Angles are
+ * formed in 64 bits, the rest in fp32, and every result is rounded once. */
+typedef struct ksana_sage_rotary {
+  int32_t B, L, D, Hq, Hkv;  /* Hq or Hkv 0: no q (no k)                                                              */
+  int32_t dtype;             /* KSANA_SAGE_BF16, _FP16 or (not for a cache) _FP32                                     */
+  int32_t width;             /* even, at most D; 0: nothing turns                                                     */
+  int32_t interleaved;       /* pairs are neighbours; 0: half of the width apart                                      */
+  int32_t inverse;           /* t negated: the gradient's way back                                                    */
+  int32_t axes;              /* positions of a token, 1 to 4                                                          */
+  int32_t ends[4];           /* ascending: pairs before ends[a], and not before ends[a - 1], go by axis a; the last is width / 2 */
+  int32_t positions_64;      /* positions are int64, else int32                                                       */
+  float magnitude;
+  int64_t q_strides[4], k_strides[4], v_strides[4]; /* in elements, channels contiguous                               */
+  int64_t position_strides[3];  /* of B, L and the axes                                                               */
+  const void* positions;     /* device, or NULL: a token's own place (in a cache: in its sequence), on every axis     */
+  const double* frequencies; /* device, [width / 2], radians per position                                             */
+} ksana_sage_rotary;
+/* q_out, k_out: contiguous [B, L, H, D]. */
+int ksana_sage_rotary_rows(const ksana_sage_rotary* call, const void* q, const void* k, void* q_out, void* k_out, void* stream);
+
+/* Where a batch's sequences lie.  Token t of entry b is in page table[b table_stride + t / page_size], slot t % page_size.  Of its
+ * k_lens[b] tokens the last q_lens[b] are the call's.  Counts are clamped to what the table and the call's rows hold.  Entries that name no
+ * page (negative, or not below `pages`) are allowed everywhere: nothing is stored there, and keys there are not seen. */
+#define KSANA_SAGE_E4M3 3
+typedef struct ksana_sage_cache {
+  void *k, *v;                    /* device, [pages, Hkv, page_size, D]                                               */
+  const float *k_scale, *v_scale; /* device, [Hkv], positive: what code 1 stands for (e4m3; NULL: 1)                  */
+  int64_t strides[3];             /* of page, head and slot, in elements, multiples of 16 bytes; channels contiguous  */
+  int32_t pages, page_size;
+  int32_t dtype;                  /* the rows' type, or KSANA_SAGE_E4M3                                               */
+  int32_t table_width;            /* entries of a sequence                                                            */
+  const int32_t* table;           /* device, [B, table_width]                                                         */
+  int64_t table_stride;
+  const int32_t *q_lens, *k_lens; /* device, [B]; q_lens NULL: all rows                                               */
+} ksana_sage_cache;
+/* Stores the call's keys, turned, and values; q, if there is one, is turned on the way into q_out (contiguous; zeros behind the
+ * counts).  e4m3: to the nearest code, what lies beyond the largest at that.  D = 128 or 64.  Pages that are written to belong to one
+ * sequence.  Repeated calls give the same bits. */
+int ksana_sage_cache_append(const ksana_sage_rotary* call, const ksana_sage_cache* cache, const void* q, const void* k, const void* v,
+                            void* q_out, void* stream);
+
+/* o = softmax(sm_scale q k^T) v of the last q_lens[b] tokens of every sequence on all its k_lens[b] keys; causal: on those up to
+ * their own position.  16-bit products accumulated in fp32, softmax statistics in fp32, probabilities rounded to q's type.  Rows behind the
+ * counts, and rows that see no key, are zeros.  D = 128 or 64, Hq a multiple of Hkv.  Repeated calls give the same bits. */
+typedef struct ksana_sage_cache_attn {
+  int32_t B, Hq, Hkv, Lq, D;
+  int32_t dtype, causal;
+  float sm_scale;                 /* at most 2e38 in size                                                             */
+  int64_t q_strides[4], o_strides[4];
+} ksana_sage_cache_attn;
+/* Bytes of the call's device scratch (256-byte aligned, not kept between calls) */
+int ksana_sage_cache_attn_scratch(const ksana_sage_cache_attn* call, const ksana_sage_cache* cache, uint64_t* bytes);
+int ksana_sage_cache_attn_fwd(const ksana_sage_cache_attn* call, const ksana_sage_cache* cache, const void* q, void* o, void* scratch,
+                              void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,9 +11,9 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libksana_sage_hip.so"
-ABI_VERSION = 25
+ABI_VERSION = 26
 
-BF16, FP16, FP32 = 0, 1, 2
+BF16, FP16, FP32, E4M3 = 0, 1, 2, 3
 OK, EINVAL, ENOTSUP, EHIP = 0, -1, -2, -3
 FLAG_PWL_EXP2 = 1
 FLAG_SMOOTH_V = 2
@@ -66,6 +66,10 @@ EXPORTS = (
     "ksana_sage_train_norm_fwd",
     "ksana_sage_train_norm_scratch",
     "ksana_sage_train_norm_bwd",
+    "ksana_sage_rotary_rows",
+    "ksana_sage_cache_append",
+    "ksana_sage_cache_attn_scratch",
+    "ksana_sage_cache_attn_fwd",
 )
 
 
@@ -130,6 +134,30 @@ class TrainNorm(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "L", "C", "x_dtype", "y_dtype", "norm", "post")] + \
         [("residual_scale", C.c_float), ("eps", C.c_float), ("reserved", C.c_int32), ("x_strides", C.c_int64 * 2), ("y_strides", C.c_int64 * 2)] + \
         [(n, Vector) for n in ("gate", "scale", "shift", "weight", "bias", "post_weight")]
+
+
+class Rotary(C.Structure):
+    """``ksana_sage_rotary``: a rotary step but for its buffers and its stream."""
+
+    _fields_ = [(n, C.c_int32) for n in ("B", "L", "D", "Hq", "Hkv", "dtype", "width", "interleaved", "inverse", "axes")] + \
+        [("ends", C.c_int32 * 4), ("positions_64", C.c_int32), ("magnitude", C.c_float)] + \
+        [(n, C.c_int64 * 4) for n in ("q_strides", "k_strides", "v_strides")] + \
+        [("position_strides", C.c_int64 * 3), ("positions", C.c_void_p), ("frequencies", C.c_void_p)]
+
+
+class Cache(C.Structure):
+    """``ksana_sage_cache``: a paged cache and where a batch's sequences lie in it."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("strides", C.c_int64 * 3)] + \
+        [(n, C.c_int32) for n in ("pages", "page_size", "dtype", "table_width")] + \
+        [("table", C.c_void_p), ("table_stride", C.c_int64), ("q_lens", C.c_void_p), ("k_lens", C.c_void_p)]
+
+
+class CacheAttn(C.Structure):
+    """``ksana_sage_cache_attn``: attention on a paged cache but for the cache, its buffers and its stream."""
+
+    _fields_ = [(n, C.c_int32) for n in ("B", "Hq", "Hkv", "Lq", "D", "dtype", "causal")] + [("sm_scale", C.c_float)] + \
+        [(n, C.c_int64 * 4) for n in ("q_strides", "o_strides")]
 
 
 class SageLibraryError(RuntimeError):
@@ -202,6 +230,10 @@ def _declare(lib):
     lib.ksana_sage_train_norm_scratch.argtypes, lib.ksana_sage_train_norm_scratch.restype = [vp] * 2, i
     lib.ksana_sage_train_norm_bwd.argtypes, lib.ksana_sage_train_norm_bwd.restype = [vp] * 11, i
     lib.ksana_sage_train_attn_bwd.argtypes, lib.ksana_sage_train_attn_bwd.restype = [vp] * 13, i
+    lib.ksana_sage_rotary_rows.argtypes, lib.ksana_sage_rotary_rows.restype = [vp] * 6, i
+    lib.ksana_sage_cache_append.argtypes, lib.ksana_sage_cache_append.restype = [vp] * 7, i
+    lib.ksana_sage_cache_attn_scratch.argtypes, lib.ksana_sage_cache_attn_scratch.restype = [vp] * 3, i
+    lib.ksana_sage_cache_attn_fwd.argtypes, lib.ksana_sage_cache_attn_fwd.restype = [vp] * 6, i
 
 
 def library_present() -> bool:

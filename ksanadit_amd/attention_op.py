@@ -8,6 +8,7 @@ forward is kept out of Dynamo graphs (:72).
 
 Beyond it: ``trainable=True`` asks for a backend with a backward pass.  The Sage backend then runs ``train_ops.attention`` where its inputs
 require gradients, torch's SDPA has one as it is, and a backend without one is a ``ValueError``.
+``op(q, k, v, kv_cache=.., pages=.., k_lens=..)`` attends through a paged cache (``cache_ops``) where the Sage backend runs; elsewhere it is a ``ValueError``.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ from .config import KsanaAttentionBackend, KsanaAttentionConfig
 from .logger import log
 
 _TRAINABLE = (KsanaAttentionBackend.SAGE_ATTN, KsanaAttentionBackend.TORCH_SDPA)
+_CACHED = (KsanaAttentionBackend.SAGE_ATTN,)
 
 
 class KsanaAttentionOp(nn.Module):
@@ -62,4 +64,6 @@ class KsanaAttentionOp(nn.Module):
         if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
             raise ValueError("LocalAttentionOp expects tensors shaped [B, L, H, D].")
         self._ensure_impl(query.dtype)
+        if backend_kwargs.get("kv_cache") is not None and self.backend_type not in _CACHED:
+            raise ValueError(f"attention backend {self.backend_type} has no paged cache (kv_cache)")
         return self._attn_impl.forward(query, key, value, **backend_kwargs)

@@ -21,6 +21,9 @@ Differences, all deliberate:
   the output - the option of the same name of the library behind the reference's call;
 * ``trainable`` (constructor argument, opt-in): calls whose inputs require gradients, with gradients enabled, run the 16-bit attention
   that has a backward pass (``train_ops.attention``) in place of the quantized one, which has none; all other calls are as ever;
+* ``kv_cache`` (keyword of a call, with ``pages``, ``k_lens`` and, if wanted, ``q_lens`` and ``rotary``): the call's keys and values are stored in a paged
+  cache and its queries attend to everything their sequences have there (``cache_ops.append`` and ``cache_ops.attention``, 16-bit products; ``rotary``: a
+  dict of ``append``'s rotary arguments).  The counts are then always honoured;
 * ``pwl_exp2`` (constructor argument, opt-in): a form of exp2 without the transcendental, 1.06-1.12x the speed at
   27 000 keys and more (head size 128; no gain at 4 400 and below) at a cosine similarity lower by ~1.5e-4;
 * availability: no HIP device -> ``supports()`` is False and the selector moves on, like the
@@ -32,7 +35,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import _capi, platform, train_ops
+from .. import _capi, cache_ops, platform, train_ops
 from ..config import KsanaAttentionBackend, KsanaAttentionConfig
 from ..sage_ops import sageattn
 from .base import KsanaAttentionBackendImpl
@@ -82,8 +85,19 @@ class SageAttentionImpl(KsanaAttentionBackendImpl):
         self.attention_config = attention_config
         self.check_config()
 
+    def _forward_cached(self, query, key, value, kv_cache, *, pages, k_lens, q_lens=None, rotary=None, **_) -> torch.Tensor:
+        if rotary is None:
+            cache_ops.append(key, value, kv_cache, pages, k_lens, q_lens)
+        else:
+            query = cache_ops.append(key, value, kv_cache, pages, k_lens, q_lens, q=query, **rotary)
+        return cache_ops.attention(query, kv_cache, pages, k_lens, q_lens, is_causal=self.causal, sm_scale=self.softmax_scale)
+
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, **kwargs) -> torch.Tensor:
         original_dtype = query.dtype
+        if kwargs.get("kv_cache") is not None:
+            if original_dtype not in (torch.float16, torch.bfloat16):
+                query, key, value = (t.to(torch.bfloat16) for t in (query, key, value))
+            return self._forward_cached(query, key, value, **kwargs).to(original_dtype if self.out_dtype is None else self.out_dtype)
         if original_dtype not in (torch.float16, torch.bfloat16):
             query, key, value = (t.to(torch.bfloat16) for t in (query, key, value))
         k_lens = kwargs.get("k_lens") if self.honor_k_lens else None

@@ -1,0 +1,489 @@
+// Attention of the last tokens of a batch's sequences on all of their keys in a paged cache: o = softmax(c q k^T) v.
+//
+// Row i of entry b stands at position k_len - n + i, n being the entry's new tokens; causal rows see the keys up to their own position, others all.  Query rows
+// of the heads that share a key head are numbered together.  Keys of pages that do not exist are not seen: zeros stand in their
+// place, and their weight is zero.
+//
+// A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys with a running maximum and sum; probabilities are rounded to
+// the tensors' type where they are multiplied with the values, everything else is fp32.  A tile's pages are looked up by its 64 keys' lanes three steps ahead.
+// Of 8-bit caches the tiles are widened, exactly, on their way to LDS; the scales go into c and into the result.  Loops of few blocks are cut into runs, which a
+// second launch joins: a block's runs share the tiles that its sequence really has.
+#include "sage_cache.h"
+#include "sage_train_device.h"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <type_traits>
+
+namespace ksana_sage {
+
+namespace {
+
+extern __shared__ __align__(1024) char cache_lds[];
+__device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)cache_lds; }
+
+constexpr int kCacheBlock = 128;  // query rows of a workgroup
+constexpr int kMostRuns = 64, kLeastTiles = 4;
+constexpr float kLog2e = 1.44269504088896340736f;
+// fp16 probabilities relative to a row's largest lose bits from 2^-14 on: scaled up by 2^6 a factor of 2^6 later.  The reference point lags behind the row's maximum by
+// at most 2^kLazy.
+constexpr float kLazy = 8.0f;
+template <int DT>
+constexpr float kShift = DT == KSANA_SAGE_FP16 ? 6.0f : 0.0f;
+
+__device__ const uint4 kZeroRow[16] = {};  // what stands in a missing key's place
+
+struct Extent {
+  int rows, keys, first;  // query rows that take part (over the heads of a key head), keys, position of the first new token
+};
+__device__ __forceinline__ Extent extent_of(const CacheAttnParams& p, int b) {
+  int n = p.Lq, keys = p.pages.width * p.pages.size.by;
+  take_counts(p.pages.q_lens, p.pages.k_lens, b, n, keys);
+  return Extent{keys > 0 ? n * p.group : 0, keys, keys - n};
+}
+__device__ __forceinline__ int position_of(const CacheAttnParams& p, int row) { return quotient(row, p.by_group); }
+__device__ __forceinline__ int keys_seen(const CacheAttnParams& p, const Extent& e, int row) {
+  return p.causal ? min(e.keys, e.first + position_of(p, row) + 1) : e.keys;
+}
+
+// A block's runs: what each of them walks, and how many there are (one at least)
+struct Run {
+  int from, to, runs;
+};
+__device__ __forceinline__ Run run_of(const CacheAttnParams& p, const Extent& e, int row0, int run) {
+  const int keys = row0 < e.rows ? keys_seen(p, e, min(row0 + kCacheBlock, e.rows) - 1) : 0;
+  const int tiles = (max(keys, 0) + kTrainTile - 1) / kTrainTile, each = p.runs == 1 ? tiles : max(kLeastTiles, (tiles + p.runs - 1) / p.runs);
+  return Run{min(run * each, tiles), min((run + 1) * each, tiles), p.runs == 1 ? 1 : max(1, (tiles + each - 1) / each)};
+}
+struct Place {
+  int bh, block, run;
+};
+// Of consecutive workgroups, which land on consecutive XCDs, each has another head: where the heads are a multiple of eight, an XCD keeps its heads' keys to
+// itself.  The last blocks, which see the most, come first.
+__device__ __forceinline__ Place place_of(const CacheAttnParams& p, int at) {
+  const int heads = p.B * p.Hkv, rest = at / heads, block = rest / p.runs;
+  return Place{at - rest * heads, p.blocks - 1 - block, rest - block * p.runs};
+}
+
+// Key t 64 + lane of the sequence: the entry of its page is on its way, then where it lies
+struct Lookup {
+  int entry, slot;
+  __device__ __forceinline__ void start(const PageTable& pages, const int32_t* table, int t, int keys, int lane) {
+    const int key = t * kTrainTile + lane, number = quotient(key, pages.size);
+    slot = key - number * pages.size.by;
+    entry = -1;
+    if (key < keys) entry = table[number];
+  }
+};
+struct Tile64 {
+  unsigned at;     // of the lane's key, 16-byte units from the cache's start; all ones: there is none
+  uint64_t exist;  // the keys that do
+  __device__ __forceinline__ void finish(const CacheAttnParams& p, const Lookup& l) {
+    const bool is = (unsigned)l.entry < (unsigned)p.pages.pages;
+    at = is ? (unsigned)l.entry * (unsigned)p.page_units + (unsigned)l.slot * (unsigned)p.slot_units : ~0u;
+    exist = __ballot(is);
+  }
+};
+
+// Copies of a tile, the wave's share.  A tile in one page is one address and a lane offset, others an address of every lane's own.
+template <int DT, int D, int kWaves, bool kEight>
+struct PagedCopy {
+  using T = Tile<D>;
+  static constexpr int kCopies = T::kCopies / kWaves;
+  static constexpr int kPiece = kEight ? 8 : 16;  // bytes of eight channels
+  const char* base;
+  unsigned whole;
+  bool pages_hold_tiles;
+  __device__ __forceinline__ PagedCopy(const CacheAttnParams& p, const char* cache, int hk, int wave, int lane)
+      : base(cache + hk * p.sH), whole((unsigned)T::row_of(wave, lane) * (unsigned)p.sS + lane % T::kPieces * kPiece),
+        pages_hold_tiles(p.pages.size.by % kTrainTile == 0) {}
+  __device__ __forceinline__ const char* from(unsigned at, int lane) const {
+    return (at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % T::kPieces * kPiece;
+  }
+  // 16 bits: on the way to `tile`
+  __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, unsigned tile, int wave, int lane) const {
+    if (pages_hold_tiles && keys.exist == ~UINT64_C(0)) {
+      const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) lds_copy16_at(first + T::row_of(c * kWaves, 0) * p.sS, whole, tile + T::copy_at(c * kWaves + wave));
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c)
+        lds_copy16_from(from((unsigned)__shfl((int)keys.at, T::row_of(c * kWaves + wave, lane)), lane), tile + T::copy_at(c * kWaves + wave));
+    }
+  }
+  // 8 bits: on the way to registers, and from there
+  __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, uint2 (&raw)[kCopies], int wave, int lane) const {
+    if (pages_hold_tiles && keys.exist == ~UINT64_C(0)) {
+      const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(first + T::row_of(c * kWaves, 0) * p.sS + whole);
+    } else {
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(from((unsigned)__shfl((int)keys.at, T::row_of(c * kWaves + wave, lane)), lane));
+    }
+  }
+  static __device__ __forceinline__ v4i widened(const uint2& raw) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      typedef float v2f __attribute__((ext_vector_type(2)));
+      const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i == 0 ? raw.x : raw.y), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i == 0 ? raw.x : raw.y), true);
+      x[4 * i] = lo[0];
+      x[4 * i + 1] = lo[1];
+      x[4 * i + 2] = hi[0];
+      x[4 * i + 3] = hi[1];
+    }
+    return pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+  }
+  static __device__ __forceinline__ void finish(const uint2 (&raw)[kCopies], unsigned tile, int wave, int lane) {
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c)
+      *(__attribute__((address_space(3))) v4i*)(uintptr_t)(tile + T::copy_at(c * kWaves + wave) + lane * 16) = widened(raw[c]);
+  }
+};
+
+// A lane's query row as B operands: channels 16 s + 8 hh ..
+template <int D>
+__device__ __forceinline__ void load_row(const uint16_t* row, int hh, uint32_t flip, v4i (&out)[Tile<D>::kSteps]) {
+#pragma unroll
+  for (int s = 0; s < Tile<D>::kSteps; ++s) {
+    const uint4 x = *reinterpret_cast<const uint4*>(row + 16 * s + 8 * hh);
+    out[s] = v4i{(int)(x.x ^ flip), (int)(x.y ^ flip), (int)(x.z ^ flip), (int)(x.w ^ flip)};
+  }
+}
+// The lane's row is here from now on: without this the compiler waits for every load under way where its values are used.
+template <int N>
+__device__ __forceinline__ void row_ready(v4i (&row)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(row[s]));
+}
+// Accumulator i of 32-key block h is key 32 h + acc_row(i) + 4 hh
+__device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+template <int DT, int D, bool kEight>
+__global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttnParams p) {
+  using T = Tile<D>;
+  constexpr int kWaves = 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
+  const int all_rows = p.Lq * p.group;
+  const Place place = place_of(p, (int)blockIdx.x);
+  const int b = place.bh / p.Hkv, hk = place.bh - b * p.Hkv, row0 = place.block * kCacheBlock;
+  const Extent e = extent_of(p, b);
+  const Run range = run_of(p, e, row0, place.run);
+  if (place.run >= range.runs) return;
+
+  const unsigned lds = lds_base();
+  const float scale = fmaxf(p.c * (p.k_scale != nullptr ? p.k_scale[hk] : 1.0f), 1.2e-38f);  // (times -infinity, where a score is hidden, still that)
+  v16f acc[T::kBlocks];
+#pragma unroll
+  for (int d = 0; d < T::kBlocks; ++d) acc[d] = v16f{};
+  float top = -INFINITY, minus = kShift<DT>, sum = 0.0f;  // reference point (unscaled), what is added to scaled scores, the row's sum
+  const int row = row0 + wave * 32 + m;
+  if (range.from < range.to) {
+    typedef PagedCopy<DT, D, kWaves, kEight> Copy;
+    const Copy k_copy(p, p.k, hk, wave, lane), v_copy(p, p.v, hk, wave, lane);
+    const int32_t* table = p.pages.table + b * p.pages.sB;
+    auto k_tile = [&](int t) { return lds + (t & 1) * T::kBytes; };
+    auto v_tile = [&](int t) { return lds + (2 + (t & 1)) * T::kBytes; };
+    uint2 k_raw[kEight ? Copy::kCopies : 1], v_raw[kEight ? Copy::kCopies : 1];
+    auto copy_keys = [&](int t, const Tile64& keys) {
+      if constexpr (kEight)
+        k_copy.start(p, keys, k_raw, wave, lane);
+      else
+        k_copy.start(p, keys, k_tile(t), wave, lane);
+    };
+    auto copy_values = [&](int t, const Tile64& keys) {
+      if constexpr (kEight)
+        v_copy.start(p, keys, v_raw, wave, lane);
+      else
+        v_copy.start(p, keys, v_tile(t), wave, lane);
+    };
+    auto keys_there = [&](int t) {
+      if constexpr (kEight) Copy::finish(k_raw, k_tile(t), wave, lane);
+    };
+    auto values_there = [&](int t) {
+      if constexpr (kEight) Copy::finish(v_raw, v_tile(t), wave, lane);
+    };
+    // (behind a run's last tile: that one again)
+    Lookup next_lookup;
+    auto look_up = [&](int t) { next_lookup.start(p.pages, table, min(t, range.to - 1), e.keys, lane); };
+    Tile64 here64, next64;  // of this step's tile and the next one
+    look_up(range.from);
+    here64.finish(p, next_lookup);
+    look_up(range.from + 1);
+    next64.finish(p, next_lookup);
+    copy_keys(range.from, here64);
+    look_up(range.from + 2);
+    v4i q[T::kSteps];
+    {
+      const int r = min(row, e.rows - 1), l = position_of(p, r);
+      load_row<D>(p.q + b * p.q_sB + l * p.q_sL + (int64_t)(hk * p.group + r - l * p.group) * p.q_sH, hh, p.flip, q);
+    }
+    const unsigned row_at = row_lane_at<D>(lane), column_at = column_lane_at<D>(lane);
+    const int limit = keys_seen(p, e, row);  // keys that the row sees, and that all of the wave see
+    const int all_see = keys_seen(p, e, min(row0 + wave * 32, e.rows - 1));
+    const bool idle = row0 + wave * 32 >= e.rows;  // a wave without rows copies its share
+    float most = -INFINITY;
+    auto hide = [&](int t, uint64_t exist, v16f (&s)[2]) {
+      if ((t + 1) * kTrainTile <= all_see && exist == ~UINT64_C(0)) return;
+      const int left = max(limit - t * kTrainTile, 0);
+      const uint64_t seen = (left < kTrainTile ? exist & ((UINT64_C(1) << left) - 1) : exist) >> (4 * hh);
+      uint32_t bits[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
+      pin(bits[0]);  // (a branch that stays one: 64 instructions for every tile otherwise)
+      pin(bits[1]);
+      float x = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[h][i] = bits[h] & (1u << acc_row(i)) ? s[h][i] : -INFINITY;
+        x = largest(x, s[0][i], s[1][i]);
+      }
+      most = x;
+    };
+    // Tile t: its scores in s, the largest of the lane's in `most`; forms the scores of tile t + 1 in `next` unless `last`.
+    auto compute = [&](int t, v16f (&s)[2], v16f (&next)[2], auto last) {
+      const float here = over_halves<Max>(most);
+      if (__any(here * scale > kLazy + kShift<DT> - minus || (top == -INFINITY && here > -INFINITY))) {
+        const float at = fmaxf(top, here);
+        const float factor = top == -INFINITY ? 0.0f : fast_exp2((top - at) * scale);
+        top = at;
+        minus = at == -INFINITY ? kShift<DT> : kShift<DT> - at * scale;
+        sum *= factor;
+#pragma unroll
+        for (int d = 0; d < T::kBlocks; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= factor;
+      }
+      unsigned k_at = k_tile(t + 1) + row_at, v_at = v_tile(t) + column_at;
+      pin(k_at);  // (one address and constants, not sixteen)
+      pin(v_at);
+      v4i pr[4];
+      {
+        constexpr int kParts = 2 * T::kSteps, kEach = 32 / kParts, kAhead = 3;
+        v4i a[kAhead];
+        if constexpr (!last.value) {
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) a[i] = read_row<D>(k_at, i / T::kSteps, i % T::kSteps);
+          next[0] = next[1] = v16f{};
+        }
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          if constexpr (!last.value) {
+            const int h = i / T::kSteps, j = i + kAhead;
+            next[h] = mfma16<DT>(a[i % kAhead], q[i % T::kSteps], next[h]);
+            if (j < kParts) a[i % kAhead] = read_row<D>(k_at, j / T::kSteps, j % T::kSteps);
+          }
+#pragma unroll
+          for (int j = i * kEach; j < (i + 1) * kEach; ++j) x[j] = fast_exp2(__fmaf_rn(s[j / 16][j % 16], scale, minus));
+#pragma unroll
+          for (int j = (i - 1) * kEach; j < i * kEach; ++j)
+            if (j >= 0) sum += x[j];
+          pin(sum);  // (added up here, not later with all of x held for it)
+          if (i * kEach % 8 == 0 && i > 0) {
+            const int f = i * kEach / 8 - 1;
+            pr[f] = pack8<DT>(x[8 * f], x[8 * f + 1], x[8 * f + 2], x[8 * f + 3], x[8 * f + 4], x[8 * f + 5], x[8 * f + 6], x[8 * f + 7]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int j = 32 - kEach; j < 32; ++j) sum += x[j];
+        pr[3] = pack8<DT>(x[24], x[25], x[26], x[27], x[28], x[29], x[30], x[31]);
+      }
+      {
+        constexpr int kParts = 4 * T::kBlocks, kEach = 16 / kParts, kAhead = 3;
+        v4i a[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) a[i] = read_column<D>(v_at, i % T::kBlocks, i / T::kBlocks);
+        float x = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          const int j = i + kAhead;
+          acc[i % T::kBlocks] = mfma16<DT>(a[i % kAhead], pr[i / T::kBlocks], acc[i % T::kBlocks]);
+          if (j < kParts) a[i % kAhead] = read_column<D>(v_at, j % T::kBlocks, j / T::kBlocks);
+          if constexpr (!last.value) {
+#pragma unroll
+            for (int l = i * kEach; l < (i + 1) * kEach; ++l) x = largest(x, next[0][l], next[1][l]);
+            pin(x);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        most = x;
+      }
+    };
+    auto step = [&](int t, v16f (&s)[2], v16f (&next)[2], auto last) {
+      tile_ready<0>();
+      Tile64 after64;
+      if constexpr (!last.value) {
+        after64.finish(p, next_lookup);
+        copy_values(t + 1, next64);
+        copy_keys(t + 2, after64);
+        look_up(t + 3);
+      }
+      if (!idle) {
+        compute(t, s, next, last);
+        if constexpr (!last.value) hide(t + 1, next64.exist, next);
+      }
+      if constexpr (!last.value) {
+        values_there(t + 1);
+        keys_there(t + 2);
+        next64 = after64;
+      }
+    };
+    typedef std::integral_constant<bool, false> More;
+    typedef std::integral_constant<bool, true> Last;
+    v16f s0[2], s1[2];
+    keys_there(range.from);
+    tile_ready<0>();
+    row_ready(q);
+    copy_keys(range.from + 1, next64);
+    copy_values(range.from, here64);
+    if (!idle) {
+      s0[0] = s0[1] = v16f{};
+#pragma unroll
+      for (int i = 0; i < 2 * T::kSteps; ++i)
+        s0[i / T::kSteps] = mfma16<DT>(read_row<D>(k_tile(range.from) + row_at, i / T::kSteps, i % T::kSteps), q[i % T::kSteps], s0[i / T::kSteps]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = largest(most, s0[0][i], s0[1][i]);
+      hide(range.from, here64.exist, s0);
+    }
+    keys_there(range.from + 1);
+    values_there(range.from);
+    int t = range.from;
+#pragma unroll 1
+    for (; t + 2 < range.to; t += 2) {
+      step(t, s0, s1, More{});
+      step(t + 1, s1, s0, More{});
+    }
+    if (t + 1 < range.to) {
+      step(t, s0, s1, More{});
+      step(t + 1, s1, s0, Last{});
+    } else {
+      step(t, s0, s1, Last{});
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy may outlive the workgroup's LDS
+  }
+  const bool takes_part = row < e.rows, exists = row < all_rows;
+  const float total = over_halves<Sum>(sum);
+  if (range.runs > 1) {
+    const int kept = min(all_rows, kCacheBlock);
+    const int64_t at = (((int64_t)place.bh * p.blocks + place.block) * p.runs + place.run) * kept + row - row0;
+    store_column_part<D>(acc, 1.0f, p.part + at * D, hh, takes_part);
+    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.B * p.Hkv * p.blocks * p.runs * kept * D + 2 * at) = make_float2(minus, total);
+    return;
+  }
+  const float factor = !takes_part || total == 0.0f ? 0.0f : (p.v_scale != nullptr ? p.v_scale[hk] : 1.0f) / total;
+  if (!takes_part) {
+#pragma unroll
+    for (int d = 0; d < T::kBlocks; ++d) acc[d] = v16f{};
+  }
+  const int r = min(row, all_rows - 1), l = position_of(p, r);
+  store_column<DT, D>(acc, factor, p.o + b * p.o_sB + l * p.o_sL + (int64_t)(hk * p.group + r - l * p.group) * p.o_sH, hh, exists);
+}
+
+// A block's runs joined: each stands against a reference point of its own.  D / 8 lanes to a row.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void sage_cache_join_kernel(const CacheAttnParams p, const int groups) {
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+  const int lane = threadIdx.x % kLanes, all_rows = p.Lq * p.group, kept = min(all_rows, kCacheBlock);
+  const int at = (int)blockIdx.x / groups, bh = at / p.blocks, block = at - bh * p.blocks, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const int i = ((int)blockIdx.x - at * groups) * kRows + threadIdx.x / kLanes, r = block * kCacheBlock + i;
+  const Extent e = extent_of(p, b);
+  const int runs = run_of(p, e, block * kCacheBlock, 0).runs;
+  if (runs == 1 || i >= kept || r >= all_rows) return;
+  float sum[8] = {}, total = 0.0f;
+  if (r < e.rows) {
+    const int64_t first = (int64_t)at * p.runs * kept + i;
+    const float2* points = reinterpret_cast<const float2*>(p.part + (int64_t)p.B * p.Hkv * p.blocks * p.runs * kept * D);
+    float top = -INFINITY;
+    for (int j = lane; j < runs; j += kLanes) {
+      const float2 x = points[first + (int64_t)j * kept];
+      top = x.y != 0.0f ? fmaxf(top, -x.x) : top;  // (a run whose keys are all hidden has no reference point)
+    }
+#pragma unroll
+    for (int j = kLanes / 2; j > 0; j >>= 1) top = fmaxf(top, __shfl_xor(top, j));
+#pragma unroll 4
+    for (int j = 0; j < runs; ++j) {
+      const float2 x = points[first + (int64_t)j * kept];
+      const float factor = x.y != 0.0f ? fast_exp2(-x.x - top) : 0.0f;
+      const float4* values = reinterpret_cast<const float4*>(p.part + (first + (int64_t)j * kept) * D + 8 * lane);
+      const float4 lo = values[0], hi = values[1];
+      const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      total = __fmaf_rn(x.y, factor, total);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) sum[c] = __fmaf_rn(v[c], factor, sum[c]);
+    }
+  }
+  const int l = position_of(p, r);
+  const float factor = total == 0.0f ? 0.0f : (p.v_scale != nullptr ? p.v_scale[hk] : 1.0f) / total;
+  *reinterpret_cast<v4i*>(p.o + b * p.o_sB + l * p.o_sL + (int64_t)(hk * p.group + r - l * p.group) * p.o_sH + 8 * lane) =
+      pack8<DT>(sum[0] * factor, sum[1] * factor, sum[2] * factor, sum[3] * factor, sum[4] * factor, sum[5] * factor, sum[6] * factor, sum[7] * factor);
+}
+
+// 64 KiB of dynamic LDS and more has to be requested per kernel, once per device.
+struct LdsRequest {
+  std::atomic<bool> done[64];
+  hipError_t make(const void* kernel, int bytes) {
+    if (bytes < 65536) return hipSuccess;
+    int dev = 0;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
+    if (done[dev].load(std::memory_order_acquire)) return hipSuccess;
+    const hipError_t f = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (f == hipSuccess) done[dev].store(true, std::memory_order_release);
+    return f;
+  }
+};
+
+void fill_in(CacheAttnParams& p) {
+  p.group = p.Hq / p.Hkv;
+  p.by_group = divisor(p.group);
+  p.c = fabsf(p.sm_scale) * kLog2e;
+  p.flip = p.sm_scale < 0.0f ? 0x80008000u : 0u;
+  p.page_units = (int)(p.sP / 16);
+  p.slot_units = (int)(p.sS / 16);
+  p.blocks = (p.Lq * p.group + kCacheBlock - 1) / kCacheBlock;
+  const int64_t workgroups = (int64_t)p.B * p.Hkv * p.blocks, tiles = ((int64_t)p.pages.width * p.pages.size.by + kTrainTile - 1) / kTrainTile;
+  // two workgroups to each of 256 compute units at a time, twice over: sequences shorter than the table are cut into as many
+  p.runs = (int)std::max<int64_t>(1, std::min<int64_t>({kMostRuns, (1024 + workgroups - 1) / workgroups, (tiles + kLeastTiles - 1) / kLeastTiles}));
+  if (workgroups >= 512) p.runs = 1;
+}
+
+template <int DT, int D, bool kEight>
+hipError_t rows(const CacheAttnParams& p, hipStream_t s) {
+  constexpr int kLds = 4 * Tile<D>::kBytes;
+  static LdsRequest request;
+  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_cache_rows_kernel<DT, D, kEight>), kLds);
+  if (e != hipSuccess) return e;
+  sage_cache_rows_kernel<DT, D, kEight><<<(unsigned)((int64_t)p.B * p.Hkv * p.blocks * p.runs), 256, kLds, s>>>(p);
+  if (p.runs > 1) {
+    const int groups = (std::min(p.Lq * p.group, kCacheBlock) * (D / 8) + 255) / 256;
+    sage_cache_join_kernel<DT, D><<<(unsigned)((int64_t)p.B * p.Hkv * p.blocks * groups), 256, 0, s>>>(p, groups);
+  }
+  return hipGetLastError();
+}
+template <int DT, int D>
+hipError_t of_cache(const CacheAttnParams& p, hipStream_t s) {
+  return p.eight_bits ? rows<DT, D, true>(p, s) : rows<DT, D, false>(p, s);
+}
+
+}  // namespace
+
+uint64_t cache_attn_scratch(CacheAttnParams p) {
+  fill_in(p);
+  if (p.runs == 1) return 0;
+  return (uint64_t)p.B * p.Hkv * p.blocks * p.runs * std::min(p.Lq * p.group, kCacheBlock) * (p.D + 2) * 4;
+}
+
+hipError_t launch_cache_attn(CacheAttnParams p, void* scratch, hipStream_t s) {
+  fill_in(p);
+  p.part = static_cast<float*>(scratch);
+  const bool bf16 = p.dtype == KSANA_SAGE_BF16;
+  if (p.D == 128) return bf16 ? of_cache<KSANA_SAGE_BF16, 128>(p, s) : of_cache<KSANA_SAGE_FP16, 128>(p, s);
+  return bf16 ? of_cache<KSANA_SAGE_BF16, 64>(p, s) : of_cache<KSANA_SAGE_FP16, 64>(p, s);
+}
+
+}  // namespace ksana_sage

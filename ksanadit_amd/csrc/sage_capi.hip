@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "../../include/ksana_sage_hip.h"
+#include "sage_cache.h"
 #include "sage_kernels.h"
 #include "sage_train.h"
 
@@ -1272,4 +1273,205 @@ extern "C" int ksana_sage_train_norm_bwd(const ksana_sage_train_norm* call, cons
   const StageRange range("ksana_sage.train_norm_bwd");
   const hipError_t e = ksana_sage::launch_train_norm_bwd(p, scratch, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? 0 : hip_fail(e, "residual norm, backward");
+}
+
+// ------------------------------------------------------------------------------------ rotary positions and the paged cache
+
+namespace {
+int rotary_params(const ksana_sage_rotary* c, ksana_sage::RotaryParams* p) {
+  if (!c) return fail(KSANA_SAGE_EINVAL, "call is null");
+  if (c->B < 1 || c->L < 1 || c->D < 1 || c->Hq < 0 || c->Hkv < 0 || c->Hq + (int64_t)c->Hkv < 1)
+    return fail(KSANA_SAGE_EINVAL, "call has a non-positive extent (B=%d L=%d D=%d Hq=%d Hkv=%d)", c->B, c->L, c->D, c->Hq, c->Hkv);
+  if (c->D > 512) return fail(KSANA_SAGE_ENOTSUP, "D=%d exceeds 512", c->D);
+  if (c->Hq > 65535 || c->Hkv > 65535) return fail(KSANA_SAGE_ENOTSUP, "Hq=%d Hkv=%d: at most 65535", c->Hq, c->Hkv);
+  if ((int64_t)c->B * c->L > (1 << 24)) return fail(KSANA_SAGE_ENOTSUP, "B*L = %lld exceeds %d", (long long)c->B * c->L, 1 << 24);
+  if (c->dtype != KSANA_SAGE_BF16 && c->dtype != KSANA_SAGE_FP16 && c->dtype != KSANA_SAGE_FP32) return fail(KSANA_SAGE_EINVAL, "dtype %d unknown", c->dtype);
+  if (c->width < 0 || c->width > c->D || c->width % 2 != 0) return fail(KSANA_SAGE_EINVAL, "width %d is not even and within D=%d", c->width, c->D);
+  if (c->axes < 1 || c->axes > ksana_sage::kMostAxes) return fail(KSANA_SAGE_EINVAL, "axes %d is not 1 to %d", c->axes, ksana_sage::kMostAxes);
+  *p = ksana_sage::RotaryParams{};
+  for (int a = 0; a < c->axes; ++a) {
+    if (c->ends[a] < (a == 0 ? 0 : c->ends[a - 1])) return fail(KSANA_SAGE_EINVAL, "ends are not ascending");
+    p->ends[a] = c->ends[a];
+  }
+  if (c->ends[c->axes - 1] != c->width / 2) return fail(KSANA_SAGE_EINVAL, "ends[%d] is %d, not width / 2 = %d", c->axes - 1, c->ends[c->axes - 1], c->width / 2);
+  if (c->width > 0 && !c->frequencies) return fail(KSANA_SAGE_EINVAL, "frequencies is null");
+  if (reinterpret_cast<uintptr_t>(c->frequencies) & 7) return fail(KSANA_SAGE_EINVAL, "frequencies is not 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(c->positions) & (c->positions_64 ? 7 : 3)) return fail(KSANA_SAGE_EINVAL, "positions is not aligned to its values");
+  for (int i = 0; i < 3; ++i)
+    if (c->position_strides[i] < 0) return fail(KSANA_SAGE_EINVAL, "positions: negative stride");
+  if (!(c->magnitude >= -3e38f && c->magnitude <= 3e38f)) return fail(KSANA_SAGE_EINVAL, "magnitude is not a number");
+  p->B = c->B;
+  p->L = c->L;
+  p->D = c->D;
+  p->R = c->width;
+  p->dtype = c->dtype;
+  p->interleaved = c->interleaved ? 1 : 0;
+  p->inverse = c->inverse ? 1 : 0;
+  p->frequencies = c->frequencies;
+  p->positions = c->positions;
+  p->pos_sB = c->position_strides[0];
+  p->pos_sL = c->position_strides[1];
+  p->pos_sA = c->position_strides[2];
+  p->pos64 = c->positions_64 ? 1 : 0;
+  p->axes = c->axes;
+  p->magnitude = c->magnitude;
+  return 0;
+}
+int rotary_part(const char* name, const ksana_sage::RotaryParams& p, const void* src, const int64_t st[4], int H, int turn, ksana_sage::RotaryPart* out) {
+  if (!src) return fail(KSANA_SAGE_EINVAL, "%s is null", name);
+  if (reinterpret_cast<uintptr_t>(src) % size_of(p.dtype)) return fail(KSANA_SAGE_EINVAL, "%s: pointer not aligned to its values", name);
+  if (p.D > 1 && st[3] != 1) return fail(KSANA_SAGE_EINVAL, "%s: D stride is %lld, must be 1", name, (long long)st[3]);
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0) return fail(KSANA_SAGE_EINVAL, "%s: negative stride", name);
+  out->src = src;
+  out->sB = st[0];
+  out->sL = st[1];
+  out->sH = st[2];
+  out->H = H;
+  out->turn = turn;
+  return 0;
+}
+// .. and where its rows go, contiguous
+int rotary_rows_out(const char* name, const ksana_sage::RotaryParams& p, void* dst, ksana_sage::RotaryPart* part) {
+  if (!dst) return fail(KSANA_SAGE_EINVAL, "%s is null", name);
+  if (reinterpret_cast<uintptr_t>(dst) & 15) return fail(KSANA_SAGE_EINVAL, "%s is not 16-byte aligned", name);
+  part->dst = dst;
+  part->dH = p.D;
+  part->dL = (int64_t)part->H * p.D;
+  part->dB = (int64_t)p.L * part->dL;
+  return 0;
+}
+
+// The cache of a call of B entries with Hkv heads of D channels of `dtype`
+int cache_pages(const ksana_sage_cache* c, int dtype, int Hkv, int D, int B, ksana_sage::PageTable* t) {
+  if (!c) return fail(KSANA_SAGE_EINVAL, "cache is null");
+  if (c->pages < 1 || c->page_size < 1 || c->table_width < 1)
+    return fail(KSANA_SAGE_EINVAL, "cache has a non-positive extent (pages=%d page_size=%d table_width=%d)", c->pages, c->page_size, c->table_width);
+  if (D != 128 && D != 64) return fail(KSANA_SAGE_ENOTSUP, "head size %d not supported (128 or 64)", D);
+  if (c->dtype != dtype && c->dtype != KSANA_SAGE_E4M3) return fail(KSANA_SAGE_EINVAL, "cache of dtype %d does not go with rows of %d", c->dtype, dtype);
+  if (!c->k || !c->v || !c->table || !c->k_lens) return fail(KSANA_SAGE_EINVAL, "k, v, table or k_lens is null");
+  const bool eight = c->dtype == KSANA_SAGE_E4M3;
+  if (!eight && (c->k_scale || c->v_scale)) return fail(KSANA_SAGE_EINVAL, "scales go with an e4m3 cache");
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) return fail(KSANA_SAGE_EINVAL, "k or v is not 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale) | reinterpret_cast<uintptr_t>(c->table) |
+       reinterpret_cast<uintptr_t>(c->q_lens) | reinterpret_cast<uintptr_t>(c->k_lens)) & 3)
+    return fail(KSANA_SAGE_EINVAL, "scales, table or counts are not 4-byte aligned");
+  const int size = eight ? 1 : 2, extent[3] = {c->pages, Hkv, c->page_size};
+  const int64_t row = (int64_t)D * size;
+  for (int i = 0; i < 3; ++i)
+    if (extent[i] > 1 && (c->strides[i] * size % 16 != 0 || c->strides[i] * size < row))
+      return fail(KSANA_SAGE_EINVAL, "cache: stride[%d]=%lld must be a multiple of 16 bytes and hold a row", i, (long long)c->strides[i]);
+  // places are kept in 32 bits, in units of 16 bytes
+  const int64_t units = (int64_t)(c->pages - 1) * (c->strides[0] * size / 16) + (int64_t)(c->page_size - 1) * (c->strides[2] * size / 16);
+  if (c->strides[0] > (INT64_C(1) << 34) || units >= (INT64_C(1) << 32) - 1) return fail(KSANA_SAGE_ENOTSUP, "cache: its pages span more than 64 GiB");
+  if (c->page_size > 1 && c->strides[2] * size > (1 << 24)) return fail(KSANA_SAGE_ENOTSUP, "cache: slots are more than 16 MiB apart");
+  if ((int64_t)c->table_width * c->page_size > (1 << 30)) return fail(KSANA_SAGE_ENOTSUP, "a sequence's table holds more than %d tokens", 1 << 30);
+  if (B > 1 && c->table_stride < 0) return fail(KSANA_SAGE_EINVAL, "table: negative stride");
+  *t = ksana_sage::PageTable{c->table, B > 1 ? c->table_stride : 0, c->table_width, c->pages, ksana_sage::divisor(c->page_size), c->q_lens, c->k_lens};
+  return 0;
+}
+
+int cache_attn_params(const ksana_sage_cache_attn* c, const ksana_sage_cache* cache, ksana_sage::CacheAttnParams* p) {
+  if (!c) return fail(KSANA_SAGE_EINVAL, "call is null");
+  if (c->B < 1 || c->Hq < 1 || c->Hkv < 1 || c->Lq < 1) return fail(KSANA_SAGE_EINVAL, "call has a non-positive extent (B=%d Hq=%d Hkv=%d Lq=%d)", c->B, c->Hq, c->Hkv, c->Lq);
+  if (c->Hq % c->Hkv != 0) return fail(KSANA_SAGE_EINVAL, "Hq=%d is not a multiple of Hkv=%d", c->Hq, c->Hkv);
+  if (c->dtype != KSANA_SAGE_BF16 && c->dtype != KSANA_SAGE_FP16) return fail(KSANA_SAGE_EINVAL, "dtype %d unknown", c->dtype);
+  if (!(c->sm_scale >= -2e38f && c->sm_scale <= 2e38f)) return fail(KSANA_SAGE_EINVAL, "sm_scale is not a number of at most 2e38 in size");
+  *p = ksana_sage::CacheAttnParams{};
+  if (int rc = cache_pages(cache, c->dtype, c->Hkv, c->D, c->B, &p->pages)) return rc;
+  const int64_t rows = (int64_t)c->Lq * (c->Hq / c->Hkv);
+  if (c->Lq > (1 << 24) || rows > (1 << 28)) return fail(KSANA_SAGE_ENOTSUP, "Lq=%d with %d query heads to a key head: too many rows", c->Lq, c->Hq / c->Hkv);
+  if ((int64_t)c->B * c->Hkv > 65535 * 4 || (int64_t)c->B * c->Hkv * ((rows + 127) / 128) > (1 << 23))
+    return fail(KSANA_SAGE_ENOTSUP, "the call's workgroups exceed the launch grid");
+  const int size = cache->dtype == KSANA_SAGE_E4M3 ? 1 : 2;
+  p->k = static_cast<const char*>(cache->k);
+  p->v = static_cast<const char*>(cache->v);
+  p->sP = cache->pages > 1 ? cache->strides[0] * size : 0;
+  p->sH = cache->strides[1] * size;
+  p->sS = cache->page_size > 1 ? cache->strides[2] * size : 0;
+  p->k_scale = cache->k_scale;
+  p->v_scale = cache->v_scale;
+  p->eight_bits = size == 1;
+  p->B = c->B;
+  p->Lq = c->Lq;
+  p->Hq = c->Hq;
+  p->Hkv = c->Hkv;
+  p->D = c->D;
+  p->dtype = c->dtype;
+  p->causal = c->causal ? 1 : 0;
+  p->sm_scale = c->sm_scale;
+  return 0;
+}
+}  // namespace
+
+extern "C" int ksana_sage_rotary_rows(const ksana_sage_rotary* call, const void* q, const void* k, void* q_out, void* k_out, void* stream) {
+  ksana_sage::RotaryParams p;
+  if (int rc = rotary_params(call, &p)) return rc;
+  if (call->Hq > 0) {
+    if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, 1, &p.part[0])) return rc;
+    if (int rc = rotary_rows_out("q_out", p, q_out, &p.part[0])) return rc;
+  }
+  if (call->Hkv > 0) {
+    if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, 1, &p.part[1])) return rc;
+    if (int rc = rotary_rows_out("k_out", p, k_out, &p.part[1])) return rc;
+  }
+  const StageRange range("ksana_sage.rotary_rows");
+  const hipError_t e = ksana_sage::launch_rotary(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "rotary positions");
+}
+
+extern "C" int ksana_sage_cache_append(const ksana_sage_rotary* call, const ksana_sage_cache* cache, const void* q, const void* k, const void* v,
+                                       void* q_out, void* stream) {
+  ksana_sage::RotaryParams p;
+  if (int rc = rotary_params(call, &p)) return rc;
+  if (call->Hkv < 1) return fail(KSANA_SAGE_EINVAL, "Hkv is 0");
+  if (call->dtype == KSANA_SAGE_FP32) return fail(KSANA_SAGE_EINVAL, "dtype %d does not go into a cache", call->dtype);
+  if (int rc = cache_pages(cache, call->dtype, call->Hkv, call->D, call->B, &p.pages)) return rc;
+  p.eight_bits = cache->dtype == KSANA_SAGE_E4M3;
+  if (call->Hq > 0) {
+    if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, 1, &p.part[0])) return rc;
+    if (int rc = rotary_rows_out("q_out", p, q_out, &p.part[0])) return rc;
+  }
+  if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, 1, &p.part[1])) return rc;
+  if (int rc = rotary_part("v", p, v, call->v_strides, call->Hkv, 0, &p.part[2])) return rc;
+  for (int i = 1; i < 3; ++i) {
+    ksana_sage::RotaryPart& part = p.part[i];
+    part.paged = 1;
+    part.dst = i == 1 ? cache->k : cache->v;
+    part.scale = i == 1 ? cache->k_scale : cache->v_scale;
+    part.dB = cache->strides[0];
+    part.dH = cache->strides[1];
+    part.dL = cache->strides[2];
+  }
+  const StageRange range("ksana_sage.cache_append");
+  const hipError_t e = ksana_sage::launch_rotary(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "paged cache, append");
+}
+
+extern "C" int ksana_sage_cache_attn_scratch(const ksana_sage_cache_attn* call, const ksana_sage_cache* cache, uint64_t* bytes) {
+  ksana_sage::CacheAttnParams p;
+  if (int rc = cache_attn_params(call, cache, &p)) return rc;
+  if (!bytes) return fail(KSANA_SAGE_EINVAL, "bytes is null");
+  *bytes = ksana_sage::cache_attn_scratch(p);
+  return 0;
+}
+
+extern "C" int ksana_sage_cache_attn_fwd(const ksana_sage_cache_attn* call, const ksana_sage_cache* cache, const void* q, void* o, void* scratch,
+                                         void* stream) {
+  ksana_sage::CacheAttnParams p;
+  if (int rc = cache_attn_params(call, cache, &p)) return rc;
+  if (int rc = check_tensor("q", q, p.dtype, call->q_strides, p.B, p.Lq, p.Hq)) return rc;
+  if (int rc = check_tensor("o", o, p.dtype, call->o_strides, p.B, p.Lq, p.Hq)) return rc;
+  if (int rc = train_scratch_given(ksana_sage::cache_attn_scratch(p), scratch)) return rc;
+  p.q = static_cast<const uint16_t*>(q);
+  p.o = static_cast<uint16_t*>(o);
+  p.q_sB = call->q_strides[0];
+  p.q_sL = call->q_strides[1];
+  p.q_sH = call->q_strides[2];
+  p.o_sB = call->o_strides[0];
+  p.o_sL = call->o_strides[1];
+  p.o_sH = call->o_strides[2];
+  const StageRange range("ksana_sage.cache_attn_fwd");
+  const hipError_t e = ksana_sage::launch_cache_attn(p, scratch, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? 0 : hip_fail(e, "attention on a paged cache");
 }

@@ -3,10 +3,11 @@
 ``attention`` takes the place of ``sageattn`` where gradients are wanted: the same layouts, key and query counts and causal
 masking, 16-bit products without quantization, and a backward pass that recomputes the probabilities.
 ``residual_norm`` is what stands between two parts of a block: gate, residual sum, norm and modulation in one pass.
+``rotary`` gives q and k their rotary positions ahead of the attention.
 
-Both run on the tensors' HIP device, on torch's current stream there; scratch comes from torch's caching allocator.  They do not synchronise and may be
+They run on the tensors' HIP device, on torch's current stream there; scratch comes from torch's caching allocator.  They do not synchronise and may be
 captured into a graph, with counts, if any, as int32 tensors on that device (others are copied there in the call, which waits for the copy and cannot be captured).
-Repeated calls give the same bits.  Gradients of gradients, forward-mode derivatives and tracing are refused; ``torch.compile`` leaves its graph for them.
+Repeated calls give the same bits.  Gradients of gradients (``rotary``, which is linear, has them), forward-mode derivatives and tracing are refused; ``torch.compile`` leaves its graph for them.
 """
 
 from __future__ import annotations
@@ -375,3 +376,173 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, gate=None, 
     call = _norm_call(x_rows, y_rows, vectors, norm, post_norm, residual_scale, eps, n_dtype)
     h, n, _ = _residual_norm_forward(x_rows, y_rows, call, n_dtype, False)
     return (x if y is None else h), n
+
+
+# ------------------------------------------------------------------------------------------------ rotary positions
+
+_ROTARY = struct.Struct("=15if15q2Q")  # ksana_sage_rotary
+_MOST_AXES = 4
+
+
+def rotary_frequencies(width: int, base: float = 10000.0, *, sections=None, scaling: str | None = None, factor: float = 1.0,
+                       original_length: int | None = None, low: float = 1.0, high: float = 32.0, device="cuda") -> torch.Tensor:
+    """The radians that each of ``width // 2`` pairs turns by from one position to the next, float64 as ``rotary`` takes them:
+    ``base ** (-i / n)`` for pair i of n; with ``sections`` the n pairs of every axis by themselves.
+
+    For sequences ``factor`` times as long as a model was trained on, ``scaling`` is "linear" (all frequencies divided by the factor), "base" (the
+    base raised so that the slowest pair's is divided by it) or "parts" (pairs that make ``high`` turns and more over ``original_length`` positions
+    keep theirs, those that make ``low`` and fewer have it divided, between them it goes over evenly with the number of turns)."""
+    sections = (width // 2,) if sections is None else tuple(sections)
+    if width < 2 or width % 2 or sum(sections) != width // 2 or min(sections) < 0:
+        raise ValueError(f"width {width} is not even, or its pairs are not those of sections {sections}")
+    if scaling not in (None, "linear", "base", "parts") or not factor > 0.0:
+        raise ValueError(f"scaling {scaling!r} with factor {factor} unknown")
+    parts = []
+    for n in sections:
+        i = torch.arange(n, dtype=torch.float64) / max(n, 1)
+        own = base * factor ** (n / (n - 1)) if scaling == "base" and n > 1 else base
+        parts.append(torch.pow(torch.tensor(own, dtype=torch.float64), -i))
+    f = torch.cat(parts)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "parts":
+        if original_length is None or not 0.0 < low < high:
+            raise ValueError("scaling by parts goes with original_length and 0 < low < high")
+        kept = ((f * (original_length / (2.0 * torch.pi)) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * kept + f / factor * (1.0 - kept)
+    return f.to(device)
+
+
+def _channels_last(t: torch.Tensor) -> torch.Tensor:
+    """``[B, L, H, D]`` with contiguous channels and strides that are not negative."""
+    return t if t.is_contiguous() or t.stride(3) == 1 and min(t.stride()[:3]) >= 0 else t.contiguous()
+
+
+def _check_rotary(frequencies, positions, sections, B: int, L: int, D: int, device: int) -> tuple:
+    """(axes, ends of the axes' pairs, whether positions have an axis behind) as the library takes them."""
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or frequencies.get_device() != device or not frequencies.is_contiguous():
+        raise ValueError(f"frequencies must be a contiguous vector of float64 on the tensors' device, got {frequencies.dtype} {tuple(frequencies.shape)} on {frequencies.device}")
+    if frequencies.requires_grad:
+        raise ValueError("frequencies have no gradient here")
+    pairs = frequencies.shape[0]
+    if not 1 <= pairs <= D // 2:
+        raise ValueError(f"{pairs} frequencies do not go with heads of {D} channels")
+    axes, ends, end = 1 if sections is None else len(sections), [], 0
+    for n in (pairs,) if sections is None else sections:
+        if n < 0:
+            raise ValueError(f"sections {sections} hold a negative number")
+        end += n
+        ends.append(end)
+    if not 1 <= axes <= _MOST_AXES or end != pairs:
+        raise ValueError(f"sections {sections} must be at most {_MOST_AXES} numbers of pairs, {pairs} in all")
+    if positions is not None:
+        lead = () if sections is None else (axes,)
+        if positions.dtype not in (torch.int32, torch.int64) or positions.get_device() != device or positions.shape not in ((L, *lead), (1, L, *lead), (B, L, *lead)):
+            raise ValueError(f"positions must be int32 or int64 [{L}] or [{B}, {L}]{f' with {axes} axes behind' if lead else ''} on the tensors' device, "
+                             f"got {positions.dtype} {tuple(positions.shape)} on {positions.device}")
+    return axes, ends + [0] * (_MOST_AXES - axes), sections is not None
+
+
+def _position_strides(positions: torch.Tensor | None, with_axes: bool) -> tuple:
+    if positions is None:
+        return 0, 0, 0
+    strides = positions.stride() if with_axes else (*positions.stride(), 0)
+    return (0, *strides) if len(strides) == 2 else (strides[0] if positions.shape[0] > 1 else 0, *strides[1:])
+
+
+_NO_ROWS = (0, 0, 0, 1)
+
+
+def _rotary_call(q, k, v, frequencies, positions, checked, interleaved: bool, magnitude: float, inverse: bool) -> bytes:
+    x = k if q is None else q
+    B, L, _, D = x.shape
+    axes, ends, with_axes = checked
+    return _ROTARY.pack(B, L, D, 0 if q is None else q.shape[2], 0 if k is None else k.shape[2], _NORM_DTYPES[x.dtype],
+                        0 if frequencies is None else 2 * frequencies.shape[0], interleaved, inverse, axes, *ends,
+                        positions is not None and positions.dtype is torch.int64, magnitude, *(_NO_ROWS if q is None else q.stride()),
+                        *(_NO_ROWS if k is None else k.stride()), *(_NO_ROWS if v is None else v.stride()), *_position_strides(positions, with_axes),
+                        0 if positions is None else positions.data_ptr(), 0 if frequencies is None else frequencies.data_ptr())
+
+
+def _turn(q, k, frequencies, positions, checked, interleaved, magnitude, inverse) -> tuple:
+    out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    rows = [None if t is None or t.numel() == 0 else _channels_last(t) for t in (q, k)]
+    given = rows[1] if rows[0] is None else rows[0]
+    if given is None:
+        return out
+    call = _rotary_call(*rows, None, frequencies, positions, checked, interleaved, magnitude, inverse)
+    with _on(given.device):
+        rc = _capi.load().ksana_sage_rotary_rows(call, _ptr(rows[0]), _ptr(rows[1]), _ptr(out[0]), _ptr(out[1]), _stream_ptr(given.device))
+    if rc != _capi.OK:
+        _capi.check(rc, "train_ops.rotary")
+    return out
+
+
+class _Rotary(torch.autograd.Function):
+    """Its gradients are turned back by the function itself, so that they have gradients too."""
+
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, checked, interleaved, magnitude, inverse):
+        ctx.save_for_backward(frequencies, positions)
+        ctx.options = (checked, interleaved, magnitude, inverse)
+        ctx.was = (frequencies.shape, None if positions is None else (positions.dtype, positions.shape))
+        ctx.set_materialize_grads(False)
+        q, k = _turn(q, k, frequencies, positions, *ctx.options)
+        return q if k is None else (q, k)
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        _refuse_unseen("rotary's backward pass", dq, dk)
+        want_q, want_k = ctx.needs_input_grad[:2]
+        given = [t for t, want in ((dq, want_q), (dk, want_k)) if want and t is not None]
+        if not given:
+            return (None,) * 8
+        frequencies, positions = ctx.saved_tensors
+        device = given[0].get_device()
+        frequencies = _kept(frequencies, torch.float64, ctx.was[0], device)
+        if positions is not None:
+            positions = _kept(positions, *ctx.was[1], device)
+        checked, interleaved, magnitude, inverse = ctx.options
+        out = _Rotary.apply(given[0], given[1] if len(given) > 1 else None, frequencies, positions, checked, interleaved, magnitude, not inverse)
+        out = iter(out if len(given) > 1 else (out,))
+        return (next(out) if want_q and dq is not None else None, next(out) if want_k and dk is not None else None, *(None,) * 6)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None = None, *, frequencies: torch.Tensor, positions: torch.Tensor | None = None, sections=None,
+           interleaved: bool = True, magnitude: float = 1.0, tensor_layout: str = "NHD") -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions of ``q`` - and of ``k``, in the same pass - with gradients: ``[B, L, H, D]`` ("NHD") or ``[B, H, L, D]`` ("HND") in and out, bf16, fp16 or
+    fp32, any strides, heads of up to 512 channels.
+
+    Of every head the first ``2 * len(frequencies)`` channels turn, in pairs: channels 2 i and 2 i + 1 (``interleaved``) or i and i + len(frequencies);
+    the others are copied.  Pair i of a token turns by its position times ``frequencies[i]`` radians (float64, see ``rotary_frequencies``), and
+    ``magnitude`` is multiplied on.  ``positions``: int32 or int64, ``[L]`` or ``[B, L]``, negative ones too; 0, 1, .. by default.  With ``sections``,
+    as (22, 21, 21) for a video's frames, rows and columns, the first 22 pairs go by the first of a token's positions, ``[L, 3]`` or ``[B, L, 3]``,
+    and so on.
+
+    Angles are formed in 64 bits, everything else in fp32, and results and gradients are rounded once."""
+    if tensor_layout not in ("NHD", "HND"):
+        raise ValueError(f"tensor_layout {tensor_layout!r} unknown")
+    for t in (q,) if k is None else (q, k):
+        if t.dim() != 4:
+            raise ValueError("rotary expects 4-D tensors")
+        if not t.is_cuda:
+            raise RuntimeError(f"rotary needs tensors on a HIP device; there is no CPU path (got device {t.device})")
+        if t.dtype not in _NORM_DTYPES or t.dtype != q.dtype or t.get_device() != q.get_device():
+            raise ValueError(f"q and k must be float32, float16 or bfloat16 of one type on one device, got {t.dtype} on {t.device}")
+    if tensor_layout == "HND":
+        q, k = q.transpose(1, 2), None if k is None else k.transpose(1, 2)
+    B, L, _, D = q.shape
+    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != D):
+        raise ValueError(f"incompatible shapes q{tuple(q.shape)} k{tuple(k.shape)}")
+    checked, magnitude = _check_rotary(frequencies, positions, sections, B, L, D, q.get_device()), float(magnitude)
+    if not abs(magnitude) <= 3e38:
+        raise ValueError(f"magnitude {magnitude} is not a number of fp32")
+    _refuse_unseen("rotary", q, k)
+    if torch.is_grad_enabled() and _wants_gradient(q, k):
+        out = _Rotary.apply(q, k, frequencies, positions, checked, bool(interleaved), magnitude, False)
+    else:
+        out = _turn(q, k, frequencies, positions, checked, bool(interleaved), magnitude, False)
+        out = out[0] if k is None else out
+    if tensor_layout == "HND":
+        return out.transpose(1, 2) if k is None else (out[0].transpose(1, 2), out[1].transpose(1, 2))
+    return out
