@@ -124,18 +124,21 @@ struct PagedCopy {
       for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(from((unsigned)__shfl((int)keys.at, T::row_of(c * kWaves + wave, lane)), lane));
     }
   }
+  // (exact: e4m3 numbers are numbers of both types)
   static __device__ __forceinline__ v4i widened(const uint2& raw) {
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      typedef float v2f __attribute__((ext_vector_type(2)));
-      const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i == 0 ? raw.x : raw.y), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)(i == 0 ? raw.x : raw.y), true);
-      x[4 * i] = lo[0];
-      x[4 * i + 1] = lo[1];
-      x[4 * i + 2] = hi[0];
-      x[4 * i + 3] = hi[1];
+    v4i out;
+    if constexpr (DT == KSANA_SAGE_BF16) {
+      out[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, 1.0f, false));
+      out[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, 1.0f, true));
+      out[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, 1.0f, false));
+      out[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, 1.0f, true));
+    } else {
+      out[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.x, 1.0f, false));
+      out[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.x, 1.0f, true));
+      out[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.y, 1.0f, false));
+      out[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.y, 1.0f, true));
     }
-    return pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+    return out;
   }
   static __device__ __forceinline__ void finish(const uint2 (&raw)[kCopies], unsigned tile, int wave, int lane) {
 #pragma unroll
@@ -161,6 +164,23 @@ __device__ __forceinline__ void row_ready(v4i (&row)[N]) {
 }
 // Accumulator i of 32-key block h is key 32 h + acc_row(i) + 4 hh
 __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
+
+// Scores of keys that the lane's row does not see: `limit` of the tile's, and those of no page.  The largest of the others.
+__device__ __forceinline__ float hide_scores(v16f (&s)[2], int limit, uint64_t exist, int hh) {
+  const int left = max(limit, 0);
+  const uint64_t seen = (left < kTrainTile ? exist & ((UINT64_C(1) << left) - 1) : exist) >> (4 * hh);
+  uint32_t bits[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
+  pin(bits[0]);  // (a branch that stays one: 64 instructions for every tile otherwise)
+  pin(bits[1]);
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s[h][i] = bits[h] & (1u << acc_row(i)) ? s[h][i] : -INFINITY;
+    most = largest(most, s[0][i], s[1][i]);
+  }
+  return most;
+}
 
 template <int DT, int D, bool kEight>
 __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttnParams p) {
@@ -228,19 +248,7 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
     float most = -INFINITY;
     auto hide = [&](int t, uint64_t exist, v16f (&s)[2]) {
       if ((t + 1) * kTrainTile <= all_see && exist == ~UINT64_C(0)) return;
-      const int left = max(limit - t * kTrainTile, 0);
-      const uint64_t seen = (left < kTrainTile ? exist & ((UINT64_C(1) << left) - 1) : exist) >> (4 * hh);
-      uint32_t bits[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
-      pin(bits[0]);  // (a branch that stays one: 64 instructions for every tile otherwise)
-      pin(bits[1]);
-      float x = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[h][i] = bits[h] & (1u << acc_row(i)) ? s[h][i] : -INFINITY;
-        x = largest(x, s[0][i], s[1][i]);
-      }
-      most = x;
+      most = hide_scores(s, limit - t * kTrainTile, exist, hh);
     };
     // Tile t: its scores in s, the largest of the lane's in `most`; forms the scores of tile t + 1 in `next` unless `last`.
     auto compute = [&](int t, v16f (&s)[2], v16f (&next)[2], auto last) {
@@ -383,42 +391,278 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
   store_column<DT, D>(acc, factor, p.o + b * p.o_sB + l * p.o_sL + (int64_t)(hk * p.group + r - l * p.group) * p.o_sH, hh, exists);
 }
 
-// A block's runs joined: each stands against a reference point of its own.  D / 8 lanes to a row.
+// Up to 32 query rows in all: waves share the rows and take a run's tiles in turn, each through LDS of its own, without a barrier.  A tile's values are on their way
+// while its scores are formed and the next one's keys while its probabilities and their product are.  In the end the waves' sums are added up.
+constexpr int kFewRows = 32, kFewWaves = 2;
+// A wave's keys, values and entries; of 8 bits keys and values take the same place in turn, since they are on their way in registers: four workgroups to a
+// compute unit where two are, XX_FP8
+template <int D, bool kEight>
+constexpr int kFewWaveLds = (kEight ? 1 : 2) * Tile<D>::kBytes + 512;
+template <int D, bool kEight>
+constexpr int kFewLds = kFewWaves * kFewWaveLds<D, kEight>;
+
+template <int kLater>
+__device__ __forceinline__ void copies_there() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLater) : "memory");
+}
+// What was read of LDS is in registers: copies may go there
+__device__ __forceinline__ void reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void lds_copy4_from(const void* lane_at, unsigned lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(lane_at) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
+// A tile of 8-bit rows on its way through registers: 16 channels of row 8 c + .. at a time (of 64 channels: 16 c + ..)
 template <int DT, int D>
-__global__ __launch_bounds__(256) void sage_cache_join_kernel(const CacheAttnParams p, const int groups) {
-  constexpr int kLanes = D / 8, kRows = 256 / kLanes;
-  const int lane = threadIdx.x % kLanes, all_rows = p.Lq * p.group, kept = min(all_rows, kCacheBlock);
-  const int at = (int)blockIdx.x / groups, bh = at / p.blocks, block = at - bh * p.blocks, b = bh / p.Hkv, hk = bh - b * p.Hkv;
-  const int i = ((int)blockIdx.x - at * groups) * kRows + threadIdx.x / kLanes, r = block * kCacheBlock + i;
+struct WideCopy {
+  using T = Tile<D>;
+  static constexpr int kPieces = D / 16, kRows = 64 / kPieces, kCopies = kTrainTile / kRows;
+  uint4 raw[kCopies];
+  __device__ __forceinline__ void start(const CacheAttnParams& p, const char* base, const Tile64& keys, int lane) {
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      const unsigned at = (unsigned)__shfl((int)keys.at, kRows * c + lane / kPieces);
+      raw[c] = *reinterpret_cast<const uint4*>((at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % kPieces * 16);
+    }
+  }
+  __device__ __forceinline__ void finish(unsigned tile, int lane) const {
+    typedef __attribute__((address_space(3))) v4i* Lds;
+    const unsigned lane_at = tile + T::at(lane / kPieces) + lane % kPieces * 32;
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) {
+      *(Lds)(uintptr_t)(lane_at + T::at(kRows * c)) = PagedCopy<DT, D, 1, true>::widened(make_uint2(raw[c].x, raw[c].y));
+      *(Lds)(uintptr_t)(lane_at + T::at(kRows * c) + 16) = PagedCopy<DT, D, 1, true>::widened(make_uint2(raw[c].z, raw[c].w));
+    }
+  }
+};
+
+template <int DT, int D, bool kEight>
+__global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few_kernel(const CacheAttnParams p) {
+  using T = Tile<D>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
+  const int all_rows = p.Lq * p.group;
+  const Place place = place_of(p, (int)blockIdx.x);
+  const int b = place.bh / p.Hkv, hk = place.bh - b * p.Hkv;
+  const Extent e = extent_of(p, b);
+  const Run range = run_of(p, e, 0, place.run);
+  if (place.run >= range.runs) return;
+
+  constexpr int kOwn = kFewWaveLds<D, kEight>;
+  const unsigned lds = lds_base() + wave * kOwn, k_tile = lds, v_tile = lds + (kEight ? 0 : T::kBytes), entries = lds + kOwn - 512;
+  const float scale = fmaxf(p.c * (p.k_scale != nullptr ? p.k_scale[hk] : 1.0f), 1.2e-38f);  // (times -infinity, where a score is hidden, still that)
+  v16f acc[T::kBlocks];
+#pragma unroll
+  for (int d = 0; d < T::kBlocks; ++d) acc[d] = v16f{};
+  float top = -INFINITY, minus = kShift<DT>, sum = 0.0f;
+  const int row = m, tiles = (range.to - range.from - wave + kFewWaves - 1) / kFewWaves;  // of this wave
+  auto tile_of = [&](int i) { return range.from + wave + i * kFewWaves; };
+  if (range.from + wave < range.to) {
+    const int32_t* table = p.pages.table + b * p.pages.sB;
+    // The entries of a tile's pages, through LDS so that nothing waits for them but what is in order before them
+    int slot = 0;
+    auto look_up = [&](int i) {
+      const int key = min(tile_of(min(i, tiles - 1)) * kTrainTile + lane, e.keys - 1), number = quotient(key, p.pages.size);
+      slot = key - number * p.pages.size.by;
+      lds_copy4_from(table + number, entries + (i & 1) * 256);
+    };
+    auto found = [&](int i, Tile64& keys) {
+      const int entry = *(const __attribute__((address_space(3))) int*)(uintptr_t)(entries + (i & 1) * 256 + lane * 4);
+      const bool is = (unsigned)entry < (unsigned)p.pages.pages && tile_of(i) * kTrainTile + lane < e.keys;
+      keys.at = is ? (unsigned)entry * (unsigned)p.page_units + (unsigned)slot * (unsigned)p.slot_units : ~0u;
+      keys.exist = __ballot(is);
+    };
+    typedef PagedCopy<DT, D, 1, false> Copy;
+    typedef WideCopy<DT, D> Wide;
+    constexpr int kCopies = kEight ? Wide::kCopies : Copy::kCopies;
+    const Copy k_copy(p, p.k, hk, 0, lane), v_copy(p, p.v, hk, 0, lane);
+    Wide k_wide, v_wide;
+    auto copy_keys = [&](const Tile64& keys) {
+      if constexpr (kEight)
+        k_wide.start(p, k_copy.base, keys, lane);
+      else
+        k_copy.start(p, keys, k_tile, 0, lane);
+    };
+    auto copy_values = [&](const Tile64& keys) {
+      if constexpr (kEight)
+        v_wide.start(p, v_copy.base, keys, lane);
+      else
+        v_copy.start(p, keys, v_tile, 0, lane);
+    };
+    v4i q[T::kSteps];
+    {
+      const int r = min(row, e.rows - 1), l = position_of(p, r);
+      load_row<D>(p.q + b * p.q_sB + l * p.q_sL + (int64_t)(hk * p.group + r - l * p.group) * p.q_sH, hh, p.flip, q);
+    }
+    Tile64 here64, next64;
+    look_up(0);
+    copies_there<0>();
+    row_ready(q);
+    found(0, here64);
+    look_up(1);
+    copy_keys(here64);
+    copy_values(here64);
+    const unsigned row_at = k_tile + row_lane_at<D>(lane), column_at = v_tile + column_lane_at<D>(lane);
+    const int limit = keys_seen(p, e, row), all_see = keys_seen(p, e, 0);
+    // On their way here: the entries of tile i + 1, tile i's keys, its values
+    auto step = [&](int i, auto last) {
+      copies_there<kCopies>();
+      if constexpr (kEight) k_wide.finish(k_tile, lane);
+      reads_done();
+      v16f s[2] = {v16f{}, v16f{}};
+#pragma unroll
+      for (int j = 0; j < 2 * T::kSteps; ++j)
+        s[j / T::kSteps] = mfma16<DT>(read_row<D>(row_at, j / T::kSteps, j % T::kSteps), q[j % T::kSteps], s[j / T::kSteps]);
+      if constexpr (!last.value) {
+        found(i + 1, next64);
+        reads_done();
+        look_up(i + 2);
+        copy_keys(next64);
+      }
+      float most = -INFINITY;
+      const int first = tile_of(i) * kTrainTile;
+      if (first + kTrainTile <= all_see && here64.exist == ~UINT64_C(0)) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = largest(most, s[0][j], s[1][j]);
+      } else {
+        most = hide_scores(s, limit - first, here64.exist, hh);
+      }
+      const float here = over_halves<Max>(most);
+      if (__any(here * scale > kLazy + kShift<DT> - minus || (top == -INFINITY && here > -INFINITY))) {
+        const float at = fmaxf(top, here);
+        const float factor = top == -INFINITY ? 0.0f : fast_exp2((top - at) * scale);
+        top = at;
+        minus = at == -INFINITY ? kShift<DT> : kShift<DT> - at * scale;
+        sum *= factor;
+#pragma unroll
+        for (int d = 0; d < T::kBlocks; ++d)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[d][j] *= factor;
+      }
+      v4i pr[4];
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = fast_exp2(__fmaf_rn(s[f / 2][8 * (f % 2) + j], scale, minus));
+          sum += x[j];
+        }
+        pr[f] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+      }
+      if constexpr (last.value)
+        copies_there<0>();
+      else
+        copies_there<kCopies + 1>();
+      if constexpr (kEight) v_wide.finish(v_tile, lane);
+      reads_done();
+#pragma unroll
+      for (int j = 0; j < 4 * T::kBlocks; ++j)
+        acc[j % T::kBlocks] = mfma16<DT>(read_column<D>(column_at, j % T::kBlocks, j / T::kBlocks), pr[j / T::kBlocks], acc[j % T::kBlocks]);
+      if constexpr (!last.value) {
+        reads_done();
+        copy_values(next64);
+        here64 = next64;
+      }
+    };
+    int i = 0;
+#pragma unroll 1
+    for (; i + 1 < tiles; ++i) step(i, std::integral_constant<bool, false>{});
+    step(i, std::integral_constant<bool, true>{});
+  }
+  float total = over_halves<Sum>(sum);
+  // The waves' sums against one reference point (a wave whose keys are all hidden has none), added up by the first
+  __syncthreads();
+  typedef __attribute__((address_space(3))) float* LdsFloat;
+  const LdsFloat points = (LdsFloat)(uintptr_t)(lds_base() + kFewWaves * kOwn - 512);
+  const LdsFloat sums = (LdsFloat)(uintptr_t)lds_base();
+  static_assert(kFewWaves == 2 && kOwn - 512 >= 64 * 4 * 16 * T::kBlocks);
+  if (wave != 0) {
+    if (hh == 0) {
+      points[m] = minus;
+      points[32 + m] = total;
+    }
+#pragma unroll
+    for (int d = 0; d < T::kBlocks; ++d)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sums[(16 * d + j) * 64 + lane] = acc[d][j];
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const float other_minus = points[m], other_total = points[32 + m];
+  const float point = fmaxf(total != 0.0f ? -minus : -INFINITY, other_total != 0.0f ? -other_minus : -INFINITY);
+  const float own_factor = total != 0.0f ? fast_exp2(-minus - point) : 0.0f, other_factor = other_total != 0.0f ? fast_exp2(-other_minus - point) : 0.0f;
+#pragma unroll
+  for (int d = 0; d < T::kBlocks; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[d][j] = __fmaf_rn(sums[(16 * d + j) * 64 + lane], other_factor, acc[d][j] * own_factor);
+  total = __fmaf_rn(other_total, other_factor, total * own_factor);
+  const bool takes_part = row < e.rows, exists = row < all_rows;
+  if (range.runs > 1) {
+    const int64_t at = ((int64_t)place.bh * p.runs + place.run) * all_rows + row;
+    store_column_part<D>(acc, 1.0f, p.part + at * D, hh, takes_part);
+    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.B * p.Hkv * p.runs * all_rows * D + 2 * at) = make_float2(-point, total);
+    return;
+  }
+  const float factor = !takes_part || total == 0.0f ? 0.0f : (p.v_scale != nullptr ? p.v_scale[hk] : 1.0f) / total;
+  if (!takes_part) {
+#pragma unroll
+    for (int d = 0; d < T::kBlocks; ++d) acc[d] = v16f{};
+  }
+  const int r = min(row, all_rows - 1), l = position_of(p, r);
+  store_column<DT, D>(acc, factor, p.o + b * p.o_sB + l * p.o_sL + (int64_t)(hk * p.group + r - l * p.group) * p.o_sH, hh, exists);
+}
+
+// A row's runs joined, by a wave: each stands against a reference point of its own, which lane j holds of run j.  D / 8 lanes to a run's channels, the others have
+// other runs, kEach a lane, and ask for all of them before they look at any.  Bound by latency where rows are few: XX_JOIN
+template <int DT, int D, int kEach>
+__global__ __launch_bounds__(256) void sage_cache_join_kernel(const CacheAttnParams p) {
+  constexpr int kLanes = D / 8, kSlots = 64 / kLanes;
+  static_assert(kMostRuns == 64);
+  const int lane = threadIdx.x & 63, part = lane % kLanes, slot = lane / kLanes, all_rows = p.Lq * p.group, kept = min(all_rows, kCacheBlock);
+  const int number = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6)), at = number / kept, i = number - at * kept;
+  const int bh = at / p.blocks, block = at - bh * p.blocks, b = bh / p.Hkv, hk = bh - b * p.Hkv, r = block * kCacheBlock + i;
+  if (bh >= p.B * p.Hkv || r >= all_rows) return;
   const Extent e = extent_of(p, b);
   const int runs = run_of(p, e, block * kCacheBlock, 0).runs;
-  if (runs == 1 || i >= kept || r >= all_rows) return;
+  if (runs == 1) return;
   float sum[8] = {}, total = 0.0f;
   if (r < e.rows) {
     const int64_t first = (int64_t)at * p.runs * kept + i;
-    const float2* points = reinterpret_cast<const float2*>(p.part + (int64_t)p.B * p.Hkv * p.blocks * p.runs * kept * D);
-    float top = -INFINITY;
-    for (int j = lane; j < runs; j += kLanes) {
-      const float2 x = points[first + (int64_t)j * kept];
-      top = x.y != 0.0f ? fmaxf(top, -x.x) : top;  // (a run whose keys are all hidden has no reference point)
+    const float2 x = reinterpret_cast<const float2*>(p.part + (int64_t)p.B * p.Hkv * p.blocks * p.runs * kept * D)[first + (int64_t)min(lane, runs - 1) * kept];
+    float4 lo[kEach], hi[kEach];
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const float4* values = reinterpret_cast<const float4*>(p.part + (first + (int64_t)min(slot + n * kSlots, runs - 1) * kept) * D + 8 * part);
+      lo[n] = values[0];
+      hi[n] = values[1];
+    }
+    const bool some = lane < runs && x.y != 0.0f;  // (a run whose keys are all hidden has no reference point)
+    const float top = over_lanes<Max>(some ? -x.x : -INFINITY);
+    const float own = some ? fast_exp2(-x.x - top) : 0.0f;
+    total = over_lanes<Sum>(some ? x.y * own : 0.0f);
+#pragma unroll
+    for (int n = 0; n < kEach; ++n) {
+      const float factor = __shfl(own, slot + n * kSlots);  // (of lanes without a run: 0)
+      sum[0] = __fmaf_rn(lo[n].x, factor, sum[0]);
+      sum[1] = __fmaf_rn(lo[n].y, factor, sum[1]);
+      sum[2] = __fmaf_rn(lo[n].z, factor, sum[2]);
+      sum[3] = __fmaf_rn(lo[n].w, factor, sum[3]);
+      sum[4] = __fmaf_rn(hi[n].x, factor, sum[4]);
+      sum[5] = __fmaf_rn(hi[n].y, factor, sum[5]);
+      sum[6] = __fmaf_rn(hi[n].z, factor, sum[6]);
+      sum[7] = __fmaf_rn(hi[n].w, factor, sum[7]);
     }
 #pragma unroll
-    for (int j = kLanes / 2; j > 0; j >>= 1) top = fmaxf(top, __shfl_xor(top, j));
-#pragma unroll 4
-    for (int j = 0; j < runs; ++j) {
-      const float2 x = points[first + (int64_t)j * kept];
-      const float factor = x.y != 0.0f ? fast_exp2(-x.x - top) : 0.0f;
-      const float4* values = reinterpret_cast<const float4*>(p.part + (first + (int64_t)j * kept) * D + 8 * lane);
-      const float4 lo = values[0], hi = values[1];
-      const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      total = __fmaf_rn(x.y, factor, total);
+    for (int j = kLanes; j < 64; j <<= 1)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) sum[c] = __fmaf_rn(v[c], factor, sum[c]);
-    }
+      for (int c = 0; c < 8; ++c) sum[c] += __shfl_xor(sum[c], j);
   }
+  if (slot != 0) return;
   const int l = position_of(p, r);
   const float factor = total == 0.0f ? 0.0f : (p.v_scale != nullptr ? p.v_scale[hk] : 1.0f) / total;
-  *reinterpret_cast<v4i*>(p.o + b * p.o_sB + l * p.o_sL + (int64_t)(hk * p.group + r - l * p.group) * p.o_sH + 8 * lane) =
+  *reinterpret_cast<v4i*>(p.o + b * p.o_sB + l * p.o_sL + (int64_t)(hk * p.group + r - l * p.group) * p.o_sH + 8 * part) =
       pack8<DT>(sum[0] * factor, sum[1] * factor, sum[2] * factor, sum[3] * factor, sum[4] * factor, sum[5] * factor, sum[6] * factor, sum[7] * factor);
 }
 
@@ -447,6 +691,11 @@ void fill_in(CacheAttnParams& p) {
   p.slot_units = (int)(p.sS / 16);
   p.blocks = (p.Lq * p.group + kCacheBlock - 1) / kCacheBlock;
   const int64_t workgroups = (int64_t)p.B * p.Hkv * p.blocks, tiles = ((int64_t)p.pages.width * p.pages.size.by + kTrainTile - 1) / kTrainTile;
+  if (p.Lq * p.group <= kFewRows) {
+    // two workgroups to each of 256 compute units at a time, four times over
+    p.runs = (int)std::max<int64_t>(1, std::min<int64_t>({kMostRuns, (2048 + workgroups - 1) / workgroups, (tiles + kLeastTiles - 1) / kLeastTiles}));
+    return;
+  }
   // two workgroups to each of 256 compute units at a time, twice over: sequences shorter than the table are cut into as many
   p.runs = (int)std::max<int64_t>(1, std::min<int64_t>({kMostRuns, (1024 + workgroups - 1) / workgroups, (tiles + kLeastTiles - 1) / kLeastTiles}));
   if (workgroups >= 512) p.runs = 1;
@@ -454,14 +703,26 @@ void fill_in(CacheAttnParams& p) {
 
 template <int DT, int D, bool kEight>
 hipError_t rows(const CacheAttnParams& p, hipStream_t s) {
-  constexpr int kLds = 4 * Tile<D>::kBytes;
-  static LdsRequest request;
-  const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_cache_rows_kernel<DT, D, kEight>), kLds);
-  if (e != hipSuccess) return e;
-  sage_cache_rows_kernel<DT, D, kEight><<<(unsigned)((int64_t)p.B * p.Hkv * p.blocks * p.runs), 256, kLds, s>>>(p);
+  const unsigned workgroups = (unsigned)((int64_t)p.B * p.Hkv * p.blocks * p.runs);
+  if (p.Lq * p.group <= kFewRows) {
+    static LdsRequest request;
+    const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_cache_few_kernel<DT, D, kEight>), kFewLds<D, kEight>);
+    if (e != hipSuccess) return e;
+    sage_cache_few_kernel<DT, D, kEight><<<workgroups, 64 * kFewWaves, kFewLds<D, kEight>, s>>>(p);
+  } else {
+    constexpr int kLds = 4 * Tile<D>::kBytes;
+    static LdsRequest request;
+    const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_cache_rows_kernel<DT, D, kEight>), kLds);
+    if (e != hipSuccess) return e;
+    sage_cache_rows_kernel<DT, D, kEight><<<workgroups, 256, kLds, s>>>(p);
+  }
   if (p.runs > 1) {
-    const int groups = (std::min(p.Lq * p.group, kCacheBlock) * (D / 8) + 255) / 256;
-    sage_cache_join_kernel<DT, D><<<(unsigned)((int64_t)p.B * p.Hkv * p.blocks * groups), 256, 0, s>>>(p, groups);
+    constexpr int kSlots = 512 / D;
+    const unsigned groups = (unsigned)(((int64_t)p.B * p.Hkv * p.blocks * std::min(p.Lq * p.group, kCacheBlock) + 3) / 4);
+    if (p.runs <= 2 * kSlots)
+      sage_cache_join_kernel<DT, D, 2><<<groups, 256, 0, s>>>(p);
+    else
+      sage_cache_join_kernel<DT, D, kMostRuns / kSlots><<<groups, 256, 0, s>>>(p);
   }
   return hipGetLastError();
 }
