@@ -421,6 +421,13 @@ struct WideCopy {
   static constexpr int kPieces = D / 16, kRows = 64 / kPieces, kCopies = kTrainTile / kRows;
   uint4 raw[kCopies];
   __device__ __forceinline__ void start(const CacheAttnParams& p, const char* base, const Tile64& keys, int lane) {
+    if (p.pages.size.by % kTrainTile == 0 && keys.exist == ~UINT64_C(0)) {
+      const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
+      const unsigned own = (unsigned)(lane / kPieces) * (unsigned)p.sS + lane % kPieces * 16;
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint4*>(first + kRows * c * p.sS + own);
+      return;
+    }
 #pragma unroll
     for (int c = 0; c < kCopies; ++c) {
       const unsigned at = (unsigned)__shfl((int)keys.at, kRows * c + lane / kPieces);
@@ -505,21 +512,25 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
     copy_values(here64);
     const unsigned row_at = k_tile + row_lane_at<D>(lane), column_at = v_tile + column_lane_at<D>(lane);
     const int limit = keys_seen(p, e, row), all_see = keys_seen(p, e, 0);
-    // On their way here: the entries of tile i + 1, tile i's keys, its values
+    auto next_keys = [&](int i) {
+      found(i + 1, next64);
+      reads_done();
+      look_up(i + 2);
+      copy_keys(next64);
+    };
+    // On their way here: the entries of tile i + 1, tile i's keys, its values.  (8 bits: the next ones as soon as these are in LDS.)
     auto step = [&](int i, auto last) {
       copies_there<kCopies>();
-      if constexpr (kEight) k_wide.finish(k_tile, lane);
+      if constexpr (kEight) {
+        k_wide.finish(k_tile, lane);
+        if constexpr (!last.value) next_keys(i);
+      }
       reads_done();
       v16f s[2] = {v16f{}, v16f{}};
 #pragma unroll
       for (int j = 0; j < 2 * T::kSteps; ++j)
         s[j / T::kSteps] = mfma16<DT>(read_row<D>(row_at, j / T::kSteps, j % T::kSteps), q[j % T::kSteps], s[j / T::kSteps]);
-      if constexpr (!last.value) {
-        found(i + 1, next64);
-        reads_done();
-        look_up(i + 2);
-        copy_keys(next64);
-      }
+      if constexpr (!kEight && !last.value) next_keys(i);
       float most = -INFINITY;
       const int first = tile_of(i) * kTrainTile;
       if (first + kTrainTile <= all_see && here64.exist == ~UINT64_C(0)) {
@@ -555,14 +566,17 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
         copies_there<0>();
       else
         copies_there<kCopies + 1>();
-      if constexpr (kEight) v_wide.finish(v_tile, lane);
+      if constexpr (kEight) {
+        v_wide.finish(v_tile, lane);
+        if constexpr (!last.value) copy_values(next64);
+      }
       reads_done();
 #pragma unroll
       for (int j = 0; j < 4 * T::kBlocks; ++j)
         acc[j % T::kBlocks] = mfma16<DT>(read_column<D>(column_at, j % T::kBlocks, j / T::kBlocks), pr[j / T::kBlocks], acc[j % T::kBlocks]);
       if constexpr (!last.value) {
         reads_done();
-        copy_values(next64);
+        if constexpr (!kEight) copy_values(next64);
         here64 = next64;
       }
     };
