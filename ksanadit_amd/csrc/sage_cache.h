@@ -74,8 +74,9 @@ struct CacheAttnParams {
   float c;                     // |sm_scale| log2(e)
   uint32_t flip;               // sign bits of two 16-bit values where sm_scale is negative
   int page_units, slot_units;  // sP and sS in 16 bytes
-  int blocks, runs;            // of query rows of a key head, of a block's keys
-  float* part;                 // [workgroups, rows of a block, D], then a pair for every row
+  int blocks;                  // of query rows of a key head
+  int whole, cut, runs;        // blocks that a workgroup walks, and those that up to `runs` do
+  float* part;                 // [cut, runs, rows of a block, D], then a pair for every row
 };
 uint64_t cache_attn_scratch(CacheAttnParams p);
 hipError_t launch_cache_attn(CacheAttnParams p, void* scratch, hipStream_t s);

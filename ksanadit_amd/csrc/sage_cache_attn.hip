@@ -47,23 +47,35 @@ __device__ __forceinline__ int keys_seen(const CacheAttnParams& p, const Extent&
   return p.causal ? min(e.keys, e.first + position_of(p, row) + 1) : e.keys;
 }
 
+// What a workgroup works on: a key head, a block of its rows and a run of the block's tiles
+struct Place {
+  int bh, block, run, cut;  // cut: number of the block among those that are cut; -1: a whole block
+};
+
 // A block's runs: what each of them walks, and how many there are (one at least)
 struct Run {
   int from, to, runs;
 };
-__device__ __forceinline__ Run run_of(const CacheAttnParams& p, const Extent& e, int row0, int run) {
+__device__ __forceinline__ Run run_of(const CacheAttnParams& p, const Extent& e, const Place& place) {
+  const int row0 = place.block * kCacheBlock, run = place.run;
+  const bool one = place.cut < 0 || p.runs == 1;
   const int keys = row0 < e.rows ? keys_seen(p, e, min(row0 + kCacheBlock, e.rows) - 1) : 0;
-  const int tiles = (max(keys, 0) + kTrainTile - 1) / kTrainTile, each = p.runs == 1 ? tiles : max(kLeastTiles, (tiles + p.runs - 1) / p.runs);
-  return Run{min(run * each, tiles), min((run + 1) * each, tiles), p.runs == 1 ? 1 : max(1, (tiles + each - 1) / each)};
+  const int tiles = (max(keys, 0) + kTrainTile - 1) / kTrainTile, each = one ? tiles : max(kLeastTiles, (tiles + p.runs - 1) / p.runs);
+  return Run{min(run * each, tiles), min((run + 1) * each, tiles), one ? 1 : max(1, (tiles + each - 1) / each)};
 }
-struct Place {
-  int bh, block, run;
-};
 // Of consecutive workgroups, which land on consecutive XCDs, each has another head: where the heads are a multiple of eight, an XCD keeps its heads' keys to
 // itself.  The last blocks, which see the most, come first.
+__device__ __forceinline__ Place block_place(const CacheAttnParams& p, int i) {
+  const int heads = p.B * p.Hkv, block = i / heads;
+  return Place{i - block * heads, p.blocks - 1 - block, 0, -1};
+}
 __device__ __forceinline__ Place place_of(const CacheAttnParams& p, int at) {
-  const int heads = p.B * p.Hkv, rest = at / heads, block = rest / p.runs;
-  return Place{at - rest * heads, p.blocks - 1 - block, rest - block * p.runs};
+  if (at < p.whole) return block_place(p, at);
+  const int run = (at - p.whole) / p.cut, cut = at - p.whole - run * p.cut;
+  Place place = block_place(p, p.whole + cut);
+  place.run = run;
+  place.cut = cut;
+  return place;
 }
 
 // Key t 64 + lane of the sequence: the entry of its page is on its way, then where it lies
@@ -79,6 +91,11 @@ struct Lookup {
 struct Tile64 {
   unsigned at;     // of the lane's key, 16-byte units from the cache's start; all ones: there is none
   uint64_t exist;  // the keys that do
+  // All 64 there, a slot apart.  (Of pages of 64 slots and more a tile has two at most: if its ends lie 63 slots apart, so does all between.)
+  __device__ __forceinline__ bool in_a_row(const CacheAttnParams& p) const {
+    return p.pages.size.by >= kTrainTile && exist == ~UINT64_C(0) &&
+           (unsigned)__builtin_amdgcn_readlane((int)at, 63) - (unsigned)__builtin_amdgcn_readfirstlane((int)at) == 63u * (unsigned)p.slot_units;
+  }
   __device__ __forceinline__ void finish(const CacheAttnParams& p, const Lookup& l) {
     const bool is = (unsigned)l.entry < (unsigned)p.pages.pages;
     at = is ? (unsigned)l.entry * (unsigned)p.page_units + (unsigned)l.slot * (unsigned)p.slot_units : ~0u;
@@ -86,7 +103,7 @@ struct Tile64 {
   }
 };
 
-// Copies of a tile, the wave's share.  A tile in one page is one address and a lane offset, others an address of every lane's own.
+// Copies of a tile, the wave's share.  One whose keys lie in a row is one address and a lane offset, others an address of every lane's own.
 template <int DT, int D, int kWaves, bool kEight>
 struct PagedCopy {
   using T = Tile<D>;
@@ -94,16 +111,14 @@ struct PagedCopy {
   static constexpr int kPiece = kEight ? 8 : 16;  // bytes of eight channels
   const char* base;
   unsigned whole;
-  bool pages_hold_tiles;
   __device__ __forceinline__ PagedCopy(const CacheAttnParams& p, const char* cache, int hk, int wave, int lane)
-      : base(cache + hk * p.sH), whole((unsigned)T::row_of(wave, lane) * (unsigned)p.sS + lane % T::kPieces * kPiece),
-        pages_hold_tiles(p.pages.size.by % kTrainTile == 0) {}
+      : base(cache + hk * p.sH), whole((unsigned)T::row_of(wave, lane) * (unsigned)p.sS + lane % T::kPieces * kPiece) {}
   __device__ __forceinline__ const char* from(unsigned at, int lane) const {
     return (at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % T::kPieces * kPiece;
   }
   // 16 bits: on the way to `tile`
   __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, unsigned tile, int wave, int lane) const {
-    if (pages_hold_tiles && keys.exist == ~UINT64_C(0)) {
+    if (keys.in_a_row(p)) {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) lds_copy16_at(first + T::row_of(c * kWaves, 0) * p.sS, whole, tile + T::copy_at(c * kWaves + wave));
@@ -115,7 +130,7 @@ struct PagedCopy {
   }
   // 8 bits: on the way to registers, and from there
   __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, uint2 (&raw)[kCopies], int wave, int lane) const {
-    if (pages_hold_tiles && keys.exist == ~UINT64_C(0)) {
+    if (keys.in_a_row(p)) {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(first + T::row_of(c * kWaves, 0) * p.sS + whole);
@@ -191,7 +206,7 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
   const Place place = place_of(p, (int)blockIdx.x);
   const int b = place.bh / p.Hkv, hk = place.bh - b * p.Hkv, row0 = place.block * kCacheBlock;
   const Extent e = extent_of(p, b);
-  const Run range = run_of(p, e, row0, place.run);
+  const Run range = run_of(p, e, place);
   if (place.run >= range.runs) return;
 
   const unsigned lds = lds_base();
@@ -377,9 +392,9 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
   const float total = over_halves<Sum>(sum);
   if (range.runs > 1) {
     const int kept = min(all_rows, kCacheBlock);
-    const int64_t at = (((int64_t)place.bh * p.blocks + place.block) * p.runs + place.run) * kept + row - row0;
+    const int64_t at = ((int64_t)place.cut * p.runs + place.run) * kept + row - row0;
     store_column_part<D>(acc, 1.0f, p.part + at * D, hh, takes_part);
-    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.B * p.Hkv * p.blocks * p.runs * kept * D + 2 * at) = make_float2(minus, total);
+    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.cut * p.runs * kept * D + 2 * at) = make_float2(minus, total);
     return;
   }
   const float factor = !takes_part || total == 0.0f ? 0.0f : (p.v_scale != nullptr ? p.v_scale[hk] : 1.0f) / total;
@@ -421,7 +436,7 @@ struct WideCopy {
   static constexpr int kPieces = D / 16, kRows = 64 / kPieces, kCopies = kTrainTile / kRows;
   uint4 raw[kCopies];
   __device__ __forceinline__ void start(const CacheAttnParams& p, const char* base, const Tile64& keys, int lane) {
-    if (p.pages.size.by % kTrainTile == 0 && keys.exist == ~UINT64_C(0)) {
+    if (keys.in_a_row(p)) {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
       const unsigned own = (unsigned)(lane / kPieces) * (unsigned)p.sS + lane % kPieces * 16;
 #pragma unroll
@@ -453,7 +468,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
   const Place place = place_of(p, (int)blockIdx.x);
   const int b = place.bh / p.Hkv, hk = place.bh - b * p.Hkv;
   const Extent e = extent_of(p, b);
-  const Run range = run_of(p, e, 0, place.run);
+  const Run range = run_of(p, e, place);
   if (place.run >= range.runs) return;
 
   constexpr int kOwn = kFewWaveLds<D, kEight>;
@@ -614,9 +629,9 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
   total = __fmaf_rn(other_total, other_factor, total * own_factor);
   const bool takes_part = row < e.rows, exists = row < all_rows;
   if (range.runs > 1) {
-    const int64_t at = ((int64_t)place.bh * p.runs + place.run) * all_rows + row;
+    const int64_t at = ((int64_t)place.cut * p.runs + place.run) * all_rows + row;
     store_column_part<D>(acc, 1.0f, p.part + at * D, hh, takes_part);
-    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.B * p.Hkv * p.runs * all_rows * D + 2 * at) = make_float2(-point, total);
+    if (takes_part && hh == 0) *reinterpret_cast<float2*>(p.part + (int64_t)p.cut * p.runs * all_rows * D + 2 * at) = make_float2(-point, total);
     return;
   }
   const float factor = !takes_part || total == 0.0f ? 0.0f : (p.v_scale != nullptr ? p.v_scale[hk] : 1.0f) / total;
@@ -636,15 +651,18 @@ __global__ __launch_bounds__(256) void sage_cache_join_kernel(const CacheAttnPar
   static_assert(kMostRuns == 64);
   const int lane = threadIdx.x & 63, part = lane % kLanes, slot = lane / kLanes, all_rows = p.Lq * p.group, kept = min(all_rows, kCacheBlock);
   const int number = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6)), at = number / kept, i = number - at * kept;
-  const int bh = at / p.blocks, block = at - bh * p.blocks, b = bh / p.Hkv, hk = bh - b * p.Hkv, r = block * kCacheBlock + i;
-  if (bh >= p.B * p.Hkv || r >= all_rows) return;
+  if (at >= p.cut) return;
+  Place place = block_place(p, p.whole + at);
+  place.cut = at;
+  const int b = place.bh / p.Hkv, hk = place.bh - b * p.Hkv, r = place.block * kCacheBlock + i;
+  if (r >= all_rows) return;
   const Extent e = extent_of(p, b);
-  const int runs = run_of(p, e, block * kCacheBlock, 0).runs;
+  const int runs = run_of(p, e, place).runs;
   if (runs == 1) return;
   float sum[8] = {}, total = 0.0f;
   if (r < e.rows) {
     const int64_t first = (int64_t)at * p.runs * kept + i;
-    const float2 x = reinterpret_cast<const float2*>(p.part + (int64_t)p.B * p.Hkv * p.blocks * p.runs * kept * D)[first + (int64_t)min(lane, runs - 1) * kept];
+    const float2 x = reinterpret_cast<const float2*>(p.part + (int64_t)p.cut * p.runs * kept * D)[first + (int64_t)min(lane, runs - 1) * kept];
     float4 lo[kEach], hi[kEach];
 #pragma unroll
     for (int n = 0; n < kEach; ++n) {
@@ -704,20 +722,42 @@ void fill_in(CacheAttnParams& p) {
   p.page_units = (int)(p.sP / 16);
   p.slot_units = (int)(p.sS / 16);
   p.blocks = (p.Lq * p.group + kCacheBlock - 1) / kCacheBlock;
-  const int64_t workgroups = (int64_t)p.B * p.Hkv * p.blocks, tiles = ((int64_t)p.pages.width * p.pages.size.by + kTrainTile - 1) / kTrainTile;
+  const int64_t blocks = (int64_t)p.B * p.Hkv * p.blocks, tiles = ((int64_t)p.pages.width * p.pages.size.by + kTrainTile - 1) / kTrainTile;
+  const int most = (int)std::min<int64_t>(kMostRuns, (tiles + kLeastTiles - 1) / kLeastTiles);
+  p.whole = 0;
+  p.cut = (int)blocks;
   if (p.Lq * p.group <= kFewRows) {
-    // two workgroups to each of 256 compute units at a time, four times over
-    p.runs = (int)std::max<int64_t>(1, std::min<int64_t>({kMostRuns, (2048 + workgroups - 1) / workgroups, (tiles + kLeastTiles - 1) / kLeastTiles}));
+    // two workgroups to each of 256 compute units at a time, four times over: sequences shorter than the table are cut into as many
+    p.runs = (int)std::max<int64_t>(1, std::min<int64_t>(most, (2048 + blocks - 1) / blocks));
     return;
   }
-  // two workgroups to each of 256 compute units at a time, twice over: sequences shorter than the table are cut into as many
-  p.runs = (int)std::max<int64_t>(1, std::min<int64_t>({kMostRuns, (1024 + workgroups - 1) / workgroups, (tiles + kLeastTiles - 1) / kLeastTiles}));
-  if (workgroups >= 512) p.runs = 1;
+  // Blocks that fill whole rounds of 512 places are left whole, the others are cut so that they fill one more.  In units of a tile's time (about
+  // 2 us with all there) a workgroup costs two besides its tiles, a second launch two and what its bytes take, written and read.
+  constexpr int kPlaces = 512;
+  constexpr double kSetup = 2.0, kJoin = 2.0, kBytesPerTile = 4e12 * 2e-6;
+  p.whole = (int)(blocks / kPlaces * kPlaces);
+  p.cut = (int)(blocks - p.whole);
+  p.runs = 1;
+  double least = 1e30;
+  for (int n = 1; n <= most; ++n) {
+    const double each = (double)((tiles + n - 1) / n);
+    const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * p.cut * 4.0 * std::min(p.Lq * p.group, kCacheBlock) * p.D / kBytesPerTile;
+    const double cost = std::ceil((double)n * p.cut / kPlaces) * (each + kSetup) + join;
+    if (cost < 0.97 * least) {
+      least = cost;
+      p.runs = n;
+    }
+  }
+  if (p.cut == 0 || p.runs == 1) {
+    p.whole = (int)blocks;
+    p.cut = 0;
+    p.runs = 1;
+  }
 }
 
 template <int DT, int D, bool kEight>
 hipError_t rows(const CacheAttnParams& p, hipStream_t s) {
-  const unsigned workgroups = (unsigned)((int64_t)p.B * p.Hkv * p.blocks * p.runs);
+  const unsigned workgroups = (unsigned)(p.whole + (int64_t)p.cut * p.runs);
   if (p.Lq * p.group <= kFewRows) {
     static LdsRequest request;
     const hipError_t e = request.make(reinterpret_cast<const void*>(&sage_cache_few_kernel<DT, D, kEight>), kFewLds<D, kEight>);
@@ -732,7 +772,7 @@ hipError_t rows(const CacheAttnParams& p, hipStream_t s) {
   }
   if (p.runs > 1) {
     constexpr int kSlots = 512 / D;
-    const unsigned groups = (unsigned)(((int64_t)p.B * p.Hkv * p.blocks * std::min(p.Lq * p.group, kCacheBlock) + 3) / 4);
+    const unsigned groups = (unsigned)(((int64_t)p.cut * std::min(p.Lq * p.group, kCacheBlock) + 3) / 4);
     if (p.runs <= 2 * kSlots)
       sage_cache_join_kernel<DT, D, 2><<<groups, 256, 0, s>>>(p);
     else
@@ -750,7 +790,7 @@ hipError_t of_cache(const CacheAttnParams& p, hipStream_t s) {
 uint64_t cache_attn_scratch(CacheAttnParams p) {
   fill_in(p);
   if (p.runs == 1) return 0;
-  return (uint64_t)p.B * p.Hkv * p.blocks * p.runs * std::min(p.Lq * p.group, kCacheBlock) * (p.D + 2) * 4;
+  return (uint64_t)p.cut * p.runs * std::min(p.Lq * p.group, kCacheBlock) * (p.D + 2) * 4;
 }
 
 hipError_t launch_cache_attn(CacheAttnParams p, void* scratch, hipStream_t s) {

@@ -121,6 +121,10 @@ ATTENTION = [
     ([3000], [33], 32, 1, 128, 256, True, BF16, BF16, "heads first"),
     ([700], [5], 7, 1, 128, 1560, True, BF16, BF16, "heads first"),
     ([1561, 3], [1560, 3], 1, 1, 128, 1560, False, FP16, FP16, "heads first"),
+    ([2000], [1664], 40, 8, 64, 100, True, BF16, BF16, "heads first"),  # more blocks than fill a round: the last ones cut
+    ([2000], [1664], 40, 8, 128, 100, False, FP16, FP16, "slots first"),
+    ([2300, 900], [4, 4], 8, 1, 128, 65, True, BF16, BF16, "heads first"),  # 32 rows
+    ([2300, 900], [11, 3], 3, 1, 64, 63, True, BF16, FP8, "heads first"),  # 33 rows
 ]
 
 
