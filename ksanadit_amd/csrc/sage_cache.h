@@ -39,7 +39,7 @@ struct RotaryPart {
   const void* src;
   int64_t sB, sL, sH;  // in elements
   void* dst;
-  int64_t dB, dL, dH;  // of pages: page, slot, head
+  int64_t dB, dL, dH;  // of pages: page, slot and head, in elements (other rows are contiguous)
   const float* scale;  // of 8-bit pages: one per head, or nullptr
   int H, turn, paged;
 };
@@ -54,7 +54,8 @@ struct RotaryParams {
   int inverse;
   PageTable pages;            // table nullptr: no cache
   // filled in by the launcher
-  int heads, units, head_slots, token_slots, tokens_each;
+  int heads, units, slots, tokens_each;
+  Divisor by_heads, by_length;
 };
 hipError_t launch_rotary(RotaryParams p, hipStream_t s);
 

@@ -1332,13 +1332,10 @@ int rotary_part(const char* name, const ksana_sage::RotaryParams& p, const void*
   return 0;
 }
 // .. and where its rows go, contiguous
-int rotary_rows_out(const char* name, const ksana_sage::RotaryParams& p, void* dst, ksana_sage::RotaryPart* part) {
+int rotary_rows_out(const char* name, void* dst, ksana_sage::RotaryPart* part) {
   if (!dst) return fail(KSANA_SAGE_EINVAL, "%s is null", name);
   if (reinterpret_cast<uintptr_t>(dst) & 15) return fail(KSANA_SAGE_EINVAL, "%s is not 16-byte aligned", name);
   part->dst = dst;
-  part->dH = p.D;
-  part->dL = (int64_t)part->H * p.D;
-  part->dB = (int64_t)p.L * part->dL;
   return 0;
 }
 
@@ -1409,11 +1406,11 @@ extern "C" int ksana_sage_rotary_rows(const ksana_sage_rotary* call, const void*
   if (int rc = rotary_params(call, &p)) return rc;
   if (call->Hq > 0) {
     if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, 1, &p.part[0])) return rc;
-    if (int rc = rotary_rows_out("q_out", p, q_out, &p.part[0])) return rc;
+    if (int rc = rotary_rows_out("q_out", q_out, &p.part[0])) return rc;
   }
   if (call->Hkv > 0) {
     if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, 1, &p.part[1])) return rc;
-    if (int rc = rotary_rows_out("k_out", p, k_out, &p.part[1])) return rc;
+    if (int rc = rotary_rows_out("k_out", k_out, &p.part[1])) return rc;
   }
   const StageRange range("ksana_sage.rotary_rows");
   const hipError_t e = ksana_sage::launch_rotary(p, static_cast<hipStream_t>(stream));
@@ -1430,7 +1427,7 @@ extern "C" int ksana_sage_cache_append(const ksana_sage_rotary* call, const ksan
   p.eight_bits = cache->dtype == KSANA_SAGE_E4M3;
   if (call->Hq > 0) {
     if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, 1, &p.part[0])) return rc;
-    if (int rc = rotary_rows_out("q_out", p, q_out, &p.part[0])) return rc;
+    if (int rc = rotary_rows_out("q_out", q_out, &p.part[0])) return rc;
   }
   if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, 1, &p.part[1])) return rc;
   if (int rc = rotary_part("v", p, v, call->v_strides, call->Hkv, 0, &p.part[2])) return rc;

@@ -39,24 +39,30 @@ __device__ __forceinline__ void turn_of(double position, double frequency, float
 template <int DT>
 constexpr int kWidth = DT == kFp32 ? 4 : 2;
 
+// E values as they lie in memory (16-byte accesses at any address)
 template <int DT, int E>
-__device__ __forceinline__ void load_values(const void* row, int64_t at, float (&x)[E]) {
-  if constexpr (E == 1) {
-    if constexpr (DT == kFp32) x[0] = static_cast<const float*>(row)[at];
-    if constexpr (DT == KSANA_SAGE_BF16) x[0] = __uint_as_float((uint32_t)static_cast<const uint16_t*>(row)[at] << 16);
-    if constexpr (DT == KSANA_SAGE_FP16) x[0] = (float)static_cast<const _Float16*>(row)[at];
-  } else {  // (16-byte accesses at any address)
-    const char* p = static_cast<const char*>(row) + at * kWidth<DT>;
-    if constexpr (DT == kFp32) {
-      __builtin_memcpy(x, p, 16);
-      __builtin_memcpy(x + 4, p + 16, 16);
+struct Raw {
+  uint4 w[DT == kFp32 ? 2 : 1];
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (E == 1) {
+      w[0].x = DT == kFp32 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
     } else {
-      uint4 raw;
-      __builtin_memcpy(&raw, p, 16);
-      widen8<DT>(raw, x);
+      __builtin_memcpy(&w[0], p, 16);
+      if constexpr (DT == kFp32) __builtin_memcpy(&w[1], p + 16, 16);
     }
   }
-}
+  __device__ __forceinline__ void values(float (&x)[E]) const {
+    if constexpr (E == 1) {
+      if constexpr (DT == kFp32) x[0] = __uint_as_float(w[0].x);
+      if constexpr (DT == KSANA_SAGE_BF16) x[0] = __uint_as_float(w[0].x << 16);
+      if constexpr (DT == KSANA_SAGE_FP16) x[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[0].x);
+    } else if constexpr (DT == kFp32) {
+      __builtin_memcpy(x, w, 32);
+    } else {
+      widen8<DT>(w[0], x);
+    }
+  }
+};
 // e4m3 as it is nearest, what lies beyond its largest number at that; not-a-numbers stay such
 __device__ __forceinline__ float within_e4m3(float x) {
   x = x > 448.0f ? 448.0f : x;
@@ -96,17 +102,29 @@ __device__ __forceinline__ void store_values(void* row, int64_t at, const float 
         w[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
       }
     }
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    // (first out of the caches, as what has been read: rotary step of 32760 tokens, 2 x 40 heads, 265 us, kept like others 271)
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(u4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u4*>(static_cast<uint16_t*>(row) + at));
   }
 }
 
-// A thread's unit: E channels at `lo` and E at `hi` of a row; units up to `turned` are turned whole or by group (interleaved).
+// What a workgroup holds of its tokens
+struct Token {
+  int there;        // in the batch's counts
+  int page, slot;   // of the cache; page -1: not stored
+};
+constexpr int kMostTokens = 16;
+
+// A workgroup takes a few tokens: first its threads form a cosine and a sine each, of a pair of a token, then all rows go through, a thread with E channels at `lo`
+// and E at `hi` of every one.  (Every thread forming what it needs itself, eight pairs for three rows: 360 us
+// of 32760 tokens, 2 x 40 heads, where this takes 250.)
 template <int DT, Layout kLayout, bool kCache, bool kEight>
 __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) {
-  constexpr int E = kLayout == kSingle ? 1 : 8;
+  constexpr int E = kLayout == kSingle ? 1 : 8, kAhead = 2;
+  extern __shared__ __align__(16) float2 turns[];  // [tokens][R / 2]: cosine and sine
+  __shared__ Token token_of[kMostTokens];
+  const int pairs = p.R / 2, all = p.B * p.L, token0 = (int)blockIdx.x * p.tokens_each, tokens = min(p.tokens_each, all - token0), rows = tokens * p.heads;
   const int unit = (int)threadIdx.x % p.units, slot = (int)threadIdx.x / p.units;
-  if (slot >= p.head_slots * p.token_slots) return;
-  const int head0 = slot % p.head_slots, token0 = slot / p.head_slots;
   // where the unit lies, and the numbers of its pairs
   int lo, hi, pair_lo, pair_hi;
   bool turn_lo, turn_hi;
@@ -134,100 +152,133 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
     }
   }
   const bool has_hi = hi < p.D;
-  const int tokens = p.B * p.L;
-  int token = (int)blockIdx.x * p.token_slots * p.tokens_each + token0;
-  for (int i = 0; i < p.tokens_each && token < tokens; ++i, token += p.token_slots) {
-    const int b = token / p.L, l = token - b * p.L;
-    int place = l;
-    bool there = true, stored = false;
-    int page = 0, in_page = 0;
+
+  struct Row {
+    int t, part, head;
+    bool is;
+    Raw<DT, E> x, y;
+  } row[kAhead];
+  auto part = [&](int i) -> const RotaryPart& { return i == 0 ? p.part[0] : i == 1 ? p.part[1] : p.part[2]; };
+  auto fetch = [&](int first) {  // (rows behind the counts too: they are there, and zeros or nothing is made of them)
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      Row& r = row[n];
+      const int number = first + n * p.slots;
+      r.is = number < rows;
+      r.t = quotient(min(number, rows - 1), p.by_heads);
+      r.head = min(number, rows - 1) - r.t * p.heads;
+      r.part = r.head < p.part[0].H ? 0 : r.head < p.part[0].H + p.part[1].H ? 1 : 2;
+      r.head -= r.part == 0 ? 0 : r.part == 1 ? p.part[0].H : p.part[0].H + p.part[1].H;
+      const int b = quotient(token0 + r.t, p.by_length), l = token0 + r.t - b * p.L;
+      const RotaryPart& from = part(r.part);
+      const char* at = static_cast<const char*>(from.src) + (b * from.sB + l * from.sL + r.head * from.sH) * kWidth<DT>;
+      if (r.is) {
+        r.x.load(at + lo * kWidth<DT>);
+        if (has_hi) r.y.load(at + hi * kWidth<DT>);
+      }
+    }
+  };
+  const bool works = slot < p.slots;
+  if (works) fetch(slot);
+
+  auto place_of = [&](int b, int l, int& n) {
+    n = p.L;
     if constexpr (kCache) {
-      const int n = p.pages.q_lens != nullptr ? rows_counted(p.pages.q_lens[b], p.L) : p.L;
-      place = (int)((int64_t)max(p.pages.k_lens[b], 0) - n + l);
-      there = l < n;
-      if (there && place >= 0) {
-        const int number = quotient(place, p.pages.size);
-        in_page = place - number * p.pages.size.by;
-        if (number < p.pages.width) {
-          page = p.pages.table[b * p.pages.sB + number];
-          stored = (unsigned)page < (unsigned)p.pages.pages;
-        }
+      if (p.pages.q_lens != nullptr) n = rows_counted(p.pages.q_lens[b], p.L);
+      return (int)((int64_t)max(p.pages.k_lens[b], 0) - n + l);
+    }
+    return l;
+  };
+  for (int i = (int)threadIdx.x; i < tokens * pairs; i += 256) {
+    const int t = i / pairs, pair = i - t * pairs, b = quotient(token0 + t, p.by_length), l = token0 + t - b * p.L;
+    double position;
+    if (p.positions != nullptr) {
+      int axis = 0;
+#pragma unroll
+      for (int a = 1; a < kMostAxes; ++a) axis = a < p.axes && pair >= p.ends[a - 1] ? a : axis;
+      const int64_t offset = b * p.pos_sB + l * p.pos_sL + axis * p.pos_sA;
+      position = p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[offset] : (double)static_cast<const int32_t*>(p.positions)[offset];
+    } else {
+      int n;
+      position = (double)place_of(b, l, n);
+    }
+    float c, s;
+    turn_of(position, p.frequencies[pair], c, s);
+    turns[i] = make_float2(c * p.magnitude, s * (p.inverse ? -p.magnitude : p.magnitude));
+  }
+  if (kCache && (int)threadIdx.x < tokens) {
+    const int t = (int)threadIdx.x, b = quotient(token0 + t, p.by_length), l = token0 + t - b * p.L;
+    int n;
+    const int place = place_of(b, l, n);
+    Token own{l < n, -1, 0};
+    if (own.there && place >= 0) {
+      const int number = quotient(place, p.pages.size);
+      own.slot = place - number * p.pages.size.by;
+      if (number < p.pages.width) {
+        const int page = p.pages.table[b * p.pages.sB + number];
+        own.page = (unsigned)page < (unsigned)p.pages.pages ? page : -1;
       }
     }
-    float c[E], s[E];
-    if (turn_lo || turn_hi) {
-      double at[kMostAxes];
+    token_of[t] = own;
+  }
+  __syncthreads();
+  if (!works) return;
+
+  for (int first = slot; first < rows; first += kAhead * p.slots) {
+    if (first != slot) fetch(first);
 #pragma unroll
-      for (int a = 0; a < kMostAxes; ++a) {
-        at[a] = (double)place;
-        if (p.positions != nullptr && a < p.axes) {
-          const int64_t offset = b * p.pos_sB + l * p.pos_sL + a * p.pos_sA;
-          at[a] = p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[offset] : (double)static_cast<const int32_t*>(p.positions)[offset];
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        // (a group that is not turned has no pairs: the last one's then, and nothing is made of them)
-        const int pair = min(e < (E + 1) / 2 ? pair_lo + e : pair_hi + e - (E + 1) / 2, p.R / 2 - 1);
-        double position = at[0];
-#pragma unroll
-        for (int a = 1; a < kMostAxes; ++a) position = a < p.axes && pair >= p.ends[a - 1] ? at[a] : position;
-        turn_of(position, p.frequencies[pair], c[e], s[e]);
-        c[e] *= p.magnitude;
-        s[e] *= p.inverse ? -p.magnitude : p.magnitude;
-      }
-    }
-    for (int h = head0; h < p.heads; h += p.head_slots) {
-      int head = h;
-      const bool second = head >= p.part[0].H;
-      head -= second ? p.part[0].H : 0;
-      const bool third = second && head >= p.part[1].H;
-      head -= third ? p.part[1].H : 0;
-      const RotaryPart& part = third ? p.part[2] : second ? p.part[1] : p.part[0];
+    for (int n = 0; n < kAhead; ++n) {
+      const Row& r = row[n];
+      if (!r.is) continue;
+      const RotaryPart& to = part(r.part);
+      Token token{1, 0, 0};
+      if constexpr (kCache) token = token_of[r.t];
+      if (kCache && to.paged && token.page < 0) continue;
       float x[E], y[E];
-      if (kCache && !there) {
-        if (part.paged) continue;
+      r.x.values(x);
+      r.y.values(y);
+      if (kCache && !token.there) {
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = y[e] = 0.0f;
-      } else {
-        if (kCache && part.paged && !stored) continue;
-        const char* row = static_cast<const char*>(part.src) + (b * part.sB + l * part.sL + head * part.sH) * kWidth<DT>;
-        load_values<DT, E>(row, lo, x);
-        if (has_hi) load_values<DT, E>(row, hi, y);
-        if (part.turn) {
-          if constexpr (kLayout == kInterleaved) {
+      }
+      if (to.turn) {
+        const float2* own = turns + r.t * pairs;
+        if constexpr (kLayout == kInterleaved) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float a = x[2 * e], d = y[2 * e];
-              if (turn_lo) {
-                x[2 * e] = __fmaf_rn(a, c[e], -x[2 * e + 1] * s[e]);
-                x[2 * e + 1] = __fmaf_rn(a, s[e], x[2 * e + 1] * c[e]);
-              }
-              if (turn_hi) {
-                y[2 * e] = __fmaf_rn(d, c[4 + e], -y[2 * e + 1] * s[4 + e]);
-                y[2 * e + 1] = __fmaf_rn(d, s[4 + e], y[2 * e + 1] * c[4 + e]);
-              }
+          for (int e = 0; e < 4; ++e) {
+            if (turn_lo) {
+              const float2 z = own[pair_lo + e];
+              const float a = x[2 * e];
+              x[2 * e] = __fmaf_rn(a, z.x, -x[2 * e + 1] * z.y);
+              x[2 * e + 1] = __fmaf_rn(a, z.y, x[2 * e + 1] * z.x);
             }
-          } else if (turn_lo) {
+            if (turn_hi) {
+              const float2 z = own[pair_hi + e];
+              const float a = y[2 * e];
+              y[2 * e] = __fmaf_rn(a, z.x, -y[2 * e + 1] * z.y);
+              y[2 * e + 1] = __fmaf_rn(a, z.y, y[2 * e + 1] * z.x);
+            }
+          }
+        } else if (turn_lo) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float a = x[e];
-              x[e] = __fmaf_rn(a, c[e], -y[e] * s[e]);
-              y[e] = __fmaf_rn(a, s[e], y[e] * c[e]);
-            }
+          for (int e = 0; e < E; ++e) {
+            const float2 z = own[pair_lo + e];
+            const float a = x[e];
+            x[e] = __fmaf_rn(a, z.x, -y[e] * z.y);
+            y[e] = __fmaf_rn(a, z.y, y[e] * z.x);
           }
         }
       }
-      if (kCache && part.paged) {
+      if (kCache && to.paged) {
         constexpr int kSize = kEight ? 1 : kWidth<DT>;
-        char* row = static_cast<char*>(part.dst) + (page * part.dB + in_page * part.dL + head * part.dH) * kSize;
-        const float inv = kEight && part.scale != nullptr ? 1.0f / part.scale[head] : 1.0f;
-        store_values<DT, E, kEight>(row, lo, x, inv);
-        if (has_hi) store_values<DT, E, kEight>(row, hi, y, inv);
+        char* at = static_cast<char*>(to.dst) + (token.page * to.dB + token.slot * to.dL + r.head * to.dH) * kSize;
+        const float inv = kEight && to.scale != nullptr ? 1.0f / to.scale[r.head] : 1.0f;
+        store_values<DT, E, kEight>(at, lo, x, inv);
+        if (has_hi) store_values<DT, E, kEight>(at, hi, y, inv);
       } else {
-        char* row = static_cast<char*>(part.dst) + (b * part.dB + l * part.dL + head * part.dH) * kWidth<DT>;
-        store_values<DT, E, false>(row, lo, x, 1.0f);
-        if (has_hi) store_values<DT, E, false>(row, hi, y, 1.0f);
+        char* at = static_cast<char*>(to.dst) + ((int64_t)(token0 + r.t) * to.H + r.head) * p.D * kWidth<DT>;
+        store_values<DT, E, false>(at, lo, x, 1.0f);
+        if (has_hi) store_values<DT, E, false>(at, hi, y, 1.0f);
       }
     }
   }
@@ -235,13 +286,14 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
 
 template <int DT, Layout kLayout>
 void start(const RotaryParams& p, unsigned groups, hipStream_t s) {
+  const unsigned lds = (unsigned)(p.tokens_each * (p.R / 2) * 8);
   if (p.pages.table == nullptr) {
-    sage_rotary_kernel<DT, kLayout, false, false><<<groups, 256, 0, s>>>(p);
+    sage_rotary_kernel<DT, kLayout, false, false><<<groups, 256, lds, s>>>(p);
   } else if constexpr (DT != kFp32) {
     if (p.eight_bits)
-      sage_rotary_kernel<DT, kLayout, true, true><<<groups, 256, 0, s>>>(p);
+      sage_rotary_kernel<DT, kLayout, true, true><<<groups, 256, lds, s>>>(p);
     else
-      sage_rotary_kernel<DT, kLayout, true, false><<<groups, 256, 0, s>>>(p);
+      sage_rotary_kernel<DT, kLayout, true, false><<<groups, 256, lds, s>>>(p);
   }
 }
 template <int DT>
@@ -261,13 +313,14 @@ hipError_t launch_rotary(RotaryParams p, hipStream_t s) {
   if (p.D % 8 == 0 && p.R % (p.interleaved ? 8 : 16) == 0) layout = p.interleaved ? kInterleaved : kHalves;
   p.heads = p.part[0].H + p.part[1].H + p.part[2].H;
   p.units = layout == kInterleaved ? (p.D / 8 + 1) / 2 : layout == kHalves ? p.R / 16 + (p.D - p.R + 15) / 16 : p.R / 2 + (p.D - p.R + 1) / 2;
-  // rows at a time: those of a token's heads, spread evenly over its passes, and of as many tokens as there is place for
-  const int slots = 256 / p.units, passes = (p.heads + slots - 1) / slots;
-  p.head_slots = (p.heads + passes - 1) / passes;
-  p.token_slots = slots / p.head_slots;
-  p.tokens_each = 1;
-  const int64_t tokens = (int64_t)p.B * p.L;
-  const unsigned groups = (unsigned)((tokens + (int64_t)p.token_slots * p.tokens_each - 1) / ((int64_t)p.token_slots * p.tokens_each));
+  p.slots = 256 / p.units;  // rows at a time
+  p.by_heads = divisor(p.heads);
+  p.by_length = divisor(p.L);
+  // About five rows to a thread where that leaves four workgroups to each of 256 compute units.  Forward and backward of 32760 tokens, 2 x 40 heads: of two
+  // tokens 501 us, of four 530, of sixteen 598.
+  const int tokens = p.B * p.L;
+  p.tokens_each = std::max(1, std::min({kMostTokens, 5 * p.slots / p.heads, (tokens + 1023) / 1024}));
+  const unsigned groups = (unsigned)((tokens + p.tokens_each - 1) / p.tokens_each);
   if (p.dtype == KSANA_SAGE_BF16)
     start_layout<KSANA_SAGE_BF16>(p, layout, groups, s);
   else if (p.dtype == KSANA_SAGE_FP16)
