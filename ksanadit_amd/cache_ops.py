@@ -23,7 +23,7 @@ import torch
 
 from . import _capi
 from .sage_ops import _DTYPES, _k_lens_arg, _stream_ptr
-from .train_ops import _channels_last, _check_rotary, _on, _ptr, _readable, _refuse_unseen, _rotary_call, _scratch, _wants_gradient
+from .train_ops import _channels_last, _check_rotary, _contiguous_like, _on, _ptr, _readable, _refuse_unseen, _rotary_call, _scratch
 
 # The library's structures, packed (see train_ops)
 _CACHE = struct.Struct("=4Q3q4iQq2Q")  # ksana_sage_cache
@@ -49,24 +49,25 @@ def allocate(pages: int, page_size: int, heads: int, head_size: int, dtype: torc
 
 def _check_cache(cache: PagedCache, pages: torch.Tensor, x: torch.Tensor, heads: int | None) -> int:
     """The cache's type as the library takes it; x: rows of q or k."""
-    k, v = cache.k, cache.v
-    device = x.get_device()
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride() or k.get_device() != device or v.get_device() != device:
+    k, v, k_scale, v_scale = cache
+    device, dtype, shape = x.get_device(), k.dtype, k.shape
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype or k.stride() != v.stride() or k.get_device() != device or v.get_device() != device:
         raise ValueError(f"the cache must be two tensors [pages, heads, page_size, head_size] laid out alike on {x.device}, "
                          f"got {k.dtype} {tuple(k.shape)} on {k.device} and {v.dtype} {tuple(v.shape)} on {v.device}")
-    if k.dtype != x.dtype and k.dtype != torch.float8_e4m3fn:
-        raise ValueError(f"a cache of {k.dtype} does not go with {x.dtype}")
-    if k.shape[3] != x.shape[3] or (heads is not None and k.shape[1] != heads):
-        raise ValueError(f"the cache holds {k.shape[1]} heads of {k.shape[3]} channels, the tensors {x.shape[2]} of {x.shape[3]}")
+    if dtype != x.dtype and dtype != torch.float8_e4m3fn:
+        raise ValueError(f"a cache of {dtype} does not go with {x.dtype}")
+    if shape[3] != x.shape[3] or (heads is not None and shape[1] != heads):
+        raise ValueError(f"the cache holds {shape[1]} heads of {shape[3]} channels, the tensors {x.shape[2]} of {x.shape[3]}")
     if k.numel() == 0 or k.stride(3) != 1:
         raise ValueError("the cache must not be empty, and its channels must be contiguous")
-    for name, t in (("k_scale", cache.k_scale), ("v_scale", cache.v_scale)):
-        if t is not None and (k.dtype != torch.float8_e4m3fn or t.dtype != torch.float32 or t.shape != k.shape[1:2] or t.get_device() != device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 [{k.shape[1]}] on {x.device}, for a float8_e4m3fn cache")
+    if k_scale is not None or v_scale is not None:
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is not None and (dtype != torch.float8_e4m3fn or t.dtype != torch.float32 or t.shape != shape[1:2] or t.get_device() != device or not t.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous float32 [{shape[1]}] on {x.device}, for a float8_e4m3fn cache")
     if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != x.shape[0] or pages.get_device() != device or pages.shape[1] == 0 or (
             pages.stride(1) != 1 and pages.shape[1] > 1):
         raise ValueError(f"pages must be int32 [{x.shape[0]}, entries] with contiguous entries on {x.device}, got {pages.dtype} {tuple(pages.shape)} on {pages.device}")
-    return _capi.E4M3 if k.dtype == torch.float8_e4m3fn else _DTYPES[k.dtype]
+    return _capi.E4M3 if dtype == torch.float8_e4m3fn else _DTYPES[dtype]
 
 
 def _cache_call(cache: PagedCache, kind: int, pages, q_lens, k_lens) -> bytes:
@@ -78,22 +79,25 @@ def _cache_call(cache: PagedCache, kind: int, pages, q_lens, k_lens) -> bytes:
 
 
 def _check_rows(name: str, *tensors: torch.Tensor) -> None:
-    first = tensors[0]
+    first, wanted = tensors[0], False
+    dtype, device = first.dtype, first.get_device()
     for t in tensors:
         if t.dim() != 4:
             raise ValueError(f"{name} expects 4-D tensors")
         if not t.is_cuda:
             raise RuntimeError(f"{name} needs tensors on a HIP device; there is no CPU path (got device {t.device})")
-        if t.dtype not in _DTYPES or t.dtype != first.dtype or t.get_device() != first.get_device():
+        if t.dtype != dtype or dtype not in _DTYPES or t.get_device() != device:
             raise ValueError(f"{name} takes bfloat16 or float16 tensors of one type on one device, got {t.dtype} on {t.device}")
-    if torch.is_grad_enabled() and _wants_gradient(*tensors):
+        wanted = wanted or t.requires_grad
+    if wanted and torch.is_grad_enabled():
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad(), or train with train_ops")
 
 
-def _counts(k_lens, q_lens, batch: int, device) -> tuple:
-    if k_lens is None:
-        raise ValueError("k_lens is needed: how many tokens every sequence has")
-    return _k_lens_arg(k_lens, batch, device), _k_lens_arg(q_lens, batch, device, "q_lens")
+def _counts(counts, name: str, batch: int, x: torch.Tensor) -> torch.Tensor | None:
+    """Counts as the kernels read them; those that are so already cost nothing."""
+    if isinstance(counts, torch.Tensor) and counts.dtype is torch.int32 and counts.shape == (batch,) and counts.get_device() == x.get_device() and counts.is_contiguous():
+        return counts
+    return _k_lens_arg(counts, batch, x.device, name)
 
 
 def append(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, pages: torch.Tensor, k_lens, q_lens=None, *, q: torch.Tensor | None = None,
@@ -121,13 +125,15 @@ def append(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, pages: torch.Ten
         checked = _check_rotary(frequencies, positions, sections, B, L, D, k.get_device())
     if not abs(magnitude) <= 3e38:
         raise ValueError(f"magnitude {magnitude} is not a number of fp32")
+    if k_lens is None:
+        raise ValueError("k_lens is needed: how many tokens every sequence has")
     _refuse_unseen("append", k, v, q)
-    k_lens, q_lens = _counts(k_lens, q_lens, B, k.device)
-    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_lens, q_lens = _counts(k_lens, "k_lens", B, k), _counts(q_lens, "q_lens", B, k)
+    out = None if q is None else _contiguous_like(q)
     if k.numel() == 0:
         return out if out is None or out.numel() == 0 else out.zero_()
     k, v = _channels_last(k), _channels_last(v)
-    q = None if q is None or q.numel() == 0 else _channels_last(q)
+    q = None if q is None or q.shape[2] == 0 else _channels_last(q)
     call = _rotary_call(q, k, v, frequencies, positions, checked, bool(interleaved), float(magnitude), False)
     with _on(k.device):
         rc = _capi.load().ksana_sage_cache_append(call, _cache_call(cache, kind, pages, q_lens, k_lens), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(out), _stream_ptr(k.device))
@@ -152,9 +158,11 @@ def attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, k_lens, q
         raise ValueError(f"{H} query heads are no multiple of the cache's {cache.k.shape[1]}")
     if sm_scale is not None and not abs(sm_scale) <= 2e38:
         raise ValueError(f"sm_scale {sm_scale} is not a number of at most 2e38 in size")
+    if k_lens is None:
+        raise ValueError("k_lens is needed: how many tokens every sequence has")
     _refuse_unseen("attention", q)
-    k_lens, q_lens = _counts(k_lens, q_lens, B, q.device)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_lens, q_lens = _counts(k_lens, "k_lens", B, q), _counts(q_lens, "q_lens", B, q)
+    o = _contiguous_like(q)
     if q.numel() == 0:
         return o
     q = _readable(q)

@@ -465,17 +465,17 @@ def _rotary_call(q, k, v, frequencies, positions, checked, interleaved: bool, ma
 
 
 def _turn(q, k, frequencies, positions, checked, interleaved, magnitude, inverse) -> tuple:
-    out = tuple(None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    rows = [None if t is None or t.numel() == 0 else _channels_last(t) for t in (q, k)]
-    given = rows[1] if rows[0] is None else rows[0]
-    if given is None:
-        return out
-    call = _rotary_call(*rows, None, frequencies, positions, checked, interleaved, magnitude, inverse)
-    with _on(given.device):
-        rc = _capi.load().ksana_sage_rotary_rows(call, _ptr(rows[0]), _ptr(rows[1]), _ptr(out[0]), _ptr(out[1]), _stream_ptr(given.device))
+    q_out, k_out = _contiguous_like(q), None if k is None else _contiguous_like(k)
+    q_rows = None if q.numel() == 0 else _channels_last(q)
+    k_rows = None if k is None or k.numel() == 0 else _channels_last(k)
+    if q_rows is None and k_rows is None:
+        return q_out, k_out
+    call, device = _rotary_call(q_rows, k_rows, None, frequencies, positions, checked, interleaved, magnitude, inverse), q.device
+    with _on(device):
+        rc = _capi.load().ksana_sage_rotary_rows(call, _ptr(q_rows), _ptr(k_rows), q_out.data_ptr(), _ptr(k_out), _stream_ptr(device))
     if rc != _capi.OK:
         _capi.check(rc, "train_ops.rotary")
-    return out
+    return q_out, k_out
 
 
 class _Rotary(torch.autograd.Function):
