@@ -24,7 +24,7 @@ extern __shared__ __align__(1024) char cache_lds[];
 __device__ __forceinline__ unsigned lds_base() { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)cache_lds; }
 
 constexpr int kCacheBlock = 128;  // query rows of a workgroup
-constexpr int kMostRuns = 64, kLeastTiles = 4;
+constexpr int kMostRuns = 64, kLeastTiles = 2;
 constexpr float kLog2e = 1.44269504088896340736f;
 // fp16 probabilities relative to a row's largest lose bits from 2^-14 on: scaled up by 2^6 a factor of 2^6 later.  The reference point lags behind the row's maximum by
 // at most 2^kLazy.
@@ -91,6 +91,8 @@ struct Lookup {
 struct Tile64 {
   unsigned at;     // of the lane's key, 16-byte units from the cache's start; all ones: there is none
   uint64_t exist;  // the keys that do
+  // Runs of 16 are (aligned ones, of the tile's 64)
+  __device__ __forceinline__ bool in_sixteens(const CacheAttnParams& p) const { return p.pages.size.by % 16 == 0 && exist == ~UINT64_C(0); }
   // All 64 there, a slot apart.  (Of pages of 64 slots and more a tile has two at most: if its ends lie 63 slots apart, so does all between.)
   __device__ __forceinline__ bool in_a_row(const CacheAttnParams& p) const {
     return p.pages.size.by >= kTrainTile && exist == ~UINT64_C(0) &&
@@ -103,7 +105,9 @@ struct Tile64 {
   }
 };
 
-// Copies of a tile, the wave's share.  One whose keys lie in a row is one address and a lane offset, others an address of every lane's own.
+// Copies of a tile, the wave's share.  One whose keys lie in a row is one address and a lane offset.  Otherwise a lane's rows of all copies are of 16 neighbours
+// (Tile::row_of): where those lie in a row, they are an address of the lane's own and constants.  Elsewhere every copy is looked up.
+// (Chunk of 4096 rows on 32768 keys, 40 heads on 8: 2320 us in pages of 64, XX16 in pages of 16, XX20 in pages of 20.)
 template <int DT, int D, int kWaves, bool kEight>
 struct PagedCopy {
   using T = Tile<D>;
@@ -122,6 +126,10 @@ struct PagedCopy {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) lds_copy16_at(first + T::row_of(c * kWaves, 0) * p.sS, whole, tile + T::copy_at(c * kWaves + wave));
+    } else if (keys.in_sixteens(p)) {
+      const char* own = from((unsigned)__shfl((int)keys.at, T::row_of(wave, lane)), lane);
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) lds_copy16_from(own + T::row_of(c * kWaves, 0) * p.sS, tile + T::copy_at(c * kWaves + wave));
     } else {
 #pragma unroll
       for (int c = 0; c < kCopies; ++c)
@@ -134,6 +142,10 @@ struct PagedCopy {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(first + T::row_of(c * kWaves, 0) * p.sS + whole);
+    } else if (keys.in_sixteens(p)) {
+      const char* own = from((unsigned)__shfl((int)keys.at, T::row_of(wave, lane)), lane);
+#pragma unroll
+      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(own + T::row_of(c * kWaves, 0) * p.sS);
     } else {
 #pragma unroll
       for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(from((unsigned)__shfl((int)keys.at, T::row_of(c * kWaves + wave, lane)), lane));
@@ -724,11 +736,23 @@ void fill_in(CacheAttnParams& p) {
   p.blocks = (p.Lq * p.group + kCacheBlock - 1) / kCacheBlock;
   const int64_t blocks = (int64_t)p.B * p.Hkv * p.blocks, tiles = ((int64_t)p.pages.width * p.pages.size.by + kTrainTile - 1) / kTrainTile;
   const int most = (int)std::min<int64_t>(kMostRuns, (tiles + kLeastTiles - 1) / kLeastTiles);
+  const double rows = std::min(p.Lq * p.group, kCacheBlock);
   p.whole = 0;
   p.cut = (int)blocks;
+  p.runs = 1;
+  double least = 1e30;
   if (p.Lq * p.group <= kFewRows) {
-    // two workgroups to each of 256 compute units at a time, four times over: sequences shorter than the table are cut into as many
-    p.runs = (int)std::max<int64_t>(1, std::min<int64_t>(most, (2048 + blocks - 1) / blocks));
+    // In us: the keys' and values' bytes at the memory's rate, half of what a wave takes for its tiles one after the other, workgroups that come and go, the second launch and
+    // its bytes.  (One token on 32760 keys, 8 heads: 64 runs 28, 10 runs 52; 64 sequences of up to 8192: 2 runs 229, 4 232, 8 245; one of 2000: 17 runs 11.5, 9 12.5, 5 15.8.)
+    const double places = p.eight_bits ? 1024.0 : 512.0, all = 2.0 * kTrainTile * p.D * (p.eight_bits ? 1.0 / 4.2e6 : 2.0 / 5.0e6) * tiles * blocks;
+    for (int n = 1; n <= most; ++n) {
+      const double each = (double)((tiles + n - 1) / n), workgroups = (double)n * blocks;
+      const double cost = all + 0.85 * std::ceil(each / kFewWaves) + 2.0 * std::max(1.0, workgroups / places) + (n == 1 ? 0.0 : 3.0 + 2.0 * workgroups * rows * p.D * 4.0 / 4e6);
+      if (cost < 0.98 * least) {
+        least = cost;
+        p.runs = n;
+      }
+    }
     return;
   }
   // Blocks that fill whole rounds of 512 places are left whole, the others are cut so that they fill one more.  In units of a tile's time (about
@@ -737,11 +761,9 @@ void fill_in(CacheAttnParams& p) {
   constexpr double kSetup = 2.0, kJoin = 2.0, kBytesPerTile = 4e12 * 2e-6;
   p.whole = (int)(blocks / kPlaces * kPlaces);
   p.cut = (int)(blocks - p.whole);
-  p.runs = 1;
-  double least = 1e30;
   for (int n = 1; n <= most; ++n) {
     const double each = (double)((tiles + n - 1) / n);
-    const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * p.cut * 4.0 * std::min(p.Lq * p.group, kCacheBlock) * p.D / kBytesPerTile;
+    const double join = n == 1 ? 0.0 : kJoin + 2.0 * n * p.cut * 4.0 * rows * p.D / kBytesPerTile;
     const double cost = std::ceil((double)n * p.cut / kPlaces) * (each + kSetup) + join;
     if (cost < 0.97 * least) {
       least = cost;
