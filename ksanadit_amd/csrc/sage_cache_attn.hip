@@ -108,19 +108,17 @@ struct Tile64 {
 // Copies of a tile, the wave's share.  One whose keys lie in a row is one address and a lane offset.  Otherwise a lane's rows of all copies are of 16 neighbours
 // (Tile::row_of): where those lie in a row, they are an address of the lane's own and constants.  Elsewhere every copy is looked up.
 // (Chunk of 4096 rows on 32768 keys, 40 heads on 8: 2320 us in pages of 64, XX16 in pages of 16, XX20 in pages of 20.)
-template <int DT, int D, int kWaves, bool kEight>
+template <int D, int kWaves>
 struct PagedCopy {
   using T = Tile<D>;
   static constexpr int kCopies = T::kCopies / kWaves;
-  static constexpr int kPiece = kEight ? 8 : 16;  // bytes of eight channels
   const char* base;
   unsigned whole;
   __device__ __forceinline__ PagedCopy(const CacheAttnParams& p, const char* cache, int hk, int wave, int lane)
-      : base(cache + hk * p.sH), whole((unsigned)T::row_of(wave, lane) * (unsigned)p.sS + lane % T::kPieces * kPiece) {}
+      : base(cache + hk * p.sH), whole((unsigned)T::row_of(wave, lane) * (unsigned)p.sS + lane % T::kPieces * 16) {}
   __device__ __forceinline__ const char* from(unsigned at, int lane) const {
-    return (at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % T::kPieces * kPiece;
+    return (at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % T::kPieces * 16;
   }
-  // 16 bits: on the way to `tile`
   __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, unsigned tile, int wave, int lane) const {
     if (keys.in_a_row(p)) {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
@@ -136,41 +134,48 @@ struct PagedCopy {
         lds_copy16_from(from((unsigned)__shfl((int)keys.at, T::row_of(c * kWaves + wave, lane)), lane), tile + T::copy_at(c * kWaves + wave));
     }
   }
-  // 8 bits: on the way to registers, and from there
-  __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, uint2 (&raw)[kCopies], int wave, int lane) const {
+};
+
+// A tile of 8-bit rows, the wave's share, on its way through registers: sixteen channels at an access, D / 16 lanes to a row
+template <int DT, int D, int kWaves>
+struct WideCopy {
+  using T = Tile<D>;
+  static constexpr int kPieces = D / 16, kRows = 64 / kPieces, kCopies = kTrainTile / (kRows * kWaves);
+  const char* base;
+  unsigned whole;
+  uint4 raw[kCopies];
+  __device__ __forceinline__ WideCopy(const CacheAttnParams& p, const char* cache, int hk, int wave, int lane)
+      : base(cache + hk * p.sH), whole((unsigned)(kRows * wave + lane / kPieces) * (unsigned)p.sS + lane % kPieces * 16) {}
+  __device__ __forceinline__ void start(const CacheAttnParams& p, const Tile64& keys, int wave, int lane) {
     if (keys.in_a_row(p)) {
       const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
 #pragma unroll
-      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(first + T::row_of(c * kWaves, 0) * p.sS + whole);
-    } else if (keys.in_sixteens(p)) {
-      const char* own = from((unsigned)__shfl((int)keys.at, T::row_of(wave, lane)), lane);
+      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint4*>(first + kRows * kWaves * c * p.sS + whole);
+      return;
+    }
 #pragma unroll
-      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(own + T::row_of(c * kWaves, 0) * p.sS);
-    } else {
-#pragma unroll
-      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint2*>(from((unsigned)__shfl((int)keys.at, T::row_of(c * kWaves + wave, lane)), lane));
+    for (int c = 0; c < kCopies; ++c) {
+      const unsigned at = (unsigned)__shfl((int)keys.at, kRows * (c * kWaves + wave) + lane / kPieces);
+      raw[c] = *reinterpret_cast<const uint4*>((at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % kPieces * 16);
     }
   }
   // (exact: e4m3 numbers are numbers of both types)
-  static __device__ __forceinline__ v4i widened(const uint2& raw) {
-    v4i out;
-    if constexpr (DT == KSANA_SAGE_BF16) {
-      out[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, 1.0f, false));
-      out[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.x, 1.0f, true));
-      out[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, 1.0f, false));
-      out[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw.y, 1.0f, true));
-    } else {
-      out[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.x, 1.0f, false));
-      out[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.x, 1.0f, true));
-      out[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.y, 1.0f, false));
-      out[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw.y, 1.0f, true));
-    }
-    return out;
+  static __device__ __forceinline__ v4i widened(unsigned lo, unsigned hi) {
+    if constexpr (DT == KSANA_SAGE_BF16)
+      return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
+    else
+      return v4i{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
+                 __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
   }
-  static __device__ __forceinline__ void finish(const uint2 (&raw)[kCopies], unsigned tile, int wave, int lane) {
+  __device__ __forceinline__ void finish(unsigned tile, int wave, int lane) const {
+    typedef __attribute__((address_space(3))) v4i* Lds;
+    const unsigned lane_at = tile + T::at(kRows * wave + lane / kPieces) + lane % kPieces * 32;  // (T::at is a sum over a row's bits)
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c)
-      *(__attribute__((address_space(3))) v4i*)(uintptr_t)(tile + T::copy_at(c * kWaves + wave) + lane * 16) = widened(raw[c]);
+    for (int c = 0; c < kCopies; ++c) {
+      *(Lds)(uintptr_t)(lane_at + T::at(kRows * kWaves * c)) = widened(raw[c].x, raw[c].y);
+      *(Lds)(uintptr_t)(lane_at + T::at(kRows * kWaves * c) + 16) = widened(raw[c].z, raw[c].w);
+    }
   }
 };
 
@@ -229,29 +234,28 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
   float top = -INFINITY, minus = kShift<DT>, sum = 0.0f;  // reference point (unscaled), what is added to scaled scores, the row's sum
   const int row = row0 + wave * 32 + m;
   if (range.from < range.to) {
-    typedef PagedCopy<DT, D, kWaves, kEight> Copy;
-    const Copy k_copy(p, p.k, hk, wave, lane), v_copy(p, p.v, hk, wave, lane);
+    using Copy = std::conditional_t<kEight, WideCopy<DT, D, kWaves>, PagedCopy<D, kWaves>>;
+    Copy k_copy(p, p.k, hk, wave, lane), v_copy(p, p.v, hk, wave, lane);
     const int32_t* table = p.pages.table + b * p.pages.sB;
     auto k_tile = [&](int t) { return lds + (t & 1) * T::kBytes; };
     auto v_tile = [&](int t) { return lds + (2 + (t & 1)) * T::kBytes; };
-    uint2 k_raw[kEight ? Copy::kCopies : 1], v_raw[kEight ? Copy::kCopies : 1];
     auto copy_keys = [&](int t, const Tile64& keys) {
       if constexpr (kEight)
-        k_copy.start(p, keys, k_raw, wave, lane);
+        k_copy.start(p, keys, wave, lane);
       else
         k_copy.start(p, keys, k_tile(t), wave, lane);
     };
     auto copy_values = [&](int t, const Tile64& keys) {
       if constexpr (kEight)
-        v_copy.start(p, keys, v_raw, wave, lane);
+        v_copy.start(p, keys, wave, lane);
       else
         v_copy.start(p, keys, v_tile(t), wave, lane);
     };
     auto keys_there = [&](int t) {
-      if constexpr (kEight) Copy::finish(k_raw, k_tile(t), wave, lane);
+      if constexpr (kEight) k_copy.finish(k_tile(t), wave, lane);
     };
     auto values_there = [&](int t) {
-      if constexpr (kEight) Copy::finish(v_raw, v_tile(t), wave, lane);
+      if constexpr (kEight) v_copy.finish(v_tile(t), wave, lane);
     };
     // (behind a run's last tile: that one again)
     Lookup next_lookup;
@@ -441,37 +445,6 @@ __device__ __forceinline__ void lds_copy4_from(const void* lane_at, unsigned lds
 #pragma clang diagnostic pop
 }
 
-// A tile of 8-bit rows on its way through registers: 16 channels of row 8 c + .. at a time (of 64 channels: 16 c + ..)
-template <int DT, int D>
-struct WideCopy {
-  using T = Tile<D>;
-  static constexpr int kPieces = D / 16, kRows = 64 / kPieces, kCopies = kTrainTile / kRows;
-  uint4 raw[kCopies];
-  __device__ __forceinline__ void start(const CacheAttnParams& p, const char* base, const Tile64& keys, int lane) {
-    if (keys.in_a_row(p)) {
-      const char* first = base + (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane(keys.at) * 16;
-      const unsigned own = (unsigned)(lane / kPieces) * (unsigned)p.sS + lane % kPieces * 16;
-#pragma unroll
-      for (int c = 0; c < kCopies; ++c) raw[c] = *reinterpret_cast<const uint4*>(first + kRows * c * p.sS + own);
-      return;
-    }
-#pragma unroll
-    for (int c = 0; c < kCopies; ++c) {
-      const unsigned at = (unsigned)__shfl((int)keys.at, kRows * c + lane / kPieces);
-      raw[c] = *reinterpret_cast<const uint4*>((at == ~0u ? reinterpret_cast<const char*>(kZeroRow) : base + (uint64_t)at * 16) + lane % kPieces * 16);
-    }
-  }
-  __device__ __forceinline__ void finish(unsigned tile, int lane) const {
-    typedef __attribute__((address_space(3))) v4i* Lds;
-    const unsigned lane_at = tile + T::at(lane / kPieces) + lane % kPieces * 32;
-#pragma unroll
-    for (int c = 0; c < kCopies; ++c) {
-      *(Lds)(uintptr_t)(lane_at + T::at(kRows * c)) = PagedCopy<DT, D, 1, true>::widened(make_uint2(raw[c].x, raw[c].y));
-      *(Lds)(uintptr_t)(lane_at + T::at(kRows * c) + 16) = PagedCopy<DT, D, 1, true>::widened(make_uint2(raw[c].z, raw[c].w));
-    }
-  }
-};
-
 template <int DT, int D, bool kEight>
 __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few_kernel(const CacheAttnParams p) {
   using T = Tile<D>;
@@ -507,20 +480,18 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
       keys.at = is ? (unsigned)entry * (unsigned)p.page_units + (unsigned)slot * (unsigned)p.slot_units : ~0u;
       keys.exist = __ballot(is);
     };
-    typedef PagedCopy<DT, D, 1, false> Copy;
-    typedef WideCopy<DT, D> Wide;
-    constexpr int kCopies = kEight ? Wide::kCopies : Copy::kCopies;
-    const Copy k_copy(p, p.k, hk, 0, lane), v_copy(p, p.v, hk, 0, lane);
-    Wide k_wide, v_wide;
+    using Copy = std::conditional_t<kEight, WideCopy<DT, D, 1>, PagedCopy<D, 1>>;
+    constexpr int kCopies = Copy::kCopies;
+    Copy k_copy(p, p.k, hk, 0, lane), v_copy(p, p.v, hk, 0, lane);
     auto copy_keys = [&](const Tile64& keys) {
       if constexpr (kEight)
-        k_wide.start(p, k_copy.base, keys, lane);
+        k_copy.start(p, keys, 0, lane);
       else
         k_copy.start(p, keys, k_tile, 0, lane);
     };
     auto copy_values = [&](const Tile64& keys) {
       if constexpr (kEight)
-        v_wide.start(p, v_copy.base, keys, lane);
+        v_copy.start(p, keys, 0, lane);
       else
         v_copy.start(p, keys, v_tile, 0, lane);
     };
@@ -549,7 +520,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
     auto step = [&](int i, auto last) {
       copies_there<kCopies>();
       if constexpr (kEight) {
-        k_wide.finish(k_tile, lane);
+        k_copy.finish(k_tile, 0, lane);
         if constexpr (!last.value) next_keys(i);
       }
       reads_done();
@@ -594,7 +565,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
       else
         copies_there<kCopies + 1>();
       if constexpr (kEight) {
-        v_wide.finish(v_tile, lane);
+        v_copy.finish(v_tile, 0, lane);
         if constexpr (!last.value) copy_values(next64);
       }
       reads_done();
