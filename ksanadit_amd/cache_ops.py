@@ -9,8 +9,9 @@ everything their sequences have in the cache.  Both take the same table and coun
 so row i of the chunk stands at position ``k_lens[b] - q_lens[b] + i``.  Every layer has a cache of its own; table and counts are the same for all of them.
 
 Both run on the tensors' HIP device, on torch's current stream there; scratch comes from torch's caching allocator.  They do not synchronise and may be captured into a
-graph; table and counts are read by the kernels, so that replays go by what they hold then.  Repeated calls give the same bits.  There is no backward pass:
-``train_ops`` has those.
+graph, with counts as int32 tensors on that device (others are copied there in the call, which waits for the copy and cannot be captured); table and counts are read by the
+kernels, so that replays go by what they hold then.  Counts are taken as what the table and the call's rows hold at most.  Repeated calls give the same
+bits.  There is no backward pass: ``train_ops`` has those.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _capi
 from .sage_ops import _DTYPES, _k_lens_arg, _stream_ptr
@@ -58,8 +60,8 @@ def _check_cache(cache: PagedCache, pages: torch.Tensor, x: torch.Tensor, heads:
         raise ValueError(f"a cache of {dtype} does not go with {x.dtype}")
     if shape[3] != x.shape[3] or (heads is not None and shape[1] != heads):
         raise ValueError(f"the cache holds {shape[1]} heads of {shape[3]} channels, the tensors {x.shape[2]} of {x.shape[3]}")
-    if k.numel() == 0 or k.stride(3) != 1:
-        raise ValueError("the cache must not be empty, and its channels must be contiguous")
+    if k.numel() == 0 or k.stride(3) != 1 or k.requires_grad or v.requires_grad:
+        raise ValueError("the cache must not be empty nor require gradients, and its channels must be contiguous")
     if k_scale is not None or v_scale is not None:
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
             if t is not None and (dtype != torch.float8_e4m3fn or t.dtype != torch.float32 or t.shape != shape[1:2] or t.get_device() != device or not t.is_contiguous()):
@@ -111,7 +113,7 @@ def append(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, pages: torch.Ten
     nearest of its numbers, beyond the largest that one.
 
     Rows behind ``q_lens[b]`` are not stored, and zeros in the result.  Nor are rows at negative positions, behind the table's end or in pages that do not exist
-    (entries that are negative or not below the cache's pages).  Pages that are written to belong to one sequence."""
+    (entries that are negative or not below the cache's pages).  A page that is written to belongs to one sequence and stands in its table once."""
     _check_rows("append", *((k, v) if q is None else (k, v, q)))
     B, L, H, D = k.shape
     if v.shape != k.shape or (q is not None and (q.shape[:2] != k.shape[:2] or q.shape[3] != D)):
@@ -139,6 +141,8 @@ def append(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, pages: torch.Ten
         rc = _capi.load().ksana_sage_cache_append(call, _cache_call(cache, kind, pages, q_lens, k_lens), _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(out), _stream_ptr(k.device))
     if rc != _capi.OK:
         _capi.check(rc, "cache_ops.append")
+    if not cache.k.is_inference() and not cache.v.is_inference():
+        increment_version((cache.k, cache.v))  # (autograd notices writes to what it has saved)
     return out
 
 

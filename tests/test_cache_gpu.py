@@ -438,6 +438,35 @@ def test_refusals(hip_device):
         cache_ops.attention(q.clone().requires_grad_(), cache, table, [40])
 
 
+def test_a_compiled_function_calls_it(hip_device):
+    """The kernels are no operators of torch: a compiled function leaves its graph for them, in every call."""
+    cache, table, dense = filled([40], 16, 2, 64, BF16, hip_device)
+    f, lens = train_ops.rotary_frequencies(64, device=hip_device), torch.tensor([40], dtype=torch.int32, device=hip_device)
+    q, k = torch.randn(1, 3, 4, 64, device=hip_device).bfloat16(), torch.randn(1, 3, 2, 64, device=hip_device).bfloat16()
+
+    def step(q, k, cache):
+        return cache_ops.attention(cache_ops.append(k, k * 2, cache, table, lens, q=q + 1, frequencies=f), cache, table, lens) * 2
+
+    compiled = torch.compile(step, backend="aot_eager")
+    for i in range(3):
+        assert torch.equal(compiled(q + i, k, cache), step(q + i, k, cache))
+
+
+def test_autograd_notices_writes(hip_device):
+    cache, table, _ = filled([40], 16, 2, 64, BF16, hip_device)
+    k = torch.zeros((1, 1, 2, 64), dtype=BF16, device=hip_device)
+    x = torch.ones_like(cache.k, requires_grad=True)
+    y = (x * cache.k).nan_to_num().sum()
+    cache_ops.append(k, k, cache, table, [40])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        own = cache_ops.allocate(3, 16, 2, 64)
+        cache_ops.append(k, k, own, table, [40])
+    with pytest.raises(ValueError, match="require gradients"):
+        cache_ops.append(k, k, cache._replace(k=cache.k.clone().requires_grad_()), table, [40])
+
+
 def test_nothing_to_do(hip_device):
     cache, table, _ = filled([40], 16, 2, 64, BF16, hip_device)
     for shape in ((1, 0, 4, 64), (1, 3, 0, 64)):

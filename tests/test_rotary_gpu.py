@@ -209,6 +209,26 @@ def test_streams_and_graphs(hip_device):
         assert all(torch.equal(a, b) for a, b in zip(held, step()))
 
 
+def test_what_records_operators_is_refused(hip_device):
+    f = train_ops.rotary_frequencies(64, device=hip_device)
+    x = torch.randn(1, 4, 2, 64, device=hip_device)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        train_ops.rotary(torch.autograd.forward_ad.make_dual(x, x), frequencies=f)
+    with pytest.raises(NotImplementedError, match="traced"):
+        torch.fx.experimental.proxy_tensor.make_fx(lambda x: train_ops.rotary(x, frequencies=f))(x)
+
+
+def test_a_compiled_function_calls_it(hip_device):
+    f = train_ops.rotary_frequencies(64, device=hip_device)
+    x = torch.randn(1, 4, 2, 64, device=hip_device, requires_grad=True)
+    compiled = torch.compile(lambda x: train_ops.rotary(x * 2, frequencies=f) * 2, backend="aot_eager")
+    for _ in range(3):
+        y = compiled(x)
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        z = train_ops.rotary(x * 2, frequencies=f) * 2
+        assert torch.equal(y, z) and torch.equal(dx, torch.autograd.grad(z, x, torch.ones_like(z))[0])
+
+
 def test_nothing_to_turn(hip_device):
     f = train_ops.rotary_frequencies(64, device=hip_device)
     for shape in ((0, 4, 2, 64), (2, 0, 2, 64), (2, 4, 0, 64)):
