@@ -159,7 +159,9 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
     Raw<DT, E> x, y;
   } row[kAhead];
   auto part = [&](int i) -> const RotaryPart& { return i == 0 ? p.part[0] : i == 1 ? p.part[1] : p.part[2]; };
-  auto fetch = [&](int first) {  // (rows behind the counts too: they are there, and zeros or nothing is made of them)
+  // (Rows behind the counts are read as others where L is 1, whatever is made of them: their entry's count would be waited for first.)
+  const bool counted = kCache && p.pages.q_lens != nullptr && p.L > 1;
+  auto fetch = [&](int first) {
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) {
       Row& r = row[n];
@@ -172,7 +174,8 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
       const int b = quotient(token0 + r.t, p.by_length), l = token0 + r.t - b * p.L;
       const RotaryPart& from = part(r.part);
       const char* at = static_cast<const char*>(from.src) + (b * from.sB + l * from.sL + r.head * from.sH) * kWidth<DT>;
-      if (r.is) {
+      r.x = r.y = Raw<DT, E>{};
+      if (r.is && (!counted || l < p.pages.q_lens[b])) {
         r.x.load(at + lo * kWidth<DT>);
         if (has_hi) r.y.load(at + hi * kWidth<DT>);
       }
@@ -316,10 +319,10 @@ hipError_t launch_rotary(RotaryParams p, hipStream_t s) {
   p.slots = 256 / p.units;  // rows at a time
   p.by_heads = divisor(p.heads);
   p.by_length = divisor(p.L);
-  // About five rows to a thread where that leaves four workgroups to each of 256 compute units.  Forward and backward of 32760 tokens, 2 x 40 heads: of two
-  // tokens 501 us, of four 530, of sixteen 598.
+  // About three rows to a thread where that leaves four workgroups to each of 256 compute units.  Forward and backward of 32760 tokens, 2 x 40 heads: of one
+  // token 503 us, of two 508, of four 530, of sixteen 598.
   const int tokens = p.B * p.L;
-  p.tokens_each = std::max(1, std::min({kMostTokens, 5 * p.slots / p.heads, (tokens + 1023) / 1024}));
+  p.tokens_each = std::max(1, std::min({kMostTokens, 3 * p.slots / p.heads, (tokens + 1023) / 1024}));
   const unsigned groups = (unsigned)((tokens + p.tokens_each - 1) / p.tokens_each);
   if (p.dtype == KSANA_SAGE_BF16)
     start_layout<KSANA_SAGE_BF16>(p, layout, groups, s);
