@@ -168,6 +168,29 @@ def test_differences(hip_device):
     assert abs(float(((moved[0] - moved[1]) / 2 * dy.double()).sum() - (dx.double() * d.double()).sum())) < 192 * 25 * 2.0**-22
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_ahead_of_the_training_attention(hip_device, dtype):
+    """A block's way: norm, rotary, attention, back to the leaves.  The gradients are those of the attention's inputs turned back."""
+    g = torch.Generator(device=hip_device).manual_seed(6)
+    B, L, H, Hkv, D, sections = 2, 150, 4, 2, 128, (22, 21, 21)
+    f = train_ops.rotary_frequencies(D, sections=sections, device=hip_device)
+    at = torch.randint(0, 60, (B, L, 3), generator=g, device=hip_device, dtype=torch.int32)
+    x = {n: torch.randn((B, L, h * D), generator=g, device=hip_device).to(DTYPES[dtype]).requires_grad_() for n, h in (("q", H), ("k", Hkv))}
+    v = torch.randn((B, L, Hkv, D), generator=g, device=hip_device).to(DTYPES[dtype])
+    do = torch.randn((B, L, H, D), generator=g, device=hip_device).to(DTYPES[dtype])
+    weight = torch.rand(H * D, generator=g, device=hip_device)
+    q, k = (train_ops.residual_norm(t, norm="rms", weight=weight[: t.shape[2]])[1].unflatten(2, (-1, D)) for t in x.values())
+    qr, kr = train_ops.rotary(q, k, frequencies=f, positions=at, sections=sections)
+    o = train_ops.attention(qr, kr, v)
+    inner = torch.autograd.grad(o, (qr, kr), do, retain_graph=True)
+    outer = torch.autograd.grad(o, (q, k), do, retain_graph=True)
+    for dy, dx in zip(inner, outer):
+        check(dx, dy, f, at, sections, True, sign=-1.0)
+    leaves = torch.autograd.grad(o, tuple(x.values()), do, retain_graph=True)
+    again = torch.autograd.grad((q, k), tuple(x.values()), outer)
+    assert all(torch.equal(a, b) for a, b in zip(leaves, again))
+
+
 def test_hooks_may_lay_saved_tensors_out_anew(hip_device):
     f = train_ops.rotary_frequencies(64, sections=(16, 16), device=hip_device)
     at = torch.randint(0, 99, (2, 5, 4), device=hip_device)[..., ::2]
