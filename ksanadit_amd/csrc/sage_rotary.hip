@@ -322,7 +322,7 @@ hipError_t launch_rotary(RotaryParams p, hipStream_t s) {
   // About three rows to a thread where that leaves four workgroups to each of 256 compute units.  Forward and backward of 32760 tokens, 2 x 40 heads: of one
   // token 503 us, of two 508, of four 530, of sixteen 598.
   const int tokens = p.B * p.L;
-  p.tokens_each = std::max(1, std::min({kMostTokens, 3 * p.slots / p.heads, (tokens + 1023) / 1024}));
+  p.tokens_each = std::max({1, std::min({kMostTokens, 3 * p.slots / p.heads, (tokens + 1023) / 1024}), (tokens + (1 << 23) - 1) >> 23});  // (a launch has fewer than 2^32 threads)
   const unsigned groups = (unsigned)((tokens + p.tokens_each - 1) / p.tokens_each);
   if (p.dtype == KSANA_SAGE_BF16)
     start_layout<KSANA_SAGE_BF16>(p, layout, groups, s);

@@ -293,6 +293,42 @@ def test_append_saturates_and_keeps_not_a_numbers(hip_device):
     assert cache.v[1, 0, 0, 4:6].float().tolist() == [224.0, 0.25]
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_every_code_of_an_8_bit_cache(hip_device, dtype):
+    """Codes are what torch's cast gives, for every 16-bit number there is; values come back as they stand, for every code there is (one key: its weight is 1)."""
+    numbers = torch.arange(-(2**15), 2**15, device=hip_device).short().view(dtype).reshape(1, 256, 2, 128)
+    cache = cache_ops.PagedCache(*pages_of(16, 2, 16, 128, FP8, hip_device, fill=0.0))
+    table = torch.arange(16, dtype=torch.int32, device=hip_device)[None]
+    cache_ops.append(numbers, -numbers, cache, table, [256])
+    for t, x in zip(cache[:2], (numbers, -numbers)):
+        want = x[0].float().clamp(-448, 448).to(FP8).float()
+        got = t.transpose(1, 2).reshape(256, 2, 128).float()
+        assert torch.equal(got.nan_to_num(9.0), want.nan_to_num(9.0)) and torch.equal(got.isnan(), x[0].isnan())
+    codes = torch.arange(256, device=hip_device).to(torch.uint8).reshape(2, 1, 1, 128)
+    v = codes.clone().view(FP8)
+    one = cache_ops.PagedCache(torch.zeros_like(codes).view(FP8), v, None, torch.tensor([0.5], device=hip_device))
+    for L in (1, 40):
+        o = cache_ops.attention(torch.ones((2, L, 1, 128), dtype=dtype, device=hip_device), one, torch.tensor([[0], [1]], dtype=torch.int32, device=hip_device), [1, 1], is_causal=False)
+        want = (v.float().reshape(2, 1, 1, 128) * 0.5).expand(2, L, 1, 128)
+        assert torch.equal(o.float().nan_to_num(9.0), want.nan_to_num(9.0)) and torch.equal(o.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("L", [1, 40])
+@pytest.mark.parametrize("kind", [BF16, FP8])
+def test_keys_of_many_sizes(hip_device, L, kind):
+    """A query picks one channel of every key: small and subnormal codes, and large ones, come into the scores as they are."""
+    n = 127
+    k = torch.zeros((n, 1, 1, 64), dtype=torch.uint8, device=hip_device)
+    k[:, 0, 0, 3] = torch.arange(n, device=hip_device).to(torch.uint8)
+    k = k.view(FP8)
+    cache = cache_ops.PagedCache(*(t.to(kind) if kind != FP8 else t for t in (k, torch.randn((n, 1, 1, 64), device=hip_device).clamp(-4, 4).to(FP8))))
+    q = torch.zeros((1, L, 1, 64), dtype=BF16, device=hip_device)
+    q[..., 3] = torch.linspace(-0.25, 0.25, L, device=hip_device)[None, :, None] if L > 1 else 0.125
+    table = torch.arange(n, dtype=torch.int32, device=hip_device)[None]
+    dense = [[t.float().double().reshape(n, 1, 64) for t in cache[:2]]]
+    check_attention(cache_ops.attention(q, cache, table, [n], is_causal=False, sm_scale=1.0), q, dense, [L], False, 1.0)
+
+
 def test_append_stores_nothing_where_there_is_no_page(hip_device):
     cache = cache_ops.PagedCache(*pages_of(3, 1, 4, 64, BF16, hip_device, fill=7.0))
     k = torch.ones((4, 6, 1, 64), dtype=BF16, device=hip_device)
