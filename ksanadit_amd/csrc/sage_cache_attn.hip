@@ -218,6 +218,10 @@ __device__ __forceinline__ float hide_scores(v16f (&s)[2], int limit, uint64_t e
   return most;
 }
 
+// Many rows: four waves of 32 share a tile's copies, two workgroups to a compute unit, so that each SIMD has two waves.  While the probabilities of tile t are formed and
+// multiplied with its values, the scores of tile t + 1 are: a few vector instructions stand behind every matrix instruction and run beside it.  So values are
+// wanted a step after their keys; each have two places in LDS.  Of 128 channels about 20 registers go through memory, outside the loop.
+// 4096 causal rows on 32768 keys, 40 heads on 8: bf16 2330 us, fp16 2480, 8 bits 2500; of 64 channels, 32 heads on 8, 1190, where exponentials count twice as much.
 template <int DT, int D, bool kEight>
 __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttnParams p) {
   using T = Tile<D>;

@@ -24,9 +24,12 @@ from . import _capi
 from .sage_ops import _DTYPES, _k_lens_arg, _require_hip, _stream_ptr, _usable
 
 
+_HERE = nullcontext()
+
+
 def _on(device: torch.device):
-    """The device made current where it is not: kernels start on the current one."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    """The device made current where it is not: kernels start on the current one.  (Asked for without the detour through torch.cuda, which costs autograd's thread 4 us.)"""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _refuse_unseen(name: str, *tensors: torch.Tensor | None) -> None:
@@ -503,8 +506,9 @@ class _Rotary(torch.autograd.Function):
         if positions is not None:
             positions = _kept(positions, *ctx.was[1], device)
         checked, interleaved, magnitude, inverse = ctx.options
-        out = _Rotary.apply(given[0], given[1] if len(given) > 1 else None, frequencies, positions, checked, interleaved, magnitude, not inverse)
-        out = iter(out if len(given) > 1 else (out,))
+        turn = _Rotary.apply if torch.is_grad_enabled() else _turn
+        out = turn(given[0], given[1] if len(given) > 1 else None, frequencies, positions, checked, interleaved, magnitude, not inverse)
+        out = iter(out if isinstance(out, tuple) else (out,))
         return (next(out) if want_q and dq is not None else None, next(out) if want_k and dk is not None else None, *(None,) * 6)
 
 
