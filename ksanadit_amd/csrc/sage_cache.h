@@ -54,7 +54,7 @@ struct RotaryParams {
   int inverse;
   PageTable pages;            // table nullptr: no cache
   // filled in by the launcher
-  int heads, units, slots, tokens_each;
+  int heads, units, slots, tokens_each, stream;
   Divisor by_heads, by_length;
 };
 hipError_t launch_rotary(RotaryParams p, hipStream_t s);

@@ -5,8 +5,11 @@
 // for the pairs (a, b) of a row's first R channels: channels 2 i and 2 i + 1, or i and i + R / 2.  The others are copied.  Backward: t negated.
 //
 // The angle is formed in turns in 64 bits - fp32 would be off by 2^-24 of it, 0.06 radians at a position of 10^6 - and what is left of it after its
-// quarter turns are taken off goes on in 32.  Bound by the rows' bytes: a thread keeps the cosines and sines of sixteen channels of a token and takes its
-// heads' rows through one after the other.
+// quarter turns are taken off goes on in 32.
+//
+// Bound by the rows' bytes: a workgroup forms its tokens' cosines and sines once, into LDS, and takes the rows of all heads through, the first ones asked for before.
+// 32760 tokens, 2 x 40 heads of 128 channels, bf16: 230 us a direction from memory, 5.8 TB/s; of 64 channels 138, 4.9 TB/s; prompts of 16384 and 9011 tokens into
+// pages, 32 + 8 + 8 heads: 149 us, 4.6 TB/s.  Few tokens are a chain of latencies: 5 us.
 #include "sage_cache.h"
 #include "sage_device.h"
 #include "sage_train.h"
@@ -17,7 +20,9 @@ namespace ksana_sage {
 
 namespace {
 
-enum Layout { kInterleaved, kHalves, kSingle };  // eight channels at an access, or (either order of pairs) one
+enum Layout { kInterleaved, kHalves, kSingle };  // 16 bytes at an access, or (either order of pairs) one value
+template <int DT, Layout kLayout>
+constexpr int kAtOnce = kLayout == kSingle ? 1 : DT == kFp32 ? 4 : 8;
 
 // cos and sin of x / 4 turns for |x| <= 1 / 2, by their series: the first terms left out are below 2e-9 and 2e-10 there
 __device__ __forceinline__ void quarter_turn(float x, float& c, float& s) {
@@ -42,24 +47,22 @@ constexpr int kWidth = DT == kFp32 ? 4 : 2;
 // E values as they lie in memory (16-byte accesses at any address)
 template <int DT, int E>
 struct Raw {
-  uint4 w[DT == kFp32 ? 2 : 1];
+  uint4 w;
   __device__ __forceinline__ void load(const char* p) {
-    if constexpr (E == 1) {
-      w[0].x = DT == kFp32 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
-    } else {
-      __builtin_memcpy(&w[0], p, 16);
-      if constexpr (DT == kFp32) __builtin_memcpy(&w[1], p + 16, 16);
-    }
+    if constexpr (E == 1)
+      w.x = DT == kFp32 ? *reinterpret_cast<const uint32_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
+    else
+      __builtin_memcpy(&w, p, 16);
   }
   __device__ __forceinline__ void values(float (&x)[E]) const {
     if constexpr (E == 1) {
-      if constexpr (DT == kFp32) x[0] = __uint_as_float(w[0].x);
-      if constexpr (DT == KSANA_SAGE_BF16) x[0] = __uint_as_float(w[0].x << 16);
-      if constexpr (DT == KSANA_SAGE_FP16) x[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[0].x);
+      if constexpr (DT == kFp32) x[0] = __uint_as_float(w.x);
+      if constexpr (DT == KSANA_SAGE_BF16) x[0] = __uint_as_float(w.x << 16);
+      if constexpr (DT == KSANA_SAGE_FP16) x[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)w.x);
     } else if constexpr (DT == kFp32) {
-      __builtin_memcpy(x, w, 32);
+      __builtin_memcpy(x, &w, 16);
     } else {
-      widen8<DT>(w[0], x);
+      widen8<DT>(w, x);
     }
   }
 };
@@ -69,7 +72,7 @@ __device__ __forceinline__ float within_e4m3(float x) {
   return x < -448.0f ? -448.0f : x;
 }
 template <int DT, int E, bool kEight>
-__device__ __forceinline__ void store_values(void* row, int64_t at, const float (&x)[E], float inv) {
+__device__ __forceinline__ void store_values(void* row, int64_t at, const float (&x)[E], float inv, int stream) {
   if constexpr (kEight) {
     float y[E];
 #pragma unroll
@@ -86,15 +89,13 @@ __device__ __forceinline__ void store_values(void* row, int64_t at, const float 
     if constexpr (DT == kFp32) static_cast<float*>(row)[at] = x[0];
     if constexpr (DT == KSANA_SAGE_BF16) static_cast<__bf16*>(row)[at] = (__bf16)x[0];
     if constexpr (DT == KSANA_SAGE_FP16) static_cast<_Float16*>(row)[at] = (_Float16)x[0];
-  } else if constexpr (DT == kFp32) {
-    float4* p = reinterpret_cast<float4*>(static_cast<float*>(row) + at);
-    p[0] = make_float4(x[0], x[1], x[2], x[3]);
-    p[1] = make_float4(x[4], x[5], x[6], x[7]);
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == KSANA_SAGE_BF16) {
+      if constexpr (DT == kFp32) {
+        w[i] = __float_as_uint(x[i]);
+      } else if constexpr (DT == KSANA_SAGE_BF16) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         w[i] = __builtin_bit_cast(uint32_t, (b2){(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
       } else {
@@ -102,9 +103,15 @@ __device__ __forceinline__ void store_values(void* row, int64_t at, const float 
         w[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
       }
     }
-    // (first out of the caches, as what has been read: rotary step of 32760 tokens, 2 x 40 heads, 265 us, kept like others 271)
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    __builtin_nontemporal_store(u4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u4*>(static_cast<uint16_t*>(row) + at));
+    u4* to = reinterpret_cast<u4*>(static_cast<char*>(row) + at * kWidth<DT>);
+    if (DT != kFp32 && stream) {
+      asm volatile("" ::: "memory");  // (the two are made one otherwise, before or behind the branch, and that is not the first)
+      __builtin_nontemporal_store(u4{w[0], w[1], w[2], w[3]}, to);
+      asm volatile("" ::: "memory");
+    } else {
+      *to = u4{w[0], w[1], w[2], w[3]};
+    }
   }
 }
 
@@ -116,11 +123,12 @@ struct Token {
 constexpr int kMostTokens = 16;
 
 // A workgroup takes a few tokens: first its threads form a cosine and a sine each, of a pair of a token, then all rows go through, a thread with E channels at `lo`
-// and E at `hi` of every one.  (Every thread forming what it needs itself, eight pairs for three rows: 360 us
-// of 32760 tokens, 2 x 40 heads, where this takes 250.)
+// and E at `hi` of every one, neighbours beside each other.  (Every thread forming what it needs itself, eight pairs for three rows: 360 us
+// of 32760 tokens, 2 x 40 heads, where this takes 230.)  Seven waves to a SIMD: with six the 1560 workgroups of a frame in 8 bits take a round more, 29.4 us for 27.4, and
+// the 32760 tokens 237.
 template <int DT, Layout kLayout, bool kCache, bool kEight>
-__global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) {
-  constexpr int E = kLayout == kSingle ? 1 : 8, kAhead = 2;
+__global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams p) {
+  constexpr int E = kAtOnce<DT, kLayout>, kAhead = 2;
   extern __shared__ __align__(16) float2 turns[];  // [tokens][R / 2]: cosine and sine
   __shared__ Token token_of[kMostTokens];
   const int pairs = p.R / 2, all = p.B * p.L, token0 = (int)blockIdx.x * p.tokens_each, tokens = min(p.tokens_each, all - token0), rows = tokens * p.heads;
@@ -129,8 +137,8 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
   int lo, hi, pair_lo, pair_hi;
   bool turn_lo, turn_hi;
   if constexpr (kLayout == kInterleaved) {
-    lo = 8 * unit;
-    hi = 8 * (unit + p.units);
+    lo = E * unit;
+    hi = E * (unit + p.units);
     turn_lo = lo < p.R;
     turn_hi = hi < p.R;
     pair_lo = lo / 2;
@@ -147,8 +155,8 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
       lo = E * unit;
       hi = lo + p.R / 2;
     } else {
-      lo = p.R + 2 * E * rest;
-      hi = lo + E;
+      lo = p.R + E * rest;
+      hi = lo + E * (p.units - turned);
     }
   }
   const bool has_hi = hi < p.D;
@@ -248,7 +256,7 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
         const float2* own = turns + r.t * pairs;
         if constexpr (kLayout == kInterleaved) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < E / 2; ++e) {
             if (turn_lo) {
               const float2 z = own[pair_lo + e];
               const float a = x[2 * e];
@@ -276,12 +284,12 @@ __global__ __launch_bounds__(256) void sage_rotary_kernel(const RotaryParams p) 
         constexpr int kSize = kEight ? 1 : kWidth<DT>;
         char* at = static_cast<char*>(to.dst) + (token.page * to.dB + token.slot * to.dL + r.head * to.dH) * kSize;
         const float inv = kEight && to.scale != nullptr ? 1.0f / to.scale[r.head] : 1.0f;
-        store_values<DT, E, kEight>(at, lo, x, inv);
-        if (has_hi) store_values<DT, E, kEight>(at, hi, y, inv);
+        store_values<DT, E, kEight>(at, lo, x, inv, p.stream);
+        if (has_hi) store_values<DT, E, kEight>(at, hi, y, inv, p.stream);
       } else {
         char* at = static_cast<char*>(to.dst) + ((int64_t)(token0 + r.t) * to.H + r.head) * p.D * kWidth<DT>;
-        store_values<DT, E, false>(at, lo, x, 1.0f);
-        if (has_hi) store_values<DT, E, false>(at, hi, y, 1.0f);
+        store_values<DT, E, false>(at, lo, x, 1.0f, p.stream);
+        if (has_hi) store_values<DT, E, false>(at, hi, y, 1.0f, p.stream);
       }
     }
   }
@@ -313,9 +321,16 @@ void start_layout(const RotaryParams& p, Layout layout, unsigned groups, hipStre
 
 hipError_t launch_rotary(RotaryParams p, hipStream_t s) {
   Layout layout = kSingle;
-  if (p.D % 8 == 0 && p.R % (p.interleaved ? 8 : 16) == 0) layout = p.interleaved ? kInterleaved : kHalves;
+  const int at_once = p.dtype == kFp32 ? 4 : 8;
+  if (p.D % at_once == 0 && p.R % (p.interleaved ? at_once : 2 * at_once) == 0) layout = p.interleaved ? kInterleaved : kHalves;
   p.heads = p.part[0].H + p.part[1].H + p.part[2].H;
-  p.units = layout == kInterleaved ? (p.D / 8 + 1) / 2 : layout == kHalves ? p.R / 16 + (p.D - p.R + 15) / 16 : p.R / 2 + (p.D - p.R + 1) / 2;
+  p.units = layout == kInterleaved ? (p.D / at_once + 1) / 2
+            : layout == kHalves    ? p.R / (2 * at_once) + (p.D - p.R + 2 * at_once - 1) / (2 * at_once)
+                                   : p.R / 2 + (p.D - p.R + 1) / 2;
+  // 16-bit results go first out of the caches, as what has been read, where an access of neighbours fills whole lines.  32760 tokens, 2 x 40 heads of 128: 244 us, kept
+  // like others 256; of 80 channels, 32 of them turned, 221 and 177.
+  const int piece = layout == kInterleaved ? p.units * 16 : p.R;
+  p.stream = layout != kSingle && p.dtype != kFp32 && piece % 128 == 0 && (layout == kInterleaved ? p.D == 16 * p.units : p.R == p.D);
   p.slots = 256 / p.units;  // rows at a time
   p.by_heads = divisor(p.heads);
   p.by_length = divisor(p.L);
