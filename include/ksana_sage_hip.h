@@ -559,7 +559,7 @@ int ksana_sage_cache_append(const ksana_sage_rotary* call, const ksana_sage_cach
                             void* q_out, void* stream);
 
 /* o = softmax(sm_scale q k^T) v of the last q_lens[b] tokens of every sequence on all its k_lens[b] keys; causal: on those up to
- * their own position.  16-bit products accumulated in fp32, softmax statistics in fp32, probabilities rounded to q's type.  Rows behind the
+ * their own position.  16-bit products accumulated in fp32, softmax statistics in fp32, probabilities rounded to q's type (few rows, 16-bit caches: in two parts).  Rows behind the
  * counts, and rows that see no key, are zeros.  D = 128 or 64, Hq a multiple of Hkv.  Repeated calls give the same bits. */
 typedef struct ksana_sage_cache_attn {
   int32_t B, Hq, Hkv, Lq, D;

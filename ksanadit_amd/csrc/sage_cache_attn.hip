@@ -5,7 +5,8 @@
 // place, and their weight is zero.
 //
 // A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys with a running maximum and sum.  Probabilities are rounded to the
-// tensors' type where they are multiplied with the values, as the matrix instructions want them (off by 2^-8 or 2^-11 of each at most), and everything else is fp32.
+// tensors' type where they are multiplied with the values, as the matrix instructions want them (off by 2^-8 or 2^-11 of each at most; few rows on 16-bit caches: twice, off
+// by 2^-16 or 2^-22), and everything else is fp32.
 // A tile's pages are looked up by its 64 keys' lanes ahead of its copies.  Of 8-bit caches the tiles are widened, exactly, on their way to LDS; the scales go into c and into
 // the result.  Loops of few blocks are cut into runs, which a second launch joins: a block's runs share the tiles that its sequence really has.
 //
@@ -558,7 +559,11 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
 #pragma unroll
           for (int j = 0; j < 16; ++j) acc[d][j] *= factor;
       }
-      v4i pr[4];
+      // Probabilities in two parts of 16 bits, the second what rounding takes off the first: the matrix pipes have the time while memory is waited for (64 sequences of up to
+      // 8192 tokens 233.3 -> 233.9 us, one token on 32760 keys 35.1 -> 35.5), and the result's error is that of its own rounding (0.0016 for 0.0023).  Of 8 bits, where half as
+      // many bytes are waited for, it costs 2 to 5 %, and the cache's own rounding is far larger: one part.
+      constexpr int kParts = kEight ? 1 : 2;
+      v4i pr[kParts][4];
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
         float x[8];
@@ -567,7 +572,12 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
           x[j] = fast_exp2(__fmaf_rn(s[f / 2][8 * (f % 2) + j], scale, minus));
           sum += x[j];
         }
-        pr[f] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+        pr[0][f] = pack8<DT>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+        if constexpr (kParts == 2) {
+          float y[8];
+          widen8<DT>(make_uint4((unsigned)pr[0][f][0], (unsigned)pr[0][f][1], (unsigned)pr[0][f][2], (unsigned)pr[0][f][3]), y);
+          pr[1][f] = pack8<DT>(x[0] - y[0], x[1] - y[1], x[2] - y[2], x[3] - y[3], x[4] - y[4], x[5] - y[5], x[6] - y[6], x[7] - y[7]);
+        }
       }
       if constexpr (last.value)
         copies_there<0>();
@@ -579,8 +589,11 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
       }
       reads_done();
 #pragma unroll
-      for (int j = 0; j < 4 * T::kBlocks; ++j)
-        acc[j % T::kBlocks] = mfma16<DT>(read_column<D>(column_at, j % T::kBlocks, j / T::kBlocks), pr[j / T::kBlocks], acc[j % T::kBlocks]);
+      for (int j = 0; j < 4 * T::kBlocks; ++j) {
+        const v4i v = read_column<D>(column_at, j % T::kBlocks, j / T::kBlocks);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) acc[j % T::kBlocks] = mfma16<DT>(v, pr[part][j / T::kBlocks], acc[j % T::kBlocks]);
+      }
       if constexpr (!last.value) {
         reads_done();
         if constexpr (!kEight) copy_values(next64);

@@ -66,9 +66,9 @@ def filled(lens, page, heads, D, dtype, device, layout="heads first", seed=0, sc
     return cache_ops.PagedCache(k, v, *(scales or (None, None))), table, dense
 
 
-def check_attention(o, q, dense, new, causal, sm_scale=None, hidden=None):
+def check_attention(o, q, dense, new, causal, sm_scale=None, hidden=None, parts=1):
     """Against the definition; off by
-    - half a step of q's type of every weight where it is multiplied on, and of the result;
+    - half a step of q's type of every weight where it is multiplied on (its square where that is done in two parts), and of the result;
     - fp32's: a score of D products and sums, by its terms' sizes (D + 8) 2^-24, counted twice in the normalised weight, and 2^-20 for exponentials, sums and factors;
     - in fp16, weights that are subnormal: 2^-31 of the row's largest each."""
     B, L, H, D = q.shape
@@ -96,7 +96,7 @@ def check_attention(o, q, dense, new, causal, sm_scale=None, hidden=None):
         ds = size.masked_fill(~seen, 0.0).amax(-1, keepdim=True) * (D + 8) * 2.0**-24 if n else torch.zeros((H, m, 1), device=q.device)
         weighed = w @ v.abs()
         largest = v.abs().amax(1, keepdim=True) if n else torch.zeros_like(want)
-        bound = (half + 2 * ds + 2.0**-20) * weighed + half * want.abs() + n * 2.0**-31 * largest * (q.dtype == FP16) + torch.finfo(q.dtype).smallest_normal * half * 2
+        bound = (half**parts + 2 * ds + 2.0**-20) * weighed + half * want.abs() + n * 2.0**-31 * largest * (q.dtype == FP16) + torch.finfo(q.dtype).smallest_normal * half * 2
         off = (o[b, :m].double().transpose(0, 1) - want).abs()
         worst = max(worst, float((off / bound).max()))
         assert bool((off <= bound).all()), (b, float((off / bound).max()), off.isnan().sum())
@@ -144,6 +144,14 @@ def test_attention(hip_device, lens, new, H, Hkv, D, page, causal, dtype, kind, 
     assert torch.equal(o, cache_ops.attention(q, cache, table, lens, new, is_causal=causal))
     if L == new[0] and len(lens) == 1:
         assert torch.equal(o, cache_ops.attention(q, cache, table, counts[0], is_causal=causal))
+
+
+@pytest.mark.parametrize("lens,new,H,Hkv,D,page,dtype", [([5000, 77], [1, 1], 40, 8, 128, 16, BF16), ([700, 3, 0], [4, 3, 0], 8, 1, 64, 64, FP16), ([129], [32], 2, 2, 128, 20, BF16)])
+def test_few_rows_are_rounded_once(hip_device, lens, new, H, Hkv, D, page, dtype):
+    """On 16-bit caches: their probabilities are multiplied on in two parts."""
+    cache, table, dense = filled(lens, page, Hkv, D, dtype, hip_device)
+    q = torch.randn((len(lens), max(new), H, D), generator=torch.Generator().manual_seed(2)).to(hip_device, dtype)
+    check_attention(cache_ops.attention(q, cache, table, lens, new), q, dense, new, True, parts=2)
 
 
 @pytest.mark.parametrize("sm_scale", [0.0, -0.3, 3.0])
