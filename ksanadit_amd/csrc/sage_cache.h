@@ -39,12 +39,12 @@ struct RotaryPart {
   const void* src;
   int64_t sB, sL, sH;  // in elements
   void* dst;
-  int64_t dB, dL, dH;  // of pages: page, slot and head, in elements (other rows are contiguous)
+  int64_t dB, dL, dH;  // of pages: page, slot and head, in elements, the same of keys and values (other rows are contiguous)
   const float* scale;  // of 8-bit pages: one per head, or nullptr
-  int H, turn, paged;
+  int H;
 };
 struct RotaryParams {
-  RotaryPart part[3];  // those without heads take no part
+  RotaryPart part[3];  // q and k, which turn, and a cache's values; with a cache keys and values go into pages.  Those without heads take no part
   int B, L, D, R, dtype, interleaved, eight_bits;
   const double* frequencies;  // R / 2 radians per position
   const void* positions;      // nullptr: of the token itself

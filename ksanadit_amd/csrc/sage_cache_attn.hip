@@ -203,9 +203,10 @@ __device__ __forceinline__ void row_ready(v4i (&row)[N]) {
 __device__ __forceinline__ constexpr int acc_row(int i) { return 8 * (i >> 2) + (i & 3); }
 
 // Scores of keys that the lane's row does not see: `limit` of the tile's, and those of no page.  The largest of the others.
-__device__ __forceinline__ float hide_scores(v16f (&s)[2], int limit, uint64_t exist, int hh) {
+__device__ __forceinline__ float hide_scores(v16f (&s)[2], int limit, uint64_t exist) {
   const int left = max(limit, 0);
-  const uint64_t seen = (left < kTrainTile ? exist & ((UINT64_C(1) << left) - 1) : exist) >> (4 * hh);
+  const uint64_t of_tile = left < kTrainTile ? exist & ((UINT64_C(1) << left) - 1) : exist;
+  const uint64_t seen = __builtin_amdgcn_inverse_ballot_w64(UINT64_C(0xffffffff) << 32) ? of_tile >> 4 : of_tile;  // (by hh, which would be kept through the loop for it)
   uint32_t bits[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
   pin(bits[0]);  // (a branch that stays one: 64 instructions for every tile otherwise)
   pin(bits[1]);
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
     float most = -INFINITY;
     auto hide = [&](int t, uint64_t exist, v16f (&s)[2]) {
       if ((t + 1) * kTrainTile <= all_see && exist == ~UINT64_C(0)) return;
-      most = hide_scores(s, limit - t * kTrainTile, exist, hh);
+      most = hide_scores(s, limit - t * kTrainTile, exist);
     };
     // Tile t: its scores in s, the largest of the lane's in `most`; forms the scores of tile t + 1 in `next` unless `last`.  Its weights are added up by themselves, then to the
     // row's sum: added to that one by one, equal weights are all rounded the same way, 0.34 % of it after 524288 keys.  (Products take 16 keys at an addition.)
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
       pin(v_at);
       v4i pr[4];
       {
-        constexpr int kParts = 2 * T::kSteps, kEach = 32 / kParts, kAhead = 3;
+        constexpr int kParts = 2 * T::kSteps, kEach = 32 / kParts, kAhead = kEight ? 2 : 3;  // (8 bits: with three a register of q is read from memory in every step)
         v4i a[kAhead];
         if constexpr (!last.value) {
 #pragma unroll
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
 #pragma unroll
         for (int j = 0; j < 16; ++j) most = largest(most, s[0][j], s[1][j]);
       } else {
-        most = hide_scores(s, limit - first, here64.exist, hh);
+        most = hide_scores(s, limit - first, here64.exist);
       }
       const float here = over_halves<Max>(most);
       if (__any(here * scale > kLazy + kShift<DT> - minus || (top == -INFINITY && here > -INFINITY))) {

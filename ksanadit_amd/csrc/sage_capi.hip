@@ -1317,7 +1317,7 @@ int rotary_params(const ksana_sage_rotary* c, ksana_sage::RotaryParams* p) {
   p->magnitude = c->magnitude;
   return 0;
 }
-int rotary_part(const char* name, const ksana_sage::RotaryParams& p, const void* src, const int64_t st[4], int H, int turn, ksana_sage::RotaryPart* out) {
+int rotary_part(const char* name, const ksana_sage::RotaryParams& p, const void* src, const int64_t st[4], int H, ksana_sage::RotaryPart* out) {
   if (!src) return fail(KSANA_SAGE_EINVAL, "%s is null", name);
   if (reinterpret_cast<uintptr_t>(src) % size_of(p.dtype)) return fail(KSANA_SAGE_EINVAL, "%s: pointer not aligned to its values", name);
   if (p.D > 1 && st[3] != 1) return fail(KSANA_SAGE_EINVAL, "%s: D stride is %lld, must be 1", name, (long long)st[3]);
@@ -1328,7 +1328,6 @@ int rotary_part(const char* name, const ksana_sage::RotaryParams& p, const void*
   out->sL = st[1];
   out->sH = st[2];
   out->H = H;
-  out->turn = turn;
   return 0;
 }
 // .. and where its rows go, contiguous
@@ -1405,11 +1404,11 @@ extern "C" int ksana_sage_rotary_rows(const ksana_sage_rotary* call, const void*
   ksana_sage::RotaryParams p;
   if (int rc = rotary_params(call, &p)) return rc;
   if (call->Hq > 0) {
-    if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, 1, &p.part[0])) return rc;
+    if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, &p.part[0])) return rc;
     if (int rc = rotary_rows_out("q_out", q_out, &p.part[0])) return rc;
   }
   if (call->Hkv > 0) {
-    if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, 1, &p.part[1])) return rc;
+    if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, &p.part[1])) return rc;
     if (int rc = rotary_rows_out("k_out", k_out, &p.part[1])) return rc;
   }
   const StageRange range("ksana_sage.rotary_rows");
@@ -1426,14 +1425,13 @@ extern "C" int ksana_sage_cache_append(const ksana_sage_rotary* call, const ksan
   if (int rc = cache_pages(cache, call->dtype, call->Hkv, call->D, call->B, &p.pages)) return rc;
   p.eight_bits = cache->dtype == KSANA_SAGE_E4M3;
   if (call->Hq > 0) {
-    if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, 1, &p.part[0])) return rc;
+    if (int rc = rotary_part("q", p, q, call->q_strides, call->Hq, &p.part[0])) return rc;
     if (int rc = rotary_rows_out("q_out", q_out, &p.part[0])) return rc;
   }
-  if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, 1, &p.part[1])) return rc;
-  if (int rc = rotary_part("v", p, v, call->v_strides, call->Hkv, 0, &p.part[2])) return rc;
+  if (int rc = rotary_part("k", p, k, call->k_strides, call->Hkv, &p.part[1])) return rc;
+  if (int rc = rotary_part("v", p, v, call->v_strides, call->Hkv, &p.part[2])) return rc;
   for (int i = 1; i < 3; ++i) {
     ksana_sage::RotaryPart& part = p.part[i];
-    part.paged = 1;
     part.dst = i == 1 ? cache->k : cache->v;
     part.scale = i == 1 ? cache->k_scale : cache->v_scale;
     part.dB = cache->strides[0];

@@ -72,23 +72,23 @@ __device__ __forceinline__ float within_e4m3(float x) {
   return x < -448.0f ? -448.0f : x;
 }
 template <int DT, int E, bool kEight>
-__device__ __forceinline__ void store_values(void* row, int64_t at, const float (&x)[E], float inv, int stream) {
+__device__ __forceinline__ void store_values(void* at, const float (&x)[E], float inv, int stream) {
   if constexpr (kEight) {
     float y[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] = within_e4m3(x[e] * inv);
     if constexpr (E == 1) {
-      static_cast<uint8_t*>(row)[at] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[0], 0, false);
+      *static_cast<uint8_t*>(at) = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[0], 0, false);
     } else {
       uint2 w;
       w.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
       w.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false), true);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(row) + at) = w;
+      *static_cast<uint2*>(at) = w;
     }
   } else if constexpr (E == 1) {
-    if constexpr (DT == kFp32) static_cast<float*>(row)[at] = x[0];
-    if constexpr (DT == KSANA_SAGE_BF16) static_cast<__bf16*>(row)[at] = (__bf16)x[0];
-    if constexpr (DT == KSANA_SAGE_FP16) static_cast<_Float16*>(row)[at] = (_Float16)x[0];
+    if constexpr (DT == kFp32) *static_cast<float*>(at) = x[0];
+    if constexpr (DT == KSANA_SAGE_BF16) *static_cast<__bf16*>(at) = (__bf16)x[0];
+    if constexpr (DT == KSANA_SAGE_FP16) *static_cast<_Float16*>(at) = (_Float16)x[0];
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -104,7 +104,7 @@ __device__ __forceinline__ void store_values(void* row, int64_t at, const float 
       }
     }
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    u4* to = reinterpret_cast<u4*>(static_cast<char*>(row) + at * kWidth<DT>);
+    u4* to = static_cast<u4*>(at);
     if (DT != kFp32 && stream) {
       asm volatile("" ::: "memory");  // (the two are made one otherwise, before or behind the branch, and that is not the first)
       __builtin_nontemporal_store(u4{w[0], w[1], w[2], w[3]}, to);
@@ -160,13 +160,15 @@ __global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams 
     }
   }
   const bool has_hi = hi < p.D;
+  const int apart = kLayout == kInterleaved ? E * p.units : hi - lo;
 
   struct Row {
     int t, part, head;
     bool is;
     Raw<DT, E> x, y;
   } row[kAhead];
-  auto part = [&](int i) -> const RotaryPart& { return i == 0 ? p.part[0] : i == 1 ? p.part[1] : p.part[2]; };
+  // A field of a row's part, by value: a reference that differs from lane to lane is read from memory, field by field, into registers that the rows need.
+  auto of = [&](int part, auto q, auto k, auto v) { return kCache && part == 2 ? v : part == 1 ? k : q; };
   // (Rows behind the counts are read as others where L is 1, whatever is made of them: their entry's count would be waited for first.)
   const bool counted = kCache && p.pages.q_lens != nullptr && p.L > 1;
   auto fetch = [&](int first) {
@@ -180,12 +182,13 @@ __global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams 
       r.part = r.head < p.part[0].H ? 0 : r.head < p.part[0].H + p.part[1].H ? 1 : 2;
       r.head -= r.part == 0 ? 0 : r.part == 1 ? p.part[0].H : p.part[0].H + p.part[1].H;
       const int b = quotient(token0 + r.t, p.by_length), l = token0 + r.t - b * p.L;
-      const RotaryPart& from = part(r.part);
-      const char* at = static_cast<const char*>(from.src) + (b * from.sB + l * from.sL + r.head * from.sH) * kWidth<DT>;
+      const RotaryPart *q = p.part, *k = p.part + 1, *v = p.part + 2;
+      const char* at = static_cast<const char*>(of(r.part, q->src, k->src, v->src)) +
+                       (b * of(r.part, q->sB, k->sB, v->sB) + l * of(r.part, q->sL, k->sL, v->sL) + r.head * of(r.part, q->sH, k->sH, v->sH) + lo) * kWidth<DT>;
       r.x = r.y = Raw<DT, E>{};
       if (r.is && (!counted || l < p.pages.q_lens[b])) {
-        r.x.load(at + lo * kWidth<DT>);
-        if (has_hi) r.y.load(at + hi * kWidth<DT>);
+        r.x.load(at);
+        if (has_hi) r.y.load(at + apart * kWidth<DT>);
       }
     }
   };
@@ -241,10 +244,10 @@ __global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams 
     for (int n = 0; n < kAhead; ++n) {
       const Row& r = row[n];
       if (!r.is) continue;
-      const RotaryPart& to = part(r.part);
+      const bool paged = kCache && r.part > 0;
       Token token{1, 0, 0};
       if constexpr (kCache) token = token_of[r.t];
-      if (kCache && to.paged && token.page < 0) continue;
+      if (paged && token.page < 0) continue;
       float x[E], y[E];
       r.x.values(x);
       r.y.values(y);
@@ -252,7 +255,7 @@ __global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams 
 #pragma unroll
         for (int e = 0; e < E; ++e) x[e] = y[e] = 0.0f;
       }
-      if (to.turn) {
+      if (!kCache || r.part < 2) {
         const float2* own = turns + r.t * pairs;
         if constexpr (kLayout == kInterleaved) {
 #pragma unroll
@@ -280,16 +283,20 @@ __global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams 
           }
         }
       }
-      if (kCache && to.paged) {
+      if (paged) {
         constexpr int kSize = kEight ? 1 : kWidth<DT>;
-        char* at = static_cast<char*>(to.dst) + (token.page * to.dB + token.slot * to.dL + r.head * to.dH) * kSize;
-        const float inv = kEight && to.scale != nullptr ? 1.0f / to.scale[r.head] : 1.0f;
-        store_values<DT, E, kEight>(at, lo, x, inv, p.stream);
-        if (has_hi) store_values<DT, E, kEight>(at, hi, y, inv, p.stream);
+        const RotaryPart &k = p.part[1], &v = p.part[2];  // (laid out alike)
+        char* at = static_cast<char*>(r.part == 1 ? k.dst : v.dst) + (token.page * k.dB + token.slot * k.dL + r.head * k.dH + lo) * kSize;
+        const float* scales = r.part == 1 ? k.scale : v.scale;
+        const float inv = kEight && scales != nullptr ? 1.0f / scales[r.head] : 1.0f;
+        store_values<DT, E, kEight>(at, x, inv, p.stream);
+        if (has_hi) store_values<DT, E, kEight>(at + apart * kSize, y, inv, p.stream);
       } else {
-        char* at = static_cast<char*>(to.dst) + ((int64_t)(token0 + r.t) * to.H + r.head) * p.D * kWidth<DT>;
-        store_values<DT, E, false>(at, lo, x, 1.0f, p.stream);
-        if (has_hi) store_values<DT, E, false>(at, hi, y, 1.0f, p.stream);
+        const RotaryPart &q = p.part[0], &k = p.part[1];
+        const bool second = !kCache && r.part == 1;
+        char* at = static_cast<char*>(second ? k.dst : q.dst) + (((int64_t)(token0 + r.t) * (second ? k.H : q.H) + r.head) * p.D + lo) * kWidth<DT>;
+        store_values<DT, E, false>(at, x, 1.0f, p.stream);
+        if (has_hi) store_values<DT, E, false>(at + apart * kWidth<DT>, y, 1.0f, p.stream);
       }
     }
   }
