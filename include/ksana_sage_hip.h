@@ -553,8 +553,8 @@ typedef struct ksana_sage_cache {
   const int32_t *q_lens, *k_lens; /* device, [B]; q_lens NULL: all rows                                               */
 } ksana_sage_cache;
 /* Stores the call's keys, turned, and values; q, if there is one, is turned on the way into q_out (contiguous; zeros behind the
- * counts).  e4m3: to the nearest code, what lies beyond the largest at that.  D = 128 or 64.  Pages that are written to belong to one
- * sequence.  Repeated calls give the same bits. */
+ * counts).  e4m3: to the code nearest to the fp32 value divided by the scale, of two as near the even one; what lies beyond the largest at
+ * that.  D = 128 or 64.  Pages that are written to belong to one sequence.  Repeated calls give the same bits. */
 int ksana_sage_cache_append(const ksana_sage_rotary* call, const ksana_sage_cache* cache, const void* q, const void* k, const void* v,
                             void* q_out, void* stream);
 

@@ -110,7 +110,7 @@ def append(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, pages: torch.Ten
 
     ``frequencies``, ``sections``, ``interleaved`` and ``magnitude`` are those of ``train_ops.rotary`` and turn k and q; so do ``positions``, which are by
     default the rows' own in their sequences.  Without ``frequencies`` nothing turns, and q is not taken.  An 8-bit cache gets the
-    nearest of its numbers, beyond the largest that one.
+    nearest of its numbers to the value (a key as it is turned, in fp32) divided by the scale, beyond the largest that one.
 
     Rows behind ``q_lens[b]`` are not stored, and zeros in the result.  Nor are rows at negative positions, behind the table's end or in pages that do not exist
     (entries that are negative or not below the cache's pages).  A page that is written to belongs to one sequence and stands in its table once."""
