@@ -538,7 +538,9 @@ typedef struct ksana_sage_rotary {
 int ksana_sage_rotary_rows(const ksana_sage_rotary* call, const void* q, const void* k, void* q_out, void* k_out, void* stream);
 
 /* Where a batch's sequences lie.  Token t of entry b is in page table[b table_stride + t / page_size], slot t % page_size.  Of its
- * k_lens[b] tokens the last q_lens[b] are the call's.  Counts are clamped to what the table and the call's rows hold.  Entries that name no
+ * k_lens[b] tokens the last q_lens[b] are the call's.  Counts below 0 are 0, q_lens at most the call's rows.  k_lens beyond
+ * table_width * page_size are the caller's error: append goes by the tokens' own positions and stores those that have a place, attention takes
+ * the table's end as the sequence's; both stay within the table.  Entries that name no
  * page (negative, or not below `pages`) are allowed everywhere: nothing is stored there, and keys there are not seen. */
 #define KSANA_SAGE_E4M3 3
 typedef struct ksana_sage_cache {

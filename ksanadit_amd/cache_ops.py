@@ -10,7 +10,9 @@ so row i of the chunk stands at position ``k_lens[b] - q_lens[b] + i``.  Every l
 
 Both run on the tensors' HIP device, on torch's current stream there; scratch comes from torch's caching allocator.  They do not synchronise and may be captured into a
 graph, with counts as int32 tensors on that device (others are copied there in the call, which waits for the copy and cannot be captured); table and counts are read by the
-kernels, so that replays go by what they hold then.  Counts are taken as what the table and the call's rows hold at most.  Repeated calls give the same
+kernels, so that replays go by what they hold then.  Counts below 0 are 0, and ``q_lens`` are at most the call's rows.  ``k_lens`` beyond ``entries * page_size``, more tokens than
+the table has room for, are the caller's error, which calls that do not synchronise cannot report.  Both stay within the table then, but do not agree: ``append`` turns and stores rows by
+their positions and leaves out those behind the table's end, ``attention`` takes that end as the sequence's.  Repeated calls give the same
 bits.  There is no backward pass: ``train_ops`` has those.
 """
 
