@@ -22,8 +22,8 @@ Differences, all deliberate:
 * ``trainable`` (constructor argument, opt-in): calls whose inputs require gradients, with gradients enabled, run the 16-bit attention
   that has a backward pass (``train_ops.attention``) in place of the quantized one, which has none; all other calls are as ever;
 * ``kv_cache`` (keyword of a call, with ``pages``, ``k_lens`` and, if wanted, ``q_lens`` and ``rotary``): the call's keys and values are stored in a paged
-  cache and its queries attend to everything their sequences have there (``cache_ops.append`` and ``cache_ops.attention``, 16-bit products; ``rotary``: a
-  dict of ``append``'s rotary arguments).  The counts are then always honoured;
+  cache and its queries attend to everything their sequences have there (``cache_ops.append`` and ``cache_ops.attention``, 16-bit products, other types rounded to an fp16 cache's or to
+  bf16; ``rotary``: a dict of ``append``'s rotary arguments).  The counts are then always honoured;
 * ``pwl_exp2`` (constructor argument, opt-in): a form of exp2 without the transcendental, 1.06-1.12x the speed at
   27 000 keys and more (head size 128; no gain at 4 400 and below) at a cosine similarity lower by ~1.5e-4;
 * availability: no HIP device -> ``supports()`` is False and the selector moves on, like the
@@ -96,7 +96,8 @@ class SageAttentionImpl(KsanaAttentionBackendImpl):
         original_dtype = query.dtype
         if kwargs.get("kv_cache") is not None:
             if original_dtype not in (torch.float16, torch.bfloat16):
-                query, key, value = (t.to(torch.bfloat16) for t in (query, key, value))
+                kept = kwargs["kv_cache"].k.dtype
+                query, key, value = (t.to(kept if kept == torch.float16 else torch.bfloat16) for t in (query, key, value))
             return self._forward_cached(query, key, value, **kwargs).to(original_dtype if self.out_dtype is None else self.out_dtype)
         if original_dtype not in (torch.float16, torch.bfloat16):
             query, key, value = (t.to(torch.bfloat16) for t in (query, key, value))
