@@ -743,7 +743,9 @@ void fill_in(CacheAttnParams& p) {
   if (p.Lq * p.group <= kFewRows) {
     // In us: the keys' and values' bytes at the memory's rate, half of what a wave takes for its tiles one after the other, workgroups that come and go, the second launch and
     // its bytes.  (One token on 32760 keys, 8 heads: 64 runs 28, 10 runs 52; 64 sequences of up to 8192: 2 runs 229, 4 232, 8 245; one of 2000: 17 runs 11.5, 9 12.5, 5 15.8.)
-    const double places = p.eight_bits ? 1024.0 : 512.0, all = 2.0 * kTrainTile * p.D * (p.eight_bits ? 1.0 / 4.2e6 : 2.0 / 5.0e6) * tiles * blocks;
+    // A compute unit has places for two workgroups of 16-bit rows of 128 channels, whose tiles fill its LDS, and for four of the others.  (64 channels with 1024 places, and with 512: 8
+    // sequences of 4096 16.4 us and 18.2, 4 of 32760 58.0 and 61.7, 64 of up to 8192 127 and 131, one of 32760, 40 key heads, 72 and 75.)
+    const double places = p.eight_bits || p.D == 64 ? 1024.0 : 512.0, all = 2.0 * kTrainTile * p.D * (p.eight_bits ? 1.0 / 4.2e6 : 2.0 / 5.0e6) * tiles * blocks;
     for (int n = 1; n <= most; ++n) {
       const double each = (double)((tiles + n - 1) / n), workgroups = (double)n * blocks;
       const double cost = all + 0.85 * std::ceil(each / kFewWaves) + 2.0 * std::max(1.0, workgroups / places) + (n == 1 ? 0.0 : 3.0 + 2.0 * workgroups * rows * p.D * 4.0 / 4e6);
