@@ -155,7 +155,8 @@ def attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, k_lens, q
 
     ``sm_scale`` is ``D ** -0.5`` by default.  Rows behind ``q_lens[b]`` and rows that see no key are zeros.  Keys behind ``k_lens[b]`` are not read, and keys in pages that
     do not exist (entries that are negative or not below the cache's pages) are not seen.  Scores, softmax statistics and sums are fp32; probabilities are rounded to q's type
-    where they are multiplied on (in two parts on 16-bit caches, up to 32 rows to a key head).  Keys that only causal masking hides have the weight 0, as in a product of matrices:
+    where they are multiplied on (in two parts on 16-bit caches, up to 32 rows to a key head).  Over n keys fp32's sums are off by about 2^-29 n of
+    themselves if all roundings go one way, half a step of fp16 at 2^18 keys; where they do not, by far less.  Keys that only causal masking hides have the weight 0, as in a product of matrices:
     not-a-numbers and infinities among them may show in the rows before."""
     _check_rows("attention", q)
     kind = _check_cache(cache, pages, q, None)

@@ -5,14 +5,15 @@
 // place, and their weight is zero.
 //
 // A wave keeps 32 query rows (S^T = k q^T: a lane holds scores of one row) and walks tiles of 64 keys with a running maximum and sum.  Probabilities are rounded to the
-// tensors' type where they are multiplied with the values, as the matrix instructions want them (off by 2^-8 or 2^-11 of each at most; few rows on 16-bit caches: twice, off
-// by 2^-16 or 2^-22), and everything else is fp32.
+// tensors' type where they are multiplied with the values, as the matrix instructions want them: off by 2^-8 (bf16) or 2^-11 (fp16) of each at most, few rows on 16-bit caches,
+// which have them in two parts, by 2^-16 or 2^-22; in fp16 besides by 2^-31 of the row's largest, the half step of its smallest numbers (2^-24, of weights scaled by 2^6).  Everything
+// else is fp32.
 // A tile's pages are looked up by its 64 keys' lanes ahead of its copies.  Of 8-bit caches the tiles are widened, exactly, on their way to LDS; the scales go into c and into
 // the result.  Loops of few blocks are cut into runs, which a second launch joins: a block's runs share the tiles that its sequence really has.
 //
-// Many rows are bound by the power that the matrix pipes draw: 4096 causal rows on 32768 keys of 128 channels, 40 heads on 8, take 2.33 ms, 1.10e15 operations /s, of zeros
-// 1.70.  (The same kernel on keys in a row takes 3 % less; a library's product reaches 1.35e15.)  Few rows are bound by the keys' and values' bytes: one token of 40
-// heads on 32760 keys 28.6 us from memory, 4.7 TB/s, and 4 for the join; 64 of up to 8192 tokens 217, 5.5 TB/s.
+// Many rows are bound by the power that the matrix pipes draw: 4096 causal rows on 32768 keys of 128 channels, 40 heads on 8, take 2.32 to 2.40 ms by the card, 1.07 to
+// 1.11e15 operations /s, of zeros 1.70.  (The same kernel on keys in a row takes 3 % less; a library's product reaches 1.35e15.)  Few rows are bound by the keys' and values' bytes: one token of 40
+// heads on 32760 keys 28.5 us from memory, 4.7 TB/s, and 4 for the join; 64 of up to 8192 tokens 216, 5.5 TB/s.
 #include "sage_cache.h"
 #include "sage_train_device.h"
 
@@ -141,7 +142,9 @@ struct PagedCopy {
   }
 };
 
-// A tile of 8-bit rows, the wave's share, on its way through registers: sixteen channels at an access, D / 16 lanes to a row
+// A tile of 8-bit rows, the wave's share, on its way through registers: sixteen channels at an access, D / 16 lanes to a row.  (Where an address is the cache's or kZeroRow's the compiler
+// makes loads of any address space of both, which count as LDS accesses too: a wait for LDS behind `start` is one for them.  Rows' 16 bytes are written every 32, where lanes of
+// neighbouring rows meet in the same banks, 8 cycles for each write.)
 template <int DT, int D, int kWaves>
 struct WideCopy {
   using T = Tile<D>;
@@ -223,7 +226,8 @@ __device__ __forceinline__ float hide_scores(v16f (&s)[2], int limit, uint64_t e
 // Many rows: four waves of 32 share a tile's copies, two workgroups to a compute unit, so that each SIMD has two waves.  While the probabilities of tile t are formed and
 // multiplied with its values, the scores of tile t + 1 are: a few vector instructions stand behind every matrix instruction and run beside it.  So values are
 // wanted a step after their keys; each have two places in LDS.  Of 128 channels about 20 registers go through memory, outside the loop.
-// 4096 causal rows on 32768 keys, 40 heads on 8: bf16 2330 us, fp16 2480, 8 bits 2500; of 64 channels, 32 heads on 8, 1190, where exponentials count twice as much.
+// 4096 causal rows on 32768 keys, 40 heads on 8, on one card: bf16 2330 us, fp16 2500, 8 bits 2510 (fp16 2600); of 64 channels, 32 heads on 8, 1200, where exponentials count
+// twice as much.
 template <int DT, int D, bool kEight>
 __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttnParams p) {
   using T = Tile<D>;
@@ -437,9 +441,9 @@ __global__ __launch_bounds__(256, 2) void sage_cache_rows_kernel(const CacheAttn
 // Up to 32 query rows in all: waves share the rows and take a run's tiles in turn, each through LDS of its own, without a barrier.  A tile's values are on their way
 // while its scores are formed and the next one's keys while its probabilities and their product are.  In the end the waves' sums are added up.
 constexpr int kFewRows = 32, kFewWaves = 2;
-// A wave's keys, values and entries.  Of 8 bits keys and values take the same place in turn, since they are on their way in registers: four workgroups to a
-// compute unit instead of two.  (16 sequences of up to 32760 tokens, 8 heads of 128 channels: 199 us with two, 167 with four, 146, 4.3 TB/s, with the next keys and values
-// asked for as soon as these are in LDS.  Without any product, exponential or write to LDS it takes 131.)
+// A wave's keys, values and entries.  Of 8 bits keys and values take the same place in turn, since they pass through registers: four workgroups to a
+// compute unit instead of two.  (16 sequences of up to 32760 tokens, 8 heads of 128 channels: 199 us with two, 167 with four, 143, 4.4 TB/s, with the next keys and values
+// asked for as soon as these are in LDS.  Without any product, exponential or write to LDS, but with the waits for LDS, it takes 131.)
 template <int D, bool kEight>
 constexpr int kFewWaveLds = (kEight ? 1 : 2) * Tile<D>::kBytes + 512;
 template <int D, bool kEight>
@@ -529,7 +533,8 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
       look_up(i + 2);
       copy_keys(next64);
     };
-    // On their way here: the entries of tile i + 1, tile i's keys, its values.  (8 bits: the next ones as soon as these are in LDS.)
+    // On their way here: the entries of tile i + 1, tile i's keys, its values.  (8 bits: the next ones are asked for as soon as these are in LDS, and are there when LDS is next waited for, see
+    // WideCopy: it is the compute unit's other waves that work meanwhile.)
     auto step = [&](int i, auto last) {
       copies_there<kCopies>();
       if constexpr (kEight) {
@@ -563,8 +568,8 @@ __global__ __launch_bounds__(64 * kFewWaves, kEight ? 2 : 1) void sage_cache_few
           for (int j = 0; j < 16; ++j) acc[d][j] *= factor;
       }
       // Probabilities in two parts of 16 bits, the second what rounding takes off the first: the matrix pipes have the time while memory is waited for (64 sequences of up to
-      // 8192 tokens 233.3 -> 233.9 us, one token on 32760 keys 35.1 -> 35.5), and the result's error is that of its own rounding (0.0016 for 0.0023).  Of 8 bits, where half as
-      // many bytes are waited for, it costs 2 to 5 %, and the cache's own rounding is far larger: one part.
+      // 8192 tokens 233.3 -> 233.9 us, one token on 32760 keys 35.1 -> 35.5), and the result's error is that of its own rounding (0.0016 for 0.0023).  Of 8 bits it costs this
+      // loop 2 to 5 %, since its loads are not in flight beside the products, and the cache's own rounding is far larger: one part.
       constexpr int kParts = kEight ? 1 : 2;
       v4i pr[kParts][4];
       float own = 0.0f;  // (of the tile, as above)

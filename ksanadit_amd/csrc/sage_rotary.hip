@@ -5,11 +5,11 @@
 // for the pairs (a, b) of a row's first R channels: channels 2 i and 2 i + 1, or i and i + R / 2.  The others are copied.  Backward: t negated.
 //
 // The angle is formed in turns in 64 bits - fp32 would be off by 2^-24 of it, 0.06 radians at a position of 10^6 - and what is left of it after its
-// quarter turns are taken off goes on in 32.
+// quarter turns are taken off goes on in 32: off by a few 2^-24, and by about 2^-52 of the angle, 2^-24 from 2^28 radians on.
 //
 // Bound by the rows' bytes: a workgroup forms its tokens' cosines and sines once, into LDS, and takes the rows of all heads through, the first ones asked for before.
-// 32760 tokens, 2 x 40 heads of 128 channels, bf16: 230 us a direction from memory, 5.8 TB/s; of 64 channels 138, 4.9 TB/s; prompts of 16384 and 9011 tokens into
-// pages, 32 + 8 + 8 heads: 149 us, 4.6 TB/s.  Few tokens are a chain of latencies: 5 us.
+// 32760 tokens, 2 x 40 heads of 128 channels, bf16: 227 to 235 us a direction from memory, 5.8 TB/s; of 64 channels 130, 5.2 TB/s; prompts of 16384 and 9011 tokens into
+// pages, 32 + 8 + 8 heads: 130 us, 5.3 TB/s.  Few tokens are a chain of latencies: 5 us.
 #include "sage_cache.h"
 #include "sage_device.h"
 #include "sage_train.h"
@@ -20,7 +20,9 @@ namespace ksana_sage {
 
 namespace {
 
-enum Layout { kInterleaved, kHalves, kSingle };  // 16 bytes at an access, or (either order of pairs) one value
+// 16 bytes at an access, or (either order of pairs) one value, where these do not divide the head, the turned channels or, of halves, each half of them.  (32760 tokens, 2 x 16 heads
+// of 80 channels of bf16, 40 of them turned: interleaved 72 us, 4.7 TB/s; halves of 20 value by value 186, 1.8 TB/s.)
+enum Layout { kInterleaved, kHalves, kSingle };
 template <int DT, Layout kLayout>
 constexpr int kAtOnce = kLayout == kSingle ? 1 : DT == kFp32 ? 4 : 8;
 
@@ -160,8 +162,8 @@ constexpr int kMostTokens = 16;
 
 // A workgroup takes a few tokens: first its threads form a cosine and a sine each, of a pair of a token, then all rows go through, a thread with E channels at `lo`
 // and E at `hi` of every one, neighbours beside each other.  (Every thread forming what it needs itself, eight pairs for three rows: 360 us
-// of 32760 tokens, 2 x 40 heads, where this takes 230.)  Seven waves to a SIMD: with six the 1560 workgroups of a frame in 8 bits take a round more, 29.4 us for 27.4, and
-// the 32760 tokens 237.
+// of 32760 tokens, 2 x 40 heads, where this takes 230.)  Seven waves to a SIMD: with six the 1560 workgroups of a frame in 8 bits take a round more, 27.4 us for 24.6, and with eight
+// registers go through memory, 27.5.
 template <int DT, Layout kLayout, bool kCache, bool kEight>
 __global__ __launch_bounds__(256, 7) void sage_rotary_kernel(const RotaryParams p) {
   constexpr int E = kAtOnce<DT, kLayout>, kAhead = 2;
@@ -370,15 +372,15 @@ hipError_t launch_rotary(RotaryParams p, hipStream_t s) {
   p.units = layout == kInterleaved ? (p.D / at_once + 1) / 2
             : layout == kHalves    ? p.R / (2 * at_once) + (p.D - p.R + 2 * at_once - 1) / (2 * at_once)
                                    : p.R / 2 + (p.D - p.R + 1) / 2;
-  // 16-bit results go first out of the caches, as what has been read, where an access of neighbours fills whole lines.  32760 tokens, 2 x 40 heads of 128: 244 us, kept
-  // like others 256; of 80 channels, 32 of them turned, 221 and 177.
+  // 16-bit results go first out of the caches, as what has been read, where an access of neighbours fills whole lines.  32760 tokens, 2 x 40 heads of 128: 236 us, kept
+  // like others 247; of 64 channels 139 and 130; of 80, 32 of them turned, 222 and 155.
   const int piece = layout == kInterleaved ? p.units * 16 : p.R;
   p.stream = layout != kSingle && p.dtype != kFp32 && piece % 128 == 0 && (layout == kInterleaved ? p.D == 16 * p.units : p.R == p.D);
   p.slots = 256 / p.units;  // rows at a time
   p.by_heads = divisor(p.heads);
   p.by_length = divisor(p.L);
-  // About three rows to a thread where that leaves four workgroups to each of 256 compute units.  Forward and backward of 32760 tokens, 2 x 40 heads: of one
-  // token 503 us, of two 508, of four 530, of sixteen 598.
+  // About three rows to a thread where that leaves four workgroups to each of 256 compute units.  32760 tokens, 2 x 40 heads: of one token 234 us, of
+  // two 254, of four 266, of sixteen 278; two prompts, 48 heads: 143, 132, 133, 157; a frame in 8 bits of one 24.5, of more 29.6.
   const int tokens = p.B * p.L;
   p.tokens_each = std::max({1, std::min({kMostTokens, 3 * p.slots / p.heads, (tokens + 1023) / 1024}), (tokens + (1 << 23) - 1) >> 23});  // (a launch has fewer than 2^32 threads)
   const unsigned groups = (unsigned)((tokens + p.tokens_each - 1) / p.tokens_each);
